@@ -1,0 +1,510 @@
+// Attention of one new token per sequence over a paged key-value cache, split
+// over the caches' lengths and joined.
+//
+//   out[b][h] = sum_t p_t v_t / sum_t p_t,  p_t = exp(scale q[b][h].k_t - max)
+//
+// Bound by reading K and V once.  The visible keys of all (sequence, KV head)
+// items are cut into blocks of 128 keys, laid end to end, and dealt to the
+// workgroups in equal runs, so that ragged batches, single long sequences and
+// many short ones fill the chip alike.  A run that covers an item's blocks only in
+// part leaves a partial (O, max, sum), and a second kernel joins these in order.
+//
+// A wave takes 32 keys at a time on MFMA, with no LDS in the loop:
+//   S^T [keys x heads] = K Q^T: a lane's A operand is 16 bytes of a key's row,
+//     loaded as they lie; the 16 columns are the KV head's query heads.
+//   O^T [dims x heads] += V^T P^T: the lane's S^T values are its B operand as
+//     they are (the order of the contraction's keys is free), and the A operand
+//     is a transposition of 8 keys x D / 16 dims within the lane's registers.
+// Row maximum and sum belong to a column, so each lane holds its own head's.
+#include "fpv2_common.h"
+#include "fpv2_decode.h"
+
+namespace fpv2 {
+namespace {
+
+constexpr int kBlockKeys = 128;  // keys of a block: 32 for each of the 4 waves
+constexpr int kWaveKeys = 32;
+constexpr int kMaxHeads = 16;  // query heads of an item (columns of an MFMA tile)
+
+struct DecodeArgs {
+  const uint16_t* q;
+  const uint16_t* k;
+  const uint16_t* v;
+  uint16_t* out;
+  const int32_t* table;
+  const int32_t* lengths;
+  float* part_o;   // [2 * grid][item_heads][D]
+  float* part_ml;  // [2 * grid][item_heads][2]
+  int64_t q_bs, q_hs, k_ps, k_hs, k_rs, v_ps, v_hs, v_rs, o_bs, o_hs, table_stride;
+  int batch, kv_heads, group, item_heads, head_items;  // head_items * item_heads >= group
+  int pages, page_size, capacity, length, window, sinks, grid;
+  uint32_t page_mul, page_shift;  // t / page_size = (umulhi(t, mul) + t) >> shift
+  float scale_log2;
+};
+
+struct Sequence {
+  int n;      // visible keys
+  int sinks;  // of which at the start
+  int skip;   // key of visible index u >= sinks: u + skip
+  int blocks;
+};
+
+__device__ __forceinline__ Sequence sequence_of(const DecodeArgs& a, int b) {
+  int len = a.lengths != nullptr ? a.lengths[b] : a.length;
+  len = min(max(len, 0), a.capacity);
+  Sequence s;
+  s.sinks = min(a.sinks, len);
+  const int start = max(s.sinks, len - a.window);
+  s.skip = start - s.sinks;
+  s.n = len - s.skip;
+  s.blocks = max(1, (s.n + kBlockKeys - 1) / kBlockKeys);  // (an empty one writes its zeros)
+  return s;
+}
+
+// Blocks of one item of every sequence, and of the ones before sequence `end`.
+__device__ __forceinline__ int wave_total(const DecodeArgs& a, int lane, int end, int* before) {
+  int all = 0, some = 0;
+  for (int b = lane; b < a.batch; b += 64) {
+    const int n = sequence_of(a, b).blocks;
+    all += n;
+    some += b < end ? n : 0;
+  }
+#pragma unroll
+  for (int off = 32; off >= 1; off >>= 1) {
+    all += __shfl_xor(all, off, 64);
+    some += __shfl_xor(some, off, 64);
+  }
+  *before = some;
+  return all;
+}
+
+template <int NW>
+struct Words { uint32_t w[NW]; };
+
+template <int NW>
+__device__ __forceinline__ Words<NW> load_words(const uint16_t* p) {
+  Words<NW> r;
+  if constexpr (NW % 4 == 0) {
+#pragma unroll
+    for (int i = 0; i < NW / 4; ++i) {
+      const u32x4 x = load16(p + 8 * i);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) r.w[4 * i + j] = x[j];
+    }
+  } else if constexpr (NW == 2) {
+    const u32x2 x = *reinterpret_cast<const u32x2*>(p);
+    r.w[0] = x[0];
+    r.w[1] = x[1];
+  } else {
+#pragma unroll
+    for (int i = 0; i < NW; ++i) r.w[i] = reinterpret_cast<const uint32_t*>(p)[i];
+  }
+  return r;
+}
+
+template <typename T, int D>
+__global__ __launch_bounds__(256, 2) void decode_attn_kernel(DecodeArgs a) {
+  constexpr int KK = D / 32;  // MFMA steps of a key's dot product
+  constexpr int DV = D / 16;  // dims of a lane
+  __shared__ float sh_o[4][kMaxHeads][D + 4];
+  __shared__ float sh_ml[4][kMaxHeads][2];
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int col = lane & 15, quad = lane >> 4;
+  const int items = a.kv_heads * a.head_items;
+
+  int before;
+  const int per_item = wave_total(a, lane, 0, &before);
+  const int total = per_item * items;
+  const int per = (total + a.grid - 1) / a.grid;
+  const int lo = min(total, static_cast<int>(blockIdx.x) * per), hi = min(total, lo + per);
+  if (lo >= hi) return;
+
+  // the sequence that holds block lo: base is its first block
+  int b = 0, base = 0;
+  for (int b0 = 0; b0 < a.batch; b0 += 64) {
+    int sum = b0 + lane < a.batch ? sequence_of(a, b0 + lane).blocks * items : 0;
+#pragma unroll
+    for (int off = 1; off < 64; off <<= 1) {
+      const int up = __shfl_up(sum, off, 64);
+      sum += lane >= off ? up : 0;
+    }
+    const uint64_t past = __ballot(base + sum > lo);
+    if (past != 0) {
+      const int at = __ffsll(static_cast<unsigned long long>(past)) - 1;
+      b = b0 + at;
+      base += at > 0 ? __shfl(sum, at - 1, 64) : 0;
+      break;
+    }
+    base += __shfl(sum, 63, 64);
+  }
+  b = __builtin_amdgcn_readfirstlane(b);
+  base = __builtin_amdgcn_readfirstlane(base);
+
+  Sequence s = sequence_of(a, b);
+  for (int cur = lo; cur < hi;) {
+    const int item = (cur - base) / s.blocks;
+    const int item_start = base + item * s.blocks;
+    const int first = cur - item_start;
+    const int end = min(hi, item_start + s.blocks);
+    const int last = end - item_start;  // blocks [first, last) of the item
+    const int kvh = item / a.head_items;
+    const int h0 = (item - kvh * a.head_items) * a.item_heads;
+    const int heads = min(a.item_heads, a.group - h0);
+    const int head = kvh * a.group + h0 + col;
+
+    u32x4 qf[KK];
+#pragma unroll
+    for (int kk = 0; kk < KK; ++kk) {
+      qf[kk] = u32x4{0, 0, 0, 0};
+      if (col < heads) qf[kk] = load16(a.q + b * a.q_bs + head * a.q_hs + 32 * kk + 8 * quad);
+    }
+    f32x4 o[DV];
+#pragma unroll
+    for (int d = 0; d < DV; ++d) o[d] = f32x4{0.f, 0.f, 0.f, 0.f};
+    float m = neg_inf(), l = 0.f;
+
+    const uint16_t* kb = a.k + kvh * a.k_hs;
+    const uint16_t* vb = a.v + kvh * a.v_hs;
+    const int32_t* table = a.table != nullptr ? a.table + b * a.table_stride : nullptr;
+    // lane i (and i + 32) looks up the row of the tile's key i
+    auto lookup = [&](int u0, int* row) {
+      const int u = min(u0 + (lane & 31), s.n - 1);
+      const uint32_t t = u < s.sinks ? u : u + s.skip;
+      const uint32_t page = (__umulhi(t, a.page_mul) + t) >> a.page_shift;
+      *row = t - page * a.page_size;
+      const int id = table != nullptr ? table[page] : b;
+      return min(max(id, 0), a.pages - 1);
+    };
+    int u0 = first * kBlockKeys + wave * kWaveKeys;
+    const int u_end = min(s.n, last * kBlockKeys);
+    int row = 0, page = 0;
+    if (u0 < u_end) page = lookup(u0, &row);
+    for (; u0 < u_end; u0 += kBlockKeys) {
+      const int64_t koff = page * a.k_ps + row * a.k_rs;
+      const int64_t voff = page * a.v_ps + row * a.v_rs;
+      u32x4 kf[2][KK];
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        const uint16_t* p = kb + __shfl(koff, 16 * t + col, 64) + 8 * quad;
+#pragma unroll
+        for (int kk = 0; kk < KK; ++kk) kf[t][kk] = load16(p + 32 * kk);
+      }
+      Words<DV / 2> vf[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        vf[j] = load_words<DV / 2>(vb + __shfl(voff, 16 * (j / 4) + 4 * quad + j % 4, 64) + DV * col);
+      if (u0 + kBlockKeys < u_end) page = lookup(u0 + kBlockKeys, &row);
+
+      f32x4 sc[2];
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        sc[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int kk = 0; kk < KK; ++kk)
+          sc[t] = Elem<T>::mfma16(as_vec8<T>(kf[t][kk]), as_vec8<T>(qf[kk]), sc[t]);
+      }
+      const bool cut = u0 + kWaveKeys > s.n;
+      float x[8], top = neg_inf();
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        x[j] = sc[j / 4][j % 4] * a.scale_log2;
+        if (cut && u0 + 16 * (j / 4) + 4 * quad + j % 4 >= s.n) {
+          x[j] = neg_inf();
+          // (a zero weight would make NaN of what an unused row may hold)
+#pragma unroll
+          for (int w = 0; w < DV / 2; ++w) vf[j].w[w] = 0;
+        }
+        top = fmaxf(top, x[j]);
+      }
+      top = fmaxf(top, __shfl_xor(top, 16, 64));
+      top = fmaxf(top, __shfl_xor(top, 32, 64));
+      const float m_new = fmaxf(m, top);
+      // (nothing but -inf so far: weights of zero instead of NaN)
+      const float ref = m_new == neg_inf() ? 0.f : m_new;
+      const float fix = __builtin_amdgcn_exp2f(m - ref);
+      m = m_new;
+      l *= fix;
+      u32x4 pf;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) x[j] = __builtin_amdgcn_exp2f(x[j] - ref);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        pf[j] = pack2<T>(x[2 * j], x[2 * j + 1]);
+        l += x[2 * j] + x[2 * j + 1];
+      }
+#pragma unroll
+      for (int d = 0; d < DV; ++d) {
+        o[d] *= fix;
+        u32x4 vt;  // dim d of the lane's 8 keys
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          vt[j] = __builtin_amdgcn_perm(vf[2 * j + 1].w[d / 2], vf[2 * j].w[d / 2],
+                                        d % 2 ? 0x07060302u : 0x05040100u);
+        o[d] = Elem<T>::mfma16(as_vec8<T>(vt), as_vec8<T>(pf), o[d]);
+      }
+    }
+    l += __shfl_xor(l, 16, 64);
+    l += __shfl_xor(l, 32, 64);
+
+    // join the four waves
+    if (quad == 0) {
+      sh_ml[wave][col][0] = m;
+      sh_ml[wave][col][1] = l;
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int d = 0; d < DV; ++d) sh_o[wave][col][(4 * quad + i) * DV + d] = o[d][i];
+    __syncthreads();
+    const bool whole = first == 0 && last == s.blocks;
+    const int64_t slot = 2 * static_cast<int64_t>(blockIdx.x) + (cur == lo ? 0 : 1);
+    for (int e = tid; e < heads * D; e += 256) {
+      const int h = e / D, d = e % D;
+      float top = neg_inf();
+#pragma unroll
+      for (int w = 0; w < 4; ++w) top = fmaxf(top, sh_ml[w][h][0]);
+      const float ref = top == neg_inf() ? 0.f : top;
+      float sum = 0.f, den = 0.f;
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        // (a wave without keys has max -inf, sum 0 and O 0)
+        const float f = __builtin_amdgcn_exp2f(sh_ml[w][h][0] - ref);
+        sum += f * sh_o[w][h][d];
+        den += f * sh_ml[w][h][1];
+      }
+      if (whole) {
+        const float r = s.n == 0 ? 0.f : sum / den;
+        a.out[b * a.o_bs + (kvh * a.group + h0 + h) * a.o_hs + d] = Elem<T>::from_float(r);
+      } else {
+        a.part_o[(slot * a.item_heads + h) * D + d] = sum;
+        if (d == 0) {
+          a.part_ml[(slot * a.item_heads + h) * 2] = top;
+          a.part_ml[(slot * a.item_heads + h) * 2 + 1] = den;
+        }
+      }
+    }
+    __syncthreads();
+    cur = end;
+    if (cur < hi && cur == base + items * s.blocks) {
+      base = cur;
+      s = sequence_of(a, ++b);
+    }
+  }
+}
+
+// Joins the partials of an item that several workgroups shared: one workgroup
+// per (item, query head), the partials dealt to its waves in order.
+template <typename T, int D>
+__global__ __launch_bounds__(256) void decode_join_kernel(DecodeArgs a) {
+  __shared__ float sh_o[4][D];
+  __shared__ float sh_ml[4][2];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int items = a.kv_heads * a.head_items;
+  const int h = blockIdx.x % a.item_heads;
+  const int at = blockIdx.x / a.item_heads;
+  const int b = at / items, item = at - b * items;
+  const int kvh = item / a.head_items, h0 = (item - kvh * a.head_items) * a.item_heads;
+  if (h0 + h >= a.group) return;
+  int before;
+  const int total = wave_total(a, lane, b, &before) * items;
+  const int per = (total + a.grid - 1) / a.grid;
+  const Sequence s = sequence_of(a, b);
+  const int start = before * items + item * s.blocks;
+  const int w0 = start / per, w1 = (start + s.blocks - 1) / per;
+  if (w0 == w1) return;  // written by its workgroup
+  constexpr int E = (D + 63) / 64;
+  float m = neg_inf(), l = 0.f, o[E];
+#pragma unroll
+  for (int e = 0; e < E; ++e) o[e] = 0.f;
+  for (int w = w0 + wave; w <= w1; w += 4) {
+    const int64_t slot = 2 * static_cast<int64_t>(w) + (start > w * per ? 1 : 0);
+    const float* po = a.part_o + (slot * a.item_heads + h) * D;
+    const float pm = a.part_ml[(slot * a.item_heads + h) * 2];
+    const float pl = a.part_ml[(slot * a.item_heads + h) * 2 + 1];
+    const float m_new = fmaxf(m, pm);
+    const float ref = m_new == neg_inf() ? 0.f : m_new;
+    const float f0 = __builtin_amdgcn_exp2f(m - ref), f1 = __builtin_amdgcn_exp2f(pm - ref);
+    m = m_new;
+    l = l * f0 + pl * f1;
+#pragma unroll
+    for (int e = 0; e < E; ++e)
+      if (64 * e + lane < D) o[e] = o[e] * f0 + po[64 * e + lane] * f1;
+  }
+#pragma unroll
+  for (int e = 0; e < E; ++e)
+    if (64 * e + lane < D) sh_o[wave][64 * e + lane] = o[e];
+  if (lane == 0) {
+    sh_ml[wave][0] = m;
+    sh_ml[wave][1] = l;
+  }
+  __syncthreads();
+  for (int d = tid; d < D; d += 256) {
+    float top = neg_inf();
+#pragma unroll
+    for (int w = 0; w < 4; ++w) top = fmaxf(top, sh_ml[w][0]);
+    const float ref = top == neg_inf() ? 0.f : top;
+    float sum = 0.f, den = 0.f;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      const float f = __builtin_amdgcn_exp2f(sh_ml[w][0] - ref);
+      sum += f * sh_o[w][d];
+      den += f * sh_ml[w][1];
+    }
+    a.out[b * a.o_bs + (kvh * a.group + h0 + h) * a.o_hs + d] = Elem<T>::from_float(sum / den);
+  }
+}
+
+struct DecodePlan {
+  int head_items, item_heads, grid;
+  int64_t most_blocks;  // of an item
+};
+
+// The launch of a call; its workspace goes by the same numbers.
+DecodePlan decode_plan(const fpv2_decode_params& p) {
+  DecodePlan plan;
+  const int64_t group = p.query_heads / p.kv_heads;
+  plan.head_items = static_cast<int>((group + kMaxHeads - 1) / kMaxHeads);
+  plan.item_heads = static_cast<int>((group + plan.head_items - 1) / plan.head_items);
+  int64_t keys = p.table_width * p.page_size;
+  if (p.window_tokens > 0 && p.window_tokens + p.sink_tokens < keys)
+    keys = p.window_tokens + p.sink_tokens;
+  plan.most_blocks = (keys + kBlockKeys - 1) / kBlockKeys;
+  if (plan.most_blocks < 1) plan.most_blocks = 1;
+  const int64_t blocks = p.batch * p.kv_heads * plan.head_items * plan.most_blocks;
+  const int64_t resident = 2 * static_cast<int64_t>(cu_count());
+  plan.grid = static_cast<int>(blocks < resident ? blocks : resident);
+  return plan;
+}
+
+int check_params(const char* name, const fpv2_decode_params* p) {
+  if (p == nullptr) return fail(FPV2_ERR_ARGUMENT, "%s: null params", name);
+  if (p->batch < 0 || p->query_heads <= 0 || p->kv_heads <= 0 || p->query_heads % p->kv_heads)
+    return fail(FPV2_ERR_ARGUMENT, "%s: query heads must be divisible by KV heads", name);
+  if (p->head_dim != 64 && p->head_dim != 96 && p->head_dim != 128 && p->head_dim != 256)
+    return fail(FPV2_ERR_UNSUPPORTED, "%s: head_dim must be 64, 96, 128 or 256", name);
+  if (p->batch > 0xffff || p->query_heads > 0xffff)
+    return fail(FPV2_ERR_UNSUPPORTED, "%s: more than 65535 sequences or query heads", name);
+  if (p->pages <= 0 || p->page_size <= 0 || p->table_width <= 0 || p->pages > 0x7fffffff ||
+      p->page_size > 0x3fffffff || p->table_width > 0x3fffffff ||
+      p->table_width * p->page_size > 0x3fffffff)
+    return fail(FPV2_ERR_ARGUMENT, "%s: pages, page_size and table_width must be positive and a "
+                "sequence's pages hold fewer than 2^30 tokens", name);
+  if (p->window_tokens < 0 || p->sink_tokens < 0 || p->length < 0)
+    return fail(FPV2_ERR_ARGUMENT, "%s: length, window_tokens and sink_tokens must not be negative", name);
+  const int64_t group = p->query_heads / p->kv_heads;
+  const int64_t items = p->batch * p->kv_heads * ((group + kMaxHeads - 1) / kMaxHeads);
+  if (items * kMaxHeads > 0x7fffffff ||
+      items * ((p->table_width * p->page_size + kBlockKeys - 1) / kBlockKeys) > 0x3fffffff)
+    return fail(FPV2_ERR_UNSUPPORTED, "%s: the call has too many blocks of keys", name);
+  return FPV2_OK;
+}
+
+int64_t partial_bytes(const fpv2_decode_params& p, const DecodePlan& plan) {
+  if (p.batch == 0 || plan.most_blocks <= 1) return 0;  // every item has one workgroup
+  return 2LL * plan.grid * plan.item_heads * (p.head_dim + 2) * 4;
+}
+
+template <typename T, int D>
+int launch(const DecodeArgs& a, bool join, hipStream_t s) {
+  hipLaunchKernelGGL((decode_attn_kernel<T, D>), dim3(a.grid), dim3(256), 0, s, a);
+  if (join) {
+    const unsigned grid = static_cast<unsigned>(a.batch) * a.kv_heads * a.head_items * a.item_heads;
+    hipLaunchKernelGGL((decode_join_kernel<T, D>), dim3(grid), dim3(256), 0, s, a);
+  }
+  return check_launch("decode_attn_kernel");
+}
+
+template <typename T>
+int launch_dim(const DecodeArgs& a, int64_t dim, bool join, hipStream_t s) {
+  switch (dim) {
+    case 64: return launch<T, 64>(a, join, s);
+    case 96: return launch<T, 96>(a, join, s);
+    case 128: return launch<T, 128>(a, join, s);
+    default: return launch<T, 256>(a, join, s);
+  }
+}
+
+}  // namespace
+}  // namespace fpv2
+
+extern "C" int64_t fpv2_decode_attention_workspace_bytes(const fpv2_decode_params* params) {
+  using namespace fpv2;
+  if (const int rc = check_params("fpv2_decode_attention", params)) return rc;
+  return partial_bytes(*params, decode_plan(*params));
+}
+
+extern "C" int fpv2_decode_attention(const void* q, const void* k_pages, const void* v_pages,
+                                     const int32_t* page_table, const int32_t* lengths, void* out,
+                                     int dtype, const fpv2_decode_params* params, void* workspace,
+                                     int64_t workspace_bytes, void* stream) {
+  using namespace fpv2;
+  const char* name = "fpv2_decode_attention";
+  const auto a16 = [](const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; };
+  if (const int rc = check_params(name, params)) return rc;
+  const fpv2_decode_params& p = *params;
+  if (dtype != FPV2_BF16 && dtype != FPV2_F16)
+    return fail(FPV2_ERR_UNSUPPORTED, "%s: dtype must be bf16 or f16", name);
+  if (p.batch == 0) return FPV2_OK;
+  if (!q || !k_pages || !v_pages || !out) return fail(FPV2_ERR_ARGUMENT, "%s: null pointer", name);
+  if (page_table == nullptr && (p.table_width != 1 || p.pages < p.batch))
+    return fail(FPV2_ERR_ARGUMENT, "%s: without a page table every sequence has one page", name);
+  if (page_table != nullptr && p.table_stride < 0)
+    return fail(FPV2_ERR_ARGUMENT, "%s: table_stride must not be negative", name);
+  const int64_t strides[] = {p.q_batch_stride, p.q_head_stride, p.k_page_stride, p.k_head_stride,
+                             p.k_row_stride,   p.v_page_stride, p.v_head_stride, p.v_row_stride};
+  for (const int64_t x : strides)
+    if (x < 0 || x % 8)
+      return fail(FPV2_ERR_ARGUMENT, "%s: strides of q, k and v must be multiples of 8", name);
+  if (p.o_batch_stride < 0 || p.o_head_stride < 0)
+    return fail(FPV2_ERR_ARGUMENT, "%s: output strides must not be negative", name);
+  if (!a16(q) || !a16(k_pages) || !a16(v_pages))
+    return fail(FPV2_ERR_ARGUMENT, "%s: q, k and v must be 16-byte aligned", name);
+  const DecodePlan plan = decode_plan(p);
+  const int64_t need = partial_bytes(p, plan);
+  if (need > 0 && (workspace == nullptr || workspace_bytes < need || !a16(workspace)))
+    return fail(FPV2_ERR_ARGUMENT, "%s: needs a 16-byte aligned workspace of %lld bytes", name,
+                static_cast<long long>(need));
+  DecodeArgs a{};
+  a.q = static_cast<const uint16_t*>(q);
+  a.k = static_cast<const uint16_t*>(k_pages);
+  a.v = static_cast<const uint16_t*>(v_pages);
+  a.out = static_cast<uint16_t*>(out);
+  a.table = page_table;
+  a.lengths = lengths;
+  a.part_o = static_cast<float*>(workspace);
+  a.part_ml = a.part_o + 2LL * plan.grid * plan.item_heads * p.head_dim;
+  a.q_bs = p.q_batch_stride;
+  a.q_hs = p.q_head_stride;
+  a.k_ps = p.k_page_stride;
+  a.k_hs = p.k_head_stride;
+  a.k_rs = p.k_row_stride;
+  a.v_ps = p.v_page_stride;
+  a.v_hs = p.v_head_stride;
+  a.v_rs = p.v_row_stride;
+  a.o_bs = p.o_batch_stride;
+  a.o_hs = p.o_head_stride;
+  a.table_stride = p.table_stride;
+  a.batch = static_cast<int>(p.batch);
+  a.kv_heads = static_cast<int>(p.kv_heads);
+  a.group = static_cast<int>(p.query_heads / p.kv_heads);
+  a.head_items = plan.head_items;
+  a.item_heads = plan.item_heads;
+  a.pages = static_cast<int>(p.pages);
+  a.page_size = static_cast<int>(p.page_size);
+  a.capacity = static_cast<int>(p.table_width * p.page_size);
+  a.length = static_cast<int>(p.length < a.capacity ? p.length : a.capacity);
+  a.window = static_cast<int>(p.window_tokens > 0 && p.window_tokens < a.capacity ? p.window_tokens
+                                                                                  : a.capacity);
+  a.sinks = static_cast<int>(p.sink_tokens < a.capacity ? p.sink_tokens : a.capacity);
+  a.grid = plan.grid;
+  uint32_t shift = 0;
+  while ((1ull << shift) < static_cast<uint64_t>(p.page_size)) ++shift;
+  a.page_shift = shift;
+  a.page_mul = static_cast<uint32_t>((((1ull << shift) - p.page_size) << 32) / p.page_size + 1);
+  a.scale_log2 = static_cast<float>(p.scale * 1.4426950408889634);
+  const hipStream_t s = static_cast<hipStream_t>(stream);
+  const bool join = plan.most_blocks > 1;
+  return dtype == FPV2_BF16 ? launch_dim<bf16_t>(a, p.head_dim, join, s)
+                            : launch_dim<f16_t>(a, p.head_dim, join, s);
+}

@@ -6,9 +6,12 @@ selection front end (``FPV2Config``/``pool_blocks``/``block_scores_and_select``/
 ``density``).  ``fpv2.kernel`` holds ``compact_block_indices`` and
 ``sparse_attention``.  ``ChunkedPrefill`` (``fpv2.chunked``) drives one
 layer's chunked prefill over a growing KV cache with incremental pooling.
+``fpv2.decode`` holds the operators of the decode step that follows:
+``decode_attention``.
 """
 
 from fpv2.chunked import ChunkedPrefill
+from fpv2.decode import decode_attention
 from fpv2.patch import block_sparsity, disable, enable, fpv2_sdpa, is_enabled
 from fpv2.selection import FPV2Config, block_scores_and_select, density, pool_blocks
 
@@ -17,6 +20,7 @@ __all__ = [
     "FPV2Config",
     "block_scores_and_select",
     "block_sparsity",
+    "decode_attention",
     "density",
     "disable",
     "enable",

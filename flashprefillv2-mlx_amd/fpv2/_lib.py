@@ -1,5 +1,5 @@
-"""ctypes binding of ``libfpv2_hip.so`` (C ABI declared in ``include/fpv2.h`` and
-``include/fpv2_decoder.h``).
+"""ctypes binding of ``libfpv2_hip.so`` (C ABI declared in ``include/fpv2.h``,
+``include/fpv2_decoder.h`` and ``include/fpv2_decode.h``).
 
 The library is built in-tree by ``flashprefillv2-mlx_amd/build.py``.  There is
 no fallback: if the library is missing or a tensor is not on a ROCm device,
@@ -53,6 +53,9 @@ EXPORTED_SYMBOLS = (
     "fpv2_qk_norm_rope",
     "fpv2_silu_mul",
     "fpv2_row_logits",
+    # a decode step's operators (fpv2_decode.h)
+    "fpv2_decode_attention_workspace_bytes",
+    "fpv2_decode_attention",
 )
 
 
@@ -107,6 +110,35 @@ class AttnParams(ctypes.Structure):
         ("o_head_stride", ctypes.c_int64),
         ("o_row_stride", ctypes.c_int64),
         ("pooled_head_stride", ctypes.c_int64),
+    ]
+
+
+class DecodeParams(ctypes.Structure):
+    """``fpv2_decode_params`` (field order and types as in fpv2_decode.h)."""
+
+    _fields_ = [
+        ("batch", ctypes.c_int64),
+        ("query_heads", ctypes.c_int64),
+        ("kv_heads", ctypes.c_int64),
+        ("head_dim", ctypes.c_int64),
+        ("pages", ctypes.c_int64),
+        ("page_size", ctypes.c_int64),
+        ("table_width", ctypes.c_int64),
+        ("table_stride", ctypes.c_int64),
+        ("length", ctypes.c_int64),
+        ("window_tokens", ctypes.c_int64),
+        ("sink_tokens", ctypes.c_int64),
+        ("scale", ctypes.c_double),
+        ("q_batch_stride", ctypes.c_int64),
+        ("q_head_stride", ctypes.c_int64),
+        ("k_page_stride", ctypes.c_int64),
+        ("k_head_stride", ctypes.c_int64),
+        ("k_row_stride", ctypes.c_int64),
+        ("v_page_stride", ctypes.c_int64),
+        ("v_head_stride", ctypes.c_int64),
+        ("v_row_stride", ctypes.c_int64),
+        ("o_batch_stride", ctypes.c_int64),
+        ("o_head_stride", ctypes.c_int64),
     ]
 
 
@@ -169,6 +201,10 @@ def _declare(lib: ctypes.CDLL) -> None:
     lib.fpv2_silu_mul.argtypes = [vp, vp, i32, i64, i64, i64, i64, vp]
     lib.fpv2_row_logits.restype = ctypes.c_int
     lib.fpv2_row_logits.argtypes = [vp, vp, vp, i32, i64, i64, i64, vp]
+    lib.fpv2_decode_attention_workspace_bytes.restype = i64
+    lib.fpv2_decode_attention_workspace_bytes.argtypes = [ctypes.POINTER(DecodeParams)]
+    lib.fpv2_decode_attention.restype = ctypes.c_int
+    lib.fpv2_decode_attention.argtypes = [vp] * 6 + [i32, ctypes.POINTER(DecodeParams), vp, i64, vp]
 
 
 def load(path: str | os.PathLike | None = None) -> ctypes.CDLL:

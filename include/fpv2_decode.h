@@ -1,0 +1,69 @@
+/*
+ * fpv2_decode.h — operators of a decode step (one new token per sequence
+ * after the FPV2 prefill), exported by libfpv2_hip.so.
+ *
+ * The reference ends where the prompt is prefilled (fpv2/generate.py:97-130
+ * hands the caches to mlx-lm, an external dependency, whose models decode
+ * over the cache with 4-bit weights and sample the tokens).  These are the
+ * gfx950 operators of that step: attention of single tokens over a paged or
+ * contiguous cache, norms and rotation with the cache write, products with
+ * 4-bit weights, and sampling.
+ *
+ * Conventions as in fpv2.h: device pointers, element strides, a hipStream_t
+ * passed as void*, work enqueued on that stream on the current device, no
+ * allocation, no host synchronisation, FPV2_OK or a negative fpv2_status with
+ * fpv2_last_error() set.  Lengths, page ids, positions and slots are read on
+ * the device; the ones out of range are clipped or skipped as stated.
+ */
+#ifndef FPV2_DECODE_H_
+#define FPV2_DECODE_H_
+
+#include <stdint.h>
+
+#ifdef __cplusplus
+extern "C" {
+#endif
+
+/* Attention of one new token per sequence over a cache in pages. */
+typedef struct fpv2_decode_params {
+  int64_t batch;
+  int64_t query_heads;
+  int64_t kv_heads;      /* divides query_heads                               */
+  int64_t head_dim;      /* 64, 96, 128 or 256                                */
+  int64_t pages;         /* pages of k_pages / v_pages                        */
+  int64_t page_size;     /* tokens of a page                                  */
+  int64_t table_width;   /* pages of a sequence (columns of page_table)       */
+  int64_t table_stride;  /* elements between its rows                         */
+  int64_t length;        /* every sequence's length where `lengths` is NULL   */
+  int64_t window_tokens; /* keys at the end that are visible; 0: all          */
+  int64_t sink_tokens;   /* keys at the start that stay visible               */
+  double scale;
+  int64_t q_batch_stride, q_head_stride;
+  int64_t k_page_stride, k_head_stride, k_row_stride;
+  int64_t v_page_stride, v_head_stride, v_row_stride;
+  int64_t o_batch_stride, o_head_stride;
+} fpv2_decode_params;
+
+/*
+ * out[b][h] = sum_t softmax_t(scale q[b][h].k_t) v_t over the visible keys t of
+ * sequence b: t < length, and t < sink_tokens or t >= length - window_tokens
+ * where a window is given.  Token t of sequence b is row t % page_size of page
+ * page_table[b][t / page_size] (int32; without page_table of page b).  Page ids
+ * are clipped to [0, pages) and lengths to [0, table_width * page_size]; a
+ * sequence of length 0 gives zeros.  Rows behind a length are not used.
+ * bf16 or f16; the strides of q, k and v multiples of 8 and their pointers
+ * 16-byte aligned.  workspace: fpv2_decode_attention_workspace_bytes bytes for
+ * the current device (0: none), 16-byte aligned, not kept between calls; calls
+ * that share one on different streams race.  Deterministic.
+ */
+int64_t fpv2_decode_attention_workspace_bytes(const fpv2_decode_params* params);
+int fpv2_decode_attention(const void* q, const void* k_pages, const void* v_pages,
+                          const int32_t* page_table, const int32_t* lengths, void* out, int dtype,
+                          const fpv2_decode_params* params, void* workspace,
+                          int64_t workspace_bytes, void* stream);
+
+#ifdef __cplusplus
+}
+#endif
+
+#endif /* FPV2_DECODE_H_ */

@@ -7,11 +7,12 @@ selection front end (``FPV2Config``/``pool_blocks``/``block_scores_and_select``/
 ``sparse_attention``.  ``ChunkedPrefill`` (``fpv2.chunked``) drives one
 layer's chunked prefill over a growing KV cache with incremental pooling.
 ``fpv2.decode`` holds the operators of the decode step that follows:
-``decode_attention``.
+``decode_attention``, ``rope_to_pages``, ``quantized_linear``.
 """
 
 from fpv2.chunked import ChunkedPrefill
-from fpv2.decode import decode_attention
+from fpv2.decode import (decode_attention, dequantize_weight, quantize_weight, quantized_linear,
+                         rope_to_pages)
 from fpv2.patch import block_sparsity, disable, enable, fpv2_sdpa, is_enabled
 from fpv2.selection import FPV2Config, block_scores_and_select, density, pool_blocks
 
@@ -22,9 +23,13 @@ __all__ = [
     "block_sparsity",
     "decode_attention",
     "density",
+    "dequantize_weight",
     "disable",
     "enable",
     "fpv2_sdpa",
     "is_enabled",
     "pool_blocks",
+    "quantize_weight",
+    "quantized_linear",
+    "rope_to_pages",
 ]

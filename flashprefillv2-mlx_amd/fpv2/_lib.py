@@ -56,6 +56,8 @@ EXPORTED_SYMBOLS = (
     # a decode step's operators (fpv2_decode.h)
     "fpv2_decode_attention_workspace_bytes",
     "fpv2_decode_attention",
+    "fpv2_rope_to_pages",
+    "fpv2_quantized_linear",
 )
 
 
@@ -142,6 +144,17 @@ class DecodeParams(ctypes.Structure):
     ]
 
 
+class RopePagesParams(ctypes.Structure):
+    """``fpv2_rope_pages_params`` (field order and types as in fpv2_decode.h)."""
+
+    _fields_ = [(name, ctypes.c_int64) for name in (
+        "tokens", "query_heads", "kv_heads", "head_dim", "rotary_half", "table_rows",
+        "interleaved", "pages", "page_size", "position_bytes", "slot_bytes", "first_position",
+        "first_slot", "qkv_row_stride", "q_token_stride", "q_head_stride", "k_page_stride",
+        "k_head_stride", "k_row_stride", "v_page_stride", "v_head_stride", "v_row_stride",
+    )] + [("eps", ctypes.c_double)]
+
+
 _lib = None
 
 
@@ -205,6 +218,10 @@ def _declare(lib: ctypes.CDLL) -> None:
     lib.fpv2_decode_attention_workspace_bytes.argtypes = [ctypes.POINTER(DecodeParams)]
     lib.fpv2_decode_attention.restype = ctypes.c_int
     lib.fpv2_decode_attention.argtypes = [vp] * 6 + [i32, ctypes.POINTER(DecodeParams), vp, i64, vp]
+    lib.fpv2_rope_to_pages.restype = ctypes.c_int
+    lib.fpv2_rope_to_pages.argtypes = [vp] * 10 + [i32, ctypes.POINTER(RopePagesParams), vp]
+    lib.fpv2_quantized_linear.restype = ctypes.c_int
+    lib.fpv2_quantized_linear.argtypes = [vp] * 5 + [i32, i32] + [i64] * 8 + [vp]
 
 
 def load(path: str | os.PathLike | None = None) -> ctypes.CDLL:

@@ -6,6 +6,10 @@ HIP kernels of the same library (``include/fpv2_decode.h``):
 
 ``decode_attention``   one new token per sequence over a paged or contiguous
                        KV cache, optionally with a window and sinks.
+``rope_to_pages``      norms of the query and key heads, the position rotation
+                       and the K/V write into a paged cache.
+``quantized_linear``   rows times 4-bit weights with group scales and biases
+                       (``quantize_weight`` / ``dequantize_weight`` convert).
 
 All of them run on the current stream of their tensors' device, whichever
 device is current, allocate from torch's allocator only (so they can be
@@ -155,3 +159,206 @@ def _strides(t: torch.Tensor):
     """Strides of all dimensions but the last; 0 where a dimension has one entry
     (torch leaves any value there)."""
     return [s if n > 1 else 0 for s, n in zip(t.stride()[:-1], t.shape)]
+
+
+def _index(value, name: str, tokens: int):
+    """Positions or slots: an integer tensor of one per token, or the first one."""
+    if isinstance(value, torch.Tensor):
+        if (value.shape != (tokens,) or value.dtype not in (torch.int32, torch.int64)
+                or not value.is_contiguous()):
+            raise ValueError(f"{name} must be contiguous int32 or int64 [tokens], or an integer")
+        return value, value.element_size(), 0
+    return None, 0, _count(value, name)
+
+
+def rope_to_pages(qkv: torch.Tensor, q_weight: torch.Tensor | None, k_weight: torch.Tensor | None,
+                  cos: torch.Tensor, sin: torch.Tensor, positions: torch.Tensor | int,
+                  slots: torch.Tensor | int, k_pages: torch.Tensor, v_pages: torch.Tensor, *,
+                  query_heads: int, eps: float = 1e-6, interleaved: bool = False,
+                  out: torch.Tensor | None = None) -> torch.Tensor:
+    """Norm and rotate the heads of fused projection rows; K and V go into pages.
+
+    ``qkv`` ``[T, (Hq + 2 Hkv) D]`` holds each token's query, key and value heads.
+    Query and key heads are RMS-normalised with ``q_weight``/``k_weight`` ``[D]``
+    (``None``: not normalised) and rotated by row ``positions[t]`` of the float32
+    tables ``cos``/``sin`` ``[positions, R]``: pairs ``(j, j + R)``, or ``(2j, 2j +
+    1)`` with ``interleaved``, of the first ``2R`` dimensions.  Key and value heads
+    are written to row ``slots[t] % page_size`` of page ``slots[t] // page_size``;
+    a token whose slot lies outside the pages (say -1) is padding and is not
+    written.  ``positions`` and ``slots`` are int32 or int64 ``[T]``, or an
+    integer: the first token's, the others following.  Returns the query
+    heads ``[T, Hq, D]`` (``out`` where given).
+
+    Everything is computed in float32 and rounded once.  Positions are clipped
+    to the tables.  Slots must be distinct: of two tokens with one slot,
+    either's values may stay.
+    """
+    if qkv.ndim != 2 or qkv.dtype not in _HALF:
+        raise ValueError("qkv must be [tokens, heads * head dim] in float16 or bfloat16")
+    _pages(k_pages, v_pages)
+    tokens = qkv.shape[0]
+    pages, kv_heads, page_size, dim = k_pages.shape
+    _count(query_heads, "query_heads", 1)
+    if k_pages.dtype != qkv.dtype:
+        raise ValueError("qkv and the caches must share a dtype")
+    if dim % 16 or not 0 < dim <= 512:
+        raise ValueError("head dimension must be a multiple of 16 and at most 512")
+    if kv_heads == 0 or qkv.shape[1] != (query_heads + 2 * kv_heads) * dim:
+        raise ValueError("qkv rows must hold the query, key and value heads")
+    if not _row_aligned(k_pages) or not _row_aligned(v_pages):
+        raise ValueError("the caches' rows must be contiguous and 16-byte aligned")
+    for name, t in (("q_weight", q_weight), ("k_weight", k_weight)):
+        if t is not None and (t.shape != (dim,) or t.dtype != qkv.dtype or not t.is_contiguous()
+                              or t.data_ptr() % 16):
+            raise ValueError(f"{name} must be contiguous [head dim] of qkv's dtype, 16-byte aligned")
+    for name, t in (("cos", cos), ("sin", sin)):
+        if (t.ndim != 2 or t.shape != cos.shape or t.dtype != torch.float32
+                or not t.is_contiguous() or t.data_ptr() % 16):
+            raise ValueError(f"{name} must be a contiguous float32 [positions, R] table")
+    half = cos.shape[1]
+    if cos.shape[0] == 0 or half == 0 or half % 8 or 2 * half > dim:
+        raise ValueError("cos and sin must have rows of a multiple of 8 angles, at most half the "
+                         "head dimension")
+    positions, position_bytes, first_position = _index(positions, "positions", tokens)
+    slots, slot_bytes, first_slot = _index(slots, "slots", tokens)
+    if out is None:
+        out = torch.empty((tokens, query_heads, dim), dtype=qkv.dtype, device=qkv.device)
+    elif out.shape != (tokens, query_heads, dim) or out.dtype != qkv.dtype or not _row_aligned(out):
+        raise ValueError("out must be [tokens, query heads, head dim] of qkv's dtype with 16-byte "
+                         "aligned rows")
+    tensors = [t for t in (qkv, k_pages, v_pages, q_weight, k_weight, cos, sin, positions, slots, out)
+               if t is not None]
+    _no_grad_needed(*tensors)
+    device = _lib.require_device(*tensors)
+    if not _row_aligned(qkv):
+        qkv = qkv.clone(memory_format=torch.contiguous_format)
+    if tokens == 0:
+        return out
+    lib = _lib.load()
+    p = _lib.RopePagesParams(
+        tokens, query_heads, kv_heads, dim, half, cos.shape[0], bool(interleaved), pages, page_size,
+        position_bytes, slot_bytes, first_position, first_slot, *_strides(qkv), *_strides(out),
+        *_strides(k_pages), *_strides(v_pages), eps)
+
+    def call(stream):
+        _lib.check(lib.fpv2_rope_to_pages(
+            qkv.data_ptr(), _lib.ptr(q_weight), _lib.ptr(k_weight), cos.data_ptr(), sin.data_ptr(),
+            _lib.ptr(positions), _lib.ptr(slots), out.data_ptr(), k_pages.data_ptr(),
+            v_pages.data_ptr(), _lib.dtype_code(qkv.dtype), ctypes.byref(p), stream),
+            "rope_to_pages")
+
+    _on_device(device, call)
+    return out
+
+
+GROUP_SIZES = (32, 64, 128)
+
+
+def quantize_weight(weight: torch.Tensor, *, group_size: int = 64):
+    """4-bit weights of ``weight`` ``[N, K]``: ``(packed, scales, biases)``.
+
+    Each group of ``group_size`` weights along ``K`` is cut into 15 equal steps
+    from its least to its greatest: ``w ~ scale q + bias``.  ``packed`` is int32
+    ``[N, K / 8]`` with weight ``k`` in bits ``4 (k % 8)`` of word ``k // 8``, ``scales``
+    and ``biases`` ``[N, K / group_size]`` are of ``weight``'s dtype: the layout of
+    MLX's affine quantization.  Runs on any device."""
+    if weight.ndim != 2 or not weight.is_floating_point():
+        raise ValueError("weight must be [out, in] of a floating type")
+    if group_size not in GROUP_SIZES or weight.shape[1] % group_size or weight.shape[1] == 0:
+        raise ValueError(f"group_size must be one of {GROUP_SIZES} and divide the columns")
+    n, k = weight.shape
+    w = weight.detach().float().view(n, k // group_size, group_size)
+    low, high = w.amin(-1, keepdim=True), w.amax(-1, keepdim=True)
+    # (a division by a number would be a product with its reciprocal on some
+    # devices; the steps are counted with the scale and bias that will be stored)
+    scales = ((high - low) / torch.full_like(high, 15)).to(weight.dtype)
+    biases = low.to(weight.dtype)
+    step = scales.float()
+    q = ((w - biases.float()) / torch.where(step == 0, 1.0, step)).round().clamp(0, 15)
+    q = q.to(torch.int32).view(n, k // 8, 8)
+    shifts = torch.arange(0, 32, 4, dtype=torch.int32, device=weight.device)
+    packed = (q << shifts).sum(-1, dtype=torch.int32)
+    return packed, scales[..., 0].contiguous(), biases[..., 0].contiguous()
+
+
+def dequantize_weight(packed: torch.Tensor, scales: torch.Tensor, biases: torch.Tensor, *,
+                      dtype: torch.dtype | None = None) -> torch.Tensor:
+    """``[N, K]`` weights of ``quantize_weight``'s result (float32 arithmetic,
+    rounded once to ``dtype``, by default the scales')."""
+    group = _group_size(packed, scales, biases)
+    n = packed.shape[0]
+    shifts = torch.arange(0, 32, 4, dtype=torch.int32, device=packed.device)
+    q = ((packed.view(torch.int32)[..., None] >> shifts) & 15).view(n, -1, group)
+    w = q * scales.float()[..., None] + biases.float()[..., None]
+    return w.view(n, -1).to(scales.dtype if dtype is None else dtype)
+
+
+def _group_size(packed, scales, biases) -> int:
+    if packed.ndim != 2 or packed.dtype not in (torch.int32, torch.uint32):
+        raise ValueError("packed must be int32 [out, in / 8]")
+    if scales.ndim != 2 or scales.shape != biases.shape or scales.shape[0] != packed.shape[0]:
+        raise ValueError("scales and biases must be [out, groups]")
+    groups = scales.shape[1]
+    for group in GROUP_SIZES:
+        if groups and groups * group == packed.shape[1] * 8:
+            return group
+    raise ValueError(f"the groups must be of one of {GROUP_SIZES} columns")
+
+
+def quantized_linear(x: torch.Tensor, packed: torch.Tensor, scales: torch.Tensor,
+                     biases: torch.Tensor, *, out_dtype: torch.dtype | None = None,
+                     out: torch.Tensor | None = None) -> torch.Tensor:
+    """``x @ w.T`` with the 4-bit weights of ``quantize_weight``.
+
+    ``x`` ``[..., K]`` in float16 or bfloat16, ``scales``/``biases`` of the same
+    dtype; returns ``[..., N]`` in that dtype or, with ``out_dtype``, in float32.
+    ``out``: optional ``[M, N]`` destination (``x`` ``[M, K]``) with contiguous
+    rows.  Products and sums are in float32 with the weights exact; ``x`` must be
+    finite (an infinite value gives NaN).  Made for the few rows of a decode
+    step: the weights are read once for every 16 rows or more (64 with groups
+    of 128), so a large prompt is better served by a product with
+    ``dequantize_weight``'s result."""
+    if x.ndim < 1 or x.dtype not in _HALF:
+        raise ValueError("x must be [..., in] in float16 or bfloat16")
+    group = _group_size(packed, scales, biases)
+    n, k = packed.shape[0], packed.shape[1] * 8
+    if x.shape[-1] != k:
+        raise ValueError("x must have as many columns as the weights")
+    if scales.dtype != x.dtype or biases.dtype != x.dtype:
+        raise ValueError("x, scales and biases must share a dtype")
+    kind = x.dtype if out_dtype is None else out_dtype
+    if kind not in (x.dtype, torch.float32):
+        raise ValueError("out_dtype must be x's dtype or float32")
+    if packed.stride(1) != 1 or (n > 1 and packed.stride(0) % 4) or packed.data_ptr() % 16:
+        raise ValueError("packed must have contiguous, 16-byte aligned rows")
+    for name, t in (("scales", scales), ("biases", biases)):
+        if t.shape[1] > 1 and t.stride(1) != 1 or n > 1 and t.stride(0) != scales.stride(0):
+            raise ValueError(f"{name} must have contiguous rows, both with one row stride")
+    rows = x if x.ndim == 2 else x.reshape(-1, k)
+    m = rows.shape[0]
+    if out is None:
+        result = torch.empty((*x.shape[:-1], n), dtype=kind, device=x.device)
+        flat, stride = result, n
+    else:
+        if (x.ndim != 2 or out.shape != (m, n) or out.dtype != kind
+                or n > 1 and out.stride(1) != 1 or m > 1 and out.stride(0) < n):
+            raise ValueError("out must be [rows, out] of out_dtype with contiguous rows, x [rows, in]")
+        result = flat = out
+        stride = out.stride(0) if m > 1 else n
+    _no_grad_needed(x, packed, scales, biases, result)
+    device = _lib.require_device(x, packed, scales, biases, result)
+    if not _row_aligned(rows) or m > 1 and rows.stride(0) < k:
+        rows = rows.clone(memory_format=torch.contiguous_format)
+    if m == 0 or n == 0:
+        return result
+    lib = _lib.load()
+
+    def call(stream):
+        _lib.check(lib.fpv2_quantized_linear(
+            rows.data_ptr(), packed.data_ptr(), scales.data_ptr(), biases.data_ptr(),
+            flat.data_ptr(), _lib.dtype_code(x.dtype), _lib.dtype_code(kind), m, n, k, group,
+            rows.stride(0) if m > 1 else k, packed.stride(0) if n > 1 else k // 8,
+            scales.stride(0) if n > 1 else k // group, stride, stream), "quantized_linear")
+
+    _on_device(device, call)
+    return result

@@ -62,6 +62,63 @@ int fpv2_decode_attention(const void* q, const void* k_pages, const void* v_page
                           const fpv2_decode_params* params, void* workspace,
                           int64_t workspace_bytes, void* stream);
 
+/* Norms and rotation of fused projection rows, K and V into pages. */
+typedef struct fpv2_rope_pages_params {
+  int64_t tokens;
+  int64_t query_heads;
+  int64_t kv_heads;
+  int64_t head_dim;       /* a multiple of 16, at most 512                     */
+  int64_t rotary_half;    /* columns of cos / sin: a multiple of 8, at most
+                             head_dim / 2                                      */
+  int64_t table_rows;     /* positions that cos / sin hold                     */
+  int64_t interleaved;    /* 0: pairs (j, j + rotary_half); 1: (2j, 2j + 1)    */
+  int64_t pages, page_size;
+  int64_t position_bytes; /* 4 or 8: type of positions[t]; 0: first_position + t */
+  int64_t slot_bytes;     /* 4 or 8: type of slots[t]; 0: first_slot + t       */
+  int64_t first_position, first_slot;
+  int64_t qkv_row_stride;
+  int64_t q_token_stride, q_head_stride;
+  int64_t k_page_stride, k_head_stride, k_row_stride;
+  int64_t v_page_stride, v_head_stride, v_row_stride;
+  double eps;
+} fpv2_rope_pages_params;
+
+/*
+ * Per-head RMSNorm (skipped for a NULL weight) and rotary embedding of the
+ * query and key heads of fused projection rows qkv[t] = [q | k | v heads]:
+ *   n = x rsqrt(mean(x^2) + eps) weight
+ *   (n_a, n_b) -> (n_a cos - n_b sin, n_b cos + n_a sin), the pair's angle
+ *   from row positions[t] (clipped to the table) of cos / sin
+ * in float32, rounded once.  Query heads go to q_out, key heads and the
+ * unchanged value heads to row slots[t] % page_size of page slots[t] / page_size;
+ * a token whose slot lies outside the pages is padding: its K and V are not
+ * written.  Slots must be distinct.  Dimensions from 2 rotary_half on are not
+ * rotated.  bf16 or f16; cos / sin float32 [table_rows, rotary_half]
+ * contiguous; strides multiples of 8 and pointers 16-byte aligned
+ * (positions / slots by their type).
+ * Counterpart of mlx-lm's q_norm / k_norm, nn.RoPE and cache update.
+ */
+int fpv2_rope_to_pages(const void* qkv, const void* q_weight, const void* k_weight,
+                       const float* cos, const float* sin, const void* positions,
+                       const void* slots, void* q_out, void* k_pages, void* v_pages, int dtype,
+                       const fpv2_rope_pages_params* params, void* stream);
+
+/*
+ * out[m][n] = sum_k x[m][k] w[n][k] with 4-bit weights in groups along k:
+ *   w[n][k] = scales[n][k / group] q[n][k] + biases[n][k / group]
+ * q[n][k] is bits 4 (k % 8) .. + 3 of 32-bit word packed[n][k / 8] (the layout of
+ * MLX's affine quantization).  group 32, 64 or 128 divides cols.  x, scales
+ * and biases share dtype (bf16 or f16), out has it too or float32 (out_dtype);
+ * products and sums in float32.  Row strides in elements (packed: in words);
+ * x_row_stride a multiple of 8, packed_row_stride of 4; x and packed 16-byte
+ * aligned; scales / biases rows contiguous, scale_row_stride elements apart.
+ */
+int fpv2_quantized_linear(const void* x, const void* packed, const void* scales,
+                          const void* biases, void* out, int dtype, int out_dtype, int64_t rows,
+                          int64_t out_cols, int64_t cols, int64_t group, int64_t x_row_stride,
+                          int64_t packed_row_stride, int64_t scale_row_stride,
+                          int64_t out_row_stride, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

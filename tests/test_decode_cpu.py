@@ -80,3 +80,103 @@ def test_decode_params_layout_matches_the_header(tmp_path):
     import ctypes
     assert got == [ctypes.sizeof(_lib.DecodeParams)] + [
         getattr(_lib.DecodeParams, name).offset for name, _ in _lib.DecodeParams._fields_]
+
+
+def _rope_args(**change):
+    bf16 = torch.bfloat16
+    args = dict(qkv=torch.zeros(3, 6 * 64, dtype=bf16), q_weight=torch.ones(64, dtype=bf16),
+                k_weight=torch.ones(64, dtype=bf16), cos=torch.zeros(9, 32), sin=torch.zeros(9, 32),
+                positions=torch.zeros(3, dtype=torch.int64), slots=torch.arange(3),
+                k_pages=torch.zeros(2, 1, 16, 64, dtype=bf16),
+                v_pages=torch.zeros(2, 1, 16, 64, dtype=bf16), query_heads=4)
+    args.update(change)
+    return args
+
+
+@pytest.mark.parametrize("change,message", [
+    (dict(qkv=torch.zeros(3, 6 * 64)), "qkv must be"),
+    (dict(qkv=torch.zeros(3, 6, 64, dtype=torch.bfloat16)), "qkv must be"),
+    (dict(qkv=torch.zeros(3, 7 * 64, dtype=torch.bfloat16)), "qkv rows must hold"),
+    (dict(qkv=torch.zeros(3, 6 * 64, dtype=torch.float16)), "share a dtype"),
+    (dict(query_heads=0), "query_heads"),
+    (dict(query_heads=True), "query_heads"),
+    (dict(q_weight=torch.ones(64)), "q_weight must be"),
+    (dict(k_weight=torch.ones(32, dtype=torch.bfloat16)), "k_weight must be"),
+    (dict(cos=torch.zeros(9, 32, dtype=torch.float64)), "cos must be"),
+    (dict(sin=torch.zeros(8, 32)), "sin must be"),
+    (dict(cos=torch.zeros(9, 28), sin=torch.zeros(9, 28)), "multiple of 8 angles"),
+    (dict(cos=torch.zeros(9, 40), sin=torch.zeros(9, 40)), "half the head dimension"),
+    (dict(cos=torch.zeros(0, 32), sin=torch.zeros(0, 32)), "cos and sin"),
+    (dict(positions=torch.zeros(2, dtype=torch.int64)), "positions must be"),
+    (dict(positions=torch.zeros(3)), "positions must be"),
+    (dict(positions=-1), "positions must be"),
+    (dict(slots=torch.zeros(6, dtype=torch.int64)[::2]), "slots must be"),
+    (dict(slots=1.0), "slots must be"),
+    (dict(k_pages=torch.zeros(2, 1, 16, 72, dtype=torch.bfloat16),
+          v_pages=torch.zeros(2, 1, 16, 72, dtype=torch.bfloat16)), "multiple of 16"),
+    (dict(v_pages=torch.zeros(2, 1, 64, 16, dtype=torch.bfloat16).transpose(2, 3)), "16-byte aligned"),
+    (dict(out=torch.zeros(3, 4, 64)), "out must be"),
+])
+def test_rope_to_pages_refuses(change, message):
+    with pytest.raises(ValueError, match=message):
+        fpv2.rope_to_pages(**_rope_args(**change))
+
+
+def test_rope_to_pages_refuses_cpu_tensors_and_gradients():
+    with pytest.raises(RuntimeError, match="ROCm"):
+        fpv2.rope_to_pages(**_rope_args())
+    weight = torch.ones(64, dtype=torch.bfloat16, requires_grad=True)
+    with pytest.raises(RuntimeError, match="no backward"):
+        fpv2.rope_to_pages(**_rope_args(q_weight=weight))
+
+
+def _linear_args(**change):
+    bf16 = torch.bfloat16
+    args = dict(x=torch.zeros(3, 128, dtype=bf16), packed=torch.zeros(10, 16, dtype=torch.int32),
+                scales=torch.zeros(10, 2, dtype=bf16), biases=torch.zeros(10, 2, dtype=bf16))
+    args.update(change)
+    return args
+
+
+@pytest.mark.parametrize("change,message", [
+    (dict(x=torch.zeros(3, 128)), "x must be"),
+    (dict(x=torch.zeros(3, 120, dtype=torch.bfloat16)), "as many columns"),
+    (dict(packed=torch.zeros(10, 16)), "packed must be"),
+    (dict(packed=torch.zeros(16, 10, dtype=torch.int32).T), "packed must have"),
+    (dict(scales=torch.zeros(9, 2, dtype=torch.bfloat16)), "scales and biases must be"),
+    (dict(scales=torch.zeros(10, 3, dtype=torch.bfloat16),
+          biases=torch.zeros(10, 3, dtype=torch.bfloat16)), "groups must be"),
+    (dict(scales=torch.zeros(10, 0, dtype=torch.bfloat16),
+          biases=torch.zeros(10, 0, dtype=torch.bfloat16)), "groups must be"),
+    (dict(scales=torch.zeros(10, 2), biases=torch.zeros(10, 2)), "share a dtype"),
+    (dict(scales=torch.zeros(2, 10, dtype=torch.bfloat16).T), "scales must have"),
+    (dict(biases=torch.zeros(10, 4, dtype=torch.bfloat16)[:, :2]), "biases must have"),
+    (dict(out_dtype=torch.float16), "out_dtype"),
+    (dict(out=torch.zeros(3, 9, dtype=torch.bfloat16)), "out must be"),
+    (dict(out=torch.zeros(10, 3, dtype=torch.bfloat16).T), "out must be"),
+    (dict(out=torch.zeros(1, 10, dtype=torch.bfloat16).expand(3, 10)), "out must be"),
+])
+def test_quantized_linear_refuses(change, message):
+    with pytest.raises(ValueError, match=message):
+        fpv2.quantized_linear(**_linear_args(**change))
+
+
+def test_quantized_linear_refuses_cpu_tensors_and_gradients():
+    with pytest.raises(RuntimeError, match="ROCm"):
+        fpv2.quantized_linear(**_linear_args())
+    x = torch.zeros(3, 128, dtype=torch.bfloat16, requires_grad=True)
+    with pytest.raises(RuntimeError, match="no backward"):
+        fpv2.quantized_linear(**_linear_args(x=x))
+
+
+def test_quantize_weight_layout_and_refusals():
+    w = torch.arange(32, dtype=torch.float32).remainder(16)[None]
+    packed, scales, biases = fpv2.quantize_weight(w, group_size=32)
+    assert [int(x) & 0xffffffff for x in packed[0]] == [0x76543210, 0xfedcba98] * 2
+    assert scales.tolist() == [[1.0]] and biases.tolist() == [[0.0]]
+    assert torch.equal(fpv2.dequantize_weight(packed, scales, biases), w)
+    for bad in (dict(weight=torch.zeros(2, 100)), dict(weight=torch.zeros(2, 2, 64)),
+                dict(weight=torch.zeros(2, 64, dtype=torch.int32)),
+                dict(weight=torch.zeros(2, 48), group_size=16), dict(weight=torch.zeros(2, 0))):
+        with pytest.raises(ValueError):
+            fpv2.quantize_weight(**bad)

@@ -22,7 +22,8 @@ CSRC = HERE / "csrc"
 INCLUDE = ROOT / "include"
 OUT = HERE / "fpv2" / "libfpv2_hip.so"
 SOURCES = ["fpv2_abi.cpp", "fpv2_pool.hip", "fpv2_select.hip", "fpv2_attention.hip",
-           "fpv2_decoder.hip", "fpv2_decode.hip", "fpv2_rope_pages.hip", "fpv2_q4.hip"]
+           "fpv2_decoder.hip", "fpv2_decode.hip", "fpv2_rope_pages.hip", "fpv2_q4.hip",
+           "fpv2_sample.hip"]
 ARCH = "gfx950"
 
 

@@ -7,12 +7,12 @@ selection front end (``FPV2Config``/``pool_blocks``/``block_scores_and_select``/
 ``sparse_attention``.  ``ChunkedPrefill`` (``fpv2.chunked``) drives one
 layer's chunked prefill over a growing KV cache with incremental pooling.
 ``fpv2.decode`` holds the operators of the decode step that follows:
-``decode_attention``, ``rope_to_pages``, ``quantized_linear``.
+``decode_attention``, ``rope_to_pages``, ``quantized_linear``, ``sample_tokens``.
 """
 
 from fpv2.chunked import ChunkedPrefill
 from fpv2.decode import (decode_attention, dequantize_weight, quantize_weight, quantized_linear,
-                         rope_to_pages)
+                         rope_to_pages, sample_tokens)
 from fpv2.patch import block_sparsity, disable, enable, fpv2_sdpa, is_enabled
 from fpv2.selection import FPV2Config, block_scores_and_select, density, pool_blocks
 
@@ -32,4 +32,5 @@ __all__ = [
     "quantize_weight",
     "quantized_linear",
     "rope_to_pages",
+    "sample_tokens",
 ]

@@ -58,6 +58,7 @@ EXPORTED_SYMBOLS = (
     "fpv2_decode_attention",
     "fpv2_rope_to_pages",
     "fpv2_quantized_linear",
+    "fpv2_sample_tokens",
 )
 
 
@@ -155,6 +156,24 @@ class RopePagesParams(ctypes.Structure):
     )] + [("eps", ctypes.c_double)]
 
 
+class SampleParams(ctypes.Structure):
+    """``fpv2_sample_params`` (field order and types as in fpv2_decode.h)."""
+
+    _fields_ = [
+        ("batch", ctypes.c_int64),
+        ("vocab", ctypes.c_int64),
+        ("logits_stride", ctypes.c_int64),
+        ("temperatures", ctypes.c_void_p),
+        ("top_ks", ctypes.c_void_p),
+        ("top_ps", ctypes.c_void_p),
+        ("min_ps", ctypes.c_void_p),
+        ("temperature", ctypes.c_double),
+        ("top_k", ctypes.c_int64),
+        ("top_p", ctypes.c_double),
+        ("min_p", ctypes.c_double),
+    ]
+
+
 _lib = None
 
 
@@ -220,6 +239,8 @@ def _declare(lib: ctypes.CDLL) -> None:
     lib.fpv2_decode_attention.argtypes = [vp] * 6 + [i32, ctypes.POINTER(DecodeParams), vp, i64, vp]
     lib.fpv2_rope_to_pages.restype = ctypes.c_int
     lib.fpv2_rope_to_pages.argtypes = [vp] * 10 + [i32, ctypes.POINTER(RopePagesParams), vp]
+    lib.fpv2_sample_tokens.restype = ctypes.c_int
+    lib.fpv2_sample_tokens.argtypes = [vp, vp, i32, ctypes.POINTER(SampleParams), vp, vp, vp]
     lib.fpv2_quantized_linear.restype = ctypes.c_int
     lib.fpv2_quantized_linear.argtypes = [vp] * 5 + [i32, i32] + [i64] * 8 + [vp]
 

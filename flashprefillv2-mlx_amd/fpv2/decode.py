@@ -10,6 +10,8 @@ HIP kernels of the same library (``include/fpv2_decode.h``):
                        and the K/V write into a paged cache.
 ``quantized_linear``   rows times 4-bit weights with group scales and biases
                        (``quantize_weight`` / ``dequantize_weight`` convert).
+``sample_tokens``      temperature, top-k, top-p and min-p from given random
+                       numbers.
 
 All of them run on the current stream of their tensors' device, whichever
 device is current, allocate from torch's allocator only (so they can be
@@ -362,3 +364,77 @@ def quantized_linear(x: torch.Tensor, packed: torch.Tensor, scales: torch.Tensor
 
     _on_device(device, call)
     return result
+
+
+MAX_VOCAB = 1 << 19  # FPV2_MAX_VOCAB
+
+
+def _setting(value, name: str, batch: int, dtype: torch.dtype, low, high):
+    """A row setting: ``(tensor, number)``, the number where there is no tensor."""
+    if isinstance(value, torch.Tensor):
+        if value.shape != (batch,) or value.dtype != dtype or not value.is_contiguous():
+            raise ValueError(f"{name} must be a number or contiguous "
+                             f"{str(dtype).removeprefix('torch.')} [batch]")
+        return value, 0
+    if dtype == torch.int32:
+        return None, _count(value, name)
+    if isinstance(value, bool) or not isinstance(value, (int, float)) or not low <= value <= high:
+        raise ValueError(f"{name} must be a number in [{low}, {high}] or a tensor")
+    return None, value
+
+
+def sample_tokens(logits: torch.Tensor, uniform: torch.Tensor, *,
+                  temperature: float | torch.Tensor = 1.0, top_k: int | torch.Tensor = 0,
+                  top_p: float | torch.Tensor = 1.0, min_p: float | torch.Tensor = 0.0,
+                  return_logprobs: bool = False):
+    """One token per row of ``logits`` ``[B, V]`` by the row's number ``uniform[b]``.
+
+    ``logits`` float32, float16 or bfloat16 with contiguous rows; ``uniform``
+    float32 ``[B]`` in ``[0, 1)``.  Each setting is a number, or a tensor ``[B]``
+    with one for each row (float32; ``top_k`` int32).  With the weights ``w_i =
+    exp((logit_i - max) / temperature)`` and the tokens ordered by logit, equal
+    ones by index, the kept ones are the first ``top_k`` (0: all), of these the
+    ones whose weight before them is less than ``top_p`` of the weight of all of
+    these, and of these the ones with ``w_i >= min_p``; the first always is.
+    The token is the first one, in index order, whose running kept weight
+    exceeds ``uniform[b]`` times all kept weight.  Temperature 0: the greatest
+    logit, of equal ones the first.
+
+    Returns int64 tokens ``[B]``, with ``return_logprobs`` also the float32 log of
+    each token's share of the kept weight.  The result is the same in every
+    call and batch.  A NaN logit counts as -inf; a row of nothing but -inf gives
+    token -1 and -inf.
+    """
+    if logits.ndim != 2 or logits.dtype not in (torch.float32, *_HALF):
+        raise ValueError("logits must be [batch, vocabulary] in float32, float16 or bfloat16")
+    batch, vocab = logits.shape
+    if not 0 < vocab <= MAX_VOCAB:
+        raise ValueError(f"the vocabulary must have 1 to {MAX_VOCAB} tokens")
+    if uniform.shape != (batch,) or uniform.dtype != torch.float32 or not uniform.is_contiguous():
+        raise ValueError("uniform must be contiguous float32 [batch]")
+    inf = float("inf")
+    t_rows, t = _setting(temperature, "temperature", batch, torch.float32, 0, 1e30)
+    k_rows, k = _setting(top_k, "top_k", batch, torch.int32, 0, inf)
+    p_rows, p = _setting(top_p, "top_p", batch, torch.float32, 0, 1)
+    m_rows, m = _setting(min_p, "min_p", batch, torch.float32, 0, 1)
+    rows = [x for x in (t_rows, k_rows, p_rows, m_rows) if x is not None]
+    _no_grad_needed(logits, uniform, *rows)
+    device = _lib.require_device(logits, uniform, *rows)
+    if vocab > 1 and logits.stride(1) != 1:
+        logits = logits.contiguous()
+    tokens = torch.empty(batch, dtype=torch.int64, device=device)
+    logprobs = torch.empty(batch, dtype=torch.float32, device=device) if return_logprobs else None
+    if batch > 0:
+        lib = _lib.load()
+        params = _lib.SampleParams(
+            batch, vocab, logits.stride(0) if batch > 1 else 0, _lib.ptr(t_rows),
+            _lib.ptr(k_rows), _lib.ptr(p_rows), _lib.ptr(m_rows), t, min(k, vocab), p, m)
+
+        def call(stream):
+            _lib.check(lib.fpv2_sample_tokens(
+                logits.data_ptr(), uniform.data_ptr(), _lib.dtype_code(logits.dtype),
+                ctypes.byref(params), tokens.data_ptr(), _lib.ptr(logprobs), stream),
+                "sample_tokens")
+
+        _on_device(device, call)
+    return (tokens, logprobs) if return_logprobs else tokens

@@ -119,6 +119,43 @@ int fpv2_quantized_linear(const void* x, const void* packed, const void* scales,
                           int64_t packed_row_stride, int64_t scale_row_stride,
                           int64_t out_row_stride, void* stream);
 
+/* Largest vocabulary of fpv2_sample_tokens (its sums are integers of 64 bits). */
+#define FPV2_MAX_VOCAB (1 << 19)
+
+/* Sampling.  A NULL array takes the value beside it for every row. */
+typedef struct fpv2_sample_params {
+  int64_t batch;
+  int64_t vocab;
+  int64_t logits_stride;    /* elements between rows                          */
+  const float* temperatures;
+  const int32_t* top_ks;
+  const float* top_ps;
+  const float* min_ps;
+  double temperature;       /* 0 or less: the greatest logit                  */
+  int64_t top_k;            /* 0 or less: no limit                            */
+  double top_p;             /* 1 or more: no limit                            */
+  double min_p;
+} fpv2_sample_params;
+
+/*
+ * One token per row of logits [batch, vocab] (float32, bf16 or f16) by the row's
+ * number uniforms[b] in [0, 1):
+ *   weights w_i = exp((logit_i - max) / temperature), tokens ordered by logit,
+ *   equal ones by index, and kept: the first top_k; of these the ones whose
+ *   weight before them is less than top_p of the weight of all of these; of
+ *   these the ones with w_i >= min_p (clipped to 1).  The first is always kept.
+ *   token = the first one in index order whose running kept weight exceeds
+ *   uniforms[b] (clipped to [0, 1]) times all kept weight (the last kept one of
+ *   any weight where none does).
+ * Weights are computed in float64 and rounded to 2^-44, sums are exact, so the
+ * result does not depend on any order.  A NaN logit counts as -inf; a row of
+ * nothing but -inf gives token -1.  logprobs (NULL: not written): log of the
+ * token's share of the kept weight, 0 for a greedy row, -inf for token -1.
+ */
+int fpv2_sample_tokens(const void* logits, const float* uniforms, int dtype,
+                       const fpv2_sample_params* params, int64_t* tokens, float* logprobs,
+                       void* stream);
+
 #ifdef __cplusplus
 }
 #endif

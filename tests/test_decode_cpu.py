@@ -57,8 +57,12 @@ def test_decode_attention_refuses_cpu_tensors_and_gradients():
         fpv2.decode_attention(**_attention_args(q=q))
 
 
-def test_decode_params_layout_matches_the_header(tmp_path):
-    """The ctypes mirror of fpv2_decode_params, as gcc lays the header's out."""
+@pytest.mark.parametrize("cname,mirror", [("fpv2_decode_params", "DecodeParams"),
+                                          ("fpv2_rope_pages_params", "RopePagesParams"),
+                                          ("fpv2_sample_params", "SampleParams")])
+def test_params_layouts_match_the_header(tmp_path, cname, mirror):
+    """The ctypes mirrors, as gcc lays the header's structs out."""
+    import ctypes
     import shutil
     import subprocess
     from pathlib import Path
@@ -67,19 +71,17 @@ def test_decode_params_layout_matches_the_header(tmp_path):
     gcc = shutil.which("gcc")
     if gcc is None:
         pytest.skip("gcc not available")
+    cls = getattr(_lib, mirror)
     lines = ['#include <stddef.h>', '#include <stdio.h>', '#include "fpv2_decode.h"',
-             "int main(void) {", '  printf("%zu\\n", sizeof(fpv2_decode_params));']
-    lines += [f'  printf("%zu\\n", offsetof(fpv2_decode_params, {name}));'
-              for name, _ in _lib.DecodeParams._fields_]
+             "int main(void) {", f'  printf("%zu\\n", sizeof({cname}));']
+    lines += [f'  printf("%zu\\n", offsetof({cname}, {name}));' for name, _ in cls._fields_]
     source, program = tmp_path / "layout.c", tmp_path / "layout"
     source.write_text("\n".join(lines + ["  return 0;", "}"]))
     include = Path(__file__).resolve().parents[1] / "include"
     subprocess.run([gcc, "-I", str(include), str(source), "-o", str(program)], check=True)
     got = [int(x) for x in subprocess.run([str(program)], capture_output=True, text=True,
                                           check=True).stdout.split()]
-    import ctypes
-    assert got == [ctypes.sizeof(_lib.DecodeParams)] + [
-        getattr(_lib.DecodeParams, name).offset for name, _ in _lib.DecodeParams._fields_]
+    assert got == [ctypes.sizeof(cls)] + [getattr(cls, name).offset for name, _ in cls._fields_]
 
 
 def _rope_args(**change):
@@ -180,3 +182,42 @@ def test_quantize_weight_layout_and_refusals():
                 dict(weight=torch.zeros(2, 48), group_size=16), dict(weight=torch.zeros(2, 0))):
         with pytest.raises(ValueError):
             fpv2.quantize_weight(**bad)
+
+
+def _sample_args(**change):
+    args = dict(logits=torch.zeros(3, 50), uniform=torch.zeros(3))
+    args.update(change)
+    return args
+
+
+@pytest.mark.parametrize("change,message", [
+    (dict(logits=torch.zeros(50)), "logits must be"),
+    (dict(logits=torch.zeros(3, 50, dtype=torch.float64)), "logits must be"),
+    (dict(logits=torch.zeros(3, 0)), "vocabulary must have"),
+    (dict(logits=torch.zeros(1, 1).expand(3, (1 << 19) + 1)), "vocabulary must have"),
+    (dict(uniform=torch.zeros(2)), "uniform must be"),
+    (dict(uniform=torch.zeros(3, dtype=torch.float64)), "uniform must be"),
+    (dict(uniform=torch.zeros(6)[::2]), "uniform must be"),
+    (dict(temperature=-0.1), "temperature"),
+    (dict(temperature=float("nan")), "temperature"),
+    (dict(temperature=float("inf")), "temperature"),
+    (dict(temperature=torch.ones(2)), "temperature"),
+    (dict(top_k=-1), "top_k"),
+    (dict(top_k=2.0), "top_k"),
+    (dict(top_k=torch.ones(3)), "top_k"),
+    (dict(top_p=1.5), "top_p"),
+    (dict(top_p=True), "top_p"),
+    (dict(top_p=torch.ones(3, dtype=torch.float64)), "top_p"),
+    (dict(min_p=-0.5), "min_p"),
+    (dict(min_p="no"), "min_p"),
+])
+def test_sample_tokens_refuses(change, message):
+    with pytest.raises(ValueError, match=message):
+        fpv2.sample_tokens(**_sample_args(**change))
+
+
+def test_sample_tokens_refuses_cpu_tensors_and_gradients():
+    with pytest.raises(RuntimeError, match="ROCm"):
+        fpv2.sample_tokens(**_sample_args())
+    with pytest.raises(RuntimeError, match="no backward"):
+        fpv2.sample_tokens(**_sample_args(logits=torch.zeros(3, 50, requires_grad=True)))

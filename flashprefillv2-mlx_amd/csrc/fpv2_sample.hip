@@ -3,22 +3,36 @@
 // The weight of a token is exp((logit - max) / temperature) in float64, rounded to
 // an integer of 2^-44: sums of up to 2^19 of them are exact in 64 bits, so that
 // histograms can be added in any order and a token next to a border is the same
-// in every call.  Kept tokens are a prefix of the order (logit descending, index
-// ascending): all tokens with a greater key than the border's, and the first few of
-// the border's own (a key is the logit's bits, ordered as unsigned integers).
+// in every call.  A token's rank is a number of 52 bits: its logit's bits, ordered as
+// unsigned integers, above the complement of its index.  Ranks are distinct, and the
+// kept tokens are the ones from some least rank on: no sort is needed, only
+// the ranks at which the count (top-k) and the weight (top-p) of all tokens from
+// there on reach their limits.
 //
-// One workgroup per row.  The border of top-k is found by counts over the key's
-// four bytes, the one of top-p by weights in the same way.
+// A short row is one workgroup's.  A long one takes passes over chunks of it, bound by
+// reading the logits (the second and third time from the caches):
+//   1. the greatest logit;
+//   2. a histogram of count and weight over (max - logit) / temperature, or the
+//      chunks' sums where the row has neither top-k nor top-p;
+//   3. the tokens of the histogram's bins that hold the borders go to a list, the ones
+//      above them into the chunks' sums;
+//   4. one workgroup finds the borders in the list and the token in its chunk.
 #include "fpv2_common.h"
 #include "fpv2_decode.h"
 
 namespace fpv2 {
 namespace {
 
-constexpr int kThreads = 1024;
-constexpr int kWaves = kThreads / 64;
-constexpr int kWeightBits = 44;
 typedef unsigned long long u64;
+constexpr int kRowThreads = 1024;   // of a workgroup that has a row
+constexpr int kChunkThreads = 256;  // of one that has a chunk
+constexpr int kWeightBits = 44;
+constexpr int kIndexBits = 20;
+constexpr int kRankBits = 32 + kIndexBits;
+constexpr int kBins = 1024;     // of the histogram,
+constexpr double kPerUnit = 32; // so many to a unit of the exponent
+constexpr int kList = 4096;     // tokens of a row's list
+constexpr int kMaxChunks = 256;
 
 struct SampleArgs {
   const void* logits;
@@ -32,9 +46,19 @@ struct SampleArgs {
   double temperature, top_p, min_p;
   int64_t top_k, stride;
   int vocab;
+  // chunks of a long row, and its workspace
+  int chunks, chunk;
+  u64* best;         // [batch][chunks] greatest rank of a chunk
+  u64* sums;         // [batch][chunks] weight of a chunk's tokens that are kept for sure
+  u64* weights;      // [batch][kBins]
+  u64* list;         // [batch][kList]
+  uint32_t* counts;  // [batch][kBins]
+  uint32_t* listed;  // [batch]
 };
 
 struct f32_t { float v; };
+template <typename T> constexpr int kLogitBytes = 2;
+template <> constexpr int kLogitBytes<f32_t> = 4;
 template <typename T>
 __device__ __forceinline__ float logit_at(const void* row, int i) {
   return Elem<T>::to_float(static_cast<const uint16_t*>(row)[i]);
@@ -42,6 +66,15 @@ __device__ __forceinline__ float logit_at(const void* row, int i) {
 template <>
 __device__ __forceinline__ float logit_at<f32_t>(const void* row, int i) {
   return static_cast<const float*>(row)[i];
+}
+// Logit j of a 16-byte vector.
+template <typename T>
+__device__ __forceinline__ float logit_in(u32x4 v, int j) {
+  return Elem<T>::to_float(j % 2 ? v[j / 2] >> 16 : v[j / 2] & 0xffffu);
+}
+template <>
+__device__ __forceinline__ float logit_in<f32_t>(u32x4 v, int j) {
+  return __uint_as_float(v[j]);
 }
 
 // Order-preserving key: -inf and NaN least, both zeros alike.
@@ -54,33 +87,85 @@ __device__ __forceinline__ uint32_t key_of(float x) {
 __device__ __forceinline__ float logit_of(uint32_t key) {
   return __uint_as_float(key & 0x80000000u ? key & 0x7fffffffu : ~key);
 }
+__device__ __forceinline__ u64 rank_of(uint32_t key, int i) {
+  return (static_cast<u64>(key) << kIndexBits) | ((1u << kIndexBits) - 1 - i);
+}
+__device__ __forceinline__ uint32_t key_in(u64 rank) { return static_cast<uint32_t>(rank >> kIndexBits); }
+__device__ __forceinline__ int index_in(u64 rank) {
+  return (1 << kIndexBits) - 1 - static_cast<int>(rank & ((1u << kIndexBits) - 1));
+}
 
+// A row's settings and greatest logit.
 struct Row {
   const void* logits;
   uint32_t top;     // greatest key
   double max, inv;  // its logit, 1 / temperature
-  u64 least;        // least weight that min_p keeps
+  double least;     // exponent from which on min_p keeps
+  double top_p;
+  int64_t top_k;    // 0: no limit
+  bool greedy, limited;
 };
 
-// log of a weight, and the weight (0 below 2^-45)
+template <typename T>
+__device__ __forceinline__ const void* row_of(const SampleArgs& a, int b) {
+  return static_cast<const char*>(a.logits) + b * a.stride * kLogitBytes<T>;
+}
+template <typename T>
+__device__ __forceinline__ Row settings_of(const SampleArgs& a, int b, u64 best) {
+  Row r;
+  r.logits = row_of<T>(a, b);
+  r.top = key_in(best);
+  r.max = logit_of(r.top);
+  const double temperature = a.temperatures ? a.temperatures[b] : a.temperature;
+  r.greedy = r.top <= kLeastKey || !(temperature > 0);
+  r.inv = 1.0 / temperature;
+  r.top_p = a.top_ps ? a.top_ps[b] : a.top_p;
+  r.top_k = a.top_ks ? a.top_ks[b] : a.top_k;
+  if (r.top_k < 0 || r.top_k >= a.vocab) r.top_k = 0;
+  const double min_p = a.min_ps ? a.min_ps[b] : a.min_p;
+  r.least = min_p > 0 ? log(fmin(min_p, 1.0)) : -__builtin_inf();
+  r.limited = !r.greedy && (r.top_k > 0 || r.top_p < 1);
+  return r;
+}
+
+// log of a weight (falls with the key), and the weight: 0 below 2^-45
 __device__ __forceinline__ double exponent_of(const Row& r, uint32_t key) {
   if (key == r.top) return 0.0;
   if (key <= kLeastKey) return -__builtin_inf();
   return (static_cast<double>(logit_of(key)) - r.max) * r.inv;
 }
-__device__ __forceinline__ u64 weight_of(const Row& r, uint32_t key) {
-  const double z = exponent_of(r, key);
+__device__ __forceinline__ u64 weight_at(double z) {
   if (!(z > -31.2)) return 0;
   return static_cast<u64>(exp(z) * (1ull << kWeightBits) + 0.5);
+}
+__device__ __forceinline__ u64 weight_of(const Row& r, uint32_t key) { return weight_at(exponent_of(r, key)); }
+__device__ __forceinline__ int bin_at(double z) {
+  return z > -(kBins - 1) / kPerUnit ? static_cast<int>(z * -kPerUnit) : kBins - 1;
+}
+// Weight of a token if min_p keeps it.
+__device__ __forceinline__ u64 likely_weight(const Row& r, uint32_t key) {
+  const double z = exponent_of(r, key);
+  return z >= r.least ? weight_at(z) : 0;
 }
 
 __device__ __forceinline__ u64 shfl_xor64(u64 v, int off) {
   return static_cast<u64>(__shfl_xor(static_cast<long long>(v), off, 64));
 }
-
-// Sum (or greatest) of a value of each thread, in every thread.
-template <bool MAX>
-__device__ u64 across(u64 v, u64* sh) {
+__device__ __forceinline__ u64 shfl64(u64 v, int lane) {
+  return static_cast<u64>(__shfl(static_cast<long long>(v), lane, 64));
+}
+// Sum over a wave's lanes up to this one.
+__device__ __forceinline__ u64 wave_scan(u64 v, int lane) {
+#pragma unroll
+  for (int off = 1; off < 64; off <<= 1) {
+    const u64 up = static_cast<u64>(__shfl_up(static_cast<long long>(v), off, 64));
+    v += lane >= off ? up : 0;
+  }
+  return v;
+}
+// Sum (or greatest) of a value of each of the workgroup's threads, in every thread.
+template <int THREADS, bool MAX>
+__device__ __forceinline__ u64 across(u64 v, u64* sh) {
 #pragma unroll
   for (int off = 32; off >= 1; off >>= 1) {
     const u64 o = shfl_xor64(v, off);
@@ -91,17 +176,46 @@ __device__ u64 across(u64 v, u64* sh) {
   __syncthreads();
   v = sh[0];
 #pragma unroll
-  for (int w = 1; w < kWaves; ++w) v = MAX ? (sh[w] > v ? sh[w] : v) : v + sh[w];
+  for (int w = 1; w < THREADS / 64; ++w) v = MAX ? (sh[w] > v ? sh[w] : v) : v + sh[w];
   return v;
 }
 
-// The first index i in [0, n) for which past(sum of value(0..i)) holds, or n: sums of a
-// wave's share, then of its shares, until one wave is left with a piece.
+// f(i, logit) for the tokens [lo, hi) of a row, in any order, by THREADS threads:
+// 16-byte loads from the first aligned logit on.
+template <typename T, int THREADS, typename F>
+__device__ __forceinline__ void for_each(const void* row, int lo, int hi, F f) {
+  constexpr int N = 16 / kLogitBytes<T>;
+  const uintptr_t at = reinterpret_cast<uintptr_t>(row) + static_cast<uintptr_t>(lo) * kLogitBytes<T>;
+  const int head = min(hi - lo, static_cast<int>((16 - at % 16) % 16) / kLogitBytes<T>);
+  const int tid = threadIdx.x;
+  if (tid < head) f(lo + tid, logit_at<T>(row, lo + tid));
+  const int first = lo + head, vectors = (hi - first) / N;
+  const char* p = static_cast<const char*>(row) + static_cast<int64_t>(first) * kLogitBytes<T>;
+#pragma unroll 2
+  for (int v = tid; v < vectors; v += THREADS) {
+    const u32x4 x = load16(p + 16 * static_cast<int64_t>(v));
+#pragma unroll
+    for (int j = 0; j < N; ++j) f(first + N * v + j, logit_in<T>(x, j));
+  }
+  const int tail = first + N * vectors + tid;
+  if (tail < hi) f(tail, logit_at<T>(row, tail));
+}
+
+struct Shared {
+  u64 sums[kRowThreads / 64];
+  u64 weights[256];
+  uint32_t counts[256];
+  u64 found[4];
+  int at;
+};
+
+// The first i in [lo, hi) for which past(before + value(lo) + .. + value(i)) holds, or
+// hi: sums of the waves' shares, then of the shares of one of these, until one
+// wave is left with a piece.
 template <typename Value, typename Past>
-__device__ int find_first(int n, Value value, Past past, u64* sh, int* sh_at) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  int lo = 0, hi = n;
-  u64 before = 0;
+__device__ int find_first(int lo, int hi, u64 before, Value value, Past past, Shared& sh) {
+  constexpr int kWaves = kRowThreads / 64;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, none = hi;
   while (hi - lo > 512) {
     const int share = (hi - lo + kWaves - 1) / kWaves;
     const int a = min(hi, lo + wave * share), b = min(hi, a + share);
@@ -110,199 +224,568 @@ __device__ int find_first(int n, Value value, Past past, u64* sh, int* sh_at) {
 #pragma unroll
     for (int off = 32; off >= 1; off >>= 1) sum += shfl_xor64(sum, off);
     __syncthreads();
-    if (lane == 0) sh[wave] = sum;
+    if (lane == 0) sh.sums[wave] = sum;
     __syncthreads();
     int w = 0;
-    while (w < kWaves && !past(before + sh[w])) before += sh[w++];
-    if (w == kWaves) return n;
+    while (w < kWaves && !past(before + sh.sums[w])) before += sh.sums[w++];
+    if (w == kWaves) return none;
     const int next = min(hi, lo + w * share);
     hi = min(hi, next + share);
     lo = next;
   }
   __syncthreads();
-  if (threadIdx.x == 0) *sh_at = n;
+  if (threadIdx.x == 0) sh.at = none;
   __syncthreads();
   if (wave == 0) {
     for (int i0 = lo; i0 < hi; i0 += 64) {
-      u64 sum = i0 + lane < hi ? value(i0 + lane) : 0;
-#pragma unroll
-      for (int off = 1; off < 64; off <<= 1) {
-        const u64 up = static_cast<u64>(__shfl_up(static_cast<long long>(sum), off, 64));
-        sum += lane >= off ? up : 0;
-      }
+      const u64 sum = wave_scan(i0 + lane < hi ? value(i0 + lane) : 0, lane);
       const uint64_t hit = __ballot(i0 + lane < hi && past(before + sum));
       if (hit != 0) {
-        if (lane == 0) *sh_at = i0 + __ffsll(static_cast<unsigned long long>(hit)) - 1;
+        if (lane == 0) sh.at = i0 + __ffsll(static_cast<unsigned long long>(hit)) - 1;
         break;
       }
-      before += static_cast<u64>(__shfl(static_cast<long long>(sum), 63, 64));
+      before += shfl64(sum, 63);
     }
   }
   __syncthreads();
-  return *sh_at;
+  return sh.at;
 }
 
-struct Border {
-  uint32_t key;  // tokens of a greater key are kept,
-  uint32_t ties; // and the first so many of this key
-  u64 above;     // weight of the tokens of a greater key
-};
-
-struct Shared {
-  u64 sums[kWaves];
-  u64 weights[256];
-  uint32_t counts[256];
-  int at;
-};
-
-// The key at which `past(count, weight)` of all tokens down to it first holds, from
-// histograms over its bytes; all tokens' least key where it never does.
-template <typename T, typename Past>
-__device__ Border border_of(const Row& r, int vocab, Shared& sh, bool weigh, Past past) {
-  uint32_t prefix = 0;
-  u64 above = 0;
-  uint32_t count = 0, in_key = 0;
-  for (int shift = 24; shift >= 0; shift -= 8) {
+// Of a group of tokens (each(f) calls f(rank) for all of them) the greatest rank from
+// which on past(count, weight) holds, given the count and weight of the tokens
+// above the group; 0 where it never does.  *weight: weight of the tokens from there on.
+// Histograms over the rank's bits, 8 at a time from the first that differ, until one
+// token is left in the border's bin.
+template <typename Each, typename Past>
+__device__ u64 least_rank(const Row& r, Each each, u64 count, u64 weight, Past past, bool weigh,
+                          u64* weight_from, Shared& sh) {
+  const int tid = threadIdx.x, lane = tid & 63;
+  u64 low = ~0ull, high = 0;
+  each([&](u64 rank) {
+    low = rank < low ? rank : low;
+    high = rank > high ? rank : high;
+  });
+  high = across<kRowThreads, true>(high, sh.sums);
+  low = ~across<kRowThreads, true>(~low, sh.sums);
+  int shift = low < high ? 64 - __clzll(static_cast<long long>(low ^ high)) - 8 : 0;
+  int width = 8;  // the bits shift .. shift + width - 1 are the bin
+  if (shift < 0) shift = 0;
+  u64 prefix = high >> (shift + width);
+  for (;;) {
     __syncthreads();
-    for (int i = threadIdx.x; i < 256; i += kThreads) sh.weights[i] = 0, sh.counts[i] = 0;
+    if (tid < 256) sh.weights[tid] = 0, sh.counts[tid] = 0;
     __syncthreads();
-    for (int i = threadIdx.x; i < vocab; i += kThreads) {
-      const uint32_t key = key_of(logit_at<T>(r.logits, i));
-      if (shift < 24 && (key >> (shift + 8)) != prefix) continue;
-      const int bin = (key >> shift) & 255;
+    each([&](u64 rank) {
+      if ((rank >> (shift + width)) != prefix) return;
+      const int bin = static_cast<int>(rank >> shift) & ((1 << width) - 1);
       atomicAdd(&sh.counts[bin], 1u);
-      if (weigh) atomicAdd(&sh.weights[bin], weight_of(r, key));
+      if (weigh) atomicAdd(&sh.weights[bin], weight_of(r, key_in(rank)));
+    });
+    __syncthreads();
+    if (tid < 64) {
+      // the lane's bins 255 - 4 lane and the three below
+      u64 c[4], w[4], cs = 0, ws = 0;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int bin = 255 - 4 * lane - j;
+        c[j] = cs += sh.counts[bin];
+        w[j] = ws += sh.weights[bin];
+      }
+      const u64 c0 = count + wave_scan(cs, lane) - cs, w0 = weight + wave_scan(ws, lane) - ws;
+      int mine = -1;
+#pragma unroll
+      for (int j = 3; j >= 0; --j) {
+        const u64 own = c[j] - (j > 0 ? c[j > 0 ? j - 1 : 0] : 0);
+        if (own > 0 && past(c0 + c[j], w0 + w[j])) mine = j;
+      }
+      const uint64_t hit = __ballot(mine >= 0);
+      if (lane == 0) sh.found[0] = hit;
+      if (hit != 0 && lane == __ffsll(static_cast<unsigned long long>(hit)) - 1) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (j == mine) {
+            const u64 before_c = j > 0 ? c[j > 0 ? j - 1 : 0] : 0, before_w = j > 0 ? w[j > 0 ? j - 1 : 0] : 0;
+            sh.found[1] = (static_cast<u64>(255 - 4 * lane - j) << 32) | (c[j] - before_c);
+            sh.found[2] = c0 + before_c;
+            sh.found[3] = w0 + before_w;
+          }
+      }
     }
     __syncthreads();
-    int bin = 255, least = 0;
-    for (; bin >= 0; --bin) {
-      if (sh.counts[bin] == 0) continue;
-      least = bin;
-      if (past(count + sh.counts[bin], above + sh.weights[bin])) break;
-      count += sh.counts[bin];
-      above += sh.weights[bin];
+    if (sh.found[0] == 0) {  // never (the first time round: later the bin has it)
+      *weight_from = weight;
+      return 0;
     }
-    if (bin < 0) {  // never: the border is the least key there is
-      bin = least;
-      count -= sh.counts[bin];
-      above -= sh.weights[bin];
+    const int bin = static_cast<int>(sh.found[1] >> 32);
+    const uint32_t in_bin = static_cast<uint32_t>(sh.found[1]);
+    prefix = (prefix << width) | bin;
+    count = sh.found[2];
+    weight = sh.found[3];
+    if (in_bin == 1 || shift == 0) {
+      *weight_from = weight + sh.weights[bin];
+      return prefix << shift;
     }
-    prefix = (prefix << 8) | bin;
-    in_key = sh.counts[bin];
+    width = shift < 8 ? shift : 8;
+    shift -= width;
   }
-  // the fewest tokens of the key for which it holds
-  const u64 w = weigh ? weight_of(r, prefix) : 0;
-  uint32_t lo = 1, hi = in_key;
-  while (lo < hi) {
-    const uint32_t mid = lo + (hi - lo) / 2;
-    if (past(count + mid, above + mid * w))
-      hi = mid;
-    else
-      lo = mid + 1;
-  }
-  return {prefix, lo, above};
 }
 
-template <typename T>
-__global__ __launch_bounds__(kThreads) void sample_kernel(SampleArgs a) {
-  __shared__ Shared sh;
-  const int b = blockIdx.x, tid = threadIdx.x, vocab = a.vocab;
-  Row r;
-  r.logits = static_cast<const char*>(a.logits) +
-             b * a.stride * static_cast<int64_t>(std::is_same<T, f32_t>::value ? 4 : 2);
-  u64 best = 0;  // key, then the lowest index
-  for (int i = tid; i < vocab; i += kThreads) {
-    const u64 k = (static_cast<u64>(key_of(logit_at<T>(r.logits, i))) << 32) | ~static_cast<uint32_t>(i);
-    best = k > best ? k : best;
+// The least kept rank of a row whose borders lie in a group of tokens.
+template <typename Each>
+__device__ u64 border_of(const Row& r, Each each, u64 count, u64 weight, u64 all, Shared& sh) {
+  u64 least = 0, from = all;
+  if (r.top_k > 0)
+    least = least_rank(r, each, count, weight, [&](u64 n, u64) { return n >= static_cast<u64>(r.top_k); },
+                       r.top_p < 1, &from, sh);
+  if (r.top_p < 1) {
+    // (a token is kept while the weight before it is less than the share)
+    const double share = r.top_p * static_cast<double>(from);
+    const u64 p = least_rank(r, each, count, weight,
+                             [&](u64, u64 w) { return static_cast<double>(w) >= share; }, true, &from, sh);
+    least = p > least ? p : least;
   }
-  best = across<true>(best, sh.sums);
-  r.top = static_cast<uint32_t>(best >> 32);
-  const int first = static_cast<int>(~static_cast<uint32_t>(best));
-  const double temperature = a.temperatures ? a.temperatures[b] : a.temperature;
-  if (r.top <= kLeastKey || !(temperature > 0)) {
-    if (tid == 0) {
-      a.tokens[b] = r.top <= kLeastKey ? -1 : first;
-      if (a.logprobs) a.logprobs[b] = r.top <= kLeastKey ? -__builtin_inff() : 0.f;
-    }
-    return;
-  }
-  r.max = logit_of(r.top);
-  r.inv = 1.0 / temperature;
-  const int64_t top_k = a.top_ks ? a.top_ks[b] : a.top_k;
-  const double top_p = a.top_ps ? a.top_ps[b] : a.top_p;
-  const double min_p = fmin(a.min_ps ? a.min_ps[b] : a.min_p, 1.0);
+  return least;
+}
 
-  Border border = {0, 0, 0};  // every key is greater
-  if (top_k > 0 && top_k < vocab)
-    border = border_of<T>(r, vocab, sh, top_p < 1, [&](uint32_t n, u64) { return n >= top_k; });
-  if (top_p < 1) {
-    u64 all;
-    if (border.key != 0) {
-      all = border.above + border.ties * weight_of(r, border.key);
-    } else {
-      all = 0;
-      for (int i = tid; i < vocab; i += kThreads) all += weight_of(r, key_of(logit_at<T>(r.logits, i)));
-      all = across<false>(all, sh.sums);
-    }
-    // (the first token's weight before it is 0: it is kept whatever top_p)
-    const double share = top_p * static_cast<double>(all);
-    const Border p = border_of<T>(r, vocab, sh, true,
-                                  [&](uint32_t, u64 w) { return static_cast<double>(w) >= share; });
-    if (p.key > border.key || (p.key == border.key && p.ties < border.ties)) border = p;
-  }
-  int last_tie = -1;  // the border key's tokens up to this one are kept
-  if (border.key != 0)
-    last_tie = find_first(vocab, [&](int i) -> u64 { return key_of(logit_at<T>(r.logits, i)) == border.key; },
-                          [&](u64 n) { return n >= border.ties; }, sh.sums, &sh.at);
+__device__ __forceinline__ void write_greedy(const SampleArgs& a, int b, u64 best) {
+  const bool none = key_in(best) <= kLeastKey;
+  a.tokens[b] = none ? -1 : index_in(best);
+  if (a.logprobs) a.logprobs[b] = none ? -__builtin_inff() : 0.f;
+}
+
+// The token: kept weight `all`, of which `before` lies before the tokens [lo, hi), where
+// the one searched for is.
+template <typename T>
+__device__ void pick(const SampleArgs& a, const Row& r, int b, u64 least, u64 all, u64 before, double target,
+                     int lo, int hi, Shared& sh) {
   const auto kept = [&](int i) -> u64 {
     const uint32_t key = key_of(logit_at<T>(r.logits, i));
-    if (key < border.key || (key == border.key && i > last_tie)) return 0;
-    if (key != r.top && !(exp(exponent_of(r, key)) >= min_p)) return 0;
-    return weight_of(r, key);
+    return rank_of(key, i) >= least ? likely_weight(r, key) : 0;
   };
-  u64 all = 0;
-  for (int i = tid; i < vocab; i += kThreads) all += kept(i);
-  all = across<false>(all, sh.sums);
-  const double target = fmin(fmax(static_cast<double>(a.uniforms[b]), 0.0), 1.0) * static_cast<double>(all);
-  int token = find_first(vocab, kept, [&](u64 w) { return static_cast<double>(w) > target; }, sh.sums, &sh.at);
-  if (token >= vocab)  // (a number of 1): the last one
-    token = find_first(vocab, kept, [&](u64 w) { return w >= all; }, sh.sums, &sh.at);
-  if (tid == 0) {
+  const int token = find_first(lo, hi, before, kept,
+                               [&](u64 w) { return static_cast<double>(w) > target || w == all; }, sh);
+  if (threadIdx.x == 0) {
     a.tokens[b] = token;
     if (a.logprobs)
       a.logprobs[b] = static_cast<float>(exponent_of(r, key_of(logit_at<T>(r.logits, token))) -
                                          log(static_cast<double>(all) / (1ull << kWeightBits)));
   }
 }
+__device__ __forceinline__ double target_of(const SampleArgs& a, int b, u64 all) {
+  return fmin(fmax(static_cast<double>(a.uniforms[b]), 0.0), 1.0) * static_cast<double>(all);
+}
+
+// Kept weight of each chunk into LDS and of the row, then the token.
+template <typename T>
+__device__ void pick_in_chunks(const SampleArgs& a, const Row& r, int b, u64 least, u64* chunk_sums, Shared& sh) {
+  const int tid = threadIdx.x, lane = tid & 63;
+  __syncthreads();
+  u64 mine = tid < a.chunks ? chunk_sums[tid] : 0;
+  const u64 all = across<kRowThreads, false>(mine, sh.sums);
+  const double target = target_of(a, b, all);
+  if (tid < 64) {  // kMaxChunks: four a lane
+    u64 c[4], sum = 0;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) c[j] = sum += 4 * lane + j < a.chunks ? chunk_sums[4 * lane + j] : 0;
+    const u64 before = wave_scan(sum, lane) - sum;
+    int at = -1;
+#pragma unroll
+    for (int j = 3; j >= 0; --j)
+      if (static_cast<double>(before + c[j]) > target || before + c[j] == all) at = j;
+    const uint64_t hit = __ballot(at >= 0);
+    if (lane == __ffsll(static_cast<unsigned long long>(hit)) - 1) {
+      u64 up = before;
+#pragma unroll
+      for (int j = 1; j < 4; ++j)
+        if (j == at) up = before + c[j - 1];
+      sh.at = 4 * lane + at;
+      sh.found[0] = up;
+    }
+  }
+  __syncthreads();
+  const int chunk = sh.at;
+  const u64 before = sh.found[0];
+  __syncthreads();
+  pick<T>(a, r, b, least, all, before, target, chunk * a.chunk, min(a.vocab, (chunk + 1) * a.chunk), sh);
+}
+
+// A whole row by one workgroup.
+template <typename T>
+__global__ __launch_bounds__(kRowThreads) void sample_row_kernel(SampleArgs a) {
+  __shared__ Shared sh;
+  const int b = blockIdx.x;
+  u64 best = 0;
+  for_each<T, kRowThreads>(row_of<T>(a, b), 0, a.vocab, [&](int i, float x) {
+    const u64 rank = rank_of(key_of(x), i);
+    best = rank > best ? rank : best;
+  });
+  best = across<kRowThreads, true>(best, sh.sums);
+  const Row r = settings_of<T>(a, b, best);
+  if (r.greedy) {
+    if (threadIdx.x == 0) write_greedy(a, b, best);
+    return;
+  }
+  u64 least = 0;
+  if (r.limited) {
+    u64 all = 0;
+    if (r.top_k == 0) {
+      for_each<T, kRowThreads>(r.logits, 0, a.vocab, [&](int, float x) { all += weight_of(r, key_of(x)); });
+      all = across<kRowThreads, false>(all, sh.sums);
+    }
+    least = border_of(r, [&](auto f) {
+      for_each<T, kRowThreads>(r.logits, 0, a.vocab, [&](int i, float x) { f(rank_of(key_of(x), i)); });
+    }, 0, 0, all, sh);
+  }
+  u64 all = 0;
+  for_each<T, kRowThreads>(r.logits, 0, a.vocab, [&](int i, float x) {
+    const uint32_t key = key_of(x);
+    if (rank_of(key, i) >= least) all += likely_weight(r, key);
+  });
+  all = across<kRowThreads, false>(all, sh.sums);
+  pick<T>(a, r, b, least, all, 0, target_of(a, b, all), 0, a.vocab, sh);
+}
+
+// ---- long rows -------------------------------------------------------------
+
+template <typename T>
+__global__ __launch_bounds__(kChunkThreads) void chunk_max_kernel(SampleArgs a) {
+  __shared__ u64 sh[kChunkThreads / 64];
+  const int c = blockIdx.x, b = blockIdx.y, tid = threadIdx.x;
+  // (the row's histogram and list for the next passes)
+  if (a.counts != nullptr) {
+    for (int i = c * kChunkThreads + tid; i < kBins; i += a.chunks * kChunkThreads) {
+      a.counts[static_cast<int64_t>(b) * kBins + i] = 0;
+      a.weights[static_cast<int64_t>(b) * kBins + i] = 0;
+    }
+    if (c == 0 && tid == 0) a.listed[b] = 0;
+  }
+  u64 best = 0;
+  for_each<T, kChunkThreads>(row_of<T>(a, b), c * a.chunk, min(a.vocab, (c + 1) * a.chunk), [&](int i, float x) {
+    const u64 rank = rank_of(key_of(x), i);
+    best = rank > best ? rank : best;
+  });
+  best = across<kChunkThreads, true>(best, sh);
+  if (tid == 0) a.best[static_cast<int64_t>(b) * a.chunks + c] = best;
+}
+
+template <int THREADS>
+__device__ __forceinline__ u64 row_best(const SampleArgs& a, int b, u64* sh) {
+  u64 best = 0;
+  for (int i = threadIdx.x; i < a.chunks; i += THREADS) {
+    const u64 x = a.best[static_cast<int64_t>(b) * a.chunks + i];
+    best = x > best ? x : best;
+  }
+  return across<THREADS, true>(best, sh);
+}
+
+template <typename T>
+__global__ __launch_bounds__(kChunkThreads) void chunk_weigh_kernel(SampleArgs a) {
+  __shared__ u64 sh[kChunkThreads / 64];
+  __shared__ u64 weights[kBins];
+  __shared__ uint32_t counts[kBins];
+  const int c = blockIdx.x, b = blockIdx.y, tid = threadIdx.x;
+  const Row r = settings_of<T>(a, b, row_best<kChunkThreads>(a, b, sh));
+  if (r.greedy) return;
+  const int lo = c * a.chunk, hi = min(a.vocab, lo + a.chunk);
+  if (!r.limited) {
+    u64 sum = 0;
+    for_each<T, kChunkThreads>(r.logits, lo, hi, [&](int, float x) { sum += likely_weight(r, key_of(x)); });
+    sum = across<kChunkThreads, false>(sum, sh);
+    if (tid == 0) a.sums[static_cast<int64_t>(b) * a.chunks + c] = sum;
+    return;
+  }
+  for (int i = tid; i < kBins; i += kChunkThreads) weights[i] = 0, counts[i] = 0;
+  __syncthreads();
+  uint32_t far = 0;  // of the last bin, where masked tokens are
+  u64 far_weight = 0;
+  for_each<T, kChunkThreads>(r.logits, lo, hi, [&](int, float x) {
+    const double z = exponent_of(r, key_of(x));
+    const int bin = bin_at(z);
+    const u64 w = weight_at(z);
+    if (bin == kBins - 1) {
+      ++far;
+      far_weight += w;
+    } else {
+      atomicAdd(&counts[bin], 1u);
+      if (w > 0) atomicAdd(&weights[bin], w);
+    }
+  });
+  if (far > 0) {
+    atomicAdd(&counts[kBins - 1], far);
+    atomicAdd(&weights[kBins - 1], far_weight);
+  }
+  __syncthreads();
+  for (int i = tid; i < kBins; i += kChunkThreads)
+    if (counts[i] > 0) {
+      atomicAdd(&a.counts[static_cast<int64_t>(b) * kBins + i], counts[i]);
+      if (weights[i] > 0) atomicAdd(&a.weights[static_cast<int64_t>(b) * kBins + i], weights[i]);
+    }
+}
+
+// The bins [lo, hi] that hold a row's borders, and what lies above and in them.
+struct Bins {
+  int lo, hi;
+  uint32_t above, in;
+  u64 above_weight, all;
+};
+
+template <int THREADS>
+__device__ Bins bins_of(const SampleArgs& a, const Row& r, int b, u64* sh) {
+  // a thread's share of the bins, in order; the first threads have it
+  constexpr int kShare = kBins / 256;
+  __shared__ u64 found[6];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  uint32_t c[kShare];
+  u64 w[kShare], cs = 0, ws = 0;
+#pragma unroll
+  for (int j = 0; j < kShare; ++j) {
+    c[j] = 0, w[j] = 0;
+    if (tid < 256) {
+      c[j] = a.counts[static_cast<int64_t>(b) * kBins + tid * kShare + j];
+      w[j] = a.weights[static_cast<int64_t>(b) * kBins + tid * kShare + j];
+    }
+    cs += c[j];
+    ws += w[j];
+  }
+  const u64 all = across<THREADS, false>(ws, sh);
+  u64 c_run = wave_scan(cs, lane), w_run = wave_scan(ws, lane);
+  __syncthreads();
+  if (lane == 63 && wave < 4) sh[wave] = c_run;
+  if (tid < 6) found[tid] = 0;
+  __syncthreads();
+  for (int i = 0; i < wave && i < 4; ++i) c_run += sh[i];
+  __syncthreads();
+  if (lane == 63 && wave < 4) sh[wave] = w_run;
+  __syncthreads();
+  for (int i = 0; i < wave && i < 4; ++i) w_run += sh[i];
+  c_run -= cs;
+  w_run -= ws;
+  // top_k alone or with top_p: the bin of token top_k; top_p alone: the share's
+  const double share = r.top_p * static_cast<double>(all);
+  const auto past = [&](u64 n, u64 weight) {
+    return r.top_k > 0 ? n >= static_cast<u64>(r.top_k) : static_cast<double>(weight) >= share;
+  };
+  if (tid < 256) {
+#pragma unroll
+    for (int j = 0; j < kShare; ++j) {
+      // (an empty bin is passed over: the border is a token's)
+      if (c[j] > 0 && past(c_run + c[j], w_run + w[j]) && (c_run == 0 || !past(c_run, w_run))) {
+        found[0] = tid * kShare + j;
+        found[1] = c_run;
+        found[2] = w_run;
+        found[3] = c[j];
+      }
+      c_run += c[j];
+      w_run += w[j];
+    }
+  }
+  __syncthreads();
+  Bins s;
+  s.hi = static_cast<int>(found[0]);
+  s.all = all;
+  if (r.top_k > 0 && r.top_p < 1) {  // both: the whole list, for top_p's border lies in it
+    s.lo = 0;
+    s.above = 0;
+    s.above_weight = 0;
+    s.in = static_cast<uint32_t>(found[1] + found[3]);
+  } else {
+    s.lo = s.hi;
+    s.above = static_cast<uint32_t>(found[1]);
+    s.above_weight = found[2];
+    s.in = static_cast<uint32_t>(found[3]);
+  }
+  return s;
+}
+
+template <typename T>
+__global__ __launch_bounds__(kChunkThreads) void chunk_list_kernel(SampleArgs a) {
+  __shared__ u64 sh[kChunkThreads / 64];
+  __shared__ u64 list[kList];
+  __shared__ uint32_t listed, at;
+  const int c = blockIdx.x, b = blockIdx.y, tid = threadIdx.x;
+  const Row r = settings_of<T>(a, b, row_best<kChunkThreads>(a, b, sh));
+  if (!r.limited) return;
+  const Bins bins = bins_of<kChunkThreads>(a, r, b, sh);
+  if (bins.in > kList) return;  // the row's workgroup does it all
+  if (tid == 0) listed = 0;
+  __syncthreads();
+  const int lo = c * a.chunk, hi = min(a.vocab, lo + a.chunk);
+  u64 sum = 0;
+  for_each<T, kChunkThreads>(r.logits, lo, hi, [&](int i, float x) {
+    const uint32_t key = key_of(x);
+    const double z = exponent_of(r, key);
+    const int bin = bin_at(z);
+    if (bin > bins.hi) return;
+    if (bin >= bins.lo)
+      list[atomicAdd(&listed, 1u)] = rank_of(key, i);
+    else if (z >= r.least)
+      sum += weight_at(z);
+  });
+  sum = across<kChunkThreads, false>(sum, sh);
+  if (tid == 0) {
+    a.sums[static_cast<int64_t>(b) * a.chunks + c] = sum;
+    at = listed > 0 ? atomicAdd(&a.listed[b], listed) : 0;
+  }
+  __syncthreads();
+  for (uint32_t i = tid; i < listed; i += kChunkThreads)
+    a.list[static_cast<int64_t>(b) * kList + at + i] = list[i];
+}
+
+template <typename T>
+__global__ __launch_bounds__(kRowThreads) void sample_finish_kernel(SampleArgs a) {
+  __shared__ Shared sh;
+  __shared__ u64 chunk_sums[kMaxChunks];
+  const int b = blockIdx.x, tid = threadIdx.x;
+  const u64 best = row_best<kRowThreads>(a, b, sh.sums);
+  const Row r = settings_of<T>(a, b, best);
+  if (r.greedy) {
+    if (tid == 0) write_greedy(a, b, best);
+    return;
+  }
+  u64 least = 0;
+  bool summed = true;
+  if (r.limited) {
+    const Bins bins = bins_of<kRowThreads>(a, r, b, sh.sums);
+    summed = bins.in <= kList;
+    if (summed) {
+      const u64* list = a.list + static_cast<int64_t>(b) * kList;
+      const auto each = [&](auto f) {
+        for (uint32_t i = tid; i < bins.in; i += kRowThreads) f(list[i]);
+      };
+      least = border_of(r, each, bins.above, bins.above_weight, bins.all, sh);
+      __syncthreads();
+      if (tid < a.chunks) chunk_sums[tid] = a.sums[static_cast<int64_t>(b) * a.chunks + tid];
+      __syncthreads();
+      each([&](u64 rank) {
+        if (rank >= least) atomicAdd(&chunk_sums[index_in(rank) / a.chunk], likely_weight(r, key_in(rank)));
+      });
+    } else {  // more tokens than a list holds: by the row itself
+      least = border_of(r, [&](auto f) {
+        for_each<T, kRowThreads>(r.logits, 0, a.vocab, [&](int i, float x) { f(rank_of(key_of(x), i)); });
+      }, 0, 0, bins.all, sh);
+      for (int c = 0; c < a.chunks; ++c) {
+        u64 sum = 0;
+        for_each<T, kRowThreads>(r.logits, c * a.chunk, min(a.vocab, (c + 1) * a.chunk), [&](int i, float x) {
+          const uint32_t key = key_of(x);
+          if (rank_of(key, i) >= least) sum += likely_weight(r, key);
+        });
+        sum = across<kRowThreads, false>(sum, sh.sums);
+        if (tid == 0) chunk_sums[c] = sum;
+      }
+    }
+  } else if (tid < a.chunks) {
+    chunk_sums[tid] = a.sums[static_cast<int64_t>(b) * a.chunks + tid];
+  }
+  pick_in_chunks<T>(a, r, b, least, chunk_sums, sh);
+}
+
+// Chunks of a row in a call (0: a workgroup has a whole row).
+constexpr int kShortRow = 4096;
+constexpr int kLeastChunk = 2048;
+int chunks_of(int64_t batch, int64_t vocab) {
+  if (vocab <= kShortRow) return 0;
+  const int64_t most = (vocab + kLeastChunk - 1) / kLeastChunk;  // at most kMaxChunks
+  int64_t want = 8LL * cu_count() / batch;
+  want = want < 1 ? 1 : want;
+  return static_cast<int>(want < most ? want : most);
+}
+
+int64_t align16(int64_t n) { return (n + 15) / 16 * 16; }
+
+// Workspace: best, sums, and with a limit weights, list, counts, listed.
+bool may_limit(const fpv2_sample_params& p) {
+  return p.top_ks != nullptr || p.top_ps != nullptr || (p.top_k > 0 && p.top_k < p.vocab) || p.top_p < 1;
+}
+int64_t workspace_of(const fpv2_sample_params& p, SampleArgs* a, char* base) {
+  const int64_t chunks = chunks_of(p.batch, p.vocab);
+  if (chunks == 0) return 0;
+  int64_t at = 0;
+  const auto take = [&](int64_t bytes) {
+    const int64_t here = at;
+    at += align16(bytes);
+    return base + here;
+  };
+  a->chunks = static_cast<int>(chunks);
+  a->chunk = static_cast<int>((p.vocab + chunks - 1) / chunks);
+  a->best = reinterpret_cast<u64*>(take(8 * p.batch * chunks));
+  a->sums = reinterpret_cast<u64*>(take(8 * p.batch * chunks));
+  if (may_limit(p)) {
+    a->weights = reinterpret_cast<u64*>(take(8 * p.batch * kBins));
+    a->list = reinterpret_cast<u64*>(take(8 * p.batch * kList));
+    a->counts = reinterpret_cast<uint32_t*>(take(4 * p.batch * kBins));
+    a->listed = reinterpret_cast<uint32_t*>(take(4 * p.batch));
+  }
+  return at;
+}
+
+template <typename T>
+int launch_sample(const SampleArgs& a, int64_t batch, hipStream_t s) {
+  const dim3 rows(static_cast<unsigned>(batch)), row_threads(kRowThreads), threads(kChunkThreads);
+  if (a.chunks == 0) {
+    hipLaunchKernelGGL(sample_row_kernel<T>, rows, row_threads, 0, s, a);
+    return check_launch("sample_row_kernel");
+  }
+  const dim3 chunks(static_cast<unsigned>(a.chunks), static_cast<unsigned>(batch));
+  hipLaunchKernelGGL(chunk_max_kernel<T>, chunks, threads, 0, s, a);
+  hipLaunchKernelGGL(chunk_weigh_kernel<T>, chunks, threads, 0, s, a);
+  if (a.counts != nullptr) hipLaunchKernelGGL(chunk_list_kernel<T>, chunks, threads, 0, s, a);
+  hipLaunchKernelGGL(sample_finish_kernel<T>, rows, row_threads, 0, s, a);
+  return check_launch("sample_finish_kernel");
+}
+
+int check_sample(const char* name, const fpv2_sample_params* p) {
+  if (p == nullptr) return fail(FPV2_ERR_ARGUMENT, "%s: null params", name);
+  if (p->batch < 0 || p->batch > 0xffff || p->vocab <= 0 || p->logits_stride < 0)
+    return fail(FPV2_ERR_ARGUMENT, "%s: bad batch (at most 65535), vocab or stride", name);
+  if (p->vocab > FPV2_MAX_VOCAB)
+    return fail(FPV2_ERR_UNSUPPORTED, "%s: more than %d tokens", name, FPV2_MAX_VOCAB);
+  return FPV2_OK;
+}
 
 }  // namespace
 }  // namespace fpv2
 
+extern "C" int64_t fpv2_sample_tokens_workspace_bytes(const fpv2_sample_params* params) {
+  using namespace fpv2;
+  if (const int rc = check_sample("fpv2_sample_tokens", params)) return rc;
+  SampleArgs a{};
+  return params->batch == 0 ? 0 : workspace_of(*params, &a, nullptr);
+}
+
 extern "C" int fpv2_sample_tokens(const void* logits, const float* uniforms, int dtype,
                                   const fpv2_sample_params* params, int64_t* tokens,
-                                  float* logprobs, void* stream) {
+                                  float* logprobs, void* workspace, int64_t workspace_bytes,
+                                  void* stream) {
   using namespace fpv2;
   const char* name = "fpv2_sample_tokens";
-  if (params == nullptr) return fail(FPV2_ERR_ARGUMENT, "%s: null params", name);
+  if (const int rc = check_sample(name, params)) return rc;
   const fpv2_sample_params& p = *params;
   if (dtype != FPV2_F32 && dtype != FPV2_BF16 && dtype != FPV2_F16)
     return fail(FPV2_ERR_UNSUPPORTED, "%s: dtype must be float32, bf16 or f16", name);
-  if (p.batch < 0 || p.batch > 0x7fffffff || p.vocab <= 0 || p.logits_stride < 0)
-    return fail(FPV2_ERR_ARGUMENT, "%s: bad batch, vocab or stride", name);
-  if (p.vocab > FPV2_MAX_VOCAB)
-    return fail(FPV2_ERR_UNSUPPORTED, "%s: more than %d tokens", name, FPV2_MAX_VOCAB);
   if (p.batch == 0) return FPV2_OK;
   if (!logits || !uniforms || !tokens) return fail(FPV2_ERR_ARGUMENT, "%s: null pointer", name);
-  SampleArgs a{logits,    uniforms,      p.temperatures, p.top_ks, p.top_ps,  p.min_ps,
-               tokens,    logprobs,      p.temperature,  p.top_p,  p.min_p,   p.top_k,
-               p.logits_stride, static_cast<int>(p.vocab)};
+  SampleArgs a{};
+  const int64_t need = workspace_of(p, &a, static_cast<char*>(workspace));
+  if (need > 0 && (workspace == nullptr || workspace_bytes < need ||
+                   (reinterpret_cast<uintptr_t>(workspace) & 15u) != 0))
+    return fail(FPV2_ERR_ARGUMENT, "%s: needs a 16-byte aligned workspace of %lld bytes", name,
+                static_cast<long long>(need));
+  a.logits = logits;
+  a.uniforms = uniforms;
+  a.temperatures = p.temperatures;
+  a.top_ks = p.top_ks;
+  a.top_ps = p.top_ps;
+  a.min_ps = p.min_ps;
+  a.tokens = tokens;
+  a.logprobs = logprobs;
+  a.temperature = p.temperature;
+  a.top_p = p.top_p;
+  a.min_p = p.min_p;
+  a.top_k = p.top_k;
+  a.stride = p.logits_stride;
+  a.vocab = static_cast<int>(p.vocab);
   const hipStream_t s = static_cast<hipStream_t>(stream);
-  const dim3 grid(static_cast<unsigned>(p.batch)), block(kThreads);
-  if (dtype == FPV2_F32)
-    hipLaunchKernelGGL(sample_kernel<f32_t>, grid, block, 0, s, a);
-  else if (dtype == FPV2_BF16)
-    hipLaunchKernelGGL(sample_kernel<bf16_t>, grid, block, 0, s, a);
-  else
-    hipLaunchKernelGGL(sample_kernel<f16_t>, grid, block, 0, s, a);
-  return check_launch("sample_kernel");
+  if (dtype == FPV2_F32) return launch_sample<f32_t>(a, p.batch, s);
+  if (dtype == FPV2_BF16) return launch_sample<bf16_t>(a, p.batch, s);
+  return launch_sample<f16_t>(a, p.batch, s);
 }

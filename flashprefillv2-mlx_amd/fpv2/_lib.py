@@ -58,6 +58,7 @@ EXPORTED_SYMBOLS = (
     "fpv2_decode_attention",
     "fpv2_rope_to_pages",
     "fpv2_quantized_linear",
+    "fpv2_sample_tokens_workspace_bytes",
     "fpv2_sample_tokens",
 )
 
@@ -240,7 +241,10 @@ def _declare(lib: ctypes.CDLL) -> None:
     lib.fpv2_rope_to_pages.restype = ctypes.c_int
     lib.fpv2_rope_to_pages.argtypes = [vp] * 10 + [i32, ctypes.POINTER(RopePagesParams), vp]
     lib.fpv2_sample_tokens.restype = ctypes.c_int
-    lib.fpv2_sample_tokens.argtypes = [vp, vp, i32, ctypes.POINTER(SampleParams), vp, vp, vp]
+    lib.fpv2_sample_tokens.argtypes = [vp, vp, i32, ctypes.POINTER(SampleParams), vp, vp, vp,
+                                       i64, vp]
+    lib.fpv2_sample_tokens_workspace_bytes.restype = i64
+    lib.fpv2_sample_tokens_workspace_bytes.argtypes = [ctypes.POINTER(SampleParams)]
     lib.fpv2_quantized_linear.restype = ctypes.c_int
     lib.fpv2_quantized_linear.argtypes = [vp] * 5 + [i32, i32] + [i64] * 8 + [vp]
 

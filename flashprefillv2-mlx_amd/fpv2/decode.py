@@ -431,10 +431,12 @@ def sample_tokens(logits: torch.Tensor, uniform: torch.Tensor, *,
             _lib.ptr(k_rows), _lib.ptr(p_rows), _lib.ptr(m_rows), t, min(k, vocab), p, m)
 
         def call(stream):
+            need = lib.fpv2_sample_tokens_workspace_bytes(ctypes.byref(params))
+            work = torch.empty(need, dtype=torch.uint8, device=device) if need > 0 else None
             _lib.check(lib.fpv2_sample_tokens(
                 logits.data_ptr(), uniform.data_ptr(), _lib.dtype_code(logits.dtype),
-                ctypes.byref(params), tokens.data_ptr(), _lib.ptr(logprobs), stream),
-                "sample_tokens")
+                ctypes.byref(params), tokens.data_ptr(), _lib.ptr(logprobs), _lib.ptr(work),
+                max(need, 0), stream), "sample_tokens")
 
         _on_device(device, call)
     return (tokens, logprobs) if return_logprobs else tokens

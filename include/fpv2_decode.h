@@ -151,10 +151,14 @@ typedef struct fpv2_sample_params {
  * result does not depend on any order.  A NaN logit counts as -inf; a row of
  * nothing but -inf gives token -1.  logprobs (NULL: not written): log of the
  * token's share of the kept weight, 0 for a greedy row, -inf for token -1.
+ * workspace: fpv2_sample_tokens_workspace_bytes bytes for the current device (0:
+ * none), 16-byte aligned, not kept between calls; calls that share one on
+ * different streams race.
  */
+int64_t fpv2_sample_tokens_workspace_bytes(const fpv2_sample_params* params);
 int fpv2_sample_tokens(const void* logits, const float* uniforms, int dtype,
                        const fpv2_sample_params* params, int64_t* tokens, float* logprobs,
-                       void* stream);
+                       void* workspace, int64_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }

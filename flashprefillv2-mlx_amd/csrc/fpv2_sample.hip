@@ -24,7 +24,8 @@ namespace fpv2 {
 namespace {
 
 typedef unsigned long long u64;
-constexpr int kRowThreads = 1024;   // of a workgroup that has a row
+constexpr int kRowThreads = 1024;   // of a workgroup that has a row alone
+constexpr int kFinishThreads = 512; // of one that finishes a row of chunks
 constexpr int kChunkThreads = 256;  // of one that has a chunk
 constexpr int kWeightBits = 44;
 constexpr int kIndexBits = 20;
@@ -32,7 +33,10 @@ constexpr int kRankBits = 32 + kIndexBits;
 constexpr int kBins = 1024;     // of the histogram,
 constexpr double kPerUnit = 32; // so many to a unit of the exponent
 constexpr int kList = 4096;     // tokens of a row's list
+constexpr int kChunkList = 512; // of which a chunk's workgroup collects in LDS
 constexpr int kMaxChunks = 256;
+constexpr int kEach = 8;        // tokens of a thread where one is searched for
+constexpr int kFew = kFinishThreads / 2;  // tokens that are compared with one another
 
 struct SampleArgs {
   const void* logits;
@@ -47,7 +51,7 @@ struct SampleArgs {
   int64_t top_k, stride;
   int vocab;
   // chunks of a long row, and its workspace
-  int chunks, chunk;
+  int chunks, chunk, group;  // (in the passes after the first, `group` of them a workgroup)
   u64* best;         // [batch][chunks] greatest rank of a chunk
   u64* sums;         // [batch][chunks] weight of a chunk's tokens that are kept for sure
   u64* weights;      // [batch][kBins]
@@ -79,10 +83,10 @@ __device__ __forceinline__ float logit_in<f32_t>(u32x4 v, int j) {
 
 // Order-preserving key: -inf and NaN least, both zeros alike.
 constexpr uint32_t kLeastKey = 0x007fffffu;  // of -inf
+__device__ __forceinline__ float without_nan(float x) { return fmaxf(x, neg_inf()); }
 __device__ __forceinline__ uint32_t key_of(float x) {
-  if (x != x) return kLeastKey;
-  const uint32_t b = __float_as_uint(x + 0.f);
-  return b & 0x80000000u ? ~b : b | 0x80000000u;
+  const uint32_t b = __float_as_uint(without_nan(x) + 0.f);
+  return b ^ (static_cast<uint32_t>(static_cast<int32_t>(b) >> 31) | 0x80000000u);
 }
 __device__ __forceinline__ float logit_of(uint32_t key) {
   return __uint_as_float(key & 0x80000000u ? key & 0x7fffffffu : ~key);
@@ -99,53 +103,87 @@ __device__ __forceinline__ int index_in(u64 rank) {
 struct Row {
   const void* logits;
   uint32_t top;     // greatest key
-  double max, inv;  // its logit, 1 / temperature
-  double least;     // exponent from which on min_p keeps
+  float top_logit;
+  double max, inv;  // the same, 1 / temperature
+  u64 least;        // weight from which on min_p keeps
+  float reached;    // temperature, rounded up
+  float from;       // a logit below all that min_p keeps with any weight
   double top_p;
   int64_t top_k;    // 0: no limit
   bool greedy, limited;
+
+  // A logit below all whose weight's log is -units or more (float arithmetic, and
+  // units good to 2^-19, are off by less than what is taken off).
+  __device__ __forceinline__ float reach(float units) const {
+    if (top_logit == __builtin_inff()) return top_logit;  // (no other has weight)
+    const float down = units * reached * 1.00001f;
+    return (top_logit - down) - (fabsf(top_logit) + down) * 0x1p-20f;
+  }
 };
 
 template <typename T>
 __device__ __forceinline__ const void* row_of(const SampleArgs& a, int b) {
   return static_cast<const char*>(a.logits) + b * a.stride * kLogitBytes<T>;
 }
+// (the loads of a pass come first, so that it waits for memory once)
+struct Settings {
+  double temperature, top_p, min_p;
+  int64_t top_k;
+};
+__device__ __forceinline__ Settings load_settings(const SampleArgs& a, int b) {
+  return {a.temperatures ? a.temperatures[b] : a.temperature, a.top_ps ? a.top_ps[b] : a.top_p,
+          a.min_ps ? a.min_ps[b] : a.min_p, a.top_ks ? a.top_ks[b] : a.top_k};
+}
 template <typename T>
-__device__ __forceinline__ Row settings_of(const SampleArgs& a, int b, u64 best) {
+__device__ __forceinline__ Row row_with(const SampleArgs& a, int b, const Settings& set, u64 best) {
   Row r;
   r.logits = row_of<T>(a, b);
   r.top = key_in(best);
-  r.max = logit_of(r.top);
-  const double temperature = a.temperatures ? a.temperatures[b] : a.temperature;
+  r.max = r.top_logit = logit_of(r.top);
+  const double temperature = fmin(set.temperature, 1e30);
   r.greedy = r.top <= kLeastKey || !(temperature > 0);
-  r.inv = 1.0 / temperature;
-  r.top_p = a.top_ps ? a.top_ps[b] : a.top_p;
-  r.top_k = a.top_ks ? a.top_ks[b] : a.top_k;
+  r.inv = fmin(1.0 / temperature, 1e300);
+  r.top_p = set.top_p;
+  r.top_k = set.top_k;
   if (r.top_k < 0 || r.top_k >= a.vocab) r.top_k = 0;
-  const double min_p = a.min_ps ? a.min_ps[b] : a.min_p;
-  r.least = min_p > 0 ? log(fmin(min_p, 1.0)) : -__builtin_inf();
+  const double min_p = fmin(fmax(set.min_p, 0.0), 1.0);
+  r.least = static_cast<u64>(min_p * (1ull << kWeightBits));
+  r.reached = static_cast<float>(temperature) * 1.000001f;
   r.limited = !r.greedy && (r.top_k > 0 || r.top_p < 1);
+  r.from = r.reach(fminf(-__logf(static_cast<float>(min_p)) + 1e-5f, 32.f));
   return r;
 }
 
-// log of a weight (falls with the key), and the weight: 0 below 2^-45
-__device__ __forceinline__ double exponent_of(const Row& r, uint32_t key) {
-  if (key == r.top) return 0.0;
-  if (key <= kLeastKey) return -__builtin_inf();
-  return (static_cast<double>(logit_of(key)) - r.max) * r.inv;
+// log of a logit's weight (it rises with the logit), and the weight of a log.
+// Without branches: a pass's threads do this for every logit.
+__device__ __forceinline__ double exponent_of(const Row& r, float x) {
+  const double z = (static_cast<double>(without_nan(x)) - r.max) * r.inv;
+  return x == r.top_logit ? 0.0 : z;  // (an infinite one has no difference)
 }
 __device__ __forceinline__ u64 weight_at(double z) {
-  if (!(z > -31.2)) return 0;
-  return static_cast<u64>(exp(z) * (1ull << kWeightBits) + 0.5);
+  // exp z = 2^n e^f, |f| <= ln 2 / 2: the series to f^12 / 12! leaves 2^-52.  Rounded to
+  // an integer by the sum with 2^52, whose mantissa it then is.
+  z = fmax(z, -64.0);
+  const double n = __builtin_rint(z * 1.4426950408889634);
+  const double f = __builtin_fma(n, -0.6931471805599453, z);
+  double p = 1.0 / 479001600;
+  constexpr double c[] = {1.0 / 39916800, 1.0 / 3628800, 1.0 / 362880, 1.0 / 40320, 1.0 / 5040, 1.0 / 720,
+                          1.0 / 120, 1.0 / 24, 1.0 / 6, 0.5, 1.0, 1.0};
+#pragma unroll
+  for (int i = 0; i < 12; ++i) p = __builtin_fma(p, f, c[i]);
+  const double w = __builtin_ldexp(p, static_cast<int>(n) + kWeightBits);
+  return static_cast<u64>(__double_as_longlong(w + 4503599627370496.0)) & 0xfffffffffffffull;
 }
-__device__ __forceinline__ u64 weight_of(const Row& r, uint32_t key) { return weight_at(exponent_of(r, key)); }
+__device__ __forceinline__ u64 weight_of(const Row& r, uint32_t key) {
+  return weight_at(exponent_of(r, logit_of(key)));
+}
 __device__ __forceinline__ int bin_at(double z) {
-  return z > -(kBins - 1) / kPerUnit ? static_cast<int>(z * -kPerUnit) : kBins - 1;
+  return min(static_cast<int>(fmin(z * -kPerUnit, static_cast<double>(kBins))), kBins - 1);
 }
 // Weight of a token if min_p keeps it.
-__device__ __forceinline__ u64 likely_weight(const Row& r, uint32_t key) {
-  const double z = exponent_of(r, key);
-  return z >= r.least ? weight_at(z) : 0;
+__device__ __forceinline__ u64 likely_weight(const Row& r, float x) {
+  const u64 w = weight_at(exponent_of(r, x));
+  return w >= r.least ? w : 0;
 }
 
 __device__ __forceinline__ u64 shfl_xor64(u64 v, int off) {
@@ -188,17 +226,28 @@ __device__ __forceinline__ void for_each(const void* row, int lo, int hi, F f) {
   const uintptr_t at = reinterpret_cast<uintptr_t>(row) + static_cast<uintptr_t>(lo) * kLogitBytes<T>;
   const int head = min(hi - lo, static_cast<int>((16 - at % 16) % 16) / kLogitBytes<T>);
   const int tid = threadIdx.x;
-  if (tid < head) f(lo + tid, logit_at<T>(row, lo + tid));
-  const int first = lo + head, vectors = (hi - first) / N;
+  const int first = lo + head, vectors = (hi - first) / N, last = first + N * vectors;
+  const int edge = tid < head ? lo + tid : last + tid - head;
+  if (edge < hi && tid < 2 * N) f(edge, logit_at<T>(row, edge));
   const char* p = static_cast<const char*>(row) + static_cast<int64_t>(first) * kLogitBytes<T>;
-#pragma unroll 2
+#pragma unroll 1
   for (int v = tid; v < vectors; v += THREADS) {
     const u32x4 x = load16(p + 16 * static_cast<int64_t>(v));
 #pragma unroll
     for (int j = 0; j < N; ++j) f(first + N * v + j, logit_in<T>(x, j));
   }
-  const int tail = first + N * vectors + tid;
-  if (tail < hi) f(tail, logit_at<T>(row, tail));
+}
+
+// The greatest rank of a thread's tokens of [lo, hi).
+template <typename T, int THREADS>
+__device__ __forceinline__ u64 best_of(const void* row, int lo, int hi) {
+  float best = neg_inf();
+  int at = hi;
+  for_each<T, THREADS>(row, lo, hi, [&](int i, float x) {
+    at = x > best || (x == best && i < at) ? i : at;
+    best = fmaxf(x, best);
+  });
+  return at < hi ? rank_of(key_of(best), at) : 0;
 }
 
 struct Shared {
@@ -209,43 +258,34 @@ struct Shared {
   int at;
 };
 
-// The first i in [lo, hi) for which past(before + value(lo) + .. + value(i)) holds, or
-// hi: sums of the waves' shares, then of the shares of one of these, until one
-// wave is left with a piece.
-template <typename Value, typename Past>
+// The first i in [lo, hi), at most kEach a thread, for which past(before + value(lo) +
+// .. + value(i)) holds, or hi.
+template <int THREADS, typename Value, typename Past>
 __device__ int find_first(int lo, int hi, u64 before, Value value, Past past, Shared& sh) {
-  constexpr int kWaves = kRowThreads / 64;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, none = hi;
-  while (hi - lo > 512) {
-    const int share = (hi - lo + kWaves - 1) / kWaves;
-    const int a = min(hi, lo + wave * share), b = min(hi, a + share);
-    u64 sum = 0;
-    for (int i = a + lane; i < b; i += 64) sum += value(i);
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int each = (hi - lo + THREADS - 1) / THREADS;
+  const int from = min(hi, lo + tid * each), to = min(hi, from + each);
+  u64 v[kEach], sum = 0;
 #pragma unroll
-    for (int off = 32; off >= 1; off >>= 1) sum += shfl_xor64(sum, off);
-    __syncthreads();
-    if (lane == 0) sh.sums[wave] = sum;
-    __syncthreads();
-    int w = 0;
-    while (w < kWaves && !past(before + sh.sums[w])) before += sh.sums[w++];
-    if (w == kWaves) return none;
-    const int next = min(hi, lo + w * share);
-    hi = min(hi, next + share);
-    lo = next;
+  for (int j = 0; j < kEach; ++j) {
+    v[j] = from + j < to ? value(from + j) : 0;
+    sum += v[j];
   }
+  const u64 upto = wave_scan(sum, lane);
   __syncthreads();
-  if (threadIdx.x == 0) sh.at = none;
+  if (lane == 63) sh.sums[wave] = upto;
+  if (tid == 0) sh.at = hi;
   __syncthreads();
-  if (wave == 0) {
-    for (int i0 = lo; i0 < hi; i0 += 64) {
-      const u64 sum = wave_scan(i0 + lane < hi ? value(i0 + lane) : 0, lane);
-      const uint64_t hit = __ballot(i0 + lane < hi && past(before + sum));
-      if (hit != 0) {
-        if (lane == 0) sh.at = i0 + __ffsll(static_cast<unsigned long long>(hit)) - 1;
-        break;
-      }
-      before += shfl64(sum, 63);
+  u64 run = before + upto - sum;
+  for (int w = 0; w < wave; ++w) run += sh.sums[w];
+  if (sum > 0 && past(run + sum) && (run == before || !past(run))) {
+    int at = -1;
+#pragma unroll
+    for (int j = 0; j < kEach; ++j) {
+      run += v[j];
+      if (at < 0 && v[j] > 0 && past(run)) at = from + j;
     }
+    sh.at = at;
   }
   __syncthreads();
   return sh.at;
@@ -256,7 +296,7 @@ __device__ int find_first(int lo, int hi, u64 before, Value value, Past past, Sh
 // above the group; 0 where it never does.  *weight: weight of the tokens from there on.
 // Histograms over the rank's bits, 8 at a time from the first that differ, until one
 // token is left in the border's bin.
-template <typename Each, typename Past>
+template <int THREADS, typename Each, typename Past>
 __device__ u64 least_rank(const Row& r, Each each, u64 count, u64 weight, Past past, bool weigh,
                           u64* weight_from, Shared& sh) {
   const int tid = threadIdx.x, lane = tid & 63;
@@ -265,8 +305,8 @@ __device__ u64 least_rank(const Row& r, Each each, u64 count, u64 weight, Past p
     low = rank < low ? rank : low;
     high = rank > high ? rank : high;
   });
-  high = across<kRowThreads, true>(high, sh.sums);
-  low = ~across<kRowThreads, true>(~low, sh.sums);
+  high = across<THREADS, true>(high, sh.sums);
+  low = ~across<THREADS, true>(~low, sh.sums);
   int shift = low < high ? 64 - __clzll(static_cast<long long>(low ^ high)) - 8 : 0;
   int width = 8;  // the bits shift .. shift + width - 1 are the bin
   if (shift < 0) shift = 0;
@@ -331,16 +371,16 @@ __device__ u64 least_rank(const Row& r, Each each, u64 count, u64 weight, Past p
 }
 
 // The least kept rank of a row whose borders lie in a group of tokens.
-template <typename Each>
+template <int THREADS, typename Each>
 __device__ u64 border_of(const Row& r, Each each, u64 count, u64 weight, u64 all, Shared& sh) {
   u64 least = 0, from = all;
   if (r.top_k > 0)
-    least = least_rank(r, each, count, weight, [&](u64 n, u64) { return n >= static_cast<u64>(r.top_k); },
+    least = least_rank<THREADS>(r, each, count, weight, [&](u64 n, u64) { return n >= static_cast<u64>(r.top_k); },
                        r.top_p < 1, &from, sh);
   if (r.top_p < 1) {
     // (a token is kept while the weight before it is less than the share)
     const double share = r.top_p * static_cast<double>(from);
-    const u64 p = least_rank(r, each, count, weight,
+    const u64 p = least_rank<THREADS>(r, each, count, weight,
                              [&](u64, u64 w) { return static_cast<double>(w) >= share; }, true, &from, sh);
     least = p > least ? p : least;
   }
@@ -355,19 +395,19 @@ __device__ __forceinline__ void write_greedy(const SampleArgs& a, int b, u64 bes
 
 // The token: kept weight `all`, of which `before` lies before the tokens [lo, hi), where
 // the one searched for is.
-template <typename T>
+template <typename T, int THREADS>
 __device__ void pick(const SampleArgs& a, const Row& r, int b, u64 least, u64 all, u64 before, double target,
                      int lo, int hi, Shared& sh) {
   const auto kept = [&](int i) -> u64 {
-    const uint32_t key = key_of(logit_at<T>(r.logits, i));
-    return rank_of(key, i) >= least ? likely_weight(r, key) : 0;
+    const float x = logit_at<T>(r.logits, i);
+    return x >= r.from && rank_of(key_of(x), i) >= least ? likely_weight(r, x) : 0;
   };
-  const int token = find_first(lo, hi, before, kept,
+  const int token = find_first<THREADS>(lo, hi, before, kept,
                                [&](u64 w) { return static_cast<double>(w) > target || w == all; }, sh);
   if (threadIdx.x == 0) {
     a.tokens[b] = token;
     if (a.logprobs)
-      a.logprobs[b] = static_cast<float>(exponent_of(r, key_of(logit_at<T>(r.logits, token))) -
+      a.logprobs[b] = static_cast<float>(exponent_of(r, logit_at<T>(r.logits, token)) -
                                          log(static_cast<double>(all) / (1ull << kWeightBits)));
   }
 }
@@ -381,7 +421,7 @@ __device__ void pick_in_chunks(const SampleArgs& a, const Row& r, int b, u64 lea
   const int tid = threadIdx.x, lane = tid & 63;
   __syncthreads();
   u64 mine = tid < a.chunks ? chunk_sums[tid] : 0;
-  const u64 all = across<kRowThreads, false>(mine, sh.sums);
+  const u64 all = across<kFinishThreads, false>(mine, sh.sums);
   const double target = target_of(a, b, all);
   if (tid < 64) {  // kMaxChunks: four a lane
     u64 c[4], sum = 0;
@@ -406,7 +446,7 @@ __device__ void pick_in_chunks(const SampleArgs& a, const Row& r, int b, u64 lea
   const int chunk = sh.at;
   const u64 before = sh.found[0];
   __syncthreads();
-  pick<T>(a, r, b, least, all, before, target, chunk * a.chunk, min(a.vocab, (chunk + 1) * a.chunk), sh);
+  pick<T, kFinishThreads>(a, r, b, least, all, before, target, chunk * a.chunk, min(a.vocab, (chunk + 1) * a.chunk), sh);
 }
 
 // A whole row by one workgroup.
@@ -414,13 +454,8 @@ template <typename T>
 __global__ __launch_bounds__(kRowThreads) void sample_row_kernel(SampleArgs a) {
   __shared__ Shared sh;
   const int b = blockIdx.x;
-  u64 best = 0;
-  for_each<T, kRowThreads>(row_of<T>(a, b), 0, a.vocab, [&](int i, float x) {
-    const u64 rank = rank_of(key_of(x), i);
-    best = rank > best ? rank : best;
-  });
-  best = across<kRowThreads, true>(best, sh.sums);
-  const Row r = settings_of<T>(a, b, best);
+  const u64 best = across<kRowThreads, true>(best_of<T, kRowThreads>(row_of<T>(a, b), 0, a.vocab), sh.sums);
+  const Row r = row_with<T>(a, b, load_settings(a, b), best);
   if (r.greedy) {
     if (threadIdx.x == 0) write_greedy(a, b, best);
     return;
@@ -429,20 +464,19 @@ __global__ __launch_bounds__(kRowThreads) void sample_row_kernel(SampleArgs a) {
   if (r.limited) {
     u64 all = 0;
     if (r.top_k == 0) {
-      for_each<T, kRowThreads>(r.logits, 0, a.vocab, [&](int, float x) { all += weight_of(r, key_of(x)); });
+      for_each<T, kRowThreads>(r.logits, 0, a.vocab, [&](int, float x) { all += weight_at(exponent_of(r, x)); });
       all = across<kRowThreads, false>(all, sh.sums);
     }
-    least = border_of(r, [&](auto f) {
+    least = border_of<kRowThreads>(r, [&](auto f) {
       for_each<T, kRowThreads>(r.logits, 0, a.vocab, [&](int i, float x) { f(rank_of(key_of(x), i)); });
     }, 0, 0, all, sh);
   }
   u64 all = 0;
   for_each<T, kRowThreads>(r.logits, 0, a.vocab, [&](int i, float x) {
-    const uint32_t key = key_of(x);
-    if (rank_of(key, i) >= least) all += likely_weight(r, key);
+    if (rank_of(key_of(x), i) >= least) all += likely_weight(r, x);
   });
   all = across<kRowThreads, false>(all, sh.sums);
-  pick<T>(a, r, b, least, all, 0, target_of(a, b, all), 0, a.vocab, sh);
+  pick<T, kRowThreads>(a, r, b, least, all, 0, target_of(a, b, all), 0, a.vocab, sh);
 }
 
 // ---- long rows -------------------------------------------------------------
@@ -459,12 +493,8 @@ __global__ __launch_bounds__(kChunkThreads) void chunk_max_kernel(SampleArgs a) 
     }
     if (c == 0 && tid == 0) a.listed[b] = 0;
   }
-  u64 best = 0;
-  for_each<T, kChunkThreads>(row_of<T>(a, b), c * a.chunk, min(a.vocab, (c + 1) * a.chunk), [&](int i, float x) {
-    const u64 rank = rank_of(key_of(x), i);
-    best = rank > best ? rank : best;
-  });
-  best = across<kChunkThreads, true>(best, sh);
+  const u64 best = across<kChunkThreads, true>(
+      best_of<T, kChunkThreads>(row_of<T>(a, b), c * a.chunk, min(a.vocab, (c + 1) * a.chunk)), sh);
   if (tid == 0) a.best[static_cast<int64_t>(b) * a.chunks + c] = best;
 }
 
@@ -478,36 +508,43 @@ __device__ __forceinline__ u64 row_best(const SampleArgs& a, int b, u64* sh) {
   return across<THREADS, true>(best, sh);
 }
 
+// a.group chunks by a workgroup: one histogram of them in LDS, so that fewer are
+// added to the row's (each line of it that an atomic goes to is one in memory).
 template <typename T>
 __global__ __launch_bounds__(kChunkThreads) void chunk_weigh_kernel(SampleArgs a) {
   __shared__ u64 sh[kChunkThreads / 64];
   __shared__ u64 weights[kBins];
   __shared__ uint32_t counts[kBins];
-  const int c = blockIdx.x, b = blockIdx.y, tid = threadIdx.x;
-  const Row r = settings_of<T>(a, b, row_best<kChunkThreads>(a, b, sh));
+  const int b = blockIdx.y, tid = threadIdx.x;
+  const int c0 = blockIdx.x * a.group, c1 = min(a.chunks, c0 + a.group);
+  const Settings set = load_settings(a, b);
+  const Row r = row_with<T>(a, b, set, row_best<kChunkThreads>(a, b, sh));
   if (r.greedy) return;
-  const int lo = c * a.chunk, hi = min(a.vocab, lo + a.chunk);
   if (!r.limited) {
-    u64 sum = 0;
-    for_each<T, kChunkThreads>(r.logits, lo, hi, [&](int, float x) { sum += likely_weight(r, key_of(x)); });
-    sum = across<kChunkThreads, false>(sum, sh);
-    if (tid == 0) a.sums[static_cast<int64_t>(b) * a.chunks + c] = sum;
+    for (int c = c0; c < c1; ++c) {
+      u64 sum = 0;
+      for_each<T, kChunkThreads>(r.logits, c * a.chunk, min(a.vocab, (c + 1) * a.chunk),
+                                 [&](int, float x) { if (x >= r.from) sum += likely_weight(r, x); });
+      sum = across<kChunkThreads, false>(sum, sh);
+      if (tid == 0) a.sums[static_cast<int64_t>(b) * a.chunks + c] = sum;
+    }
     return;
   }
   for (int i = tid; i < kBins; i += kChunkThreads) weights[i] = 0, counts[i] = 0;
   __syncthreads();
+  const bool weigh = r.top_p < 1;
   uint32_t far = 0;  // of the last bin, where masked tokens are
   u64 far_weight = 0;
-  for_each<T, kChunkThreads>(r.logits, lo, hi, [&](int, float x) {
-    const double z = exponent_of(r, key_of(x));
+  for_each<T, kChunkThreads>(r.logits, c0 * a.chunk, min(a.vocab, c1 * a.chunk), [&](int, float x) {
+    const double z = exponent_of(r, x);
     const int bin = bin_at(z);
-    const u64 w = weight_at(z);
+    const u64 w = weigh ? weight_at(z) : 0;
     if (bin == kBins - 1) {
       ++far;
       far_weight += w;
     } else {
       atomicAdd(&counts[bin], 1u);
-      if (w > 0) atomicAdd(&weights[bin], w);
+      if (weigh) atomicAdd(&weights[bin], w);
     }
   });
   if (far > 0) {
@@ -529,29 +566,40 @@ struct Bins {
   u64 above_weight, all;
 };
 
-template <int THREADS>
-__device__ Bins bins_of(const SampleArgs& a, const Row& r, int b, u64* sh) {
-  // a thread's share of the bins, in order; the first threads have it
-  constexpr int kShare = kBins / 256;
-  __shared__ u64 found[6];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+// A thread's share of the histogram, in order; the first 256 threads have it.
+constexpr int kShare = kBins / 256;
+struct HistShare {
   uint32_t c[kShare];
-  u64 w[kShare], cs = 0, ws = 0;
+  u64 w[kShare];
+};
+__device__ __forceinline__ HistShare load_hist(const SampleArgs& a, int b) {
+  HistShare h;
+  const int tid = threadIdx.x;
 #pragma unroll
   for (int j = 0; j < kShare; ++j) {
-    c[j] = 0, w[j] = 0;
-    if (tid < 256) {
-      c[j] = a.counts[static_cast<int64_t>(b) * kBins + tid * kShare + j];
-      w[j] = a.weights[static_cast<int64_t>(b) * kBins + tid * kShare + j];
+    h.c[j] = 0, h.w[j] = 0;
+    if (tid < 256 && a.counts != nullptr) {
+      h.c[j] = a.counts[static_cast<int64_t>(b) * kBins + tid * kShare + j];
+      h.w[j] = a.weights[static_cast<int64_t>(b) * kBins + tid * kShare + j];
     }
-    cs += c[j];
-    ws += w[j];
   }
+  return h;
+}
+
+template <int THREADS>
+__device__ Bins bins_of(const HistShare& h, const Row& r, u64* sh) {
+  __shared__ u64 found[4];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const uint32_t(&c)[kShare] = h.c;
+  const u64(&w)[kShare] = h.w;
+  u64 cs = 0, ws = 0;
+#pragma unroll
+  for (int j = 0; j < kShare; ++j) cs += c[j], ws += w[j];
   const u64 all = across<THREADS, false>(ws, sh);
   u64 c_run = wave_scan(cs, lane), w_run = wave_scan(ws, lane);
   __syncthreads();
   if (lane == 63 && wave < 4) sh[wave] = c_run;
-  if (tid < 6) found[tid] = 0;
+  if (tid < 4) found[tid] = 0;
   __syncthreads();
   for (int i = 0; i < wave && i < 4; ++i) c_run += sh[i];
   __syncthreads();
@@ -600,95 +648,162 @@ __device__ Bins bins_of(const SampleArgs& a, const Row& r, int b, u64* sh) {
 template <typename T>
 __global__ __launch_bounds__(kChunkThreads) void chunk_list_kernel(SampleArgs a) {
   __shared__ u64 sh[kChunkThreads / 64];
-  __shared__ u64 list[kList];
+  __shared__ u64 list[kChunkList];
   __shared__ uint32_t listed, at;
-  const int c = blockIdx.x, b = blockIdx.y, tid = threadIdx.x;
-  const Row r = settings_of<T>(a, b, row_best<kChunkThreads>(a, b, sh));
+  const int b = blockIdx.y, tid = threadIdx.x;
+  const int c0 = blockIdx.x * a.group, c1 = min(a.chunks, c0 + a.group);
+  const Settings set = load_settings(a, b);
+  const HistShare hist = load_hist(a, b);
+  const Row r = row_with<T>(a, b, set, row_best<kChunkThreads>(a, b, sh));
   if (!r.limited) return;
-  const Bins bins = bins_of<kChunkThreads>(a, r, b, sh);
+  const Bins bins = bins_of<kChunkThreads>(hist, r, sh);
   if (bins.in > kList) return;  // the row's workgroup does it all
+  // (a logit below is in none of the bins: the others are looked at)
+  const float from = bins.hi == kBins - 1 ? neg_inf() : r.reach((bins.hi + 1) / static_cast<float>(kPerUnit));
   if (tid == 0) listed = 0;
   __syncthreads();
-  const int lo = c * a.chunk, hi = min(a.vocab, lo + a.chunk);
-  u64 sum = 0;
-  for_each<T, kChunkThreads>(r.logits, lo, hi, [&](int i, float x) {
-    const uint32_t key = key_of(x);
-    const double z = exponent_of(r, key);
-    const int bin = bin_at(z);
-    if (bin > bins.hi) return;
-    if (bin >= bins.lo)
-      list[atomicAdd(&listed, 1u)] = rank_of(key, i);
-    else if (z >= r.least)
-      sum += weight_at(z);
-  });
-  sum = across<kChunkThreads, false>(sum, sh);
-  if (tid == 0) {
-    a.sums[static_cast<int64_t>(b) * a.chunks + c] = sum;
-    at = listed > 0 ? atomicAdd(&a.listed[b], listed) : 0;
+  for (int c = c0; c < c1; ++c) {
+    u64 sum = 0;
+    for_each<T, kChunkThreads>(r.logits, c * a.chunk, min(a.vocab, (c + 1) * a.chunk), [&](int i, float x) {
+      if (without_nan(x) < from) return;
+      const double z = exponent_of(r, x);
+      const int bin = bin_at(z);
+      if (bin > bins.hi) return;
+      if (bin < bins.lo) {
+        const u64 w = weight_at(z);
+        sum += w >= r.least ? w : 0;
+        return;
+      }
+      const u64 rank = rank_of(key_of(x), i);
+      const uint32_t slot = atomicAdd(&listed, 1u);
+      if (slot < kChunkList)
+        list[slot] = rank;
+      else
+        a.list[static_cast<int64_t>(b) * kList + atomicAdd(&a.listed[b], 1u)] = rank;
+    });
+    sum = across<kChunkThreads, false>(sum, sh);
+    if (tid == 0) a.sums[static_cast<int64_t>(b) * a.chunks + c] = sum;
   }
   __syncthreads();
-  for (uint32_t i = tid; i < listed; i += kChunkThreads)
-    a.list[static_cast<int64_t>(b) * kList + at + i] = list[i];
+  const uint32_t n = listed < kChunkList ? listed : kChunkList;
+  if (tid == 0) at = n > 0 ? atomicAdd(&a.listed[b], n) : 0;
+  __syncthreads();
+  for (uint32_t i = tid; i < n; i += kChunkThreads) a.list[static_cast<int64_t>(b) * kList + at + i] = list[i];
+}
+
+// border_of for at most kFew tokens (rank, 0 for none, of the first threads): the count
+// and weight above each by comparing all with all, half of them by each of two
+// threads.
+__device__ u64 border_of_few(const Row& r, u64 rank, const Bins& bins, Shared& sh) {
+  __shared__ u64 ranks[kFew], weights[kFew], half_weight[kFew];
+  __shared__ uint32_t half_count[kFew];
+  const int tid = threadIdx.x, of = tid & (kFew - 1), n = static_cast<int>(bins.in);
+  if (tid < kFew) {
+    ranks[tid] = rank;
+    weights[tid] = rank != 0 && r.top_p < 1 ? weight_of(r, key_in(rank)) : 0;
+  }
+  __syncthreads();
+  const u64 own = ranks[of];
+  uint32_t count = 0;
+  u64 weight = 0;
+  const int from = tid < kFew ? 0 : (n + 1) / 2, to = tid < kFew ? (n + 1) / 2 : n;
+#pragma unroll 4
+  for (int j = from; j < to; ++j) {
+    const bool over = ranks[j] > own;
+    count += over;
+    weight += over ? weights[j] : 0;
+  }
+  if (tid >= kFew) {
+    half_count[of] = count;
+    half_weight[of] = weight;
+  }
+  __syncthreads();
+  const bool is = tid < n;
+  u64 above = bins.above, above_weight = bins.above_weight;
+  if (is) {
+    above += count + half_count[of];
+    above_weight += weight + half_weight[of];
+  }
+  bool kept = is && (r.top_k == 0 || above < static_cast<u64>(r.top_k));
+  if (r.top_p < 1) {
+    const u64 all = r.top_k == 0 ? bins.all
+                                 : across<kFinishThreads, true>(kept ? above_weight + weights[of] : 0, sh.sums);
+    // (the first token has nothing before it: it is kept whatever the share)
+    kept = kept && (above == 0 || static_cast<double>(above_weight) < r.top_p * static_cast<double>(all));
+  }
+  return ~across<kFinishThreads, true>(kept ? ~own : 0, sh.sums);
 }
 
 template <typename T>
-__global__ __launch_bounds__(kRowThreads) void sample_finish_kernel(SampleArgs a) {
+__global__ __launch_bounds__(kFinishThreads) void sample_finish_kernel(SampleArgs a) {
   __shared__ Shared sh;
   __shared__ u64 chunk_sums[kMaxChunks];
   const int b = blockIdx.x, tid = threadIdx.x;
-  const u64 best = row_best<kRowThreads>(a, b, sh.sums);
-  const Row r = settings_of<T>(a, b, best);
+  const Settings set = load_settings(a, b);
+  const HistShare hist = load_hist(a, b);
+  const u64 sum = tid < a.chunks ? a.sums[static_cast<int64_t>(b) * a.chunks + tid] : 0;
+  u64 mine[kList / kFinishThreads];  // tokens of the list: how many count is known later
+  const u64* list = a.list + static_cast<int64_t>(b) * kList;
+#pragma unroll
+  for (int j = 0; j < kList / kFinishThreads; ++j)
+    mine[j] = a.counts != nullptr ? list[tid + j * kFinishThreads] : 0;
+  const u64 best = row_best<kFinishThreads>(a, b, sh.sums);
+  const Row r = row_with<T>(a, b, set, best);
   if (r.greedy) {
     if (tid == 0) write_greedy(a, b, best);
     return;
   }
   u64 least = 0;
-  bool summed = true;
   if (r.limited) {
-    const Bins bins = bins_of<kRowThreads>(a, r, b, sh.sums);
-    summed = bins.in <= kList;
-    if (summed) {
-      const u64* list = a.list + static_cast<int64_t>(b) * kList;
+    const Bins bins = bins_of<kFinishThreads>(hist, r, sh.sums);
+    if (bins.in <= kList) {
+#pragma unroll
+      for (int j = 0; j < kList / kFinishThreads; ++j)
+        if (tid + j * kFinishThreads >= bins.in) mine[j] = 0;  // (no token's rank is 0)
       const auto each = [&](auto f) {
-        for (uint32_t i = tid; i < bins.in; i += kRowThreads) f(list[i]);
+#pragma unroll
+        for (int j = 0; j < kList / kFinishThreads; ++j)
+          if (mine[j] != 0) f(mine[j]);
       };
-      least = border_of(r, each, bins.above, bins.above_weight, bins.all, sh);
+      least = bins.in <= kFew ? border_of_few(r, mine[0], bins, sh)
+                              : border_of<kFinishThreads>(r, each, bins.above, bins.above_weight, bins.all, sh);
       __syncthreads();
-      if (tid < a.chunks) chunk_sums[tid] = a.sums[static_cast<int64_t>(b) * a.chunks + tid];
+      if (tid < a.chunks) chunk_sums[tid] = sum;
       __syncthreads();
       each([&](u64 rank) {
-        if (rank >= least) atomicAdd(&chunk_sums[index_in(rank) / a.chunk], likely_weight(r, key_in(rank)));
+        if (rank >= least) atomicAdd(&chunk_sums[index_in(rank) / a.chunk], likely_weight(r, logit_of(key_in(rank))));
       });
     } else {  // more tokens than a list holds: by the row itself
-      least = border_of(r, [&](auto f) {
-        for_each<T, kRowThreads>(r.logits, 0, a.vocab, [&](int i, float x) { f(rank_of(key_of(x), i)); });
+      least = border_of<kFinishThreads>(r, [&](auto f) {
+        for_each<T, kFinishThreads>(r.logits, 0, a.vocab, [&](int i, float x) { f(rank_of(key_of(x), i)); });
       }, 0, 0, bins.all, sh);
       for (int c = 0; c < a.chunks; ++c) {
         u64 sum = 0;
-        for_each<T, kRowThreads>(r.logits, c * a.chunk, min(a.vocab, (c + 1) * a.chunk), [&](int i, float x) {
-          const uint32_t key = key_of(x);
-          if (rank_of(key, i) >= least) sum += likely_weight(r, key);
+        for_each<T, kFinishThreads>(r.logits, c * a.chunk, min(a.vocab, (c + 1) * a.chunk), [&](int i, float x) {
+          if (rank_of(key_of(x), i) >= least) sum += likely_weight(r, x);
         });
-        sum = across<kRowThreads, false>(sum, sh.sums);
+        sum = across<kFinishThreads, false>(sum, sh.sums);
         if (tid == 0) chunk_sums[c] = sum;
       }
     }
   } else if (tid < a.chunks) {
-    chunk_sums[tid] = a.sums[static_cast<int64_t>(b) * a.chunks + tid];
+    chunk_sums[tid] = sum;
   }
   pick_in_chunks<T>(a, r, b, least, chunk_sums, sh);
 }
 
 // Chunks of a row in a call (0: a workgroup has a whole row).
 constexpr int kShortRow = 4096;
-constexpr int kLeastChunk = 2048;
+constexpr int kLeastChunk = 2048, kMostChunk = kFinishThreads * kEach;
 int chunks_of(int64_t batch, int64_t vocab) {
   if (vocab <= kShortRow) return 0;
-  const int64_t most = (vocab + kLeastChunk - 1) / kLeastChunk;  // at most kMaxChunks
-  int64_t want = 8LL * cu_count() / batch;
-  want = want < 1 ? 1 : want;
-  return static_cast<int>(want < most ? want : most);
+  const int64_t least = (vocab + kMostChunk - 1) / kMostChunk;
+  const int64_t most = (vocab + kLeastChunk - 1) / kLeastChunk;
+  const int64_t want = 8LL * cu_count() / batch;
+  return static_cast<int>(want < least ? least : want > most ? most : want);
 }
+static_assert(kShortRow <= kRowThreads * kEach, "a row's workgroup has kEach tokens a thread");
+static_assert(FPV2_MAX_VOCAB <= kMaxChunks * kLeastChunk, "chunks of the longest row");
 
 int64_t align16(int64_t n) { return (n + 15) / 16 * 16; }
 
@@ -707,6 +822,9 @@ int64_t workspace_of(const fpv2_sample_params& p, SampleArgs* a, char* base) {
   };
   a->chunks = static_cast<int>(chunks);
   a->chunk = static_cast<int>((p.vocab + chunks - 1) / chunks);
+  // (a workgroup's start costs the passes as much as half a chunk: four waves a SIMD)
+  const int64_t group = p.batch * chunks / (4 * cu_count());
+  a->group = static_cast<int>(group < 1 ? 1 : group > chunks ? chunks : group);
   a->best = reinterpret_cast<u64*>(take(8 * p.batch * chunks));
   a->sums = reinterpret_cast<u64*>(take(8 * p.batch * chunks));
   if (may_limit(p)) {
@@ -727,9 +845,10 @@ int launch_sample(const SampleArgs& a, int64_t batch, hipStream_t s) {
   }
   const dim3 chunks(static_cast<unsigned>(a.chunks), static_cast<unsigned>(batch));
   hipLaunchKernelGGL(chunk_max_kernel<T>, chunks, threads, 0, s, a);
-  hipLaunchKernelGGL(chunk_weigh_kernel<T>, chunks, threads, 0, s, a);
-  if (a.counts != nullptr) hipLaunchKernelGGL(chunk_list_kernel<T>, chunks, threads, 0, s, a);
-  hipLaunchKernelGGL(sample_finish_kernel<T>, rows, row_threads, 0, s, a);
+  const dim3 groups(static_cast<unsigned>((a.chunks + a.group - 1) / a.group), static_cast<unsigned>(batch));
+  hipLaunchKernelGGL(chunk_weigh_kernel<T>, groups, threads, 0, s, a);
+  if (a.counts != nullptr) hipLaunchKernelGGL(chunk_list_kernel<T>, groups, threads, 0, s, a);
+  hipLaunchKernelGGL(sample_finish_kernel<T>, rows, dim3(kFinishThreads), 0, s, a);
   return check_launch("sample_finish_kernel");
 }
 

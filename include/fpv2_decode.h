@@ -131,7 +131,7 @@ typedef struct fpv2_sample_params {
   const int32_t* top_ks;
   const float* top_ps;
   const float* min_ps;
-  double temperature;       /* 0 or less: the greatest logit                  */
+  double temperature;       /* 0 or less: the greatest logit; at most 1e30     */
   int64_t top_k;            /* 0 or less: no limit                            */
   double top_p;             /* 1 or more: no limit                            */
   double min_p;

@@ -12,13 +12,14 @@
 // bits allow keeps the cancellation of P against 16 X small: float32 outputs
 // are good to 2^-22 or so.)
 //
-// A step is 128 weights of a row, 32 on each quad of lanes, so a dot product over
-// all lanes would mix 128 / group groups.  The A operand keeps them apart: its
-// row m S + j (S = 128 / group) is x[m] with zeros outside the step's group j, so
-// that P comes out per group.  16 / S rows of x make a tile.
+// A step is 128 weights of a row, 32 on each quad of lanes, which is at most a
+// group's.  A product over all lanes would mix the quads' groups, so the quads first
+// exchange words (four swaps of half waves and rows): then word j of a quad is its
+// quarter of group j's 32 weights, and each product has one group.
 //
 // Waves of a workgroup take the steps of the same weight rows in turn and add
-// their sums in LDS at the end.
+// their sums in LDS at the end; the next step's loads are in flight while one is
+// computed.
 #include "fpv2_common.h"
 #include "fpv2_decode.h"
 
@@ -68,19 +69,42 @@ __device__ __forceinline__ u32x4 reorder(u32x4 d) {
   return r;
 }
 
-// S: groups of a step of 128 weights; R: tiles of 16 weight rows and MT: tiles of
-// 16 / S rows of x of a workgroup; W: its waves.
-template <typename T, int S, int R, int MT, int W>
+// out[j] of quad q = in[q] of quad j.
+__device__ __forceinline__ u32x4 exchange(u32x4 v) {
+  const auto a = __builtin_amdgcn_permlane32_swap(v[0], v[2], false, false);
+  const auto b = __builtin_amdgcn_permlane32_swap(v[1], v[3], false, false);
+  const auto c = __builtin_amdgcn_permlane16_swap(a[0], b[0], false, false);
+  const auto d = __builtin_amdgcn_permlane16_swap(a[1], b[1], false, false);
+  return u32x4{c[0], c[1], d[0], d[1]};
+}
+
+// Scales (or biases) of a step's S groups: one load where they are all there and
+// aligned.
+template <int S, bool EVEN>
+__device__ __forceinline__ void load_scales(const uint16_t* p, int g, int groups, uint16_t* out) {
+  if constexpr (EVEN && S == 4) {
+    const u32x2 v = *reinterpret_cast<const u32x2*>(p + g);
+    out[0] = v[0] & 0xffffu, out[1] = v[0] >> 16, out[2] = v[1] & 0xffffu, out[3] = v[1] >> 16;
+  } else if constexpr (EVEN && S == 2) {
+    const uint32_t v = *reinterpret_cast<const uint32_t*>(p + g);
+    out[0] = v & 0xffffu, out[1] = v >> 16;
+  } else {
+#pragma unroll
+    for (int j = 0; j < S; ++j) out[j] = EVEN || g + j < groups ? p[g + j] : 0;
+  }
+}
+
+// S: groups of a step of 128 weights; R: tiles of 16 weight rows, MT: tiles of 16
+// rows of x of a workgroup, of whose rows 4 quad .. + Y - 1 are used; W: its waves.
+// EVEN: the columns are whole steps, the scales aligned.
+template <typename T, int S, int R, int MT, int Y, int W, bool EVEN>
 __global__ __launch_bounds__(64 * W) void q4_linear_kernel(Q4Args a) {
-  constexpr int MP = 16 / S;  // rows of x of a tile
-  constexpr int Y = 4 / S;    // of which in a lane
   __shared__ float sh[W][R * MT * Y][64];
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int col = lane & 15, quad = lane >> 4;
   const int n0 = blockIdx.x * (16 * R);
-  const int m0 = blockIdx.y * (MP * MT);
-  const bool mine = col % S == quad * S / 4;  // the lane's weights are in its row's group
+  const int m0 = blockIdx.y * (16 * MT);
 
   const uint32_t* wp[R];
   const uint16_t* sp[R];
@@ -92,10 +116,10 @@ __global__ __launch_bounds__(64 * W) void q4_linear_kernel(Q4Args a) {
     sp[r] = a.scales + n * a.s_rs;
     bp[r] = a.biases + n * a.s_rs;
   }
-  const uint16_t* xp[MT];
+  const uint16_t* xp[MT];  // (rows past the last give results that are not used)
 #pragma unroll
   for (int t = 0; t < MT; ++t)
-    xp[t] = a.x + static_cast<int64_t>(min(m0 + t * MP + col / S, a.rows - 1)) * a.x_rs;
+    xp[t] = a.x + static_cast<int64_t>(min(m0 + 16 * t + col, a.rows - 1)) * a.x_rs + 8 * quad;
 
   float y[R][MT][Y];
 #pragma unroll
@@ -107,58 +131,78 @@ __global__ __launch_bounds__(64 * W) void q4_linear_kernel(Q4Args a) {
   const u32x4 ones = {Nibbles<T>::kOnes, Nibbles<T>::kOnes, Nibbles<T>::kOnes, Nibbles<T>::kOnes};
   const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
 
-  const int steps = (a.k + 127) / 128;
-  for (int step = wave; step < steps; step += W) {
-    const int k0 = 128 * step + 32 * quad;  // the lane's 32 weights
-    const bool in = k0 < a.k;
-    const int kc = in ? k0 : a.k - 32;
-    u32x4 w[R];
-    float s[R][S], c[R][S];
+  struct Stage {
+    u32x4 w[R], x[MT][4];
+    uint16_t s[R][S], b[R][S];
+  };
+  const auto load = [&](Stage& st, int step) {
+    const int k0 = 128 * step + 32 * quad;
+    const int kc = EVEN || k0 < a.k ? k0 : a.k - 32;
 #pragma unroll
     for (int r = 0; r < R; ++r) {
-      w[r] = load16(wp[r] + kc / 8);
-#pragma unroll
-      for (int j = 0; j < S; ++j) {
-        const int g = step * S + j;
-        s[r][j] = c[r][j] = 0.f;
-        if (g < a.groups) {
-          s[r][j] = Elem<T>::to_float(sp[r][g]);
-          c[r][j] = Elem<T>::to_float(bp[r][g]) - 16.f * s[r][j];
-        }
-      }
+      st.w[r] = load16(wp[r] + kc / 8);
+      load_scales<S, EVEN>(sp[r], step * S, a.groups, st.s[r]);
+      load_scales<S, EVEN>(bp[r], step * S, a.groups, st.b[r]);
     }
-    u32x4 xv[MT][4];
 #pragma unroll
     for (int t = 0; t < MT; ++t)
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        xv[t][j] = u32x4{0, 0, 0, 0};
-        if (mine && in) xv[t][j] = reorder(load16(xp[t] + k0 + 8 * j));
+        const int k = 128 * step + 32 * j;
+        st.x[t][j] = EVEN || k < a.k ? load16(xp[t] + k) : u32x4{0, 0, 0, 0};
       }
-    f32x4 xs[MT];
+  };
+  const auto compute = [&](const Stage& st) {
+    u32x4 xv[MT][4];
+    f32x4 xs[MT][S];
 #pragma unroll
     for (int t = 0; t < MT; ++t) {
-      xs[t] = zero;
 #pragma unroll
-      for (int j = 0; j < 4; ++j)
-        xs[t] = Elem<T>::mfma16(as_vec8<T>(xv[t][j]), as_vec8<T>(ones), xs[t]);
+      for (int g = 0; g < S; ++g) xs[t][g] = zero;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        xv[t][j] = reorder(st.x[t][j]);
+        xs[t][j * S / 4] = Elem<T>::mfma16(as_vec8<T>(xv[t][j]), as_vec8<T>(ones), xs[t][j * S / 4]);
+      }
     }
 #pragma unroll
     for (int r = 0; r < R; ++r) {
+      const u32x4 w = exchange(st.w[r]);
       u32x4 wide[4];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) wide[j] = widen<T>(w[r][j]);
+      for (int j = 0; j < 4; ++j) wide[j] = widen<T>(w[j]);
+      float s[S], c[S];
+#pragma unroll
+      for (int g = 0; g < S; ++g) {
+        s[g] = Elem<T>::to_float(st.s[r][g]);
+        c[g] = Elem<T>::to_float(st.b[r][g]) - 16.f * s[g];
+      }
 #pragma unroll
       for (int t = 0; t < MT; ++t) {
-        f32x4 p = zero;
+        f32x4 p[S];
+#pragma unroll
+        for (int g = 0; g < S; ++g) p[g] = zero;
 #pragma unroll
         for (int j = 0; j < 4; ++j)
-          p = Elem<T>::mfma16(as_vec8<T>(xv[t][j]), as_vec8<T>(wide[j]), p);
-        // row 4 quad + i of the tile: group i % S of x's row (4 quad + i) / S
+          p[j * S / 4] = Elem<T>::mfma16(as_vec8<T>(xv[t][j]), as_vec8<T>(wide[j]), p[j * S / 4]);
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-          y[r][t][i / S] = fmaf(s[r][i % S], p[i], fmaf(c[r][i % S], xs[t][i], y[r][t][i / S]));
+        for (int g = 0; g < S; ++g)
+#pragma unroll
+          for (int i = 0; i < Y; ++i)
+            y[r][t][i] = fmaf(s[g], p[g][i], fmaf(c[g], xs[t][g][i], y[r][t][i]));
       }
+    }
+  };
+  const int steps = (a.k + 127) / 128;
+  if (wave < steps) {
+    Stage st[2];
+    load(st[0], wave);
+    for (int step = wave; step < steps; step += 2 * W) {
+      if (step + W < steps) load(st[1], step + W);
+      compute(st[0]);
+      if (step + W >= steps) break;
+      if (step + 2 * W < steps) load(st[0], step + 2 * W);
+      compute(st[1]);
     }
   }
 #pragma unroll
@@ -174,7 +218,7 @@ __global__ __launch_bounds__(64 * W) void q4_linear_kernel(Q4Args a) {
     for (int w = 0; w < W; ++w) sum += sh[w][e][lane];
     const int i = e % Y, t = e / Y % MT, r = e / (Y * MT);
     const int n = n0 + 16 * r + col;
-    const int m = m0 + t * MP + quad * Y + i;
+    const int m = m0 + 16 * t + 4 * quad + i;
     if (n < a.n && m < a.rows) {
       if (a.out_f32)
         static_cast<float*>(a.out)[m * a.o_rs + n] = sum;
@@ -184,23 +228,26 @@ __global__ __launch_bounds__(64 * W) void q4_linear_kernel(Q4Args a) {
   }
 }
 
-template <typename T, int S, int R, int MT>
+template <typename T, int S, int R, int MT, int Y, int W>
 void launch(const Q4Args& a, hipStream_t s) {
-  constexpr int W = 8;
-  const dim3 grid((a.n + 16 * R - 1) / (16 * R), (a.rows + 16 / S * MT - 1) / (16 / S * MT));
-  hipLaunchKernelGGL((q4_linear_kernel<T, S, R, MT, W>), grid, dim3(64 * W), 0, s, a);
+  const dim3 grid((a.n + 16 * R - 1) / (16 * R), (a.rows + 16 * MT - 1) / (16 * MT));
+  const auto aligned = [](const void* p) { return reinterpret_cast<uintptr_t>(p) % (2 * S) == 0; };
+  if (a.k % 128 == 0 && a.s_rs % S == 0 && aligned(a.scales) && aligned(a.biases))
+    hipLaunchKernelGGL((q4_linear_kernel<T, S, R, MT, Y, W, true>), grid, dim3(64 * W), 0, s, a);
+  else
+    hipLaunchKernelGGL((q4_linear_kernel<T, S, R, MT, Y, W, false>), grid, dim3(64 * W), 0, s, a);
 }
 
 template <typename T, int S>
 void launch_rows(const Q4Args& a, hipStream_t s) {
-  const int tiles = (a.rows + 16 / S - 1) / (16 / S);
-  const bool wide = a.n >= 32 * 2 * cu_count();
-  if (tiles <= 1)
-    wide ? launch<T, S, 2, 1>(a, s) : launch<T, S, 1, 1>(a, s);
-  else if (tiles == 2)
-    wide ? launch<T, S, 2, 2>(a, s) : launch<T, S, 1, 2>(a, s);
+  const bool wide = a.n >= 256 * cu_count();
+  const bool few = a.n <= 16 * cu_count();
+  if (a.rows == 1)
+    wide ? launch<T, S, 2, 1, 1, 4>(a, s) : few ? launch<T, S, 1, 1, 1, 16>(a, s) : launch<T, S, 1, 1, 1, 8>(a, s);
+  else if (a.rows <= 16)
+    wide ? launch<T, S, 2, 1, 4, 4>(a, s) : few ? launch<T, S, 1, 1, 4, 16>(a, s) : launch<T, S, 1, 1, 4, 8>(a, s);
   else
-    wide ? launch<T, S, 2, 4>(a, s) : launch<T, S, 1, 4>(a, s);
+    wide ? launch<T, S, 2, 2, 4, 4>(a, s) : launch<T, S, 1, 2, 4, 8>(a, s);
 }
 
 template <typename T>

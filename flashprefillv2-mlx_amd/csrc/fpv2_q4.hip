@@ -17,9 +17,10 @@
 // exchange words (four swaps of half waves and rows): then word j of a quad is its
 // quarter of group j's 32 weights, and each product has one group.
 //
-// Waves of a workgroup take the steps of the same weight rows in turn and add
-// their sums in LDS at the end; the next step's loads are in flight while one is
-// computed.
+// Waves of a workgroup take pairs of steps of the same weight rows in turn and add
+// their sums in LDS at the end; the next pair's weights are in flight while one is
+// computed.  x lies in LDS, in the order of the operands: loaded from memory by
+// every wave, it kept the address units busier than the weights did.
 #include "fpv2_common.h"
 #include "fpv2_decode.h"
 
@@ -35,6 +36,8 @@ struct Q4Args {
   int rows, n, k, groups;
   int64_t x_rs, p_rs, s_rs, o_rs;
   int out_f32;
+  int wn;     // tiles of weight rows of a workgroup, each its own waves'
+  int panel;  // pairs of steps whose x lies in LDS at a time
 };
 
 template <typename T> struct Nibbles;
@@ -47,15 +50,16 @@ template <> struct Nibbles<f16_t> {
   static constexpr uint32_t kMask = 0x03c003c0u, kBase = 0x4c004c00u, kOnes = 0x3c003c00u;
 };
 
-// (16 + q) of a word's nibbles, in the order 0 4 1 5 2 6 3 7.
+// (16 + q) of a word's nibbles, in the order 0 4 1 5 2 6 3 7; base: kBase, in a vector
+// register, so that masking and joining are one instruction.
 template <typename T>
-__device__ __forceinline__ u32x4 widen(uint32_t w) {
+__device__ __forceinline__ u32x4 widen(uint32_t w, uint32_t base) {
   u32x4 r;
 #pragma unroll
   for (int p = 0; p < 4; ++p) {
     const int shift = 4 * p - Nibbles<T>::kBit;
     const uint32_t v = shift < 0 ? w << -shift : w >> shift;
-    r[p] = (v & Nibbles<T>::kMask) | Nibbles<T>::kBase;
+    r[p] = (v & Nibbles<T>::kMask) | base;
   }
   return r;
 }
@@ -78,176 +82,185 @@ __device__ __forceinline__ u32x4 exchange(u32x4 v) {
   return u32x4{c[0], c[1], d[0], d[1]};
 }
 
-// Scales (or biases) of a step's S groups: one load where they are all there and
-// aligned.
-template <int S, bool EVEN>
+// N scales (or biases) from group g on: one load where they are all there and aligned.
+template <int N, bool EVEN>
 __device__ __forceinline__ void load_scales(const uint16_t* p, int g, int groups, uint16_t* out) {
-  if constexpr (EVEN && S == 4) {
-    const u32x2 v = *reinterpret_cast<const u32x2*>(p + g);
-    out[0] = v[0] & 0xffffu, out[1] = v[0] >> 16, out[2] = v[1] & 0xffffu, out[3] = v[1] >> 16;
-  } else if constexpr (EVEN && S == 2) {
-    const uint32_t v = *reinterpret_cast<const uint32_t*>(p + g);
-    out[0] = v & 0xffffu, out[1] = v >> 16;
+  if constexpr (EVEN) {
+    uint32_t v[N / 2];
+    if constexpr (N == 8) {
+      const u32x4 x = load16(p + g);
+      v[0] = x[0], v[1] = x[1], v[2] = x[2], v[3] = x[3];
+    } else if constexpr (N == 4) {
+      const u32x2 x = *reinterpret_cast<const u32x2*>(p + g);
+      v[0] = x[0], v[1] = x[1];
+    } else {
+      v[0] = *reinterpret_cast<const uint32_t*>(p + g);
+    }
+#pragma unroll
+    for (int j = 0; j < N; ++j) out[j] = j % 2 ? v[j / 2] >> 16 : v[j / 2] & 0xffffu;
   } else {
 #pragma unroll
-    for (int j = 0; j < S; ++j) out[j] = EVEN || g + j < groups ? p[g + j] : 0;
+    for (int j = 0; j < N; ++j) out[j] = g + j < groups ? p[g + j] : 0;
   }
 }
 
-// S: groups of a step of 128 weights; R: tiles of 16 weight rows, MT: tiles of 16
-// rows of x of a workgroup, of whose rows 4 quad .. + Y - 1 are used; W: its waves.
-// EVEN: the columns are whole steps, the scales aligned.
-template <typename T, int S, int R, int MT, int Y, int W, bool EVEN>
+constexpr int W = 8;  // waves of a workgroup
+
+// S: groups of a step of 128 weights; M: rows of x of a workgroup (1, 4 or a number of
+// tiles of 16).  EVEN: the columns are whole pairs of steps, the scales aligned.
+template <typename T, int S, int M, bool EVEN>
 __global__ __launch_bounds__(64 * W) void q4_linear_kernel(Q4Args a) {
-  __shared__ float sh[W][R * MT * Y][64];
+  constexpr int MT = (M + 15) / 16;  // tiles of rows of x,
+  constexpr int MR = M < 16 ? M : 16;  // of so many rows,
+  constexpr int Y = M < 4 ? M : 4;   // of which rows 4 quad .. + Y - 1 in a lane
+  extern __shared__ __attribute__((aligned(16))) char sh[];
+  u32x4* sh_x = reinterpret_cast<u32x4*>(sh);  // [panel * 8][MT][4 quads][MR] of 8 columns
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int col = lane & 15, quad = lane >> 4;
-  const int n0 = blockIdx.x * (16 * R);
-  const int m0 = blockIdx.y * (16 * MT);
+  const int wk = W / a.wn, wave_n = wave / wk, wave_k = wave - wave_n * wk;
+  const int n = (blockIdx.x * a.wn + wave_n) * 16 + col;  // the lane's weight row
+  const int m0 = blockIdx.y * M;
 
-  const uint32_t* wp[R];
-  const uint16_t* sp[R];
-  const uint16_t* bp[R];
-#pragma unroll
-  for (int r = 0; r < R; ++r) {
-    const int64_t n = min(n0 + 16 * r + col, a.n - 1);
-    wp[r] = a.packed + n * a.p_rs;
-    sp[r] = a.scales + n * a.s_rs;
-    bp[r] = a.biases + n * a.s_rs;
-  }
-  const uint16_t* xp[MT];  // (rows past the last give results that are not used)
+  const int64_t row = min(n, a.n - 1);
+  const uint32_t* wp = a.packed + row * a.p_rs;
+  const uint16_t* sp = a.scales + row * a.s_rs;
+  const uint16_t* bp = a.biases + row * a.s_rs;
+  float y[MT][Y];
 #pragma unroll
   for (int t = 0; t < MT; ++t)
-    xp[t] = a.x + static_cast<int64_t>(min(m0 + 16 * t + col, a.rows - 1)) * a.x_rs + 8 * quad;
-
-  float y[R][MT][Y];
 #pragma unroll
-  for (int r = 0; r < R; ++r)
-#pragma unroll
-    for (int t = 0; t < MT; ++t)
-#pragma unroll
-      for (int i = 0; i < Y; ++i) y[r][t][i] = 0.f;
+    for (int i = 0; i < Y; ++i) y[t][i] = 0.f;
   const u32x4 ones = {Nibbles<T>::kOnes, Nibbles<T>::kOnes, Nibbles<T>::kOnes, Nibbles<T>::kOnes};
   const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
+  uint32_t base = Nibbles<T>::kBase;
+  asm("" : "+v"(base));
 
   struct Stage {
-    u32x4 w[R], x[MT][4];
-    uint16_t s[R][S], b[R][S];
+    u32x4 w[2];
+    uint16_t s[2 * S], b[2 * S];
   };
-  const auto load = [&](Stage& st, int step) {
-    const int k0 = 128 * step + 32 * quad;
-    const int kc = EVEN || k0 < a.k ? k0 : a.k - 32;
+  const auto load = [&](Stage& st, int pair) {
 #pragma unroll
-    for (int r = 0; r < R; ++r) {
-      st.w[r] = load16(wp[r] + kc / 8);
-      load_scales<S, EVEN>(sp[r], step * S, a.groups, st.s[r]);
-      load_scales<S, EVEN>(bp[r], step * S, a.groups, st.b[r]);
+    for (int h = 0; h < 2; ++h) {
+      const int k0 = 256 * pair + 128 * h + 32 * quad;
+      st.w[h] = load16(wp + (EVEN || k0 < a.k ? k0 : a.k - 32) / 8);
     }
-#pragma unroll
-    for (int t = 0; t < MT; ++t)
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int k = 128 * step + 32 * j;
-        st.x[t][j] = EVEN || k < a.k ? load16(xp[t] + k) : u32x4{0, 0, 0, 0};
-      }
+    load_scales<2 * S, EVEN>(sp, pair * 2 * S, a.groups, st.s);
+    load_scales<2 * S, EVEN>(bp, pair * 2 * S, a.groups, st.b);
   };
-  const auto compute = [&](const Stage& st) {
-    u32x4 xv[MT][4];
-    f32x4 xs[MT][S];
+  // (rows of x past the last are copies of it, columns past the last zeros)
+  const auto compute = [&](const Stage& st, int at) {  // at: the pair's place in the panel
 #pragma unroll
-    for (int t = 0; t < MT; ++t) {
-#pragma unroll
-      for (int g = 0; g < S; ++g) xs[t][g] = zero;
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        xv[t][j] = reorder(st.x[t][j]);
-        xs[t][j * S / 4] = Elem<T>::mfma16(as_vec8<T>(xv[t][j]), as_vec8<T>(ones), xs[t][j * S / 4]);
-      }
-    }
-#pragma unroll
-    for (int r = 0; r < R; ++r) {
-      const u32x4 w = exchange(st.w[r]);
+    for (int h = 0; h < 2; ++h) {
+      const u32x4 w = exchange(st.w[h]);
       u32x4 wide[4];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) wide[j] = widen<T>(w[j]);
-      float s[S], c[S];
-#pragma unroll
-      for (int g = 0; g < S; ++g) {
-        s[g] = Elem<T>::to_float(st.s[r][g]);
-        c[g] = Elem<T>::to_float(st.b[r][g]) - 16.f * s[g];
-      }
+      for (int j = 0; j < 4; ++j) wide[j] = widen<T>(w[j], base);
 #pragma unroll
       for (int t = 0; t < MT; ++t) {
-        f32x4 p[S];
+        f32x4 xs[S], p[S];
 #pragma unroll
-        for (int g = 0; g < S; ++g) p[g] = zero;
+        for (int g = 0; g < S; ++g) xs[g] = p[g] = zero;
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-          p[j * S / 4] = Elem<T>::mfma16(as_vec8<T>(xv[t][j]), as_vec8<T>(wide[j]), p[j * S / 4]);
+        for (int j = 0; j < 4; ++j) {
+          const u32x4 x = sh_x[(((8 * at + 4 * h + j) * MT + t) * 4 + quad) * MR + min(col, MR - 1)];
+          xs[j * S / 4] = Elem<T>::mfma16(as_vec8<T>(x), as_vec8<T>(ones), xs[j * S / 4]);
+          p[j * S / 4] = Elem<T>::mfma16(as_vec8<T>(x), as_vec8<T>(wide[j]), p[j * S / 4]);
+        }
 #pragma unroll
-        for (int g = 0; g < S; ++g)
+        for (int g = 0; g < S; ++g) {
+          const float s = Elem<T>::to_float(st.s[S * h + g]);
+          const float c = fmaf(-16.f, s, Elem<T>::to_float(st.b[S * h + g]));
 #pragma unroll
-          for (int i = 0; i < Y; ++i)
-            y[r][t][i] = fmaf(s[g], p[g][i], fmaf(c[g], xs[t][g][i], y[r][t][i]));
+          for (int i = 0; i < Y; ++i) y[t][i] = fmaf(s, p[g][i], fmaf(c, xs[g][i], y[t][i]));
+        }
       }
     }
   };
-  const int steps = (a.k + 127) / 128;
-  if (wave < steps) {
-    Stage st[2];
-    load(st[0], wave);
-    for (int step = wave; step < steps; step += 2 * W) {
-      if (step + W < steps) load(st[1], step + W);
-      compute(st[0]);
-      if (step + W >= steps) break;
-      if (step + 2 * W < steps) load(st[0], step + 2 * W);
-      compute(st[1]);
+  const int pairs = (a.k + 255) / 256;
+  Stage st[2];
+  if (wave_k < pairs) load(st[0], wave_k);
+  for (int p0 = 0; p0 < pairs; p0 += a.panel) {
+    const int p1 = min(pairs, p0 + a.panel);
+    if (p0 > 0) __syncthreads();
+    for (int e = tid; e < (p1 - p0) * (32 * M); e += 64 * W) {
+      const int m = e % MR, q = e / MR % 4, t = e / (MR * 4) % MT, block = e / (MR * 4 * MT);
+      const int k = 256 * p0 + 32 * block + 8 * q;
+      u32x4 v = {0, 0, 0, 0};
+      if (EVEN || k < a.k)
+        v = reorder(load16(a.x + static_cast<int64_t>(min(m0 + 16 * t + m, a.rows - 1)) * a.x_rs + k));
+      sh_x[e] = v;
+    }
+    __syncthreads();
+    // the wave's first pair of the panel is in st[0] already
+    for (int pair = p0 + (wave_k - p0 % wk + wk) % wk; pair < p1; pair += 2 * wk) {
+      if (pair + wk < pairs) load(st[1], pair + wk);
+      compute(st[0], pair - p0);
+      if (pair + wk >= p1) {
+        st[0] = st[1];
+        break;
+      }
+      if (pair + 2 * wk < pairs) load(st[0], pair + 2 * wk);
+      compute(st[1], pair + wk - p0);
     }
   }
-#pragma unroll
-  for (int r = 0; r < R; ++r)
-#pragma unroll
-    for (int t = 0; t < MT; ++t)
-#pragma unroll
-      for (int i = 0; i < Y; ++i) sh[wave][(r * MT + t) * Y + i][lane] = y[r][t][i];
   __syncthreads();
-  for (int e = wave; e < R * MT * Y; e += W) {
-    float sum = 0.f;
+  float(*sum)[MT * Y][64] = reinterpret_cast<float(*)[MT * Y][64]>(sh);
 #pragma unroll
-    for (int w = 0; w < W; ++w) sum += sh[w][e][lane];
-    const int i = e % Y, t = e / Y % MT, r = e / (Y * MT);
-    const int n = n0 + 16 * r + col;
-    const int m = m0 + 16 * t + 4 * quad + i;
-    if (n < a.n && m < a.rows) {
+  for (int t = 0; t < MT; ++t)
+#pragma unroll
+    for (int i = 0; i < Y; ++i) sum[wave][t * Y + i][lane] = y[t][i];
+  __syncthreads();
+  for (int e = wave_k; e < MT * Y; e += wk) {
+    float v = 0.f;
+    for (int w = 0; w < wk; ++w) v += sum[wave_n * wk + w][e][lane];
+    const int i = e % Y, t = e / Y, x_row = 4 * quad + i, m = m0 + 16 * t + x_row;
+    if (n < a.n && x_row < MR && m < a.rows) {
       if (a.out_f32)
-        static_cast<float*>(a.out)[m * a.o_rs + n] = sum;
+        static_cast<float*>(a.out)[m * a.o_rs + n] = v;
       else
-        static_cast<uint16_t*>(a.out)[m * a.o_rs + n] = Elem<T>::from_float(sum);
+        static_cast<uint16_t*>(a.out)[m * a.o_rs + n] = Elem<T>::from_float(v);
     }
   }
 }
 
-template <typename T, int S, int R, int MT, int Y, int W>
-void launch(const Q4Args& a, hipStream_t s) {
-  const dim3 grid((a.n + 16 * R - 1) / (16 * R), (a.rows + 16 * MT - 1) / (16 * MT));
-  const auto aligned = [](const void* p) { return reinterpret_cast<uintptr_t>(p) % (2 * S) == 0; };
-  if (a.k % 128 == 0 && a.s_rs % S == 0 && aligned(a.scales) && aligned(a.biases))
-    hipLaunchKernelGGL((q4_linear_kernel<T, S, R, MT, Y, W, true>), grid, dim3(64 * W), 0, s, a);
+constexpr int kPanelBytes = 81920;  // of x in LDS at most: two workgroups fit a CU
+
+template <typename T, int S, int M>
+void launch(Q4Args a, hipStream_t s) {
+  constexpr int kSum = W * ((M + 15) / 16) * (M < 4 ? M : 4) * 256;
+  const int tiles = (a.n + 15) / 16, many = (a.rows + M - 1) / M;
+  // A workgroup reads M rows of x and 16 wn rows of weights, so wn pays in x's
+  // reads and costs in workgroups.  Microseconds for wn = 1 / 2 / 4 / 8: 19456 x 2560
+  // one row 10.4 / 10.3 / 11.5 / 12.9, 12 rows (groups of 32) 23.6 / 19.7 / 17.9 / 19.0, 64 rows
+  // 66.7 / 44.2 / 35.6 / 31.7; 151936 x 2560 one row 61.5 / 48.5 / 46.1 / 51.0, 3 rows 86 / 65 / 56 /
+  // 49.5; 9728 x 2560 4 rows 10.7 / 9.9 / 9.1 / 14.0; 6144 x 2560 one row 5.9 / 6.6 / 8.1 / 12.4, 32
+  // rows 15.9 / 13.2 / 15.3 / 22.0; 2560 x 9728 one row 8.4 / 12.6 / 20.5 / 39.7.
+  const int least = M == 1 ? 8 * cu_count() : M == 16 ? cu_count() : cu_count() / 2;
+  a.wn = 1;
+  while (a.wn < W && tiles / (2 * a.wn) * many >= least) a.wn *= 2;
+  const int pairs = (a.k + 255) / 256, most = kPanelBytes / (512 * M);
+  a.panel = pairs < most ? pairs : most;
+  const int bytes = a.panel * 512 * M > kSum ? a.panel * 512 * M : kSum;
+  const dim3 grid((tiles + a.wn - 1) / a.wn, many);
+  const auto aligned = [](const void* p) { return reinterpret_cast<uintptr_t>(p) % (4 * S) == 0; };
+  if (a.k % 256 == 0 && a.s_rs % (2 * S) == 0 && aligned(a.scales) && aligned(a.biases))
+    hipLaunchKernelGGL((q4_linear_kernel<T, S, M, true>), grid, dim3(64 * W), bytes, s, a);
   else
-    hipLaunchKernelGGL((q4_linear_kernel<T, S, R, MT, Y, W, false>), grid, dim3(64 * W), 0, s, a);
+    hipLaunchKernelGGL((q4_linear_kernel<T, S, M, false>), grid, dim3(64 * W), bytes, s, a);
 }
 
 template <typename T, int S>
 void launch_rows(const Q4Args& a, hipStream_t s) {
-  const bool wide = a.n >= 256 * cu_count();
-  const bool few = a.n <= 16 * cu_count();
   if (a.rows == 1)
-    wide ? launch<T, S, 2, 1, 1, 4>(a, s) : few ? launch<T, S, 1, 1, 1, 16>(a, s) : launch<T, S, 1, 1, 1, 8>(a, s);
+    launch<T, S, 1>(a, s);
+  else if (a.rows <= 4)
+    launch<T, S, 4>(a, s);
   else if (a.rows <= 16)
-    wide ? launch<T, S, 2, 1, 4, 4>(a, s) : few ? launch<T, S, 1, 1, 4, 16>(a, s) : launch<T, S, 1, 1, 4, 8>(a, s);
+    launch<T, S, 16>(a, s);
   else
-    wide ? launch<T, S, 2, 2, 4, 4>(a, s) : launch<T, S, 1, 2, 4, 8>(a, s);
+    launch<T, S, 32>(a, s);
 }
 
 template <typename T>

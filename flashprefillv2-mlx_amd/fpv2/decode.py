@@ -22,6 +22,7 @@ that require a gradient are refused while gradients are recorded.
 from __future__ import annotations
 
 import ctypes
+from functools import lru_cache
 
 import torch
 
@@ -31,22 +32,29 @@ from fpv2.kernel import SUPPORTED_HEAD_DIMS
 _HALF = (torch.float16, torch.bfloat16)
 
 
-def _on_device(device: torch.device, call) -> None:
-    """``call(stream)`` with ``device`` current."""
-    stream = _lib.stream_ptr(device)
-    if device.index == torch.cuda.current_device():
-        call(stream)
-    else:
-        with torch.cuda.device(device):
-            call(stream)
-
-
-def _no_grad_needed(*tensors: torch.Tensor) -> None:
+def _device(tensors) -> int:
+    """The index of the one ROCm device that all tensors are on; raises where there is
+    none, or where a gradient would be lost.  (These calls take microseconds on
+    the device, so the checks are made in few steps.)"""
     if torch.is_grad_enabled():
         for t in tensors:
             if t.requires_grad:
                 raise RuntimeError("the decode operators have no backward: call them under "
                                    "torch.no_grad() or detach their inputs")
+    index = tensors[0].get_device()
+    for t in tensors:
+        if t.get_device() != index or index < 0:
+            _lib.require_device(*tensors)
+    return index
+
+
+def _on_device(index: int, call) -> None:
+    """``call(stream)`` with device ``index`` current and its current stream."""
+    if index == torch._C._cuda_getDevice():
+        call(torch._C._cuda_getCurrentRawStream(index))
+    else:
+        with torch.cuda.device(index):
+            call(torch._C._cuda_getCurrentRawStream(index))
 
 
 def _count(value, name: str, least: int = 0) -> int:
@@ -55,22 +63,54 @@ def _count(value, name: str, least: int = 0) -> int:
     return value
 
 
-def _row_aligned(t: torch.Tensor) -> bool:
-    """16-byte aligned rows: what the kernels read in place."""
-    return (t.stride(-1) == 1 and t.data_ptr() % 16 == 0
-            and all(s % 8 == 0 for s, n in zip(t.stride()[:-1], t.shape) if n > 1))
+def _row_strides(t: torch.Tensor):
+    """The strides of all dimensions but the last (any multiple of 8 where a
+    dimension has one entry), or ``None`` where the rows are not contiguous and
+    16-byte aligned: what the kernels read in place."""
+    if t.data_ptr() & 15:
+        return None
+    *strides, last = t.stride()
+    if last != 1 and t.shape[-1] > 1:
+        return None
+    union = 0
+    for s in strides:
+        union |= s
+    if union & 7:
+        strides = [s if n > 1 else 0 for s, n in zip(strides, t.shape)]
+        if any(s & 7 for s in strides):
+            return None
+    return strides
 
 
-def _pages(k_pages: torch.Tensor, v_pages: torch.Tensor) -> None:
-    for name, t in (("k_pages", k_pages), ("v_pages", v_pages)):
-        if t.ndim != 4:
-            raise ValueError(f"{name} must have shape [pages, KV heads, page size, head dim]")
-    if k_pages.shape != v_pages.shape:
+def _pages(k_pages: torch.Tensor, v_pages: torch.Tensor):
+    """The caches' shape and strides."""
+    if k_pages.ndim != 4 or v_pages.ndim != 4:
+        name = "v_pages" if k_pages.ndim == 4 else "k_pages"
+        raise ValueError(f"{name} must have shape [pages, KV heads, page size, head dim]")
+    shape = k_pages.shape
+    if shape != v_pages.shape:
         raise ValueError("k_pages and v_pages must have the same shape")
     if k_pages.dtype not in _HALF or v_pages.dtype != k_pages.dtype:
         raise ValueError("the caches must share float16 or bfloat16 dtype")
-    if k_pages.shape[0] == 0 or k_pages.shape[2] == 0:
+    if shape[0] == 0 or shape[2] == 0:
         raise ValueError("the caches must hold at least one row")
+    return shape
+
+
+def _page_strides(k_pages: torch.Tensor, v_pages: torch.Tensor):
+    k, v = _row_strides(k_pages), _row_strides(v_pages)
+    if k is None or v is None:
+        raise ValueError("the caches' rows must be contiguous and 16-byte aligned")
+    return *k, *v
+
+
+@lru_cache(maxsize=256)
+def _decode_plan(index: int, *fields):
+    """A call's parameters and the bytes of workspace that it needs on device
+    ``index`` (the current one)."""
+    params = _lib.DecodeParams(*fields)
+    need = _lib.load().fpv2_decode_attention_workspace_bytes(ctypes.byref(params))
+    return ctypes.byref(params), need
 
 
 def decode_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
@@ -95,72 +135,71 @@ def decode_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tens
     """
     if q.ndim != 3:
         raise ValueError("q must have shape [batch, query heads, head dim]")
-    _pages(k_pages, v_pages)
-    batch, heads, dim = q.shape
-    pages, kv_heads, page_size, _ = k_pages.shape
+    pages, kv_heads, page_size, page_dim = _pages(k_pages, v_pages)
+    shape, dtype = q.shape, q.dtype
+    batch, heads, dim = shape
     if kv_heads == 0 or heads == 0 or heads % kv_heads:
         raise ValueError("query heads must be divisible by KV heads")
-    if dim not in SUPPORTED_HEAD_DIMS or k_pages.shape[3] != dim:
+    if dim not in SUPPORTED_HEAD_DIMS or page_dim != dim:
         raise ValueError(f"head dimension must be one of {SUPPORTED_HEAD_DIMS}, the caches' too")
-    if q.dtype != k_pages.dtype:
+    if dtype != k_pages.dtype:
         raise ValueError("q and the caches must share float16 or bfloat16 dtype")
-    if not _row_aligned(k_pages) or not _row_aligned(v_pages):
-        raise ValueError("the caches' rows must be contiguous and 16-byte aligned")
+    page_strides = _page_strides(k_pages, v_pages)
     tensors = [q, k_pages, v_pages]
+    width, table_stride, table_ptr = 1, 0, None
     if page_table is not None:
         if page_table.ndim != 2 or page_table.shape[0] != batch or page_table.dtype != torch.int32:
             raise ValueError("page_table must be int32 [batch, pages of a sequence]")
-        if page_table.shape[1] == 0 or page_table.stride(1) != 1 and page_table.shape[1] > 1:
+        width = page_table.shape[1]
+        table_stride, last = page_table.stride()
+        if width == 0 or last != 1 and width > 1:
             raise ValueError("page_table must have contiguous rows of at least one page")
+        table_ptr = page_table.data_ptr()
         tensors.append(page_table)
     elif pages < batch:
         raise ValueError("without a page_table every sequence needs a page")
-    uniform = 0
+    uniform, lengths_ptr = 0, None
     if isinstance(lengths, torch.Tensor):
         if lengths.shape != (batch,) or lengths.dtype != torch.int32 or not lengths.is_contiguous():
             raise ValueError("lengths must be contiguous int32 [batch], or an integer")
+        lengths_ptr = lengths.data_ptr()
         tensors.append(lengths)
     else:
-        uniform, lengths = _count(lengths, "lengths"), None
+        uniform = _count(lengths, "lengths")
     window = 0 if window_tokens is None else _count(window_tokens, "window_tokens", 1)
     _count(sink_tokens, "sink_tokens")
-    if out is None:
-        out = torch.empty((batch, heads, dim), dtype=q.dtype, device=q.device)
-    elif out.shape != q.shape or out.dtype != q.dtype or dim > 1 and out.stride(2) != 1:
-        raise ValueError("out must be [batch, query heads, head dim] of q's dtype with a "
-                         "contiguous last dimension")
-    else:
+    if out is not None:
+        if out.shape != shape or out.dtype != dtype or out.stride(2) != 1:
+            raise ValueError("out must be [batch, query heads, head dim] of q's dtype with a "
+                             "contiguous last dimension")
         tensors.append(out)
-    _no_grad_needed(*tensors)
-    device = _lib.require_device(*tensors)
-    if not _row_aligned(q):
+    index = _device(tensors)
+    if out is None:
+        out = torch.empty(shape, dtype=dtype, device=q.device)
+    q_strides = _row_strides(q)
+    if q_strides is None:
         q = q.clone(memory_format=torch.contiguous_format)
+        q_strides = _row_strides(q)
     if batch == 0:
         return out
     lib = _lib.load()
-    p = _lib.DecodeParams(
-        batch, heads, kv_heads, dim, pages, page_size,
-        1 if page_table is None else page_table.shape[1],
-        0 if page_table is None else page_table.stride(0), uniform, window, sink_tokens,
-        dim ** -0.5 if scale is None else scale, *_strides(q), *_strides(k_pages),
-        *_strides(v_pages), out.stride(0), out.stride(1))
 
     def call(stream):
-        need = lib.fpv2_decode_attention_workspace_bytes(ctypes.byref(p))
-        work = torch.empty(need, dtype=torch.uint8, device=device) if need > 0 else None
+        params, need = _decode_plan(
+            index, batch, heads, kv_heads, dim, pages, page_size, width, table_stride,
+            uniform, window, sink_tokens, dim ** -0.5 if scale is None else scale, *q_strides,
+            *page_strides, out.stride(0), out.stride(1))
+        work = torch.empty(need, dtype=torch.uint8, device=out.device) if need > 0 else None
         _lib.check(lib.fpv2_decode_attention(
-            q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), _lib.ptr(page_table),
-            _lib.ptr(lengths), out.data_ptr(), _lib.dtype_code(q.dtype), ctypes.byref(p),
-            _lib.ptr(work), max(need, 0), stream), "decode_attention")
+            q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), table_ptr, lengths_ptr,
+            out.data_ptr(), _lib.dtype_code(dtype), params, _lib.ptr(work), max(need, 0), stream),
+            "decode_attention")
 
-    _on_device(device, call)
+    _on_device(index, call)
     return out
 
 
-def _strides(t: torch.Tensor):
-    """Strides of all dimensions but the last; 0 where a dimension has one entry
-    (torch leaves any value there)."""
-    return [s if n > 1 else 0 for s, n in zip(t.stride()[:-1], t.shape)]
+_rope_params = lru_cache(maxsize=256)(lambda *fields: _lib.RopePagesParams(*fields))
 
 
 def _index(value, name: str, tokens: int):
@@ -197,9 +236,8 @@ def rope_to_pages(qkv: torch.Tensor, q_weight: torch.Tensor | None, k_weight: to
     """
     if qkv.ndim != 2 or qkv.dtype not in _HALF:
         raise ValueError("qkv must be [tokens, heads * head dim] in float16 or bfloat16")
-    _pages(k_pages, v_pages)
+    pages, kv_heads, page_size, dim = _pages(k_pages, v_pages)
     tokens = qkv.shape[0]
-    pages, kv_heads, page_size, dim = k_pages.shape
     _count(query_heads, "query_heads", 1)
     if k_pages.dtype != qkv.dtype:
         raise ValueError("qkv and the caches must share a dtype")
@@ -207,11 +245,10 @@ def rope_to_pages(qkv: torch.Tensor, q_weight: torch.Tensor | None, k_weight: to
         raise ValueError("head dimension must be a multiple of 16 and at most 512")
     if kv_heads == 0 or qkv.shape[1] != (query_heads + 2 * kv_heads) * dim:
         raise ValueError("qkv rows must hold the query, key and value heads")
-    if not _row_aligned(k_pages) or not _row_aligned(v_pages):
-        raise ValueError("the caches' rows must be contiguous and 16-byte aligned")
+    page_strides = _page_strides(k_pages, v_pages)
     for name, t in (("q_weight", q_weight), ("k_weight", k_weight)):
-        if t is not None and (t.shape != (dim,) or t.dtype != qkv.dtype or not t.is_contiguous()
-                              or t.data_ptr() % 16):
+        if t is not None and (t.shape != (dim,) or t.dtype != qkv.dtype or t.data_ptr() & 15
+                              or not t.is_contiguous()):
             raise ValueError(f"{name} must be contiguous [head dim] of qkv's dtype, 16-byte aligned")
     for name, t in (("cos", cos), ("sin", sin)):
         if (t.ndim != 2 or t.shape != cos.shape or t.dtype != torch.float32
@@ -223,24 +260,26 @@ def rope_to_pages(qkv: torch.Tensor, q_weight: torch.Tensor | None, k_weight: to
                          "head dimension")
     positions, position_bytes, first_position = _index(positions, "positions", tokens)
     slots, slot_bytes, first_slot = _index(slots, "slots", tokens)
-    if out is None:
-        out = torch.empty((tokens, query_heads, dim), dtype=qkv.dtype, device=qkv.device)
-    elif out.shape != (tokens, query_heads, dim) or out.dtype != qkv.dtype or not _row_aligned(out):
+    tensors = [qkv, k_pages, v_pages, cos, sin]
+    tensors += [t for t in (q_weight, k_weight, positions, slots, out) if t is not None]
+    if out is not None and (out.shape != (tokens, query_heads, dim) or out.dtype != qkv.dtype
+                            or _row_strides(out) is None):
         raise ValueError("out must be [tokens, query heads, head dim] of qkv's dtype with 16-byte "
                          "aligned rows")
-    tensors = [t for t in (qkv, k_pages, v_pages, q_weight, k_weight, cos, sin, positions, slots, out)
-               if t is not None]
-    _no_grad_needed(*tensors)
-    device = _lib.require_device(*tensors)
-    if not _row_aligned(qkv):
+    index = _device(tensors)
+    if out is None:
+        out = torch.empty((tokens, query_heads, dim), dtype=qkv.dtype, device=qkv.device)
+    qkv_strides = _row_strides(qkv)
+    if qkv_strides is None:
         qkv = qkv.clone(memory_format=torch.contiguous_format)
+        qkv_strides = _row_strides(qkv)
     if tokens == 0:
         return out
     lib = _lib.load()
-    p = _lib.RopePagesParams(
+    p = (_rope_params if position_bytes and slot_bytes else _lib.RopePagesParams)(
         tokens, query_heads, kv_heads, dim, half, cos.shape[0], bool(interleaved), pages, page_size,
-        position_bytes, slot_bytes, first_position, first_slot, *_strides(qkv), *_strides(out),
-        *_strides(k_pages), *_strides(v_pages), eps)
+        position_bytes, slot_bytes, first_position, first_slot, *qkv_strides, *_row_strides(out),
+        *page_strides, eps)
 
     def call(stream):
         _lib.check(lib.fpv2_rope_to_pages(
@@ -249,7 +288,7 @@ def rope_to_pages(qkv: torch.Tensor, q_weight: torch.Tensor | None, k_weight: to
             v_pages.data_ptr(), _lib.dtype_code(qkv.dtype), ctypes.byref(p), stream),
             "rope_to_pages")
 
-    _on_device(device, call)
+    _on_device(index, call)
     return out
 
 
@@ -338,32 +377,34 @@ def quantized_linear(x: torch.Tensor, packed: torch.Tensor, scales: torch.Tensor
             raise ValueError(f"{name} must have contiguous rows, both with one row stride")
     rows = x if x.ndim == 2 else x.reshape(-1, k)
     m = rows.shape[0]
-    if out is None:
-        result = torch.empty((*x.shape[:-1], n), dtype=kind, device=x.device)
-        flat, stride = result, n
-    else:
+    tensors = [x, packed, scales, biases]
+    out_stride = n
+    if out is not None:
         if (x.ndim != 2 or out.shape != (m, n) or out.dtype != kind
                 or n > 1 and out.stride(1) != 1 or m > 1 and out.stride(0) < n):
             raise ValueError("out must be [rows, out] of out_dtype with contiguous rows, x [rows, in]")
-        result = flat = out
-        stride = out.stride(0) if m > 1 else n
-    _no_grad_needed(x, packed, scales, biases, result)
-    device = _lib.require_device(x, packed, scales, biases, result)
-    if not _row_aligned(rows) or m > 1 and rows.stride(0) < k:
+        out_stride = out.stride(0) if m > 1 else n
+        tensors.append(out)
+    index = _device(tensors)
+    if out is None:
+        out = torch.empty((*x.shape[:-1], n), dtype=kind, device=x.device)
+    strides = _row_strides(rows)
+    if strides is None or m > 1 and strides[0] < k:
         rows = rows.clone(memory_format=torch.contiguous_format)
+        strides = _row_strides(rows)
     if m == 0 or n == 0:
-        return result
+        return out
     lib = _lib.load()
 
     def call(stream):
         _lib.check(lib.fpv2_quantized_linear(
             rows.data_ptr(), packed.data_ptr(), scales.data_ptr(), biases.data_ptr(),
-            flat.data_ptr(), _lib.dtype_code(x.dtype), _lib.dtype_code(kind), m, n, k, group,
-            rows.stride(0) if m > 1 else k, packed.stride(0) if n > 1 else k // 8,
-            scales.stride(0) if n > 1 else k // group, stride, stream), "quantized_linear")
+            out.data_ptr(), _lib.dtype_code(x.dtype), _lib.dtype_code(kind), m, n, k, group,
+            strides[0] if m > 1 else k, packed.stride(0) if n > 1 else k // 8,
+            scales.stride(0) if n > 1 else k // group, out_stride, stream), "quantized_linear")
 
-    _on_device(device, call)
-    return result
+    _on_device(index, call)
+    return out
 
 
 MAX_VOCAB = 1 << 19  # FPV2_MAX_VOCAB
@@ -417,9 +458,9 @@ def sample_tokens(logits: torch.Tensor, uniform: torch.Tensor, *,
     k_rows, k = _setting(top_k, "top_k", batch, torch.int32, 0, inf)
     p_rows, p = _setting(top_p, "top_p", batch, torch.float32, 0, 1)
     m_rows, m = _setting(min_p, "min_p", batch, torch.float32, 0, 1)
-    rows = [x for x in (t_rows, k_rows, p_rows, m_rows) if x is not None]
-    _no_grad_needed(logits, uniform, *rows)
-    device = _lib.require_device(logits, uniform, *rows)
+    index = _device([logits, uniform, *(x for x in (t_rows, k_rows, p_rows, m_rows)
+                                        if x is not None)])
+    device = logits.device
     if vocab > 1 and logits.stride(1) != 1:
         logits = logits.contiguous()
     tokens = torch.empty(batch, dtype=torch.int64, device=device)
@@ -438,5 +479,5 @@ def sample_tokens(logits: torch.Tensor, uniform: torch.Tensor, *,
                 ctypes.byref(params), tokens.data_ptr(), _lib.ptr(logprobs), _lib.ptr(work),
                 max(need, 0), stream), "sample_tokens")
 
-        _on_device(device, call)
+        _on_device(index, call)
     return (tokens, logprobs) if return_logprobs else tokens

@@ -22,8 +22,12 @@
 namespace fpv2 {
 namespace {
 
-constexpr int kBlockKeys = 128;  // keys of a block: 32 for each of the 4 waves
-constexpr int kWaveKeys = 32;
+// Keys of a wave's tile, and of a block: a tile for each of the 4 waves.  KT: MFMA
+// tiles of 16 keys.
+template <int D> constexpr int kKt = D > 128 ? 1 : 2;
+constexpr int wave_keys(int64_t dim) { return 16 * (dim == 64 ? kKt<64> : dim == 96 ? kKt<96> : dim == 128 ? kKt<128> : kKt<256>); }
+constexpr int block_keys(int64_t dim) { return 4 * wave_keys(dim); }
+constexpr int kMaxGrid = 4096;   // workgroups of a call
 constexpr int kMaxHeads = 16;  // query heads of an item (columns of an MFMA tile)
 
 struct DecodeArgs {
@@ -38,6 +42,7 @@ struct DecodeArgs {
   int64_t q_bs, q_hs, k_ps, k_hs, k_rs, v_ps, v_hs, v_rs, o_bs, o_hs, table_stride;
   int batch, kv_heads, group, item_heads, head_items;  // head_items * item_heads >= group
   int pages, page_size, capacity, length, window, sinks, grid;
+  int block_keys;
   uint32_t page_mul, page_shift;  // t / page_size = (umulhi(t, mul) + t) >> shift
   float scale_log2;
 };
@@ -57,7 +62,7 @@ __device__ __forceinline__ Sequence sequence_of(const DecodeArgs& a, int b) {
   const int start = max(s.sinks, len - a.window);
   s.skip = start - s.sinks;
   s.n = len - s.skip;
-  s.blocks = max(1, (s.n + kBlockKeys - 1) / kBlockKeys);  // (an empty one writes its zeros)
+  s.blocks = max(1, (s.n + a.block_keys - 1) / a.block_keys);  // (an empty one writes its zeros)
   return s;
 }
 
@@ -76,6 +81,18 @@ __device__ __forceinline__ int wave_total(const DecodeArgs& a, int lane, int end
   }
   *before = some;
   return all;
+}
+
+// The first block of a workgroup's run (runs differ by a block at most), and the
+// workgroup that has a block.  Where there are fewer blocks than workgroups, each
+// of the first ones has one: an item's workgroups are neighbours.
+__device__ __forceinline__ int first_of(const DecodeArgs& a, uint32_t w, int total) {
+  const uint32_t grid = min(a.grid, total);
+  return static_cast<int>(static_cast<uint64_t>(min(w, grid)) * static_cast<uint32_t>(total) / grid);
+}
+__device__ __forceinline__ int workgroup_of(const DecodeArgs& a, int block, int total) {
+  const uint32_t grid = min(a.grid, total);
+  return static_cast<int>((static_cast<uint64_t>(block + 1) * grid - 1) / static_cast<uint32_t>(total));
 }
 
 template <int NW>
@@ -102,12 +119,35 @@ __device__ __forceinline__ Words<NW> load_words(const uint16_t* p) {
   return r;
 }
 
+// O^T += V^T P^T over a lane's 8 keys (of 32) or 4 (of 16), in 16-bit pairs.
+template <typename T>
+__device__ __forceinline__ f32x4 product(u32x4 v, u32x4 p, f32x4 o) {
+  return Elem<T>::mfma16(as_vec8<T>(v), as_vec8<T>(p), o);
+}
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
+template <typename T>
+__device__ __forceinline__ f32x4 product(u32x2 v, u32x2 p, f32x4 o) {
+  if constexpr (std::is_same<T, bf16_t>::value)
+    return __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(__builtin_bit_cast(s16x4, v), __builtin_bit_cast(s16x4, p),
+                                                     o, 0, 0, 0);
+  else
+    return __builtin_amdgcn_mfma_f32_16x16x16f16(__builtin_bit_cast(f16x4, v), __builtin_bit_cast(f16x4, p), o,
+                                                 0, 0, 0);
+}
+
 template <typename T, int D>
 __global__ __launch_bounds__(256, 2) void decode_attn_kernel(DecodeArgs a) {
+  constexpr int KT = kKt<D>, kWaveKeys = 16 * KT, kBlockKeys = 4 * kWaveKeys;
+  constexpr int NK = 4 * KT;  // keys of a lane
+  typedef uint32_t Pairs __attribute__((ext_vector_type(NK / 2)));
   constexpr int KK = D / 32;  // MFMA steps of a key's dot product
   constexpr int DV = D / 16;  // dims of a lane
   __shared__ float sh_o[4][kMaxHeads][D + 4];
   __shared__ float sh_ml[4][kMaxHeads][2];
+  // (at head dim 256 the queries would not fit the registers beside K, V and O)
+  constexpr bool kLdsQ = D > 128;
+  __shared__ u32x4 sh_q[kLdsQ ? 64 * KK : 1];
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int col = lane & 15, quad = lane >> 4;
@@ -116,8 +156,7 @@ __global__ __launch_bounds__(256, 2) void decode_attn_kernel(DecodeArgs a) {
   int before;
   const int per_item = wave_total(a, lane, 0, &before);
   const int total = per_item * items;
-  const int per = (total + a.grid - 1) / a.grid;
-  const int lo = min(total, static_cast<int>(blockIdx.x) * per), hi = min(total, lo + per);
+  const int lo = first_of(a, blockIdx.x, total), hi = first_of(a, blockIdx.x + 1, total);
   if (lo >= hi) return;
 
   // the sequence that holds block lo: base is its first block
@@ -153,11 +192,16 @@ __global__ __launch_bounds__(256, 2) void decode_attn_kernel(DecodeArgs a) {
     const int heads = min(a.item_heads, a.group - h0);
     const int head = kvh * a.group + h0 + col;
 
-    u32x4 qf[KK];
+    u32x4 qf[kLdsQ ? 1 : KK];
+    const auto load_q = [&](int kk) {
+      return col < heads ? load16(a.q + b * a.q_bs + head * a.q_hs + 32 * kk + 8 * quad) : u32x4{0, 0, 0, 0};
+    };
+    if constexpr (kLdsQ) {
+      for (int kk = wave; kk < KK; kk += 4) sh_q[64 * kk + lane] = load_q(kk);
+      __syncthreads();
+    } else {
 #pragma unroll
-    for (int kk = 0; kk < KK; ++kk) {
-      qf[kk] = u32x4{0, 0, 0, 0};
-      if (col < heads) qf[kk] = load16(a.q + b * a.q_bs + head * a.q_hs + 32 * kk + 8 * quad);
+      for (int kk = 0; kk < KK; ++kk) qf[kk] = load_q(kk);
     }
     f32x4 o[DV];
 #pragma unroll
@@ -167,9 +211,9 @@ __global__ __launch_bounds__(256, 2) void decode_attn_kernel(DecodeArgs a) {
     const uint16_t* kb = a.k + kvh * a.k_hs;
     const uint16_t* vb = a.v + kvh * a.v_hs;
     const int32_t* table = a.table != nullptr ? a.table + b * a.table_stride : nullptr;
-    // lane i (and i + 32) looks up the row of the tile's key i
+    // lane i (modulo the tile) looks up the row of the tile's key i
     auto lookup = [&](int u0, int* row) {
-      const int u = min(u0 + (lane & 31), s.n - 1);
+      const int u = min(u0 + (lane & (kWaveKeys - 1)), s.n - 1);
       const uint32_t t = u < s.sinks ? u : u + s.skip;
       const uint32_t page = (__umulhi(t, a.page_mul) + t) >> a.page_shift;
       *row = t - page * a.page_size;
@@ -183,31 +227,39 @@ __global__ __launch_bounds__(256, 2) void decode_attn_kernel(DecodeArgs a) {
     for (; u0 < u_end; u0 += kBlockKeys) {
       const int64_t koff = page * a.k_ps + row * a.k_rs;
       const int64_t voff = page * a.v_ps + row * a.v_rs;
-      u32x4 kf[2][KK];
+      u32x4 kf[KT][KK];
 #pragma unroll
-      for (int t = 0; t < 2; ++t) {
+      for (int t = 0; t < KT; ++t) {
         const uint16_t* p = kb + __shfl(koff, 16 * t + col, 64) + 8 * quad;
 #pragma unroll
         for (int kk = 0; kk < KK; ++kk) kf[t][kk] = load16(p + 32 * kk);
       }
-      Words<DV / 2> vf[8];
+      // (at head dim 256 half of V waits for K's registers)
+      constexpr int kEarly = D > 128 ? NK / 2 : NK;
+      Words<DV / 2> vf[NK];
+      const auto load_v = [&](int j) {
+        return load_words<DV / 2>(vb + __shfl(voff, 16 * (j / 4) + 4 * quad + j % 4, 64) + DV * col);
+      };
 #pragma unroll
-      for (int j = 0; j < 8; ++j)
-        vf[j] = load_words<DV / 2>(vb + __shfl(voff, 16 * (j / 4) + 4 * quad + j % 4, 64) + DV * col);
+      for (int j = 0; j < kEarly; ++j) vf[j] = load_v(j);
       if (u0 + kBlockKeys < u_end) page = lookup(u0 + kBlockKeys, &row);
 
-      f32x4 sc[2];
+      int q_at = lane;
+      if constexpr (kLdsQ) asm volatile("" : "+v"(q_at));  // (read again for each tile)
+      f32x4 sc[KT];
 #pragma unroll
-      for (int t = 0; t < 2; ++t) {
+      for (int t = 0; t < KT; ++t) {
         sc[t] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int kk = 0; kk < KK; ++kk)
-          sc[t] = Elem<T>::mfma16(as_vec8<T>(kf[t][kk]), as_vec8<T>(qf[kk]), sc[t]);
+          sc[t] = Elem<T>::mfma16(as_vec8<T>(kf[t][kk]), as_vec8<T>(kLdsQ ? sh_q[64 * kk + q_at] : qf[kLdsQ ? 0 : kk]), sc[t]);
       }
-      const bool cut = u0 + kWaveKeys > s.n;
-      float x[8], top = neg_inf();
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
+      for (int j = kEarly; j < NK; ++j) vf[j] = load_v(j);
+      const bool cut = u0 + kWaveKeys > s.n;
+      float x[NK], top = neg_inf();
+#pragma unroll
+      for (int j = 0; j < NK; ++j) {
         x[j] = sc[j / 4][j % 4] * a.scale_log2;
         if (cut && u0 + 16 * (j / 4) + 4 * quad + j % 4 >= s.n) {
           x[j] = neg_inf();
@@ -225,23 +277,23 @@ __global__ __launch_bounds__(256, 2) void decode_attn_kernel(DecodeArgs a) {
       const float fix = __builtin_amdgcn_exp2f(m - ref);
       m = m_new;
       l *= fix;
-      u32x4 pf;
+      Pairs pf;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) x[j] = __builtin_amdgcn_exp2f(x[j] - ref);
+      for (int j = 0; j < NK; ++j) x[j] = __builtin_amdgcn_exp2f(x[j] - ref);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
+      for (int j = 0; j < NK / 2; ++j) {
         pf[j] = pack2<T>(x[2 * j], x[2 * j + 1]);
         l += x[2 * j] + x[2 * j + 1];
       }
 #pragma unroll
       for (int d = 0; d < DV; ++d) {
         o[d] *= fix;
-        u32x4 vt;  // dim d of the lane's 8 keys
+        Pairs vt;  // dim d of the lane's keys
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
+        for (int j = 0; j < NK / 2; ++j)
           vt[j] = __builtin_amdgcn_perm(vf[2 * j + 1].w[d / 2], vf[2 * j].w[d / 2],
                                         d % 2 ? 0x07060302u : 0x05040100u);
-        o[d] = Elem<T>::mfma16(as_vec8<T>(vt), as_vec8<T>(pf), o[d]);
+        o[d] = product<T>(vt, pf, o[d]);
       }
     }
     l += __shfl_xor(l, 16, 64);
@@ -252,10 +304,12 @@ __global__ __launch_bounds__(256, 2) void decode_attn_kernel(DecodeArgs a) {
       sh_ml[wave][col][0] = m;
       sh_ml[wave][col][1] = l;
     }
+    if (col < heads) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
+      for (int i = 0; i < 4; ++i)
 #pragma unroll
-      for (int d = 0; d < DV; ++d) sh_o[wave][col][(4 * quad + i) * DV + d] = o[d][i];
+        for (int d = 0; d < DV; ++d) sh_o[wave][col][(4 * quad + i) * DV + d] = o[d][i];
+    }
     __syncthreads();
     const bool whole = first == 0 && last == s.blocks;
     const int64_t slot = 2 * static_cast<int64_t>(blockIdx.x) + (cur == lo ? 0 : 1);
@@ -294,11 +348,14 @@ __global__ __launch_bounds__(256, 2) void decode_attn_kernel(DecodeArgs a) {
 }
 
 // Joins the partials of an item that several workgroups shared: one workgroup
-// per (item, query head), the partials dealt to its waves in order.
+// per (item, query head).  First the weights of all partials, then their sum, 16
+// bytes of a partial a thread.
 template <typename T, int D>
 __global__ __launch_bounds__(256) void decode_join_kernel(DecodeArgs a) {
-  __shared__ float sh_o[4][D];
-  __shared__ float sh_ml[4][2];
+  constexpr int kLanes = D / 4, kSlots = 256 / kLanes;  // partials at a time
+  __shared__ float sh_f[kMaxGrid];
+  __shared__ float sh_r[4];
+  __shared__ f32x4 sh_o[kSlots][kLanes];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int items = a.kv_heads * a.head_items;
   const int h = blockIdx.x % a.item_heads;
@@ -308,50 +365,52 @@ __global__ __launch_bounds__(256) void decode_join_kernel(DecodeArgs a) {
   if (h0 + h >= a.group) return;
   int before;
   const int total = wave_total(a, lane, b, &before) * items;
-  const int per = (total + a.grid - 1) / a.grid;
   const Sequence s = sequence_of(a, b);
   const int start = before * items + item * s.blocks;
-  const int w0 = start / per, w1 = (start + s.blocks - 1) / per;
-  if (w0 == w1) return;  // written by its workgroup
-  constexpr int E = (D + 63) / 64;
-  float m = neg_inf(), l = 0.f, o[E];
-#pragma unroll
-  for (int e = 0; e < E; ++e) o[e] = 0.f;
-  for (int w = w0 + wave; w <= w1; w += 4) {
-    const int64_t slot = 2 * static_cast<int64_t>(w) + (start > w * per ? 1 : 0);
-    const float* po = a.part_o + (slot * a.item_heads + h) * D;
-    const float pm = a.part_ml[(slot * a.item_heads + h) * 2];
-    const float pl = a.part_ml[(slot * a.item_heads + h) * 2 + 1];
-    const float m_new = fmaxf(m, pm);
-    const float ref = m_new == neg_inf() ? 0.f : m_new;
-    const float f0 = __builtin_amdgcn_exp2f(m - ref), f1 = __builtin_amdgcn_exp2f(pm - ref);
-    m = m_new;
-    l = l * f0 + pl * f1;
-#pragma unroll
-    for (int e = 0; e < E; ++e)
-      if (64 * e + lane < D) o[e] = o[e] * f0 + po[64 * e + lane] * f1;
+  const int w0 = workgroup_of(a, start, total), n = workgroup_of(a, start + s.blocks - 1, total) - w0 + 1;
+  if (n == 1) return;  // written by its workgroup
+  // a workgroup's first item is in its slot 0, its last in slot 1
+  const int in_last = start > first_of(a, w0, total) ? 1 : 0;
+  const auto slot_of = [&](int i) { return 2 * static_cast<int64_t>(w0 + i) + (i == 0 ? in_last : 0); };
+  float top = neg_inf();
+  for (int i = tid; i < n; i += 256) {
+    const float m = a.part_ml[(slot_of(i) * a.item_heads + h) * 2];
+    sh_f[i] = m;
+    top = fmaxf(top, m);
   }
 #pragma unroll
-  for (int e = 0; e < E; ++e)
-    if (64 * e + lane < D) sh_o[wave][64 * e + lane] = o[e];
-  if (lane == 0) {
-    sh_ml[wave][0] = m;
-    sh_ml[wave][1] = l;
+  for (int off = 32; off >= 1; off >>= 1) top = fmaxf(top, __shfl_xor(top, off, 64));
+  if (lane == 0) sh_r[wave] = top;
+  __syncthreads();
+  top = fmaxf(fmaxf(sh_r[0], sh_r[1]), fmaxf(sh_r[2], sh_r[3]));
+  const float ref = top == neg_inf() ? 0.f : top;
+  __syncthreads();
+  float den = 0.f;
+  for (int i = tid; i < n; i += 256) {
+    const float f = __builtin_amdgcn_exp2f(sh_f[i] - ref);
+    sh_f[i] = f;
+    den += f * a.part_ml[(slot_of(i) * a.item_heads + h) * 2 + 1];
+  }
+#pragma unroll
+  for (int off = 32; off >= 1; off >>= 1) den += __shfl_xor(den, off, 64);
+  if (lane == 0) sh_r[wave] = den;
+  __syncthreads();
+  den = (sh_r[0] + sh_r[1]) + (sh_r[2] + sh_r[3]);
+  f32x4 o = {0.f, 0.f, 0.f, 0.f};
+  const int g = tid / kLanes, e = tid % kLanes;
+  if (g < kSlots) {
+#pragma unroll 8
+    for (int i = g; i < n; i += kSlots)
+      o += sh_f[i] * *reinterpret_cast<const f32x4*>(a.part_o + (slot_of(i) * a.item_heads + h) * D + 4 * e);
+    sh_o[g][e] = o;
   }
   __syncthreads();
-  for (int d = tid; d < D; d += 256) {
-    float top = neg_inf();
+  if (tid < kLanes) {
 #pragma unroll
-    for (int w = 0; w < 4; ++w) top = fmaxf(top, sh_ml[w][0]);
-    const float ref = top == neg_inf() ? 0.f : top;
-    float sum = 0.f, den = 0.f;
+    for (int i = 1; i < kSlots; ++i) o += sh_o[i][tid];
+    uint16_t* out = a.out + b * a.o_bs + (kvh * a.group + h0 + h) * a.o_hs + 4 * tid;
 #pragma unroll
-    for (int w = 0; w < 4; ++w) {
-      const float f = __builtin_amdgcn_exp2f(sh_ml[w][0] - ref);
-      sum += f * sh_o[w][d];
-      den += f * sh_ml[w][1];
-    }
-    a.out[b * a.o_bs + (kvh * a.group + h0 + h) * a.o_hs + d] = Elem<T>::from_float(sum / den);
+    for (int j = 0; j < 4; ++j) out[j] = Elem<T>::from_float(o[j] / den);
   }
 }
 
@@ -369,11 +428,11 @@ DecodePlan decode_plan(const fpv2_decode_params& p) {
   int64_t keys = p.table_width * p.page_size;
   if (p.window_tokens > 0 && p.window_tokens + p.sink_tokens < keys)
     keys = p.window_tokens + p.sink_tokens;
-  plan.most_blocks = (keys + kBlockKeys - 1) / kBlockKeys;
+  plan.most_blocks = (keys + block_keys(p.head_dim) - 1) / block_keys(p.head_dim);
   if (plan.most_blocks < 1) plan.most_blocks = 1;
   const int64_t blocks = p.batch * p.kv_heads * plan.head_items * plan.most_blocks;
-  const int64_t resident = 2 * static_cast<int64_t>(cu_count());
-  plan.grid = static_cast<int>(blocks < resident ? blocks : resident);
+  const int64_t most = 2 * static_cast<int64_t>(cu_count());
+  plan.grid = static_cast<int>(blocks < most ? blocks : most < kMaxGrid ? most : kMaxGrid);
   return plan;
 }
 
@@ -395,7 +454,7 @@ int check_params(const char* name, const fpv2_decode_params* p) {
   const int64_t group = p->query_heads / p->kv_heads;
   const int64_t items = p->batch * p->kv_heads * ((group + kMaxHeads - 1) / kMaxHeads);
   if (items * kMaxHeads > 0x7fffffff ||
-      items * ((p->table_width * p->page_size + kBlockKeys - 1) / kBlockKeys) > 0x3fffffff)
+      items * ((p->table_width * p->page_size + 63) / 64) > 0x3fffffff)
     return fail(FPV2_ERR_UNSUPPORTED, "%s: the call has too many blocks of keys", name);
   return FPV2_OK;
 }
@@ -490,6 +549,7 @@ extern "C" int fpv2_decode_attention(const void* q, const void* k_pages, const v
   a.group = static_cast<int>(p.query_heads / p.kv_heads);
   a.head_items = plan.head_items;
   a.item_heads = plan.item_heads;
+  a.block_keys = block_keys(p.head_dim);
   a.pages = static_cast<int>(p.pages);
   a.page_size = static_cast<int>(p.page_size);
   a.capacity = static_cast<int>(p.table_width * p.page_size);

@@ -37,6 +37,10 @@ hook's accounting rule leaves such calls out (``patch.py:255-266``).  These
 counts are the layer's own: the calls do not enter the hook's
 ``fpv2.block_sparsity()``.
 
+``decode`` attends one new token at a time against the same cache
+(``fpv2.decode_attention``), and ``pages`` hands the cache to the other operators
+of a decode step.
+
 Every call runs on the current stream.  As with a module's buffers, the KV
 and pooled caches are not synchronised across streams: a caller that moves
 between streams orders the calls itself (``wait_stream``).
@@ -49,6 +53,7 @@ from dataclasses import replace
 import torch
 
 from fpv2 import _lib
+from fpv2.decode import decode_attention
 from fpv2.kernel import SUPPORTED_HEAD_DIMS, _launch_attention
 from fpv2.patch import (SelectedBlockCounter, _causal_block_count, _effective_config, _geometry,
                         _pool_into, _request_config, _select_attend)
@@ -318,6 +323,41 @@ class ChunkedPrefill:
         if keep is not None:
             keep.update(config=config, offset=geo.offset, pooled_k=pooled_k, pooled_v=pooled_v,
                         lists=(ids, counts, ids, pruned_counts))
+
+    def pages(self) -> tuple[torch.Tensor, torch.Tensor]:
+        """The cache as one page ``[1, Hkv, capacity, D]`` of keys and one of values,
+        as the decode operators take it (a token's slot is its position)."""
+        return self.k[None], self.v[None]
+
+    def decode(self, q: torch.Tensor, k: torch.Tensor | None = None,
+               v: torch.Tensor | None = None, *, scale: float | None = None,
+               out: torch.Tensor | None = None) -> torch.Tensor:
+        """Attend one new token ``q`` (``[Hq, 1, D]`` or ``[1, Hq, 1, D]``) against the
+        whole cache, exactly, after appending its ``k``/``v`` ``[Hkv, 1, D]`` where they
+        are given (not where ``reserve(1)`` made room for them already); returns
+        ``[1, Hq, 1, D]``.
+
+        The reference leaves single tokens to the original attention
+        (``fpv2/patch.py:177-205``: fewer queries than a tile).  ``out``: optional
+        ``[Hq, 1, D]`` destination.  The new rows are pooled when a later ``attend``
+        or ``step`` needs them."""
+        q3 = self._three_d(q, "q")
+        if q3.shape != (self.query_heads, 1, self.head_dim) or q3.dtype != self.dtype:
+            raise ValueError("q must be [query_heads, 1, head_dim] of the cache's geometry and dtype")
+        if (k is None) != (v is None):
+            raise ValueError("k and v are given together")
+        if out is not None and (out.shape != q3.shape or out.dtype != self.dtype):
+            raise ValueError("out must be [query_heads, 1, head_dim] of q's dtype")
+        if k is not None:
+            k, v = self._rows(k, v)
+            if k.shape[1] != 1:
+                raise ValueError("decode takes one token's keys and values")
+            self.append(k, v)
+        if self.length == 0:
+            raise ValueError("query length cannot exceed key length for causal attention")
+        res = decode_attention(q3.transpose(0, 1), *self.pages(), None, self.length, scale=scale,
+                               out=None if out is None else out.transpose(0, 1))
+        return res.transpose(0, 1)[None]
 
     def step(self, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, **kwargs) -> torch.Tensor:
         """Append the chunk's K/V, then attend its queries."""

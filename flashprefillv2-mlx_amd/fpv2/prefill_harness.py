@@ -18,6 +18,12 @@ layers are plain 2-D GEMMs (``torch.nn.functional.linear``); the residual add
 + RMSNorm, the per-head Q/K RMSNorm + RoPE and the SwiGLU gate are fused HIP
 kernels of the same library (``include/fpv2_decoder.h``), computing in float32
 and storing bf16.
+
+``ChunkedPrefillRunner.decode`` goes on token by token over the prefill's caches
+and ``generate`` samples the tokens (``fpv2.decode``; the reference leaves both to
+mlx-lm, ``fpv2/generate.py:97-130``).  With ``RandomDecoder.quantize`` the decode
+steps read 4-bit weights, as the reference's MLX models do, and the prefill, which
+is bound by arithmetic, the dense weights of the same values.
 """
 
 from __future__ import annotations
@@ -31,6 +37,8 @@ import torch.nn.functional as F
 
 from fpv2 import _lib
 from fpv2.chunked import ChunkedPrefill
+from fpv2.decode import (decode_attention, dequantize_weight, quantize_weight, quantized_linear,
+                         rope_to_pages, sample_tokens)
 from fpv2.selection import FPV2Config
 
 
@@ -192,6 +200,23 @@ class RandomDecoder:
                 "down": w(s.hidden, s.intermediate),
             })
         self.final_norm = torch.ones(s.hidden, device=self.device, dtype=dtype)
+        self.packed: list[dict] | None = None  # 4-bit projections of each layer
+        self.packed_embed: tuple | None = None
+
+    def quantize(self, group_size: int = 64) -> None:
+        """Cut the projections and the tied head to 4 bits (``quantize_weight``).
+
+        Decode steps then read the packed weights; the dense ones, which the
+        prefill's products read, become the packed weights' values rounded to
+        the model's dtype."""
+        def cut(w):
+            packed = quantize_weight(w, group_size=group_size)
+            w.copy_(dequantize_weight(*packed))
+            return packed
+
+        self.packed = [{name: cut(layer[name]) for name in ("qkv", "o", "gate_up", "down")}
+                       for layer in self.layers]
+        self.packed_embed = cut(self.embed)
 
     def parameters(self) -> int:
         n = self.embed.numel() + self.final_norm.numel()
@@ -263,6 +288,7 @@ class ChunkedPrefillRunner:
                               last_n_blocks=base.last_n_blocks,
                               mean_correction=base.mean_correction)
         self.model, self.capacity, self.attention = model, capacity, attention
+        self._tables: tuple | None = None  # cos / sin of the cache's positions
         self.capture_layer: int | None = None
         self.captured: dict | None = None
         if attention == "sdpa":
@@ -343,13 +369,85 @@ class ChunkedPrefillRunner:
             x, delta = m.embed[tokens[start:end]], None
             for li in range(m.shape.layers):
                 x, delta = self._layer(li, x, delta, cos, sin)
-        last = _add_rms_norm(x[-1:], delta[-1:], m.final_norm, m.shape.rms_eps)
+        return self._head(x[-1:], delta[-1:])
+
+    def _head(self, x: torch.Tensor, delta: torch.Tensor) -> torch.Tensor:
+        """float32 logits ``[vocab]`` of one position's residual stream ``x + delta``."""
+        m = self.model
+        last = _add_rms_norm(x, delta, m.final_norm, m.shape.rms_eps)
         w = m.embed
         if (w.stride(1) != 1 or w.stride(0) % 8 or w.stride(0) < w.shape[1] or w.data_ptr() % 16
                 or (w.requires_grad and torch.is_grad_enabled())):
             # (rows that the kernel does not read in place, or a graph to keep)
             return F.linear(last, w).float()[0]
         return _row_logits(last[0], w)
+
+    def decode(self, token: torch.Tensor) -> torch.Tensor:
+        """Append one token (an integer tensor of one element on the model's device)
+        to the prefilled sequence; returns the logits of its position (float32
+        ``[vocab]``).  Exact attention over the whole cache in both modes; reads the
+        4-bit weights of a quantized model."""
+        m, s = self.model, self.model.shape
+        if self.attention == "sdpa":
+            raise ValueError("decode goes on over the caches of 'fpv2' or 'dense'")
+        if token.numel() != 1 or token.is_floating_point():
+            raise ValueError("token must be an integer tensor of one element")
+        position = self.caches[0].length
+        if position == 0:
+            raise ValueError("decode needs a prefilled prompt")
+        if position >= self.capacity:
+            raise ValueError("the KV cache capacity is exceeded")
+        if self._tables is None:
+            pos = torch.arange(self.capacity, device=m.device)
+            half = s.head_dim // 2
+            self._tables = tuple(t[:, :half].contiguous() for t in rope_tables(s, pos))
+
+        def linear(x, li, name):
+            if m.packed is None:
+                return F.linear(x, m.layers[li][name])
+            return quantized_linear(x, *m.packed[li][name])
+
+        x, delta = m.embed[token.reshape(1)], None
+        for li, (p, cache) in enumerate(zip(m.layers, self.caches)):
+            h = _add_rms_norm(x, delta, p["attn_norm"], s.rms_eps)
+            k_pages, v_pages = cache.pages()
+            cache.reserve(1)
+            q = rope_to_pages(linear(h, li, "qkv"), p["q_norm"], p["k_norm"], *self._tables,
+                              position, position, k_pages, v_pages, query_heads=s.query_heads,
+                              eps=s.rms_eps)
+            attn = decode_attention(q, k_pages, v_pages, None, cache.length)
+            h = _add_rms_norm(x, linear(attn.view(1, -1), li, "o"), p["mlp_norm"], s.rms_eps)
+            delta = linear(_silu_mul(linear(h, li, "gate_up"), s.intermediate), li, "down")
+        if m.packed_embed is None:
+            return self._head(x, delta)
+        last = _add_rms_norm(x, delta, m.final_norm, s.rms_eps)
+        return quantized_linear(last, *m.packed_embed, out_dtype=torch.float32)[0]
+
+    def generate(self, tokens: torch.Tensor, chunk: int, new_tokens: int, *,
+                 temperature: float = 1.0, top_k: int = 0, top_p: float = 1.0,
+                 min_p: float = 0.0, uniform: torch.Tensor | None = None) -> torch.Tensor:
+        """Prefill the prompt in ``chunk``-token pieces, then sample ``new_tokens``
+        tokens (``sample_tokens``'s settings); returns them as int64 ``[new_tokens]``.
+        ``uniform``: the float32 random numbers ``[new_tokens]`` of the tokens (by
+        default from torch's generator of the model's device)."""
+        if isinstance(new_tokens, bool) or not isinstance(new_tokens, int) or new_tokens <= 0:
+            raise ValueError("new_tokens must be a positive integer")
+        if any(cache.length for cache in self.caches):
+            raise ValueError("generate starts from empty caches: call reset() first")
+        if tokens.numel() + new_tokens - 1 > self.capacity:
+            raise ValueError("prompt and new tokens exceed the KV cache capacity")
+        if uniform is None:
+            uniform = torch.rand(new_tokens, device=self.model.device)
+        elif uniform.shape != (new_tokens,):
+            raise ValueError("uniform must be float32 [new_tokens]")
+        logits = self.prefill(tokens, chunk)
+        out = []
+        for i in range(new_tokens):
+            if i > 0:
+                logits = self.decode(out[-1])
+            out.append(sample_tokens(logits[None], uniform[i:i + 1], temperature=temperature,
+                                     top_k=top_k, top_p=top_p, min_p=min_p))
+        return torch.cat(out)
 
 
 def measure(shape: DecoderShape, *, tokens: int, chunk: int, alpha: float, device,

@@ -186,31 +186,37 @@ __device__ __forceinline__ u64 likely_weight(const Row& r, float x) {
   return w >= r.least ? w : 0;
 }
 
-__device__ __forceinline__ u64 shfl_xor64(u64 v, int off) {
-  return static_cast<u64>(__shfl_xor(static_cast<long long>(v), off, 64));
+// Sum (or greatest) of a value over a wave's lanes up to this one, by DPP: shifts
+// within rows of 16 lanes, then the rows' last lanes to the rows after them.
+// (Through shuffles the six dependent steps take three times as long.)
+template <int CTRL, int ROWS>
+__device__ __forceinline__ u64 from_lanes(u64 v) {  // 0 where there is no such lane
+  const uint32_t lo = __builtin_amdgcn_update_dpp(0, static_cast<int>(v), CTRL, ROWS, 0xf, false);
+  const uint32_t hi = __builtin_amdgcn_update_dpp(0, static_cast<int>(v >> 32), CTRL, ROWS, 0xf, false);
+  return (static_cast<u64>(hi) << 32) | lo;
 }
-__device__ __forceinline__ u64 shfl64(u64 v, int lane) {
-  return static_cast<u64>(__shfl(static_cast<long long>(v), lane, 64));
-}
-// Sum over a wave's lanes up to this one.
-__device__ __forceinline__ u64 wave_scan(u64 v, int lane) {
-#pragma unroll
-  for (int off = 1; off < 64; off <<= 1) {
-    const u64 up = static_cast<u64>(__shfl_up(static_cast<long long>(v), off, 64));
-    v += lane >= off ? up : 0;
-  }
+template <bool MAX = false>
+__device__ __forceinline__ u64 wave_scan(u64 v) {
+  const auto with = [&](u64 o) { v = MAX ? (o > v ? o : v) : v + o; };
+  with(from_lanes<0x111, 0xf>(v));  // row_shr 1, 2, 4, 8
+  with(from_lanes<0x112, 0xf>(v));
+  with(from_lanes<0x114, 0xf>(v));
+  with(from_lanes<0x118, 0xf>(v));
+  with(from_lanes<0x142, 0xa>(v));  // row_bcast 15, to the odd rows
+  with(from_lanes<0x143, 0xc>(v));  // row_bcast 31, to the upper half
   return v;
+}
+__device__ __forceinline__ u64 last_lane(u64 v) {
+  const uint32_t lo = __builtin_amdgcn_readlane(static_cast<int>(v), 63);
+  const uint32_t hi = __builtin_amdgcn_readlane(static_cast<int>(v >> 32), 63);
+  return (static_cast<u64>(hi) << 32) | lo;
 }
 // Sum (or greatest) of a value of each of the workgroup's threads, in every thread.
 template <int THREADS, bool MAX>
 __device__ __forceinline__ u64 across(u64 v, u64* sh) {
-#pragma unroll
-  for (int off = 32; off >= 1; off >>= 1) {
-    const u64 o = shfl_xor64(v, off);
-    v = MAX ? (o > v ? o : v) : v + o;
-  }
+  v = wave_scan<MAX>(v);
   __syncthreads();
-  if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = v;
+  if ((threadIdx.x & 63) == 63) sh[threadIdx.x >> 6] = v;
   __syncthreads();
   v = sh[0];
 #pragma unroll
@@ -271,7 +277,7 @@ __device__ int find_first(int lo, int hi, u64 before, Value value, Past past, Sh
     v[j] = from + j < to ? value(from + j) : 0;
     sum += v[j];
   }
-  const u64 upto = wave_scan(sum, lane);
+  const u64 upto = wave_scan(sum);
   __syncthreads();
   if (lane == 63) sh.sums[wave] = upto;
   if (tid == 0) sh.at = hi;
@@ -331,7 +337,7 @@ __device__ u64 least_rank(const Row& r, Each each, u64 count, u64 weight, Past p
         c[j] = cs += sh.counts[bin];
         w[j] = ws += sh.weights[bin];
       }
-      const u64 c0 = count + wave_scan(cs, lane) - cs, w0 = weight + wave_scan(ws, lane) - ws;
+      const u64 c0 = count + wave_scan(cs) - cs, w0 = weight + wave_scan(ws) - ws;
       int mine = -1;
 #pragma unroll
       for (int j = 3; j >= 0; --j) {
@@ -427,7 +433,7 @@ __device__ void pick_in_chunks(const SampleArgs& a, const Row& r, int b, u64 lea
     u64 c[4], sum = 0;
 #pragma unroll
     for (int j = 0; j < 4; ++j) c[j] = sum += 4 * lane + j < a.chunks ? chunk_sums[4 * lane + j] : 0;
-    const u64 before = wave_scan(sum, lane) - sum;
+    const u64 before = wave_scan(sum) - sum;
     int at = -1;
 #pragma unroll
     for (int j = 3; j >= 0; --j)
@@ -586,8 +592,7 @@ __device__ __forceinline__ HistShare load_hist(const SampleArgs& a, int b) {
   return h;
 }
 
-template <int THREADS>
-__device__ Bins bins_of(const HistShare& h, const Row& r, u64* sh) {
+__device__ Bins bins_of(const HistShare& h, const Row& r) {
   __shared__ u64 found[4];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const uint32_t(&c)[kShare] = h.c;
@@ -595,17 +600,18 @@ __device__ Bins bins_of(const HistShare& h, const Row& r, u64* sh) {
   u64 cs = 0, ws = 0;
 #pragma unroll
   for (int j = 0; j < kShare; ++j) cs += c[j], ws += w[j];
-  const u64 all = across<THREADS, false>(ws, sh);
-  u64 c_run = wave_scan(cs, lane), w_run = wave_scan(ws, lane);
-  __syncthreads();
-  if (lane == 63 && wave < 4) sh[wave] = c_run;
+  u64 c_run = wave_scan(cs), w_run = wave_scan(ws);
+  __shared__ u64 waves[2][4];
+  if (lane == 63 && wave < 4) waves[0][wave] = c_run, waves[1][wave] = w_run;
   if (tid < 4) found[tid] = 0;
   __syncthreads();
-  for (int i = 0; i < wave && i < 4; ++i) c_run += sh[i];
-  __syncthreads();
-  if (lane == 63 && wave < 4) sh[wave] = w_run;
-  __syncthreads();
-  for (int i = 0; i < wave && i < 4; ++i) w_run += sh[i];
+  u64 all = 0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    c_run += i < wave ? waves[0][i] : 0;
+    w_run += i < wave ? waves[1][i] : 0;
+    all += waves[1][i];
+  }
   c_run -= cs;
   w_run -= ws;
   // top_k alone or with top_p: the bin of token top_k; top_p alone: the share's
@@ -656,7 +662,7 @@ __global__ __launch_bounds__(kChunkThreads) void chunk_list_kernel(SampleArgs a)
   const HistShare hist = load_hist(a, b);
   const Row r = row_with<T>(a, b, set, row_best<kChunkThreads>(a, b, sh));
   if (!r.limited) return;
-  const Bins bins = bins_of<kChunkThreads>(hist, r, sh);
+  const Bins bins = bins_of(hist, r);
   if (bins.in > kList) return;  // the row's workgroup does it all
   // (a logit below is in none of the bins: the others are looked at)
   const float from = bins.hi == kBins - 1 ? neg_inf() : r.reach((bins.hi + 1) / static_cast<float>(kPerUnit));
@@ -755,7 +761,7 @@ __global__ __launch_bounds__(kFinishThreads) void sample_finish_kernel(SampleArg
   }
   u64 least = 0;
   if (r.limited) {
-    const Bins bins = bins_of<kFinishThreads>(hist, r, sh.sums);
+    const Bins bins = bins_of(hist, r);
     if (bins.in <= kList) {
 #pragma unroll
       for (int j = 0; j < kList / kFinishThreads; ++j)

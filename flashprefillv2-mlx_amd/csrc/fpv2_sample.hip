@@ -297,7 +297,7 @@ __device__ int find_first(int lo, int hi, u64 before, Value value, Past past, Sh
   return sh.at;
 }
 
-// Of a group of tokens (each(f) calls f(rank) for all of them) the greatest rank from
+// Of a group of tokens (each(f) calls f(rank, weight()) for all of them) the greatest rank from
 // which on past(count, weight) holds, given the count and weight of the tokens
 // above the group; 0 where it never does.  *weight: weight of the tokens from there on.
 // Histograms over the rank's bits, 8 at a time from the first that differ, until one
@@ -307,7 +307,7 @@ __device__ u64 least_rank(const Row& r, Each each, u64 count, u64 weight, Past p
                           u64* weight_from, Shared& sh) {
   const int tid = threadIdx.x, lane = tid & 63;
   u64 low = ~0ull, high = 0;
-  each([&](u64 rank) {
+  each([&](u64 rank, auto) {
     low = rank < low ? rank : low;
     high = rank > high ? rank : high;
   });
@@ -321,11 +321,11 @@ __device__ u64 least_rank(const Row& r, Each each, u64 count, u64 weight, Past p
     __syncthreads();
     if (tid < 256) sh.weights[tid] = 0, sh.counts[tid] = 0;
     __syncthreads();
-    each([&](u64 rank) {
+    each([&](u64 rank, auto of) {
       if ((rank >> (shift + width)) != prefix) return;
       const int bin = static_cast<int>(rank >> shift) & ((1 << width) - 1);
       atomicAdd(&sh.counts[bin], 1u);
-      if (weigh) atomicAdd(&sh.weights[bin], weight_of(r, key_in(rank)));
+      if (weigh) atomicAdd(&sh.weights[bin], of());
     });
     __syncthreads();
     if (tid < 64) {
@@ -474,7 +474,9 @@ __global__ __launch_bounds__(kRowThreads) void sample_row_kernel(SampleArgs a) {
       all = across<kRowThreads, false>(all, sh.sums);
     }
     least = border_of<kRowThreads>(r, [&](auto f) {
-      for_each<T, kRowThreads>(r.logits, 0, a.vocab, [&](int i, float x) { f(rank_of(key_of(x), i)); });
+      for_each<T, kRowThreads>(r.logits, 0, a.vocab, [&](int i, float x) {
+        f(rank_of(key_of(x), i), [&] { return weight_at(exponent_of(r, x)); });
+      });
     }, 0, 0, all, sh);
   }
   u64 all = 0;
@@ -700,13 +702,13 @@ __global__ __launch_bounds__(kChunkThreads) void chunk_list_kernel(SampleArgs a)
 // border_of for at most kFew tokens (rank, 0 for none, of the first threads): the count
 // and weight above each by comparing all with all, half of them by each of two
 // threads.
-__device__ u64 border_of_few(const Row& r, u64 rank, const Bins& bins, Shared& sh) {
+__device__ u64 border_of_few(const Row& r, u64 rank, u64 own_weight, const Bins& bins, Shared& sh) {
   __shared__ u64 ranks[kFew], weights[kFew], half_weight[kFew];
   __shared__ uint32_t half_count[kFew];
   const int tid = threadIdx.x, of = tid & (kFew - 1), n = static_cast<int>(bins.in);
   if (tid < kFew) {
     ranks[tid] = rank;
-    weights[tid] = rank != 0 && r.top_p < 1 ? weight_of(r, key_in(rank)) : 0;
+    weights[tid] = own_weight;
   }
   __syncthreads();
   const u64 own = ranks[of];
@@ -766,22 +768,29 @@ __global__ __launch_bounds__(kFinishThreads) void sample_finish_kernel(SampleArg
 #pragma unroll
       for (int j = 0; j < kList / kFinishThreads; ++j)
         if (tid + j * kFinishThreads >= bins.in) mine[j] = 0;  // (no token's rank is 0)
+      u64 weight[kList / kFinishThreads];
+#pragma unroll
+      for (int j = 0; j < kList / kFinishThreads; ++j)
+        weight[j] = mine[j] != 0 ? weight_of(r, key_in(mine[j])) : 0;
       const auto each = [&](auto f) {
 #pragma unroll
         for (int j = 0; j < kList / kFinishThreads; ++j)
-          if (mine[j] != 0) f(mine[j]);
+          if (mine[j] != 0) f(mine[j], [&] { return weight[j]; });
       };
-      least = bins.in <= kFew ? border_of_few(r, mine[0], bins, sh)
+      least = bins.in <= kFew ? border_of_few(r, mine[0], weight[0], bins, sh)
                               : border_of<kFinishThreads>(r, each, bins.above, bins.above_weight, bins.all, sh);
       __syncthreads();
       if (tid < a.chunks) chunk_sums[tid] = sum;
       __syncthreads();
-      each([&](u64 rank) {
-        if (rank >= least) atomicAdd(&chunk_sums[index_in(rank) / a.chunk], likely_weight(r, logit_of(key_in(rank))));
+      each([&](u64 rank, auto of) {
+        const u64 w = of();
+        if (rank >= least && w >= r.least) atomicAdd(&chunk_sums[index_in(rank) / a.chunk], w);
       });
     } else {  // more tokens than a list holds: by the row itself
       least = border_of<kFinishThreads>(r, [&](auto f) {
-        for_each<T, kFinishThreads>(r.logits, 0, a.vocab, [&](int i, float x) { f(rank_of(key_of(x), i)); });
+        for_each<T, kFinishThreads>(r.logits, 0, a.vocab, [&](int i, float x) {
+        f(rank_of(key_of(x), i), [&] { return weight_at(exponent_of(r, x)); });
+      });
       }, 0, 0, bins.all, sh);
       for (int c = 0; c < a.chunks; ++c) {
         u64 sum = 0;

@@ -22,11 +22,8 @@
 namespace fpv2 {
 namespace {
 
-// Keys of a wave's tile, and of a block: a tile for each of the 4 waves.  KT: MFMA
-// tiles of 16 keys.
-template <int D> constexpr int kKt = D > 128 ? 1 : 2;
-constexpr int wave_keys(int64_t dim) { return 16 * (dim == 64 ? kKt<64> : dim == 96 ? kKt<96> : dim == 128 ? kKt<128> : kKt<256>); }
-constexpr int block_keys(int64_t dim) { return 4 * wave_keys(dim); }
+constexpr int kBlockKeys = 128;  // keys of a block: a tile of 32 for each of the 4 waves
+constexpr int kWaveKeys = 32;
 constexpr int kMaxGrid = 4096;   // workgroups of a call
 constexpr int kMaxHeads = 16;  // query heads of an item (columns of an MFMA tile)
 
@@ -42,7 +39,6 @@ struct DecodeArgs {
   int64_t q_bs, q_hs, k_ps, k_hs, k_rs, v_ps, v_hs, v_rs, o_bs, o_hs, table_stride;
   int batch, kv_heads, group, item_heads, head_items;  // head_items * item_heads >= group
   int pages, page_size, capacity, length, window, sinks, grid;
-  int block_keys;
   uint32_t page_mul, page_shift;  // t / page_size = (umulhi(t, mul) + t) >> shift
   float scale_log2;
 };
@@ -62,7 +58,7 @@ __device__ __forceinline__ Sequence sequence_of(const DecodeArgs& a, int b) {
   const int start = max(s.sinks, len - a.window);
   s.skip = start - s.sinks;
   s.n = len - s.skip;
-  s.blocks = max(1, (s.n + a.block_keys - 1) / a.block_keys);  // (an empty one writes its zeros)
+  s.blocks = max(1, (s.n + kBlockKeys - 1) / kBlockKeys);  // (an empty one writes its zeros)
   return s;
 }
 
@@ -119,28 +115,8 @@ __device__ __forceinline__ Words<NW> load_words(const uint16_t* p) {
   return r;
 }
 
-// O^T += V^T P^T over a lane's 8 keys (of 32) or 4 (of 16), in 16-bit pairs.
-template <typename T>
-__device__ __forceinline__ f32x4 product(u32x4 v, u32x4 p, f32x4 o) {
-  return Elem<T>::mfma16(as_vec8<T>(v), as_vec8<T>(p), o);
-}
-typedef short s16x4 __attribute__((ext_vector_type(4)));
-typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
-template <typename T>
-__device__ __forceinline__ f32x4 product(u32x2 v, u32x2 p, f32x4 o) {
-  if constexpr (std::is_same<T, bf16_t>::value)
-    return __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(__builtin_bit_cast(s16x4, v), __builtin_bit_cast(s16x4, p),
-                                                     o, 0, 0, 0);
-  else
-    return __builtin_amdgcn_mfma_f32_16x16x16f16(__builtin_bit_cast(f16x4, v), __builtin_bit_cast(f16x4, p), o,
-                                                 0, 0, 0);
-}
-
 template <typename T, int D>
 __global__ __launch_bounds__(256, 2) void decode_attn_kernel(DecodeArgs a) {
-  constexpr int KT = kKt<D>, kWaveKeys = 16 * KT, kBlockKeys = 4 * kWaveKeys;
-  constexpr int NK = 4 * KT;  // keys of a lane
-  typedef uint32_t Pairs __attribute__((ext_vector_type(NK / 2)));
   constexpr int KK = D / 32;  // MFMA steps of a key's dot product
   constexpr int DV = D / 16;  // dims of a lane
   __shared__ float sh_o[4][kMaxHeads][D + 4];
@@ -211,9 +187,9 @@ __global__ __launch_bounds__(256, 2) void decode_attn_kernel(DecodeArgs a) {
     const uint16_t* kb = a.k + kvh * a.k_hs;
     const uint16_t* vb = a.v + kvh * a.v_hs;
     const int32_t* table = a.table != nullptr ? a.table + b * a.table_stride : nullptr;
-    // lane i (modulo the tile) looks up the row of the tile's key i
+    // lane i (and i + 32) looks up the row of the tile's key i
     auto lookup = [&](int u0, int* row) {
-      const int u = min(u0 + (lane & (kWaveKeys - 1)), s.n - 1);
+      const int u = min(u0 + (lane & 31), s.n - 1);
       const uint32_t t = u < s.sinks ? u : u + s.skip;
       const uint32_t page = (__umulhi(t, a.page_mul) + t) >> a.page_shift;
       *row = t - page * a.page_size;
@@ -227,16 +203,16 @@ __global__ __launch_bounds__(256, 2) void decode_attn_kernel(DecodeArgs a) {
     for (; u0 < u_end; u0 += kBlockKeys) {
       const int64_t koff = page * a.k_ps + row * a.k_rs;
       const int64_t voff = page * a.v_ps + row * a.v_rs;
-      u32x4 kf[KT][KK];
+      u32x4 kf[2][KK];
 #pragma unroll
-      for (int t = 0; t < KT; ++t) {
+      for (int t = 0; t < 2; ++t) {
         const uint16_t* p = kb + __shfl(koff, 16 * t + col, 64) + 8 * quad;
 #pragma unroll
         for (int kk = 0; kk < KK; ++kk) kf[t][kk] = load16(p + 32 * kk);
       }
       // (at head dim 256 half of V waits for K's registers)
-      constexpr int kEarly = D > 128 ? NK / 2 : NK;
-      Words<DV / 2> vf[NK];
+      constexpr int kEarly = D > 128 ? 4 : 8;
+      Words<DV / 2> vf[8];
       const auto load_v = [&](int j) {
         return load_words<DV / 2>(vb + __shfl(voff, 16 * (j / 4) + 4 * quad + j % 4, 64) + DV * col);
       };
@@ -246,20 +222,20 @@ __global__ __launch_bounds__(256, 2) void decode_attn_kernel(DecodeArgs a) {
 
       int q_at = lane;
       if constexpr (kLdsQ) asm volatile("" : "+v"(q_at));  // (read again for each tile)
-      f32x4 sc[KT];
+      f32x4 sc[2];
 #pragma unroll
-      for (int t = 0; t < KT; ++t) {
+      for (int t = 0; t < 2; ++t) {
         sc[t] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int kk = 0; kk < KK; ++kk)
           sc[t] = Elem<T>::mfma16(as_vec8<T>(kf[t][kk]), as_vec8<T>(kLdsQ ? sh_q[64 * kk + q_at] : qf[kLdsQ ? 0 : kk]), sc[t]);
       }
 #pragma unroll
-      for (int j = kEarly; j < NK; ++j) vf[j] = load_v(j);
+      for (int j = kEarly; j < 8; ++j) vf[j] = load_v(j);
       const bool cut = u0 + kWaveKeys > s.n;
-      float x[NK], top = neg_inf();
+      float x[8], top = neg_inf();
 #pragma unroll
-      for (int j = 0; j < NK; ++j) {
+      for (int j = 0; j < 8; ++j) {
         x[j] = sc[j / 4][j % 4] * a.scale_log2;
         if (cut && u0 + 16 * (j / 4) + 4 * quad + j % 4 >= s.n) {
           x[j] = neg_inf();
@@ -277,23 +253,23 @@ __global__ __launch_bounds__(256, 2) void decode_attn_kernel(DecodeArgs a) {
       const float fix = __builtin_amdgcn_exp2f(m - ref);
       m = m_new;
       l *= fix;
-      Pairs pf;
+      u32x4 pf;
 #pragma unroll
-      for (int j = 0; j < NK; ++j) x[j] = __builtin_amdgcn_exp2f(x[j] - ref);
+      for (int j = 0; j < 8; ++j) x[j] = __builtin_amdgcn_exp2f(x[j] - ref);
 #pragma unroll
-      for (int j = 0; j < NK / 2; ++j) {
+      for (int j = 0; j < 4; ++j) {
         pf[j] = pack2<T>(x[2 * j], x[2 * j + 1]);
         l += x[2 * j] + x[2 * j + 1];
       }
 #pragma unroll
       for (int d = 0; d < DV; ++d) {
         o[d] *= fix;
-        Pairs vt;  // dim d of the lane's keys
+        u32x4 vt;  // dim d of the lane's 8 keys
 #pragma unroll
-        for (int j = 0; j < NK / 2; ++j)
+        for (int j = 0; j < 4; ++j)
           vt[j] = __builtin_amdgcn_perm(vf[2 * j + 1].w[d / 2], vf[2 * j].w[d / 2],
                                         d % 2 ? 0x07060302u : 0x05040100u);
-        o[d] = product<T>(vt, pf, o[d]);
+        o[d] = Elem<T>::mfma16(as_vec8<T>(vt), as_vec8<T>(pf), o[d]);
       }
     }
     l += __shfl_xor(l, 16, 64);
@@ -428,7 +404,7 @@ DecodePlan decode_plan(const fpv2_decode_params& p) {
   int64_t keys = p.table_width * p.page_size;
   if (p.window_tokens > 0 && p.window_tokens + p.sink_tokens < keys)
     keys = p.window_tokens + p.sink_tokens;
-  plan.most_blocks = (keys + block_keys(p.head_dim) - 1) / block_keys(p.head_dim);
+  plan.most_blocks = (keys + kBlockKeys - 1) / kBlockKeys;
   if (plan.most_blocks < 1) plan.most_blocks = 1;
   const int64_t blocks = p.batch * p.kv_heads * plan.head_items * plan.most_blocks;
   const int64_t most = 2 * static_cast<int64_t>(cu_count());
@@ -454,7 +430,7 @@ int check_params(const char* name, const fpv2_decode_params* p) {
   const int64_t group = p->query_heads / p->kv_heads;
   const int64_t items = p->batch * p->kv_heads * ((group + kMaxHeads - 1) / kMaxHeads);
   if (items * kMaxHeads > 0x7fffffff ||
-      items * ((p->table_width * p->page_size + 63) / 64) > 0x3fffffff)
+      items * ((p->table_width * p->page_size + kBlockKeys - 1) / kBlockKeys) > 0x3fffffff)
     return fail(FPV2_ERR_UNSUPPORTED, "%s: the call has too many blocks of keys", name);
   return FPV2_OK;
 }
@@ -549,7 +525,6 @@ extern "C" int fpv2_decode_attention(const void* q, const void* k_pages, const v
   a.group = static_cast<int>(p.query_heads / p.kv_heads);
   a.head_items = plan.head_items;
   a.item_heads = plan.item_heads;
-  a.block_keys = block_keys(p.head_dim);
   a.pages = static_cast<int>(p.pages);
   a.page_size = static_cast<int>(p.page_size);
   a.capacity = static_cast<int>(p.table_width * p.page_size);

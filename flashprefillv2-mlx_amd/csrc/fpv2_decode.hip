@@ -402,7 +402,7 @@ DecodePlan decode_plan(const fpv2_decode_params& p) {
   plan.head_items = static_cast<int>((group + kMaxHeads - 1) / kMaxHeads);
   plan.item_heads = static_cast<int>((group + plan.head_items - 1) / plan.head_items);
   int64_t keys = p.table_width * p.page_size;
-  if (p.window_tokens > 0 && p.window_tokens + p.sink_tokens < keys)
+  if (p.window_tokens > 0 && p.window_tokens < keys && p.sink_tokens < keys - p.window_tokens)
     keys = p.window_tokens + p.sink_tokens;
   plan.most_blocks = (keys + kBlockKeys - 1) / kBlockKeys;
   if (plan.most_blocks < 1) plan.most_blocks = 1;

@@ -141,7 +141,7 @@ __device__ __forceinline__ Row row_with(const SampleArgs& a, int b, const Settin
   r.top = key_in(best);
   r.max = r.top_logit = logit_of(r.top);
   const double temperature = fmin(set.temperature, 1e30);
-  r.greedy = r.top <= kLeastKey || !(temperature > 0);
+  r.greedy = r.top <= kLeastKey || !(set.temperature > 0);
   r.inv = fmin(1.0 / temperature, 1e300);
   r.top_p = set.top_p;
   r.top_k = set.top_k;
@@ -408,8 +408,8 @@ __device__ void pick(const SampleArgs& a, const Row& r, int b, u64 least, u64 al
     const float x = logit_at<T>(r.logits, i);
     return x >= r.from && rank_of(key_of(x), i) >= least ? likely_weight(r, x) : 0;
   };
-  const int token = find_first<THREADS>(lo, hi, before, kept,
-                               [&](u64 w) { return static_cast<double>(w) > target || w == all; }, sh);
+  const int token = min(hi - 1, find_first<THREADS>(
+      lo, hi, before, kept, [&](u64 w) { return static_cast<double>(w) > target || w == all; }, sh));
   if (threadIdx.x == 0) {
     a.tokens[b] = token;
     if (a.logprobs)
@@ -668,6 +668,10 @@ __global__ __launch_bounds__(kChunkThreads) void chunk_list_kernel(SampleArgs a)
   if (bins.in > kList) return;  // the row's workgroup does it all
   // (a logit below is in none of the bins: the others are looked at)
   const float from = bins.hi == kBins - 1 ? neg_inf() : r.reach((bins.hi + 1) / static_cast<float>(kPerUnit));
+  // (the list holds as many as the histogram counted, if nobody writes the logits)
+  const auto put = [&](uint32_t i, u64 rank) {
+    if (i < kList) a.list[static_cast<int64_t>(b) * kList + i] = rank;
+  };
   if (tid == 0) listed = 0;
   __syncthreads();
   for (int c = c0; c < c1; ++c) {
@@ -687,7 +691,7 @@ __global__ __launch_bounds__(kChunkThreads) void chunk_list_kernel(SampleArgs a)
       if (slot < kChunkList)
         list[slot] = rank;
       else
-        a.list[static_cast<int64_t>(b) * kList + atomicAdd(&a.listed[b], 1u)] = rank;
+        put(atomicAdd(&a.listed[b], 1u), rank);
     });
     sum = across<kChunkThreads, false>(sum, sh);
     if (tid == 0) a.sums[static_cast<int64_t>(b) * a.chunks + c] = sum;
@@ -696,7 +700,7 @@ __global__ __launch_bounds__(kChunkThreads) void chunk_list_kernel(SampleArgs a)
   const uint32_t n = listed < kChunkList ? listed : kChunkList;
   if (tid == 0) at = n > 0 ? atomicAdd(&a.listed[b], n) : 0;
   __syncthreads();
-  for (uint32_t i = tid; i < n; i += kChunkThreads) a.list[static_cast<int64_t>(b) * kList + at + i] = list[i];
+  for (uint32_t i = tid; i < n; i += kChunkThreads) put(at + i, list[i]);
 }
 
 // border_of for at most kFew tokens (rank, 0 for none, of the first threads): the count

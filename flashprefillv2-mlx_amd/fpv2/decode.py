@@ -169,13 +169,14 @@ def decode_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tens
     window = 0 if window_tokens is None else _count(window_tokens, "window_tokens", 1)
     _count(sink_tokens, "sink_tokens")
     if out is not None:
-        if out.shape != shape or out.dtype != dtype or out.stride(2) != 1:
+        if (out.shape != shape or out.dtype != dtype or out.stride(2) != 1
+                or batch > 1 and out.stride(0) < dim or heads > 1 and out.stride(1) < dim):
             raise ValueError("out must be [batch, query heads, head dim] of q's dtype with a "
-                             "contiguous last dimension")
+                             "contiguous last dimension and no overlap")
         tensors.append(out)
     index = _device(tensors)
     if out is None:
-        out = torch.empty(shape, dtype=dtype, device=q.device)
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
     q_strides = _row_strides(q)
     if q_strides is None:
         q = q.clone(memory_format=torch.contiguous_format)
@@ -209,7 +210,9 @@ def _index(value, name: str, tokens: int):
                 or not value.is_contiguous()):
             raise ValueError(f"{name} must be contiguous int32 or int64 [tokens], or an integer")
         return value, value.element_size(), 0
-    return None, 0, _count(value, name)
+    if _count(value, name) >= 1 << 62:
+        raise ValueError(f"{name} must be below 2^62")
+    return None, 0, value
 
 
 def rope_to_pages(qkv: torch.Tensor, q_weight: torch.Tensor | None, k_weight: torch.Tensor | None,
@@ -263,7 +266,8 @@ def rope_to_pages(qkv: torch.Tensor, q_weight: torch.Tensor | None, k_weight: to
     tensors = [qkv, k_pages, v_pages, cos, sin]
     tensors += [t for t in (q_weight, k_weight, positions, slots, out) if t is not None]
     if out is not None and (out.shape != (tokens, query_heads, dim) or out.dtype != qkv.dtype
-                            or _row_strides(out) is None):
+                            or _row_strides(out) is None or tokens > 1 and out.stride(0) < dim
+                            or query_heads > 1 and out.stride(1) < dim):
         raise ValueError("out must be [tokens, query heads, head dim] of qkv's dtype with 16-byte "
                          "aligned rows")
     index = _device(tensors)
@@ -355,7 +359,7 @@ def quantized_linear(x: torch.Tensor, packed: torch.Tensor, scales: torch.Tensor
     dtype; returns ``[..., N]`` in that dtype or, with ``out_dtype``, in float32.
     ``out``: optional ``[M, N]`` destination (``x`` ``[M, K]``) with contiguous
     rows.  Products and sums are in float32 with the weights exact; ``x`` must be
-    finite (an infinite value gives NaN).  Made for the few rows of a decode
+    below 1e34 (an infinite value gives NaN).  Made for the few rows of a decode
     step: the weights are read once for every 16 rows or more (64 with groups
     of 128), so a large prompt is better served by a product with
     ``dequantize_weight``'s result."""
@@ -439,7 +443,9 @@ def sample_tokens(logits: torch.Tensor, uniform: torch.Tensor, *,
     these, and of these the ones with ``w_i >= min_p``; the first always is.
     The token is the first one, in index order, whose running kept weight
     exceeds ``uniform[b]`` times all kept weight.  Temperature 0: the greatest
-    logit, of equal ones the first.
+    logit, of equal ones the first.  (In tensors, temperatures of 0 or less and NaN
+    are 0, ``top_k`` of 0 or less and ``top_p`` of 1 or more are no limit, and a
+    negative ``min_p`` is 0, one above 1 is 1.)
 
     Returns int64 tokens ``[B]``, with ``return_logprobs`` also the float32 log of
     each token's share of the kept weight.  The result is the same in every

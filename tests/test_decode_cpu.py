@@ -221,3 +221,88 @@ def test_sample_tokens_refuses_cpu_tensors_and_gradients():
         fpv2.sample_tokens(**_sample_args())
     with pytest.raises(RuntimeError, match="no backward"):
         fpv2.sample_tokens(**_sample_args(logits=torch.zeros(3, 50, requires_grad=True)))
+
+
+def test_more_refusals():
+    """Destinations that overlap themselves, indexes past 64 bits."""
+    bf16 = torch.bfloat16
+    for out in (torch.zeros(1, 8, 64, dtype=bf16).expand(2, 8, 64),
+                torch.zeros(2, 1, 64, dtype=bf16).expand(2, 8, 64)):
+        with pytest.raises(ValueError, match="out must be"):
+            fpv2.decode_attention(**_attention_args(out=out))
+    for out in (torch.zeros(1, 4, 64, dtype=bf16).expand(3, 4, 64),
+                torch.zeros(3, 1, 64, dtype=bf16).expand(3, 4, 64)):
+        with pytest.raises(ValueError, match="out must be"):
+            fpv2.rope_to_pages(**_rope_args(out=out))
+    for name in ("positions", "slots"):
+        with pytest.raises(ValueError, match=name):
+            fpv2.rope_to_pages(**_rope_args(**{name: 1 << 62}))
+
+
+def test_c_entries_refuse_without_a_device():
+    """Argument errors of the C entries come before any device call."""
+    import ctypes
+
+    from fpv2 import _lib
+    if not _lib.LIB_PATH.exists():
+        pytest.skip("libfpv2_hip.so not built (run __graft_entry__.build())")
+    lib = _lib.load()
+
+    def attention(**change):
+        p = _lib.DecodeParams(batch=1, query_heads=4, kv_heads=2, head_dim=64, pages=3, page_size=16,
+                              table_width=2, table_stride=2)
+        for name, value in change.items():
+            setattr(p, name, value)
+        return lib.fpv2_decode_attention(8, 16, 16, 16, 16, 16, _lib.BF16, ctypes.byref(p), None, 0, None)
+
+    for change in (dict(batch=-1), dict(kv_heads=0), dict(query_heads=5), dict(pages=0),
+                   dict(page_size=0), dict(table_width=0), dict(window_tokens=-1), dict(sink_tokens=-2),
+                   dict(length=-1), dict(page_size=1 << 30), dict(k_row_stride=4),
+                   dict(table_stride=-1), dict()):
+        assert attention(**change) == _lib.FPV2_ERR_ARGUMENT  # (the last: q is not aligned)
+    assert attention(head_dim=80) == _lib.FPV2_ERR_UNSUPPORTED
+    assert attention(batch=1 << 16) == _lib.FPV2_ERR_UNSUPPORTED
+    assert attention(batch=0) == _lib.FPV2_OK
+    assert lib.fpv2_decode_attention(0, 0, 0, 0, 0, 0, _lib.BF16, None, None, 0, None) == -1
+
+    def rope(**change):
+        p = _lib.RopePagesParams(tokens=2, query_heads=4, kv_heads=2, head_dim=64, rotary_half=32,
+                                 table_rows=9, pages=3, page_size=16, qkv_row_stride=512,
+                                 q_token_stride=256, q_head_stride=64)
+        for name, value in change.items():
+            setattr(p, name, value)
+        return lib.fpv2_rope_to_pages(8, 16, 16, 16, 16, 16, 16, 16, 16, 16, _lib.F16,
+                                      ctypes.byref(p), None)
+
+    for change in (dict(tokens=-1), dict(kv_heads=0), dict(table_rows=0), dict(pages=0),
+                   dict(pages=1 << 27, page_size=16), dict(position_bytes=2), dict(slot_bytes=1),
+                   dict(qkv_row_stride=504), dict(q_head_stride=63), dict()):
+        assert rope(**change) == _lib.FPV2_ERR_ARGUMENT
+    for change in (dict(head_dim=72), dict(head_dim=528), dict(rotary_half=40), dict(rotary_half=12)):
+        assert rope(**change) == _lib.FPV2_ERR_UNSUPPORTED
+    assert rope(tokens=0) == _lib.FPV2_OK
+
+    def linear(rows=2, n=32, k=128, group=64, xs=128, ps=16, ss=2, os=32, dtype=_lib.BF16,
+               out_dtype=_lib.BF16, x=8):
+        return lib.fpv2_quantized_linear(x, 16, 16, 16, 16, dtype, out_dtype, rows, n, k, group, xs, ps,
+                                         ss, os, None)
+
+    for change in (dict(rows=-1), dict(k=100), dict(k=0), dict(xs=120), dict(xs=130), dict(ps=14),
+                   dict(ps=12), dict(ss=1), dict(os=31), dict(x=0), dict()):
+        assert linear(**change) == _lib.FPV2_ERR_ARGUMENT
+    for change in (dict(group=48), dict(dtype=_lib.F32), dict(out_dtype=_lib.F16)):
+        assert linear(**change) == _lib.FPV2_ERR_UNSUPPORTED
+    assert linear(rows=0) == _lib.FPV2_OK and linear(n=0) == _lib.FPV2_OK
+
+    def sample(dtype=_lib.F32, logits=16, **change):
+        p = _lib.SampleParams(batch=2, vocab=5000, logits_stride=5000, temperature=1.0, top_p=1.0)
+        for name, value in change.items():
+            setattr(p, name, value)
+        return lib.fpv2_sample_tokens(logits, 16, dtype, ctypes.byref(p), 16, None, None, 0, None)
+
+    for change in (dict(batch=-1), dict(batch=1 << 16), dict(vocab=0), dict(logits_stride=-1),
+                   dict(logits=0), dict()):  # (the last: no workspace)
+        assert sample(**change) == _lib.FPV2_ERR_ARGUMENT
+    assert sample(vocab=(1 << 19) + 1) == _lib.FPV2_ERR_UNSUPPORTED
+    assert sample(dtype=7) == _lib.FPV2_ERR_UNSUPPORTED
+    assert sample(batch=0) == _lib.FPV2_OK

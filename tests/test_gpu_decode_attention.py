@@ -258,3 +258,29 @@ def test_runs_on_the_current_stream(cuda):
         got = fpv2.decode_attention(late, k, v, None, 4000)
     side.synchronize()
     assert torch.equal(got, want)
+
+
+def test_windows_past_any_cache(cuda):
+    """Windows and sinks of the largest integers see everything."""
+    gen = torch.Generator().manual_seed(12)
+    k, v, table = _paged(gen, [700, 90], 2, 16, 64, BF16)
+    q = _rand(gen, 2, 4, 64, dtype=BF16)
+    want = _check(cuda, q, k, v, table, [700, 90])
+    for window, sinks in ((2 ** 62, 2 ** 62), (2 ** 63 - 1, 2 ** 63 - 1), (1, 2 ** 63 - 1), (2 ** 62, 0)):
+        got = fpv2.decode_attention(q.to(cuda), k.to(cuda), v.to(cuda), table.to(cuda),
+                                    torch.tensor([700, 90], dtype=torch.int32, device=cuda),
+                                    window_tokens=window, sink_tokens=sinks)
+        assert torch.equal(got, want)
+
+
+def test_small_float16_values(cuda):
+    """Subnormal keys and values count."""
+    gen = torch.Generator().manual_seed(13)
+    k, v = (_rand(gen, 1, 1, 200, 64, dtype=torch.float32) * 2e-6 for _ in "kv")
+    k, v = (x.to(F16) for x in (k, v))
+    q = _rand(gen, 1, 4, 64, dtype=F16) * 30
+    got = fpv2.decode_attention(q.to(cuda), k.to(cuda), v.to(cuda), None, 200, scale=1000.0)
+    want, tol = _reference(q, k, v, None, [200], 1000.0, None, 0)
+    # (a result this small is rounded to a multiple of 2^-24)
+    assert bool(((got.cpu().double() - want).abs() <= tol + 2.0 ** -25).all())
+    assert float(want.abs().max()) > 2.0 ** -22

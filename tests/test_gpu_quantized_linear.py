@@ -168,3 +168,13 @@ def test_captured_and_streams(cuda):
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(y, fpv2.quantized_linear(x, *weights))
+
+
+def test_small_float16_values(cuda):
+    """Subnormal activations and scales count."""
+    gen = torch.Generator().manual_seed(5)
+    packed, scales, biases = _weights(gen, 40, 256, 64, F16)
+    x = (torch.randn((3, 256), generator=gen) * 3e-6).to(F16)
+    _check(cuda, x, (packed, scales, biases), F32)
+    small = ((scales.float() * 1e-3).to(F16), (biases.float() * 1e-3).to(F16))
+    _check(cuda, (x.float() * 1e4).to(F16), (packed, *small), F32)

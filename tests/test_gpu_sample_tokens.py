@@ -199,3 +199,22 @@ def test_captured(cuda):
         torch.cuda.synchronize()
         for a, b in zip(got, call()):
             assert torch.equal(a, b)
+
+
+def test_settings_out_of_range_in_tensors(cuda):
+    """NaN and negative temperatures are greedy, other settings out of range no limit."""
+    gen = torch.Generator().manual_seed(7)
+    logits, u = _logits(gen, 4, 5003, F32), torch.rand(4, generator=gen)
+    dev = logits.to(cuda)
+    t = torch.tensor([math.nan, -1.0, 0.0, -math.inf], device=cuda)
+    assert torch.equal(fpv2.sample_tokens(dev, u.to(cuda), temperature=t).cpu(), logits.argmax(1))
+    want = fpv2.sample_tokens(dev, u.to(cuda))
+    got = fpv2.sample_tokens(dev, u.to(cuda), top_k=torch.tensor([-5, 0, 5003, 2 ** 31 - 1], device=cuda,
+                                                                 dtype=torch.int32),
+                             top_p=torch.tensor([1.0, 7.0, math.inf, math.nan], device=cuda),
+                             min_p=torch.tensor([-1.0, math.nan, 0.0, -math.inf], device=cuda))
+    assert torch.equal(got, want)
+    hot = fpv2.sample_tokens(dev, u.to(cuda), temperature=torch.full((4,), math.inf, device=cuda))
+    assert torch.equal(hot, fpv2.sample_tokens(dev, u.to(cuda), temperature=1e30))
+    top = fpv2.sample_tokens(dev, u.to(cuda), min_p=torch.full((4,), 9.0, device=cuda))
+    assert torch.equal(top.cpu(), logits.argmax(1))

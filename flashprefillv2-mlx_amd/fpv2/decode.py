@@ -36,15 +36,17 @@ def _device(tensors) -> int:
     """The index of the one ROCm device that all tensors are on; raises where there is
     none, or where a gradient would be lost.  (These calls take microseconds on
     the device, so the checks are made in few steps.)"""
-    if torch.is_grad_enabled():
-        for t in tensors:
-            if t.requires_grad:
-                raise RuntimeError("the decode operators have no backward: call them under "
-                                   "torch.no_grad() or detach their inputs")
     index = tensors[0].get_device()
-    for t in tensors:
-        if t.get_device() != index or index < 0:
-            _lib.require_device(*tensors)
+    if index >= 0:
+        for t in tensors:
+            if t.requires_grad or t.get_device() != index:
+                break
+        else:
+            return index
+    if torch.is_grad_enabled() and any(t.requires_grad for t in tensors):
+        raise RuntimeError("the decode operators have no backward: call them under "
+                           "torch.no_grad() or detach their inputs")
+    _lib.require_device(*tensors)
     return index
 
 
@@ -98,6 +100,11 @@ def _pages(k_pages: torch.Tensor, v_pages: torch.Tensor):
 
 
 def _page_strides(k_pages: torch.Tensor, v_pages: torch.Tensor):
+    a, b, c, last = k_pages.stride()
+    d, e, f, other = v_pages.stride()
+    if (last == 1 == other and not (a | b | c | d | e | f) & 7
+            and not (k_pages.data_ptr() | v_pages.data_ptr()) & 15):
+        return a, b, c, d, e, f
     k, v = _row_strides(k_pages), _row_strides(v_pages)
     if k is None or v is None:
         raise ValueError("the caches' rows must be contiguous and 16-byte aligned")
@@ -253,18 +260,23 @@ def rope_to_pages(qkv: torch.Tensor, q_weight: torch.Tensor | None, k_weight: to
         if t is not None and (t.shape != (dim,) or t.dtype != qkv.dtype or t.data_ptr() & 15
                               or not t.is_contiguous()):
             raise ValueError(f"{name} must be contiguous [head dim] of qkv's dtype, 16-byte aligned")
-    for name, t in (("cos", cos), ("sin", sin)):
-        if (t.ndim != 2 or t.shape != cos.shape or t.dtype != torch.float32
-                or not t.is_contiguous() or t.data_ptr() % 16):
-            raise ValueError(f"{name} must be a contiguous float32 [positions, R] table")
-    half = cos.shape[1]
-    if cos.shape[0] == 0 or half == 0 or half % 8 or 2 * half > dim:
+    if not (cos.ndim == 2 and cos.shape == sin.shape and cos.dtype == sin.dtype == torch.float32
+            and cos.is_contiguous() and sin.is_contiguous()
+            and not (cos.data_ptr() | sin.data_ptr()) & 15):
+        for name, t in (("cos", cos), ("sin", sin)):
+            if (t.ndim != 2 or t.shape != cos.shape or t.dtype != torch.float32
+                    or not t.is_contiguous() or t.data_ptr() % 16):
+                raise ValueError(f"{name} must be a contiguous float32 [positions, R] table")
+    rows, half = cos.shape
+    if rows == 0 or half == 0 or half % 8 or 2 * half > dim:
         raise ValueError("cos and sin must have rows of a multiple of 8 angles, at most half the "
                          "head dimension")
     positions, position_bytes, first_position = _index(positions, "positions", tokens)
     slots, slot_bytes, first_slot = _index(slots, "slots", tokens)
     tensors = [qkv, k_pages, v_pages, cos, sin]
-    tensors += [t for t in (q_weight, k_weight, positions, slots, out) if t is not None]
+    for t in (q_weight, k_weight, positions, slots, out):
+        if t is not None:
+            tensors.append(t)
     if out is not None and (out.shape != (tokens, query_heads, dim) or out.dtype != qkv.dtype
                             or _row_strides(out) is None or tokens > 1 and out.stride(0) < dim
                             or query_heads > 1 and out.stride(1) < dim):
@@ -281,7 +293,7 @@ def rope_to_pages(qkv: torch.Tensor, q_weight: torch.Tensor | None, k_weight: to
         return out
     lib = _lib.load()
     p = (_rope_params if position_bytes and slot_bytes else _lib.RopePagesParams)(
-        tokens, query_heads, kv_heads, dim, half, cos.shape[0], bool(interleaved), pages, page_size,
+        tokens, query_heads, kv_heads, dim, half, rows, bool(interleaved), pages, page_size,
         position_bytes, slot_bytes, first_position, first_slot, *qkv_strides, *_row_strides(out),
         *page_strides, eps)
 

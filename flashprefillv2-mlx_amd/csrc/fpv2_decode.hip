@@ -4,9 +4,9 @@
 //   out[b][h] = sum_t p_t v_t / sum_t p_t,  p_t = exp(scale q[b][h].k_t - max)
 //
 // Bound by reading K and V once.  The visible keys of all (sequence, KV head)
-// items are cut into blocks of 128 keys, laid end to end, and dealt to the
+// items are cut into tiles of 32 keys, laid end to end, and dealt to the
 // workgroups in equal runs, so that ragged batches, single long sequences and
-// many short ones fill the chip alike.  A run that covers an item's blocks only in
+// many short ones fill the chip alike.  A run that covers an item's tiles only in
 // part leaves a partial (O, max, sum), and a second kernel joins these in order.
 //
 // A wave takes 32 keys at a time on MFMA, with no LDS in the loop:
@@ -22,8 +22,13 @@
 namespace fpv2 {
 namespace {
 
-constexpr int kBlockKeys = 128;  // keys of a block: a tile of 32 for each of the 4 waves
-constexpr int kWaveKeys = 32;
+constexpr int kTileKeys = 32;   // keys of a wave's tile
+constexpr int kWaves = 4;
+constexpr int kStepKeys = kWaves * kTileKeys;
+// What an item costs a workgroup beside its tiles (its queries, its first rows'
+// addresses, the join of the waves), in tiles.  24 sequences of 61 to 16001 keys:
+// counted as none 69 us, as 4 62.5, 8 62.4, 16 63.6 us.
+constexpr int kItemUnits = 8;
 constexpr int kMaxGrid = 4096;   // workgroups of a call
 constexpr int kMaxHeads = 16;  // query heads of an item (columns of an MFMA tile)
 
@@ -47,7 +52,8 @@ struct Sequence {
   int n;      // visible keys
   int sinks;  // of which at the start
   int skip;   // key of visible index u >= sinks: u + skip
-  int blocks;
+  int tiles;
+  __device__ __forceinline__ int units() const { return kItemUnits + tiles; }
 };
 
 __device__ __forceinline__ Sequence sequence_of(const DecodeArgs& a, int b) {
@@ -58,15 +64,15 @@ __device__ __forceinline__ Sequence sequence_of(const DecodeArgs& a, int b) {
   const int start = max(s.sinks, len - a.window);
   s.skip = start - s.sinks;
   s.n = len - s.skip;
-  s.blocks = max(1, (s.n + kBlockKeys - 1) / kBlockKeys);  // (an empty one writes its zeros)
+  s.tiles = max(1, (s.n + kTileKeys - 1) / kTileKeys);  // (an empty one writes its zeros)
   return s;
 }
 
-// Blocks of one item of every sequence, and of the ones before sequence `end`.
+// Units of one item of every sequence, and of the ones before sequence `end`.
 __device__ __forceinline__ int wave_total(const DecodeArgs& a, int lane, int end, int* before) {
   int all = 0, some = 0;
   for (int b = lane; b < a.batch; b += 64) {
-    const int n = sequence_of(a, b).blocks;
+    const int n = sequence_of(a, b).units();
     all += n;
     some += b < end ? n : 0;
   }
@@ -79,16 +85,19 @@ __device__ __forceinline__ int wave_total(const DecodeArgs& a, int lane, int end
   return all;
 }
 
-// The first block of a workgroup's run (runs differ by a block at most), and the
-// workgroup that has a block.  Where there are fewer blocks than workgroups, each
-// of the first ones has one: an item's workgroups are neighbours.
-__device__ __forceinline__ int first_of(const DecodeArgs& a, uint32_t w, int total) {
-  const uint32_t grid = min(a.grid, total);
-  return static_cast<int>(static_cast<uint64_t>(min(w, grid)) * static_cast<uint32_t>(total) / grid);
+// The workgroups that have a run: of a tile for each wave at least.
+__device__ __forceinline__ uint32_t runs_of(const DecodeArgs& a, int total) {
+  return min(a.grid, (total + kWaves - 1) / kWaves);
 }
-__device__ __forceinline__ int workgroup_of(const DecodeArgs& a, int block, int total) {
-  const uint32_t grid = min(a.grid, total);
-  return static_cast<int>((static_cast<uint64_t>(block + 1) * grid - 1) / static_cast<uint32_t>(total));
+// The first unit of a workgroup's run (runs differ by a unit at most), and the
+// workgroup that has a unit.
+__device__ __forceinline__ int first_of(const DecodeArgs& a, uint32_t w, int total) {
+  const uint32_t runs = runs_of(a, total);
+  return static_cast<int>(static_cast<uint64_t>(min(w, runs)) * static_cast<uint32_t>(total) / runs);
+}
+__device__ __forceinline__ int workgroup_of(const DecodeArgs& a, int unit, int total) {
+  const uint32_t runs = runs_of(a, total);
+  return static_cast<int>((static_cast<uint64_t>(unit + 1) * runs - 1) / static_cast<uint32_t>(total));
 }
 
 template <int NW>
@@ -138,7 +147,7 @@ __global__ __launch_bounds__(256, 2) void decode_attn_kernel(DecodeArgs a) {
   // the sequence that holds block lo: base is its first block
   int b = 0, base = 0;
   for (int b0 = 0; b0 < a.batch; b0 += 64) {
-    int sum = b0 + lane < a.batch ? sequence_of(a, b0 + lane).blocks * items : 0;
+    int sum = b0 + lane < a.batch ? sequence_of(a, b0 + lane).units() * items : 0;
 #pragma unroll
     for (int off = 1; off < 64; off <<= 1) {
       const int up = __shfl_up(sum, off, 64);
@@ -157,12 +166,20 @@ __global__ __launch_bounds__(256, 2) void decode_attn_kernel(DecodeArgs a) {
   base = __builtin_amdgcn_readfirstlane(base);
 
   Sequence s = sequence_of(a, b);
-  for (int cur = lo; cur < hi;) {
-    const int item = (cur - base) / s.blocks;
-    const int item_start = base + item * s.blocks;
-    const int first = cur - item_start;
-    const int end = min(hi, item_start + s.blocks);
-    const int last = end - item_start;  // blocks [first, last) of the item
+  for (int cur = lo, end; cur < hi; cur = end) {
+    const int units = s.units();
+    const int item = (cur - base) / units;
+    const int item_start = base + item * units;
+    end = min(hi, item_start + units);
+    // tiles [first, last) of the item; the run may start or end among the other units
+    const int first = max(0, cur - item_start - kItemUnits), last = end - item_start - kItemUnits;
+    const int b_now = b;
+    const Sequence s_now = s;
+    if (end < hi && end == base + items * units) {
+      base = end;
+      s = sequence_of(a, ++b);
+    }
+    if (last <= first) continue;
     const int kvh = item / a.head_items;
     const int h0 = (item - kvh * a.head_items) * a.item_heads;
     const int heads = min(a.item_heads, a.group - h0);
@@ -170,7 +187,7 @@ __global__ __launch_bounds__(256, 2) void decode_attn_kernel(DecodeArgs a) {
 
     u32x4 qf[kLdsQ ? 1 : KK];
     const auto load_q = [&](int kk) {
-      return col < heads ? load16(a.q + b * a.q_bs + head * a.q_hs + 32 * kk + 8 * quad) : u32x4{0, 0, 0, 0};
+      return col < heads ? load16(a.q + b_now * a.q_bs + head * a.q_hs + 32 * kk + 8 * quad) : u32x4{0, 0, 0, 0};
     };
     if constexpr (kLdsQ) {
       for (int kk = wave; kk < KK; kk += 4) sh_q[64 * kk + lane] = load_q(kk);
@@ -186,21 +203,21 @@ __global__ __launch_bounds__(256, 2) void decode_attn_kernel(DecodeArgs a) {
 
     const uint16_t* kb = a.k + kvh * a.k_hs;
     const uint16_t* vb = a.v + kvh * a.v_hs;
-    const int32_t* table = a.table != nullptr ? a.table + b * a.table_stride : nullptr;
+    const int32_t* table = a.table != nullptr ? a.table + b_now * a.table_stride : nullptr;
     // lane i (and i + 32) looks up the row of the tile's key i
     auto lookup = [&](int u0, int* row) {
-      const int u = min(u0 + (lane & 31), s.n - 1);
-      const uint32_t t = u < s.sinks ? u : u + s.skip;
+      const int u = min(u0 + (lane & 31), s_now.n - 1);
+      const uint32_t t = u < s_now.sinks ? u : u + s_now.skip;
       const uint32_t page = (__umulhi(t, a.page_mul) + t) >> a.page_shift;
       *row = t - page * a.page_size;
-      const int id = table != nullptr ? table[page] : b;
+      const int id = table != nullptr ? table[page] : b_now;
       return min(max(id, 0), a.pages - 1);
     };
-    int u0 = first * kBlockKeys + wave * kWaveKeys;
-    const int u_end = min(s.n, last * kBlockKeys);
+    int u0 = first * kTileKeys + wave * kTileKeys;
+    const int u_end = min(s_now.n, last * kTileKeys);
     int row = 0, page = 0;
     if (u0 < u_end) page = lookup(u0, &row);
-    for (; u0 < u_end; u0 += kBlockKeys) {
+    for (; u0 < u_end; u0 += kStepKeys) {
       const int64_t koff = page * a.k_ps + row * a.k_rs;
       const int64_t voff = page * a.v_ps + row * a.v_rs;
       u32x4 kf[2][KK];
@@ -218,7 +235,7 @@ __global__ __launch_bounds__(256, 2) void decode_attn_kernel(DecodeArgs a) {
       };
 #pragma unroll
       for (int j = 0; j < kEarly; ++j) vf[j] = load_v(j);
-      if (u0 + kBlockKeys < u_end) page = lookup(u0 + kBlockKeys, &row);
+      if (u0 + kStepKeys < u_end) page = lookup(u0 + kStepKeys, &row);
 
       int q_at = lane;
       if constexpr (kLdsQ) asm volatile("" : "+v"(q_at));  // (read again for each tile)
@@ -232,12 +249,12 @@ __global__ __launch_bounds__(256, 2) void decode_attn_kernel(DecodeArgs a) {
       }
 #pragma unroll
       for (int j = kEarly; j < 8; ++j) vf[j] = load_v(j);
-      const bool cut = u0 + kWaveKeys > s.n;
+      const bool cut = u0 + kTileKeys > s_now.n;
       float x[8], top = neg_inf();
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
         x[j] = sc[j / 4][j % 4] * a.scale_log2;
-        if (cut && u0 + 16 * (j / 4) + 4 * quad + j % 4 >= s.n) {
+        if (cut && u0 + 16 * (j / 4) + 4 * quad + j % 4 >= s_now.n) {
           x[j] = neg_inf();
           // (a zero weight would make NaN of what an unused row may hold)
 #pragma unroll
@@ -287,7 +304,7 @@ __global__ __launch_bounds__(256, 2) void decode_attn_kernel(DecodeArgs a) {
         for (int d = 0; d < DV; ++d) sh_o[wave][col][(4 * quad + i) * DV + d] = o[d][i];
     }
     __syncthreads();
-    const bool whole = first == 0 && last == s.blocks;
+    const bool whole = first == 0 && last == s_now.tiles;
     const int64_t slot = 2 * static_cast<int64_t>(blockIdx.x) + (cur == lo ? 0 : 1);
     for (int e = tid; e < heads * D; e += 256) {
       const int h = e / D, d = e % D;
@@ -304,8 +321,8 @@ __global__ __launch_bounds__(256, 2) void decode_attn_kernel(DecodeArgs a) {
         den += f * sh_ml[w][h][1];
       }
       if (whole) {
-        const float r = s.n == 0 ? 0.f : sum / den;
-        a.out[b * a.o_bs + (kvh * a.group + h0 + h) * a.o_hs + d] = Elem<T>::from_float(r);
+        const float r = s_now.n == 0 ? 0.f : sum / den;
+        a.out[b_now * a.o_bs + (kvh * a.group + h0 + h) * a.o_hs + d] = Elem<T>::from_float(r);
       } else {
         a.part_o[(slot * a.item_heads + h) * D + d] = sum;
         if (d == 0) {
@@ -315,11 +332,6 @@ __global__ __launch_bounds__(256, 2) void decode_attn_kernel(DecodeArgs a) {
       }
     }
     __syncthreads();
-    cur = end;
-    if (cur < hi && cur == base + items * s.blocks) {
-      base = cur;
-      s = sequence_of(a, ++b);
-    }
   }
 }
 
@@ -342,8 +354,9 @@ __global__ __launch_bounds__(256) void decode_join_kernel(DecodeArgs a) {
   int before;
   const int total = wave_total(a, lane, b, &before) * items;
   const Sequence s = sequence_of(a, b);
-  const int start = before * items + item * s.blocks;
-  const int w0 = workgroup_of(a, start, total), n = workgroup_of(a, start + s.blocks - 1, total) - w0 + 1;
+  const int start = before * items + item * s.units();
+  const int w0 = workgroup_of(a, start + kItemUnits, total);
+  const int n = workgroup_of(a, start + s.units() - 1, total) - w0 + 1;
   if (n == 1) return;  // written by its workgroup
   // a workgroup's first item is in its slot 0, its last in slot 1
   const int in_last = start > first_of(a, w0, total) ? 1 : 0;
@@ -392,7 +405,7 @@ __global__ __launch_bounds__(256) void decode_join_kernel(DecodeArgs a) {
 
 struct DecodePlan {
   int head_items, item_heads, grid;
-  int64_t most_blocks;  // of an item
+  int64_t most_tiles;  // of an item
 };
 
 // The launch of a call; its workspace goes by the same numbers.
@@ -404,11 +417,11 @@ DecodePlan decode_plan(const fpv2_decode_params& p) {
   int64_t keys = p.table_width * p.page_size;
   if (p.window_tokens > 0 && p.window_tokens < keys && p.sink_tokens < keys - p.window_tokens)
     keys = p.window_tokens + p.sink_tokens;
-  plan.most_blocks = (keys + kBlockKeys - 1) / kBlockKeys;
-  if (plan.most_blocks < 1) plan.most_blocks = 1;
-  const int64_t blocks = p.batch * p.kv_heads * plan.head_items * plan.most_blocks;
-  const int64_t most = 2 * static_cast<int64_t>(cu_count());
-  plan.grid = static_cast<int>(blocks < most ? blocks : most < kMaxGrid ? most : kMaxGrid);
+  plan.most_tiles = (keys + kTileKeys - 1) / kTileKeys;
+  if (plan.most_tiles < 1) plan.most_tiles = 1;
+  const int64_t units = p.batch * p.kv_heads * plan.head_items * (plan.most_tiles + kItemUnits);
+  const int64_t runs = (units + kWaves - 1) / kWaves, most = 2 * static_cast<int64_t>(cu_count());
+  plan.grid = static_cast<int>(runs < most ? runs : most < kMaxGrid ? most : kMaxGrid);
   return plan;
 }
 
@@ -430,13 +443,13 @@ int check_params(const char* name, const fpv2_decode_params* p) {
   const int64_t group = p->query_heads / p->kv_heads;
   const int64_t items = p->batch * p->kv_heads * ((group + kMaxHeads - 1) / kMaxHeads);
   if (items * kMaxHeads > 0x7fffffff ||
-      items * ((p->table_width * p->page_size + kBlockKeys - 1) / kBlockKeys) > 0x3fffffff)
-    return fail(FPV2_ERR_UNSUPPORTED, "%s: the call has too many blocks of keys", name);
+      items * ((p->table_width * p->page_size + kTileKeys - 1) / kTileKeys + kItemUnits) > 0x3fffffff)
+    return fail(FPV2_ERR_UNSUPPORTED, "%s: the call has too many tiles of keys", name);
   return FPV2_OK;
 }
 
 int64_t partial_bytes(const fpv2_decode_params& p, const DecodePlan& plan) {
-  if (p.batch == 0 || plan.most_blocks <= 1) return 0;  // every item has one workgroup
+  if (p.batch == 0 || plan.most_tiles <= 1) return 0;  // every item has one workgroup
   return 2LL * plan.grid * plan.item_heads * (p.head_dim + 2) * 4;
 }
 
@@ -539,7 +552,7 @@ extern "C" int fpv2_decode_attention(const void* q, const void* k_pages, const v
   a.page_mul = static_cast<uint32_t>((((1ull << shift) - p.page_size) << 32) / p.page_size + 1);
   a.scale_log2 = static_cast<float>(p.scale * 1.4426950408889634);
   const hipStream_t s = static_cast<hipStream_t>(stream);
-  const bool join = plan.most_blocks > 1;
+  const bool join = plan.most_tiles > 1;
   return dtype == FPV2_BF16 ? launch_dim<bf16_t>(a, p.head_dim, join, s)
                             : launch_dim<f16_t>(a, p.head_dim, join, s);
 }

@@ -30,7 +30,6 @@ struct RopePagesArgs {
   int lanes;       // of a head: a power of two >= d / 16
   int chunk;       // heads of a wave
   int chunks;      // waves of a token
-  int streaming;   // stores past the caches
   float eps;
 };
 
@@ -56,7 +55,8 @@ __device__ __forceinline__ u32x4 pack8(const float* x) {
   return w;
 }
 
-template <typename T>
+// STREAM: the stores go past the caches.
+template <typename T, bool STREAM>
 __global__ __launch_bounds__(256) void rope_pages_kernel(RopePagesArgs a) {
   const int lane = threadIdx.x & 63;
   const int64_t work = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 6);
@@ -159,7 +159,7 @@ __global__ __launch_bounds__(256) void rope_pages_kernel(RopePagesArgs a) {
     else
       dst = a.v + page * a.v_ps + (h - a.qh - a.kh) * a.v_hs + row * a.v_rs;
     if (kind == 0 || stored) {
-      if (a.streaming) {
+      if constexpr (STREAM) {
         __builtin_nontemporal_store(xa, reinterpret_cast<u32x4*>(dst + 8 * ua));
         __builtin_nontemporal_store(xb, reinterpret_cast<u32x4*>(dst + 8 * ub));
       } else {
@@ -255,15 +255,23 @@ extern "C" int fpv2_rope_to_pages(const void* qkv, const void* q_weight, const v
   // many tokens overflow.  8192 tokens of 32 / 8 heads, D = 128: one round 44.5 us, two
   // 42.6, all six 49.4; with such stores 42.5, 39.7 (5.2 TB/s) and 42.4 us.
   const int heads = a.qh + 2 * a.kh, per_wave = 64 / a.lanes;
-  a.streaming = p.tokens >= 8 * static_cast<int64_t>(cu_count());
-  a.chunk = a.streaming ? 2 * per_wave : per_wave;
+  const bool many = p.tokens >= 8 * static_cast<int64_t>(cu_count());
+  a.chunk = many ? 2 * per_wave : per_wave;
   a.chunks = (heads + a.chunk - 1) / a.chunk;
   const int64_t grid = (p.tokens * a.chunks + 3) / 4;
   if (grid > 0x7fffffff) return fail(FPV2_ERR_ARGUMENT, "%s: too many tokens", name);
   const hipStream_t s = static_cast<hipStream_t>(stream);
-  if (dtype == FPV2_BF16)
-    hipLaunchKernelGGL(rope_pages_kernel<bf16_t>, dim3(static_cast<unsigned>(grid)), dim3(256), 0, s, a);
-  else
-    hipLaunchKernelGGL(rope_pages_kernel<f16_t>, dim3(static_cast<unsigned>(grid)), dim3(256), 0, s, a);
+  const dim3 blocks(static_cast<unsigned>(grid)), threads(256);
+  if (dtype == FPV2_BF16) {
+    if (many)
+      hipLaunchKernelGGL((rope_pages_kernel<bf16_t, true>), blocks, threads, 0, s, a);
+    else
+      hipLaunchKernelGGL((rope_pages_kernel<bf16_t, false>), blocks, threads, 0, s, a);
+  } else {
+    if (many)
+      hipLaunchKernelGGL((rope_pages_kernel<f16_t, true>), blocks, threads, 0, s, a);
+    else
+      hipLaunchKernelGGL((rope_pages_kernel<f16_t, false>), blocks, threads, 0, s, a);
+  }
   return check_launch("rope_pages_kernel");
 }

@@ -12,11 +12,15 @@
 // A short row is one workgroup's.  A long one takes passes over chunks of it, bound by
 // reading the logits (the second and third time from the caches):
 //   1. the greatest logit;
-//   2. a histogram of count and weight over (max - logit) / temperature, or the
-//      chunks' sums where the row has neither top-k nor top-p;
-//   3. the tokens of the histogram's bins that hold the borders go to a list, the ones
-//      above them into the chunks' sums;
-//   4. one workgroup finds the borders in the list and the token in its chunk.
+//   2. a histogram over (max - logit) / temperature, of the count and with top-p alone of
+//      the weight, or the chunks' sums where the row has neither top-k nor top-p;
+//   3. the tokens of the histogram's bin that holds the border go to a list, the ones
+//      above it into the chunks' sums, or where they are few to the list too;
+//   4. one workgroup finds the borders in the list and the token in it, or in its chunk.
+// What bounds it: for one row the four launches, each a chain of loads and barriers (151936
+// float32 logits with top-k and top-p: 3.0 + 5.2 + 6.0 + 7.6 us); for many the
+// second pass's float64 (48 bf16 rows of 151936 with settings of their own: 6 + 22 + 14 +
+// 13 us; 160 float32 rows of 50001 with min-p: 9 + 8 + 7 us, 3.5 TB/s in the first).
 #include "fpv2_common.h"
 #include "fpv2_decode.h"
 
@@ -31,12 +35,14 @@ constexpr int kWeightBits = 44;
 constexpr int kIndexBits = 20;
 constexpr int kRankBits = 32 + kIndexBits;
 constexpr int kBins = 1024;     // of the histogram,
-constexpr double kPerUnit = 32; // so many to a unit of the exponent
+constexpr float kPerUnit = 32; // so many to a unit of the exponent
 constexpr int kList = 4096;     // tokens of a row's list
 constexpr int kChunkList = 512; // of which a chunk's workgroup collects in LDS
 constexpr int kMaxChunks = 256;
 constexpr int kEach = 8;        // tokens of a thread where one is searched for
 constexpr int kFew = kFinishThreads / 2;  // tokens that are compared with one another
+constexpr int kMostChunk = kFinishThreads * kEach;
+constexpr int kRoots = 64;      // powers 2^(k / kRoots) of which a weight is made
 
 struct SampleArgs {
   const void* logits;
@@ -105,6 +111,9 @@ struct Row {
   uint32_t top;     // greatest key
   float top_logit;
   double max, inv;  // the same, 1 / temperature
+  double scale;     // kRoots log2 e / temperature
+  const double* roots;
+  float bins;       // of the histogram to a unit of the logits
   u64 least;        // weight from which on min_p keeps
   float reached;    // temperature, rounded up
   float from;       // a logit below all that min_p keeps with any weight
@@ -135,14 +144,18 @@ __device__ __forceinline__ Settings load_settings(const SampleArgs& a, int b) {
           a.min_ps ? a.min_ps[b] : a.min_p, a.top_ks ? a.top_ks[b] : a.top_k};
 }
 template <typename T>
-__device__ __forceinline__ Row row_with(const SampleArgs& a, int b, const Settings& set, u64 best) {
+__device__ __forceinline__ Row row_with(const SampleArgs& a, int b, const Settings& set, u64 best,
+                                        const double* roots) {
   Row r;
+  r.roots = roots;
   r.logits = row_of<T>(a, b);
   r.top = key_in(best);
   r.max = r.top_logit = logit_of(r.top);
   const double temperature = fmin(set.temperature, 1e30);
   r.greedy = r.top <= kLeastKey || !(set.temperature > 0);
   r.inv = fmin(1.0 / temperature, 1e300);
+  r.scale = r.inv * (1.4426950408889634 * kRoots);
+  r.bins = static_cast<float>(fmin(kPerUnit * r.inv, 1e38));
   r.top_p = set.top_p;
   r.top_k = set.top_k;
   if (r.top_k < 0 || r.top_k >= a.vocab) r.top_k = 0;
@@ -154,35 +167,55 @@ __device__ __forceinline__ Row row_with(const SampleArgs& a, int b, const Settin
   return r;
 }
 
-// log of a logit's weight (it rises with the logit), and the weight of a log.
-// Without branches: a pass's threads do this for every logit.
+// log of a logit's weight.
 __device__ __forceinline__ double exponent_of(const Row& r, float x) {
-  const double z = (static_cast<double>(without_nan(x)) - r.max) * r.inv;
-  return x == r.top_logit ? 0.0 : z;  // (an infinite one has no difference)
+  return x == r.top_logit ? 0.0 : (static_cast<double>(without_nan(x)) - r.max) * r.inv;
 }
-__device__ __forceinline__ u64 weight_at(double z) {
-  // exp z = 2^n e^f, |f| <= ln 2 / 2: the series to f^12 / 12! leaves 2^-52.  Rounded to
-  // an integer by the sum with 2^52, whose mantissa it then is.
-  z = fmax(z, -64.0);
-  const double n = __builtin_rint(z * 1.4426950408889634);
-  const double f = __builtin_fma(n, -0.6931471805599453, z);
-  double p = 1.0 / 479001600;
-  constexpr double c[] = {1.0 / 39916800, 1.0 / 3628800, 1.0 / 362880, 1.0 / 40320, 1.0 / 5040, 1.0 / 720,
-                          1.0 / 120, 1.0 / 24, 1.0 / 6, 0.5, 1.0, 1.0};
+// (by the workgroup's first threads, before a barrier: the series leaves 2^-62)
+__device__ __forceinline__ void fill_roots(double* roots) {
+  if (threadIdx.x < kRoots) {
+    const double f = threadIdx.x * (0.6931471805599453 / kRoots);
+    double p = 1;
 #pragma unroll
-  for (int i = 0; i < 12; ++i) p = __builtin_fma(p, f, c[i]);
-  const double w = __builtin_ldexp(p, static_cast<int>(n) + kWeightBits);
-  return static_cast<u64>(__double_as_longlong(w + 4503599627370496.0)) & 0xfffffffffffffull;
+    for (int i = 17; i > 0; --i) p = __builtin_fma(p, f * (1.0 / i), 1.0);
+    roots[threadIdx.x] = p;
+  }
 }
-__device__ __forceinline__ u64 weight_of(const Row& r, uint32_t key) {
-  return weight_at(exponent_of(r, logit_of(key)));
+// Weight of a logit, without branches, as a pass's threads do this for every logit:
+// e^z = 2^((n + f) / kRoots), |f| <= 1/2, is root n mod kRoots with n / kRoots added to its
+// exponent, times the series in f to the fifth power, which leaves 2^-54.  n and the
+// rounding to an integer come of sums with a large number, whose low bits they are.
+// (Half as many instructions in float64 as the series on |z| <= ln 2 / 2: the second pass
+// over 48 rows of 151936 without limits took 17.6 us, and takes 14.3.)
+__device__ __forceinline__ u64 weight_of(const Row& r, float x) {
+  const double d = static_cast<double>(without_nan(x)) - r.max;
+  const double t = fmax((x == r.top_logit ? 0.0 : d) * r.scale, -64.0 * kRoots);  // (no weight there)
+  constexpr double kWhole = 6755399441055744.0;  // 1.5 * 2^52
+  const double whole = t + kWhole;
+  const int n = static_cast<int>(__double_as_longlong(whole));
+  const double f = t - (whole - kWhole);
+  constexpr double l = 0.6931471805599453 / kRoots;
+  double p = l * l * l * l * l / 120;
+  p = __builtin_fma(p, f, l * l * l * l / 24);
+  p = __builtin_fma(p, f, l * l * l / 6);
+  p = __builtin_fma(p, f, l * l / 2);
+  p = __builtin_fma(p, f, l);
+  p = __builtin_fma(p, f, 1.0);
+  const u64 root = static_cast<u64>(__double_as_longlong(r.roots[n & (kRoots - 1)]));
+  const u64 power = static_cast<u64>(static_cast<uint32_t>((n >> 6) + kWeightBits) << 20) << 32;
+  const double w = __builtin_fma(__longlong_as_double(static_cast<long long>(root + power)), p, 4503599627370496.0);
+  return static_cast<u64>(__double_as_longlong(w)) & 0xfffffffffffffull;
 }
-__device__ __forceinline__ int bin_at(double z) {
-  return min(static_cast<int>(fmin(z * -kPerUnit, static_cast<double>(kBins))), kBins - 1);
+static_assert(kRoots == 1 << 6, "a weight's power");
+// Bin of a logit: any number that doesn't fall where the logit rises will do, for what
+// lies in a bin is decided by ranks.
+__device__ __forceinline__ int bin_of(const Row& r, float x) {
+  const float down = (r.top_logit - without_nan(x)) * r.bins;
+  return x == r.top_logit ? 0 : static_cast<int>(fminf(down, static_cast<float>(kBins - 1)));
 }
 // Weight of a token if min_p keeps it.
 __device__ __forceinline__ u64 likely_weight(const Row& r, float x) {
-  const u64 w = weight_at(exponent_of(r, x));
+  const u64 w = weight_of(r, x);
   return w >= r.least ? w : 0;
 }
 
@@ -224,37 +257,97 @@ __device__ __forceinline__ u64 across(u64 v, u64* sh) {
   return v;
 }
 
-// f(i, logit) for the tokens [lo, hi) of a row, in any order, by THREADS threads:
-// 16-byte loads from the first aligned logit on.
+// f(i, logits) is called for logits of token i and the next ones: the 16 bytes of a
+// load, or one.
+template <int N>
+struct Logits {
+  float x[N];
+  __device__ __forceinline__ float greatest() const {  // (NaN if all are)
+    float m = x[0];
+#pragma unroll
+    for (int j = 1; j < N; ++j) m = fmaxf(m, x[j]);
+    return m;
+  }
+};
+template <typename T, typename F>
+__device__ __forceinline__ void with_vector(int i, u32x4 v, F f) {
+  constexpr int N = 16 / kLogitBytes<T>;
+  Logits<N> logits;
+#pragma unroll
+  for (int j = 0; j < N; ++j) logits.x[j] = logit_in<T>(v, j);
+  f(i, logits);
+}
+// The tokens [lo, hi) of a row: whole vectors from the first aligned logit on, and a
+// thread's token before or after them.
+template <typename T, int THREADS>
+struct Span {
+  static constexpr int N = 16 / kLogitBytes<T>;
+  int first, vectors, edge;  // edge: -1 for none
+  const char* at;
+  __device__ __forceinline__ Span(const void* row, int lo, int hi) {
+    const uintptr_t from = reinterpret_cast<uintptr_t>(row) + static_cast<uintptr_t>(lo) * kLogitBytes<T>;
+    const int head = min(hi - lo, static_cast<int>((16 - from % 16) % 16) / kLogitBytes<T>);
+    const int tid = threadIdx.x;
+    first = lo + head;
+    vectors = (hi - first) / N;
+    const int last = first + N * vectors;
+    edge = tid < head ? lo + tid : last + tid - head;
+    if (edge >= hi || tid >= 2 * N) edge = -1;
+    at = static_cast<const char*>(row) + static_cast<int64_t>(first) * kLogitBytes<T>;
+  }
+  __device__ __forceinline__ u32x4 load(int v) const { return load16(at + 16 * static_cast<int64_t>(v)); }
+};
+// A workgroup's chunk, loaded at once: before the pass has its row's settings.
+template <typename T>
+struct Chunk {
+  using Vectors = Span<T, kChunkThreads>;
+  static constexpr int kEachThread = kMostChunk / (Vectors::N * kChunkThreads);
+  Vectors span;
+  u32x4 v[kEachThread];
+  float edge;
+  __device__ __forceinline__ Chunk(const SampleArgs& a, const void* row, int c)
+      : span(row, c * a.chunk, min(a.vocab, (c + 1) * a.chunk)) {
+#pragma unroll
+    for (int k = 0; k < kEachThread; ++k) {
+      const int i = threadIdx.x + k * kChunkThreads;
+      v[k] = u32x4{};
+      if (i < span.vectors) v[k] = span.load(i);
+    }
+    edge = span.edge >= 0 ? logit_at<T>(row, span.edge) : 0.f;
+  }
+  template <typename F>
+  __device__ __forceinline__ void for_vectors(F f) const {
+    if (span.edge >= 0) f(span.edge, Logits<1>{{edge}});
+#pragma unroll
+    for (int k = 0; k < kEachThread; ++k) {
+      const int i = threadIdx.x + k * kChunkThreads;
+      if (i < span.vectors) with_vector<T>(span.first + Vectors::N * i, v[k], f);
+    }
+  }
+};
+// f(i, logit) for the tokens [lo, hi) of a row, in any order, by THREADS threads.
 template <typename T, int THREADS, typename F>
 __device__ __forceinline__ void for_each(const void* row, int lo, int hi, F f) {
-  constexpr int N = 16 / kLogitBytes<T>;
-  const uintptr_t at = reinterpret_cast<uintptr_t>(row) + static_cast<uintptr_t>(lo) * kLogitBytes<T>;
-  const int head = min(hi - lo, static_cast<int>((16 - at % 16) % 16) / kLogitBytes<T>);
-  const int tid = threadIdx.x;
-  const int first = lo + head, vectors = (hi - first) / N, last = first + N * vectors;
-  const int edge = tid < head ? lo + tid : last + tid - head;
-  if (edge < hi && tid < 2 * N) f(edge, logit_at<T>(row, edge));
-  const char* p = static_cast<const char*>(row) + static_cast<int64_t>(first) * kLogitBytes<T>;
+  const Span<T, THREADS> span(row, lo, hi);
+  if (span.edge >= 0) f(span.edge, logit_at<T>(row, span.edge));
 #pragma unroll 1
-  for (int v = tid; v < vectors; v += THREADS) {
-    const u32x4 x = load16(p + 16 * static_cast<int64_t>(v));
+  for (int v = threadIdx.x; v < span.vectors; v += THREADS)
+    with_vector<T>(span.first + span.N * v, span.load(v), [&](int i, const Logits<span.N>& logits) {
 #pragma unroll
-    for (int j = 0; j < N; ++j) f(first + N * v + j, logit_in<T>(x, j));
-  }
+      for (int j = 0; j < span.N; ++j) f(i + j, logits.x[j]);
+    });
 }
 
-// The greatest rank of a thread's tokens of [lo, hi).
-template <typename T, int THREADS>
-__device__ __forceinline__ u64 best_of(const void* row, int lo, int hi) {
-  float best = neg_inf();
-  int at = hi;
-  for_each<T, THREADS>(row, lo, hi, [&](int i, float x) {
-    at = x > best || (x == best && i < at) ? i : at;
-    best = fmaxf(x, best);
-  });
-  return at < hi ? rank_of(key_of(best), at) : 0;
-}
+// The greatest rank of tokens, one after the other.
+struct Best {
+  float logit = neg_inf();
+  int at = 1 << kIndexBits;
+  __device__ __forceinline__ void add(int i, float x) {
+    at = x > logit || (x == logit && i < at) ? i : at;
+    logit = fmaxf(x, logit);
+  }
+  __device__ __forceinline__ u64 rank() const { return at < 1 << kIndexBits ? rank_of(key_of(logit), at) : 0; }
+};
 
 struct Shared {
   u64 sums[kRowThreads / 64];
@@ -399,6 +492,15 @@ __device__ __forceinline__ void write_greedy(const SampleArgs& a, int b, u64 bes
   if (a.logprobs) a.logprobs[b] = none ? -__builtin_inff() : 0.f;
 }
 
+__device__ __forceinline__ double target_of(const SampleArgs& a, int b, u64 all) {
+  return fmin(fmax(static_cast<double>(a.uniforms[b]), 0.0), 1.0) * static_cast<double>(all);
+}
+__device__ __forceinline__ void write_token(const SampleArgs& a, const Row& r, int b, int token, float logit, u64 all) {
+  a.tokens[b] = token;
+  if (a.logprobs)
+    a.logprobs[b] = static_cast<float>(exponent_of(r, logit) - log(static_cast<double>(all) / (1ull << kWeightBits)));
+}
+
 // The token: kept weight `all`, of which `before` lies before the tokens [lo, hi), where
 // the one searched for is.
 template <typename T, int THREADS>
@@ -410,15 +512,7 @@ __device__ void pick(const SampleArgs& a, const Row& r, int b, u64 least, u64 al
   };
   const int token = min(hi - 1, find_first<THREADS>(
       lo, hi, before, kept, [&](u64 w) { return static_cast<double>(w) > target || w == all; }, sh));
-  if (threadIdx.x == 0) {
-    a.tokens[b] = token;
-    if (a.logprobs)
-      a.logprobs[b] = static_cast<float>(exponent_of(r, logit_at<T>(r.logits, token)) -
-                                         log(static_cast<double>(all) / (1ull << kWeightBits)));
-  }
-}
-__device__ __forceinline__ double target_of(const SampleArgs& a, int b, u64 all) {
-  return fmin(fmax(static_cast<double>(a.uniforms[b]), 0.0), 1.0) * static_cast<double>(all);
+  if (threadIdx.x == 0) write_token(a, r, b, token, logit_at<T>(r.logits, token), all);
 }
 
 // Kept weight of each chunk into LDS and of the row, then the token.
@@ -460,8 +554,12 @@ template <typename T>
 __global__ __launch_bounds__(kRowThreads) void sample_row_kernel(SampleArgs a) {
   __shared__ Shared sh;
   const int b = blockIdx.x;
-  const u64 best = across<kRowThreads, true>(best_of<T, kRowThreads>(row_of<T>(a, b), 0, a.vocab), sh.sums);
-  const Row r = row_with<T>(a, b, load_settings(a, b), best);
+  __shared__ double roots[kRoots];
+  fill_roots(roots);
+  Best mine;
+  for_each<T, kRowThreads>(row_of<T>(a, b), 0, a.vocab, [&](int i, float x) { mine.add(i, x); });
+  const u64 best = across<kRowThreads, true>(mine.rank(), sh.sums);
+  const Row r = row_with<T>(a, b, load_settings(a, b), best, roots);
   if (r.greedy) {
     if (threadIdx.x == 0) write_greedy(a, b, best);
     return;
@@ -470,12 +568,12 @@ __global__ __launch_bounds__(kRowThreads) void sample_row_kernel(SampleArgs a) {
   if (r.limited) {
     u64 all = 0;
     if (r.top_k == 0) {
-      for_each<T, kRowThreads>(r.logits, 0, a.vocab, [&](int, float x) { all += weight_at(exponent_of(r, x)); });
+      for_each<T, kRowThreads>(r.logits, 0, a.vocab, [&](int, float x) { all += weight_of(r, x); });
       all = across<kRowThreads, false>(all, sh.sums);
     }
     least = border_of<kRowThreads>(r, [&](auto f) {
       for_each<T, kRowThreads>(r.logits, 0, a.vocab, [&](int i, float x) {
-        f(rank_of(key_of(x), i), [&] { return weight_at(exponent_of(r, x)); });
+        f(rank_of(key_of(x), i), [&] { return weight_of(r, x); });
       });
     }, 0, 0, all, sh);
   }
@@ -493,6 +591,7 @@ template <typename T>
 __global__ __launch_bounds__(kChunkThreads) void chunk_max_kernel(SampleArgs a) {
   __shared__ u64 sh[kChunkThreads / 64];
   const int c = blockIdx.x, b = blockIdx.y, tid = threadIdx.x;
+  const Chunk<T> chunk(a, row_of<T>(a, b), c);
   // (the row's histogram and list for the next passes)
   if (a.counts != nullptr) {
     for (int i = c * kChunkThreads + tid; i < kBins; i += a.chunks * kChunkThreads) {
@@ -501,8 +600,13 @@ __global__ __launch_bounds__(kChunkThreads) void chunk_max_kernel(SampleArgs a) 
     }
     if (c == 0 && tid == 0) a.listed[b] = 0;
   }
-  const u64 best = across<kChunkThreads, true>(
-      best_of<T, kChunkThreads>(row_of<T>(a, b), c * a.chunk, min(a.vocab, (c + 1) * a.chunk)), sh);
+  Best mine;
+  chunk.for_vectors([&](int i, const auto& logits) {
+    constexpr int N = sizeof(logits) / sizeof(float);
+#pragma unroll
+    for (int j = 0; j < N; ++j) mine.add(i + j, logits.x[j]);
+  });
+  const u64 best = across<kChunkThreads, true>(mine.rank(), sh);
   if (tid == 0) a.best[static_cast<int64_t>(b) * a.chunks + c] = best;
 }
 
@@ -516,6 +620,13 @@ __device__ __forceinline__ u64 row_best(const SampleArgs& a, int b, u64* sh) {
   return across<THREADS, true>(best, sh);
 }
 
+// The row of a workgroup in a grid of [chunks][batch].  Rows differ in what they need: one
+// after the other, and shifted by one from chunk to chunk, they spread over the CUs
+// in whatever order kinds of rows come.  (The second pass over 48 rows of 151936 in an
+// order of six kinds: 26.1 us with a row's chunks one after the other, when a CU had
+// eight of a kind, against 23.8.)
+__device__ __forceinline__ int spread_row() { return (blockIdx.x + blockIdx.y) % gridDim.x; }
+
 // a.group chunks by a workgroup: one histogram of them in LDS, so that fewer are
 // added to the row's (each line of it that an atomic goes to is one in memory).
 template <typename T>
@@ -523,16 +634,24 @@ __global__ __launch_bounds__(kChunkThreads) void chunk_weigh_kernel(SampleArgs a
   __shared__ u64 sh[kChunkThreads / 64];
   __shared__ u64 weights[kBins];
   __shared__ uint32_t counts[kBins];
-  const int b = blockIdx.y, tid = threadIdx.x;
-  const int c0 = blockIdx.x * a.group, c1 = min(a.chunks, c0 + a.group);
+  const int b = spread_row(), tid = threadIdx.x;
+  const int c0 = blockIdx.y * a.group, c1 = min(a.chunks, c0 + a.group);
+  Chunk<T> chunk(a, row_of<T>(a, b), c0);
   const Settings set = load_settings(a, b);
-  const Row r = row_with<T>(a, b, set, row_best<kChunkThreads>(a, b, sh));
+  __shared__ double roots[kRoots];
+  fill_roots(roots);
+  const Row r = row_with<T>(a, b, set, row_best<kChunkThreads>(a, b, sh), roots);
   if (r.greedy) return;
   if (!r.limited) {
     for (int c = c0; c < c1; ++c) {
+      if (c > c0) chunk = Chunk<T>(a, r.logits, c);
       u64 sum = 0;
-      for_each<T, kChunkThreads>(r.logits, c * a.chunk, min(a.vocab, (c + 1) * a.chunk),
-                                 [&](int, float x) { if (x >= r.from) sum += likely_weight(r, x); });
+      chunk.for_vectors([&](int, const auto& logits) {
+        if (!(logits.greatest() >= r.from)) return;
+        constexpr int N = sizeof(logits) / sizeof(float);
+#pragma unroll
+        for (int j = 0; j < N; ++j) sum += likely_weight(r, logits.x[j]);
+      });
       sum = across<kChunkThreads, false>(sum, sh);
       if (tid == 0) a.sums[static_cast<int64_t>(b) * a.chunks + c] = sum;
     }
@@ -540,21 +659,38 @@ __global__ __launch_bounds__(kChunkThreads) void chunk_weigh_kernel(SampleArgs a
   }
   for (int i = tid; i < kBins; i += kChunkThreads) weights[i] = 0, counts[i] = 0;
   __syncthreads();
-  const bool weigh = r.top_p < 1;
+  const bool weigh = r.top_k == 0;  // (with top_k the borders' list is weighed)
   uint32_t far = 0;  // of the last bin, where masked tokens are
   u64 far_weight = 0;
-  for_each<T, kChunkThreads>(r.logits, c0 * a.chunk, min(a.vocab, c1 * a.chunk), [&](int, float x) {
-    const double z = exponent_of(r, x);
-    const int bin = bin_at(z);
-    const u64 w = weigh ? weight_at(z) : 0;
-    if (bin == kBins - 1) {
-      ++far;
-      far_weight += w;
-    } else {
-      atomicAdd(&counts[bin], 1u);
-      if (weigh) atomicAdd(&weights[bin], w);
+  // (a load's weights before its atomics: the roots that are read in LDS come back in order)
+  const auto add = [&](int, const auto& logits) {
+    constexpr int N = sizeof(logits) / sizeof(float);
+    int bin[N];
+    u64 w[N];
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      bin[j] = bin_of(r, logits.x[j]);
+      w[j] = 0;
     }
-  });
+    if (weigh) {
+#pragma unroll
+      for (int j = 0; j < N; ++j) w[j] = weight_of(r, logits.x[j]);
+    }
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      if (bin[j] == kBins - 1) {
+        ++far;
+        far_weight += w[j];
+      } else {
+        atomicAdd(&counts[bin[j]], 1u);
+        if (weigh) atomicAdd(&weights[bin[j]], w[j]);
+      }
+    }
+  };
+  for (int c = c0; c < c1; ++c) {
+    if (c > c0) chunk = Chunk<T>(a, r.logits, c);
+    chunk.for_vectors(add);
+  }
   if (far > 0) {
     atomicAdd(&counts[kBins - 1], far);
     atomicAdd(&weights[kBins - 1], far_weight);
@@ -581,15 +717,11 @@ struct HistShare {
   u64 w[kShare];
 };
 __device__ __forceinline__ HistShare load_hist(const SampleArgs& a, int b) {
-  HistShare h;
-  const int tid = threadIdx.x;
-#pragma unroll
-  for (int j = 0; j < kShare; ++j) {
-    h.c[j] = 0, h.w[j] = 0;
-    if (tid < 256 && a.counts != nullptr) {
-      h.c[j] = a.counts[static_cast<int64_t>(b) * kBins + tid * kShare + j];
-      h.w[j] = a.weights[static_cast<int64_t>(b) * kBins + tid * kShare + j];
-    }
+  HistShare h{};
+  const int64_t at = static_cast<int64_t>(b) * kBins + threadIdx.x * kShare;
+  if (threadIdx.x < 256 && a.counts != nullptr) {
+    __builtin_memcpy(h.c, __builtin_assume_aligned(a.counts + at, 16), sizeof(h.c));
+    __builtin_memcpy(h.w, __builtin_assume_aligned(a.weights + at, 16), sizeof(h.w));
   }
   return h;
 }
@@ -639,7 +771,9 @@ __device__ Bins bins_of(const HistShare& h, const Row& r) {
   Bins s;
   s.hi = static_cast<int>(found[0]);
   s.all = all;
-  if (r.top_k > 0 && r.top_p < 1) {  // both: the whole list, for top_p's border lies in it
+  // all down to the bin for both limits, as top_p's border may lie anywhere above, and for
+  // few tokens, among which the token is found without its chunk
+  if ((r.top_k > 0 && r.top_p < 1) || found[1] + found[3] <= kFew) {
     s.lo = 0;
     s.above = 0;
     s.above_weight = 0;
@@ -658,16 +792,17 @@ __global__ __launch_bounds__(kChunkThreads) void chunk_list_kernel(SampleArgs a)
   __shared__ u64 sh[kChunkThreads / 64];
   __shared__ u64 list[kChunkList];
   __shared__ uint32_t listed, at;
-  const int b = blockIdx.y, tid = threadIdx.x;
-  const int c0 = blockIdx.x * a.group, c1 = min(a.chunks, c0 + a.group);
+  const int b = spread_row(), tid = threadIdx.x;
+  const int c0 = blockIdx.y * a.group, c1 = min(a.chunks, c0 + a.group);
+  Chunk<T> chunk(a, row_of<T>(a, b), c0);
   const Settings set = load_settings(a, b);
   const HistShare hist = load_hist(a, b);
-  const Row r = row_with<T>(a, b, set, row_best<kChunkThreads>(a, b, sh));
+  __shared__ double roots[kRoots];
+  fill_roots(roots);
+  const Row r = row_with<T>(a, b, set, row_best<kChunkThreads>(a, b, sh), roots);
   if (!r.limited) return;
   const Bins bins = bins_of(hist, r);
   if (bins.in > kList) return;  // the row's workgroup does it all
-  // (a logit below is in none of the bins: the others are looked at)
-  const float from = bins.hi == kBins - 1 ? neg_inf() : r.reach((bins.hi + 1) / static_cast<float>(kPerUnit));
   // (the list holds as many as the histogram counted, if nobody writes the logits)
   const auto put = [&](uint32_t i, u64 rank) {
     if (i < kList) a.list[static_cast<int64_t>(b) * kList + i] = rank;
@@ -676,22 +811,26 @@ __global__ __launch_bounds__(kChunkThreads) void chunk_list_kernel(SampleArgs a)
   __syncthreads();
   for (int c = c0; c < c1; ++c) {
     u64 sum = 0;
-    for_each<T, kChunkThreads>(r.logits, c * a.chunk, min(a.vocab, (c + 1) * a.chunk), [&](int i, float x) {
-      if (without_nan(x) < from) return;
-      const double z = exponent_of(r, x);
-      const int bin = bin_at(z);
-      if (bin > bins.hi) return;
-      if (bin < bins.lo) {
-        const u64 w = weight_at(z);
-        sum += w >= r.least ? w : 0;
-        return;
+    if (c > c0) chunk = Chunk<T>(a, r.logits, c);
+    chunk.for_vectors([&](int i, const auto& logits) {
+      if (bin_of(r, logits.greatest()) > bins.hi) return;
+      constexpr int N = sizeof(logits) / sizeof(float);
+#pragma unroll
+      for (int j = 0; j < N; ++j) {
+        const float x = logits.x[j];
+        const int bin = bin_of(r, x);
+        if (bin > bins.hi) continue;
+        if (bin < bins.lo) {
+          sum += likely_weight(r, x);
+          continue;
+        }
+        const u64 rank = rank_of(key_of(x), i + j);
+        const uint32_t slot = atomicAdd(&listed, 1u);
+        if (slot < kChunkList)
+          list[slot] = rank;
+        else
+          put(atomicAdd(&a.listed[b], 1u), rank);
       }
-      const u64 rank = rank_of(key_of(x), i);
-      const uint32_t slot = atomicAdd(&listed, 1u);
-      if (slot < kChunkList)
-        list[slot] = rank;
-      else
-        put(atomicAdd(&a.listed[b], 1u), rank);
     });
     sum = across<kChunkThreads, false>(sum, sh);
     if (tid == 0) a.sums[static_cast<int64_t>(b) * a.chunks + c] = sum;
@@ -703,52 +842,84 @@ __global__ __launch_bounds__(kChunkThreads) void chunk_list_kernel(SampleArgs a)
   for (uint32_t i = tid; i < n; i += kChunkThreads) put(at + i, list[i]);
 }
 
-// border_of for at most kFew tokens (rank, 0 for none, of the first threads): the count
-// and weight above each by comparing all with all, half of them by each of two
-// threads.
-__device__ u64 border_of_few(const Row& r, u64 rank, u64 own_weight, const Bins& bins, Shared& sh) {
-  __shared__ u64 ranks[kFew], weights[kFew], half_weight[kFew];
-  __shared__ uint32_t half_count[kFew];
-  const int tid = threadIdx.x, of = tid & (kFew - 1), n = static_cast<int>(bins.in);
-  if (tid < kFew) {
-    ranks[tid] = rank;
-    weights[tid] = own_weight;
+// At most kFew tokens of a list, compared all with all: each token by `parts` lanes next to
+// one another, which have a part of the others each.
+typedef u64 u64x2 __attribute__((ext_vector_type(2)));
+struct Few {
+  u64x2 tokens[kFew];  // rank and weight, 0 for none
+};
+struct Place {
+  int n, parts, token, part;
+  __device__ __forceinline__ explicit Place(int n)
+      : n(n), parts(n <= kFew / 8 ? 16 : n <= kFew / 4 ? 8 : n <= kFew / 2 ? 4 : 2),
+        token(static_cast<int>(threadIdx.x) / parts), part(static_cast<int>(threadIdx.x) % parts) {}
+};
+// Count and weight of the tokens that come before the lane's one.
+template <typename Before>
+__device__ __forceinline__ void sum_before(const Few& few, const Place& at, Before before, u64* count, u64* weight) {
+  const u64 own = few.tokens[at.token][0];
+  uint32_t c = 0;
+  u64 w = 0;
+#pragma unroll 1
+  for (int j = at.part; j < at.n; j += 4 * at.parts) {  // (kFew / parts is a multiple of 4)
+    u64x2 other[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) other[i] = few.tokens[j + i * at.parts];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const bool is = before(other[i][0], own);
+      c += is;
+      w += is ? other[i][1] : 0;
+    }
+  }
+  u64 n = c;
+  n += from_lanes<0xb1, 0xf>(n), w += from_lanes<0xb1, 0xf>(w);  // of pairs of lanes,
+  if (at.parts > 2) n += from_lanes<0x4e, 0xf>(n), w += from_lanes<0x4e, 0xf>(w);    // fours,
+  if (at.parts > 4) n += from_lanes<0x141, 0xf>(n), w += from_lanes<0x141, 0xf>(w);  // eights
+  if (at.parts > 8) n += from_lanes<0x140, 0xf>(n), w += from_lanes<0x140, 0xf>(w);  // and sixteens
+  *count = n;
+  *weight = w;
+}
+// border_of for them (the first kFew threads bring one each).
+__device__ u64 border_of_few(const Row& r, u64 rank, u64 weight, const Bins& bins, const Place& at, Few& few,
+                             Shared& sh) {
+  if (threadIdx.x < kFew) {
+    few.tokens[threadIdx.x][0] = rank;
+    few.tokens[threadIdx.x][1] = weight;
   }
   __syncthreads();
-  const u64 own = ranks[of];
-  uint32_t count = 0;
-  u64 weight = 0;
-  const int from = tid < kFew ? 0 : (n + 1) / 2, to = tid < kFew ? (n + 1) / 2 : n;
-#pragma unroll 4
-  for (int j = from; j < to; ++j) {
-    const bool over = ranks[j] > own;
-    count += over;
-    weight += over ? weights[j] : 0;
-  }
-  if (tid >= kFew) {
-    half_count[of] = count;
-    half_weight[of] = weight;
-  }
-  __syncthreads();
-  const bool is = tid < n;
-  u64 above = bins.above, above_weight = bins.above_weight;
-  if (is) {
-    above += count + half_count[of];
-    above_weight += weight + half_weight[of];
-  }
-  bool kept = is && (r.top_k == 0 || above < static_cast<u64>(r.top_k));
+  u64 above, above_weight;
+  sum_before(few, at, [](u64 other, u64 own) { return other > own; }, &above, &above_weight);
+  above += bins.above;
+  above_weight += bins.above_weight;
+  bool kept = at.token < at.n && (r.top_k == 0 || above < static_cast<u64>(r.top_k));
   if (r.top_p < 1) {
     const u64 all = r.top_k == 0 ? bins.all
-                                 : across<kFinishThreads, true>(kept ? above_weight + weights[of] : 0, sh.sums);
+                                 : across<kFinishThreads, true>(kept ? above_weight + few.tokens[at.token][1] : 0, sh.sums);
     // (the first token has nothing before it: it is kept whatever the share)
     kept = kept && (above == 0 || static_cast<double>(above_weight) < r.top_p * static_cast<double>(all));
   }
-  return ~across<kFinishThreads, true>(kept ? ~own : 0, sh.sums);
+  return ~across<kFinishThreads, true>(kept ? ~few.tokens[at.token][0] : 0, sh.sums);
+}
+
+// The token where all that may be kept are among them.
+__device__ void pick_of_few(const SampleArgs& a, const Row& r, int b, u64 least, const Place& at, Few& few, Shared& sh) {
+  const u64 rank = few.tokens[at.token][0], weight = few.tokens[at.token][1];
+  const u64 w = at.part == 0 && at.token < at.n && rank >= least && weight >= r.least ? weight : 0;
+  if (at.part == 0) few.tokens[at.token][1] = w;
+  const u64 all = across<kFinishThreads, false>(w, sh.sums);
+  u64 count, before;
+  sum_before(few, at, [](u64 other, u64 own) { return index_in(other) < index_in(own); }, &count, &before);
+  const double target = target_of(a, b, all);
+  const auto past = [&](u64 v) { return static_cast<double>(v) > target || v == all; };
+  if (w > 0 && past(before + w) && (before == 0 || !past(before)))
+    write_token(a, r, b, index_in(rank), logit_of(key_in(rank)), all);
 }
 
 template <typename T>
 __global__ __launch_bounds__(kFinishThreads) void sample_finish_kernel(SampleArgs a) {
   __shared__ Shared sh;
+  __shared__ Few few;
   __shared__ u64 chunk_sums[kMaxChunks];
   const int b = blockIdx.x, tid = threadIdx.x;
   const Settings set = load_settings(a, b);
@@ -759,8 +930,10 @@ __global__ __launch_bounds__(kFinishThreads) void sample_finish_kernel(SampleArg
 #pragma unroll
   for (int j = 0; j < kList / kFinishThreads; ++j)
     mine[j] = a.counts != nullptr ? list[tid + j * kFinishThreads] : 0;
+  __shared__ double roots[kRoots];
+  fill_roots(roots);
   const u64 best = row_best<kFinishThreads>(a, b, sh.sums);
-  const Row r = row_with<T>(a, b, set, best);
+  const Row r = row_with<T>(a, b, set, best, roots);
   if (r.greedy) {
     if (tid == 0) write_greedy(a, b, best);
     return;
@@ -775,14 +948,20 @@ __global__ __launch_bounds__(kFinishThreads) void sample_finish_kernel(SampleArg
       u64 weight[kList / kFinishThreads];
 #pragma unroll
       for (int j = 0; j < kList / kFinishThreads; ++j)
-        weight[j] = mine[j] != 0 ? weight_of(r, key_in(mine[j])) : 0;
+        weight[j] = j * kFinishThreads < bins.in && mine[j] != 0 ? weight_of(r, logit_of(key_in(mine[j]))) : 0;
       const auto each = [&](auto f) {
 #pragma unroll
         for (int j = 0; j < kList / kFinishThreads; ++j)
           if (mine[j] != 0) f(mine[j], [&] { return weight[j]; });
       };
-      least = bins.in <= kFew ? border_of_few(r, mine[0], weight[0], bins, sh)
-                              : border_of<kFinishThreads>(r, each, bins.above, bins.above_weight, bins.all, sh);
+      const bool is_few = bins.in <= kFew;
+      const Place place(static_cast<int>(bins.in));
+      least = is_few ? border_of_few(r, mine[0], weight[0], bins, place, few, sh)
+                     : border_of<kFinishThreads>(r, each, bins.above, bins.above_weight, bins.all, sh);
+      if (is_few && bins.lo == 0) {
+        pick_of_few(a, r, b, least, place, few, sh);
+        return;
+      }
       __syncthreads();
       if (tid < a.chunks) chunk_sums[tid] = sum;
       __syncthreads();
@@ -793,7 +972,7 @@ __global__ __launch_bounds__(kFinishThreads) void sample_finish_kernel(SampleArg
     } else {  // more tokens than a list holds: by the row itself
       least = border_of<kFinishThreads>(r, [&](auto f) {
         for_each<T, kFinishThreads>(r.logits, 0, a.vocab, [&](int i, float x) {
-        f(rank_of(key_of(x), i), [&] { return weight_at(exponent_of(r, x)); });
+        f(rank_of(key_of(x), i), [&] { return weight_of(r, x); });
       });
       }, 0, 0, bins.all, sh);
       for (int c = 0; c < a.chunks; ++c) {
@@ -813,7 +992,7 @@ __global__ __launch_bounds__(kFinishThreads) void sample_finish_kernel(SampleArg
 
 // Chunks of a row in a call (0: a workgroup has a whole row).
 constexpr int kShortRow = 4096;
-constexpr int kLeastChunk = 2048, kMostChunk = kFinishThreads * kEach;
+constexpr int kLeastChunk = 2048;
 int chunks_of(int64_t batch, int64_t vocab) {
   if (vocab <= kShortRow) return 0;
   const int64_t least = (vocab + kMostChunk - 1) / kMostChunk;
@@ -864,7 +1043,7 @@ int launch_sample(const SampleArgs& a, int64_t batch, hipStream_t s) {
   }
   const dim3 chunks(static_cast<unsigned>(a.chunks), static_cast<unsigned>(batch));
   hipLaunchKernelGGL(chunk_max_kernel<T>, chunks, threads, 0, s, a);
-  const dim3 groups(static_cast<unsigned>((a.chunks + a.group - 1) / a.group), static_cast<unsigned>(batch));
+  const dim3 groups(static_cast<unsigned>(batch), static_cast<unsigned>((a.chunks + a.group - 1) / a.group));
   hipLaunchKernelGGL(chunk_weigh_kernel<T>, groups, threads, 0, s, a);
   if (a.counts != nullptr) hipLaunchKernelGGL(chunk_list_kernel<T>, groups, threads, 0, s, a);
   hipLaunchKernelGGL(sample_finish_kernel<T>, rows, dim3(kFinishThreads), 0, s, a);

@@ -218,3 +218,25 @@ def test_settings_out_of_range_in_tensors(cuda):
     assert torch.equal(hot, fpv2.sample_tokens(dev, u.to(cuda), temperature=1e30))
     top = fpv2.sample_tokens(dev, u.to(cuda), min_p=torch.full((4,), 9.0, device=cuda))
     assert torch.equal(top.cpu(), logits.argmax(1))
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_borders_of_each_kind(cuda, dtype):
+    """Long rows whose borders have few tokens above them, many above and few next to
+    them, hundreds and thousands next to them."""
+    gen = torch.Generator().manual_seed(8)
+    vocab = 40_009
+    logits = 0.5 * torch.randn((6, vocab), generator=gen) - 30
+    at = torch.randperm(vocab, generator=gen)
+    logits[:, at[:5]] = 9 + torch.rand((6, 5), generator=gen)
+    logits[:, at[5:1005]] = 2 + 4 * torch.rand((6, 1000), generator=gen)
+    logits[:, at[1005:1705]] = 1 + 0.01 * torch.rand((6, 700), generator=gen)
+    logits[:, at[1705:7705]] = -1 + 0.01 * torch.rand((6, 6000), generator=gen)
+    logits = logits.to(dtype)
+    u = torch.tensor([0.0, 1.0, 0.25, 0.5, 0.75, 0.9375])
+    for top_p in (0.01, 0.2, 0.6, 0.9, 0.955, 0.975, 0.985, 0.99, 0.998, 0.9999):
+        _check(cuda, logits, u, top_p=top_p)
+        _check(cuda, logits, u, top_p=top_p, top_k=900, min_p=1e-6)
+    for top_k in (3, 31, 33, 64, 127, 129, 255, 256, 257, 300, 1300, 1705, 4000, 30_000):
+        _check(cuda, logits, u, top_k=top_k)
+        _check(cuda, logits, u, top_k=top_k, top_p=0.97, temperature=1.5)

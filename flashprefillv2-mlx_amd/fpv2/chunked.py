@@ -53,7 +53,7 @@ from dataclasses import replace
 import torch
 
 from fpv2 import _lib
-from fpv2.decode import decode_attention
+from fpv2.decode import _device as check_device, decode_attention
 from fpv2.kernel import SUPPORTED_HEAD_DIMS, _launch_attention
 from fpv2.patch import (SelectedBlockCounter, _causal_block_count, _effective_config, _geometry,
                         _pool_into, _request_config, _select_attend)
@@ -346,15 +346,21 @@ class ChunkedPrefill:
             raise ValueError("q must be [query_heads, 1, head_dim] of the cache's geometry and dtype")
         if (k is None) != (v is None):
             raise ValueError("k and v are given together")
-        if out is not None and (out.shape != q3.shape or out.dtype != self.dtype):
-            raise ValueError("out must be [query_heads, 1, head_dim] of q's dtype")
+        # (all that could be refused is looked at before the token is appended)
+        if out is not None and (out.shape != q3.shape or out.dtype != self.dtype
+                                or out.stride(2) != 1
+                                or self.query_heads > 1 and out.stride(0) < self.head_dim):
+            raise ValueError("out must be [query_heads, 1, head_dim] of q's dtype with contiguous "
+                             "rows and no overlap")
+        check_device([x for x in (q3, self.k, k, v, out) if x is not None])
         if k is not None:
             k, v = self._rows(k, v)
             if k.shape[1] != 1:
                 raise ValueError("decode takes one token's keys and values")
-            self.append(k, v)
-        if self.length == 0:
+        elif self.length == 0:
             raise ValueError("query length cannot exceed key length for causal attention")
+        if k is not None:
+            self.append(k, v)
         res = decode_attention(q3.transpose(0, 1), *self.pages(), None, self.length, scale=scale,
                                out=None if out is None else out.transpose(0, 1))
         return res.transpose(0, 1)[None]

@@ -256,6 +256,9 @@ def rope_to_pages(qkv: torch.Tensor, q_weight: torch.Tensor | None, k_weight: to
     if kv_heads == 0 or qkv.shape[1] != (query_heads + 2 * kv_heads) * dim:
         raise ValueError("qkv rows must hold the query, key and value heads")
     page_strides = _page_strides(k_pages, v_pages)
+    if min(page_strides) < dim and any(
+            n > 1 and s < dim for n, s in zip((pages, kv_heads, page_size) * 2, page_strides)):
+        raise ValueError("the caches' rows overlap")
     for name, t in (("q_weight", q_weight), ("k_weight", k_weight)):
         if t is not None and (t.shape != (dim,) or t.dtype != qkv.dtype or t.data_ptr() & 15
                               or not t.is_contiguous()):
@@ -372,9 +375,8 @@ def quantized_linear(x: torch.Tensor, packed: torch.Tensor, scales: torch.Tensor
     ``out``: optional ``[M, N]`` destination (``x`` ``[M, K]``) with contiguous
     rows.  Products and sums are in float32 with the weights exact; ``x`` must be
     below 1e34 (an infinite value gives NaN).  Made for the few rows of a decode
-    step: the weights are read once for every 16 rows or more (64 with groups
-    of 128), so a large prompt is better served by a product with
-    ``dequantize_weight``'s result."""
+    step: the weights are read once for every 32 rows, so a large prompt is better
+    served by a product with ``dequantize_weight``'s result."""
     if x.ndim < 1 or x.dtype not in _HALF:
         raise ValueError("x must be [..., in] in float16 or bfloat16")
     group = _group_size(packed, scales, biases)
@@ -440,6 +442,14 @@ def _setting(value, name: str, batch: int, dtype: torch.dtype, low, high):
     return None, value
 
 
+def _settings(temperature, top_k, top_p, min_p, batch: int):
+    inf = float("inf")
+    return (_setting(temperature, "temperature", batch, torch.float32, 0, 1e30),
+            _setting(top_k, "top_k", batch, torch.int32, 0, inf),
+            _setting(top_p, "top_p", batch, torch.float32, 0, 1),
+            _setting(min_p, "min_p", batch, torch.float32, 0, 1))
+
+
 def sample_tokens(logits: torch.Tensor, uniform: torch.Tensor, *,
                   temperature: float | torch.Tensor = 1.0, top_k: int | torch.Tensor = 0,
                   top_p: float | torch.Tensor = 1.0, min_p: float | torch.Tensor = 0.0,
@@ -471,11 +481,8 @@ def sample_tokens(logits: torch.Tensor, uniform: torch.Tensor, *,
         raise ValueError(f"the vocabulary must have 1 to {MAX_VOCAB} tokens")
     if uniform.shape != (batch,) or uniform.dtype != torch.float32 or not uniform.is_contiguous():
         raise ValueError("uniform must be contiguous float32 [batch]")
-    inf = float("inf")
-    t_rows, t = _setting(temperature, "temperature", batch, torch.float32, 0, 1e30)
-    k_rows, k = _setting(top_k, "top_k", batch, torch.int32, 0, inf)
-    p_rows, p = _setting(top_p, "top_p", batch, torch.float32, 0, 1)
-    m_rows, m = _setting(min_p, "min_p", batch, torch.float32, 0, 1)
+    (t_rows, t), (k_rows, k), (p_rows, p), (m_rows, m) = _settings(
+        temperature, top_k, top_p, min_p, batch)
     index = _device([logits, uniform, *(x for x in (t_rows, k_rows, p_rows, m_rows)
                                         if x is not None)])
     device = logits.device

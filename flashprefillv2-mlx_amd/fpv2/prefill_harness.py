@@ -37,7 +37,7 @@ import torch.nn.functional as F
 
 from fpv2 import _lib
 from fpv2.chunked import ChunkedPrefill
-from fpv2.decode import (decode_attention, dequantize_weight, quantize_weight, quantized_linear,
+from fpv2.decode import (_settings, decode_attention, dequantize_weight, quantize_weight, quantized_linear,
                          rope_to_pages, sample_tokens)
 from fpv2.selection import FPV2Config
 
@@ -432,14 +432,19 @@ class ChunkedPrefillRunner:
         default from torch's generator of the model's device)."""
         if isinstance(new_tokens, bool) or not isinstance(new_tokens, int) or new_tokens <= 0:
             raise ValueError("new_tokens must be a positive integer")
+        # (what could be refused is looked at before the prompt is prefilled)
+        if self.attention == "sdpa":
+            raise ValueError("generate goes on over the caches of 'fpv2' or 'dense'")
+        _settings(temperature, top_k, top_p, min_p, 1)
         if any(cache.length for cache in self.caches):
             raise ValueError("generate starts from empty caches: call reset() first")
         if tokens.numel() + new_tokens - 1 > self.capacity:
             raise ValueError("prompt and new tokens exceed the KV cache capacity")
         if uniform is None:
             uniform = torch.rand(new_tokens, device=self.model.device)
-        elif uniform.shape != (new_tokens,):
-            raise ValueError("uniform must be float32 [new_tokens]")
+        elif (uniform.shape != (new_tokens,) or uniform.dtype != torch.float32
+              or uniform.device != self.model.embed.device):
+            raise ValueError("uniform must be float32 [new_tokens] on the model's device")
         logits = self.prefill(tokens, chunk)
         out = []
         for i in range(new_tokens):

@@ -239,6 +239,18 @@ def test_more_refusals():
             fpv2.rope_to_pages(**_rope_args(**{name: 1 << 62}))
 
 
+def test_rope_to_pages_refuses_caches_that_overlap():
+    """Tokens' rows would be written over one another."""
+    bf16 = torch.bfloat16
+    k, v = (torch.zeros(2, 1, 16, 64, dtype=bf16) for _ in "kv")
+    for name in ("k_pages", "v_pages"):
+        for bad in (torch.zeros(1, 1, 16, 64, dtype=bf16).expand(2, 1, 16, 64),
+                    torch.zeros(2, 1, 1, 64, dtype=bf16).expand(2, 1, 16, 64),
+                    torch.zeros(2000, dtype=bf16).as_strided((2, 1, 16, 64), (1024, 1024, 8, 1))):
+            with pytest.raises(ValueError, match="overlap"):
+                fpv2.rope_to_pages(**_rope_args(**{"k_pages": k, "v_pages": v, name: bad}))
+
+
 def test_c_entries_refuse_without_a_device():
     """Argument errors of the C entries come before any device call."""
     import ctypes

@@ -10,6 +10,8 @@ are within 2^-5 of their norm, and tokens are sampled from the step's own logits
 
 from __future__ import annotations
 
+import math
+
 import pytest
 import torch
 
@@ -133,6 +135,37 @@ def test_decode_refusals(cuda):
         runner.decode(token.repeat(2))
     with pytest.raises(ValueError, match="'fpv2' or 'dense'"):
         ChunkedPrefillRunner(model, 64, attention="sdpa").decode(token)
+
+
+def test_refused_calls_leave_the_caches(cuda):
+    """What is refused is refused before a token is appended or a prompt prefilled."""
+    cache = ChunkedPrefill(4, 2, 64, 8, device=cuda)
+    q, k = (torch.zeros((h, 1, 64), dtype=BF16, device=cuda) for h in (4, 2))
+    wide = torch.zeros((4, 64, 2), dtype=BF16, device=cuda)
+    for error, bad in ((ValueError, dict(out=wide[..., :1].transpose(1, 2))),
+                       (ValueError, dict(out=q[:1].expand(4, 1, 64))),
+                       (RuntimeError, dict(out=q.cpu())), (RuntimeError, dict(v=k.cpu())),
+                       (RuntimeError, dict(k=k.clone().requires_grad_())),
+                       (RuntimeError, dict(q=q.clone().requires_grad_()))):
+        with pytest.raises(error):
+            cache.decode(**{"q": q, "k": k, "v": k, **bad})
+        assert cache.length == 0 and not cache.k.requires_grad
+    cache.decode(q, k, k)
+    assert cache.length == 1
+
+    model = RandomDecoder(SHAPE, device=cuda, seed=7)
+    runner = ChunkedPrefillRunner(model, 64)
+    prompt = torch.zeros(5, dtype=torch.int64, device=cuda)
+    for bad in (dict(temperature=-1.0), dict(top_k=-1), dict(top_p=1.5), dict(min_p=math.nan),
+                dict(uniform=torch.rand(2)),
+                dict(uniform=torch.rand(2, device=cuda, dtype=torch.float64))):
+        with pytest.raises(ValueError):
+            runner.generate(prompt, 64, 2, **bad)
+        assert runner.caches[0].length == 0
+    stock = ChunkedPrefillRunner(model, 64, attention="sdpa")
+    with pytest.raises(ValueError, match="'fpv2' or 'dense'"):
+        stock.generate(prompt, 64, 1)
+    assert runner.generate(prompt, 64, 2).shape == (2,)
 
 
 def test_single_tokens_between_chunks(cuda):

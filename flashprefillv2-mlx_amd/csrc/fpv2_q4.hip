@@ -21,6 +21,11 @@
 // their sums in LDS at the end; the next pair's weights are in flight while one is
 // computed.  x lies in LDS, in the order of the operands: loaded from memory by
 // every wave, it kept the address units busier than the weights did.
+//
+// Measured: 151936 x 2560, groups of 128, 3 rows 50 us (4.2 TB/s); 19456 x 2560, groups of
+// 32, 12 rows of float16 17 us (1.9 TB/s); 2560 x 9728, groups of 64, one row 8.1 us (1.7
+// TB/s: a launch, x, two turns of loads and the sum).  Without gain: two or three
+// pairs in flight (8.8 and 9.6 us for the last), 16 waves, two rows' tiles a wave.
 #include "fpv2_common.h"
 #include "fpv2_decode.h"
 

@@ -119,7 +119,10 @@ __global__ __launch_bounds__(64 * W) void q4_linear_kernel(Q4Args a) {
   constexpr int MR = M < 16 ? M : 16;  // of so many rows,
   constexpr int Y = M < 4 ? M : 4;   // of which rows 4 quad .. + Y - 1 in a lane
   extern __shared__ __attribute__((aligned(16))) char sh[];
-  u32x4* sh_x = reinterpret_cast<u32x4*>(sh);  // [panel * 8][MT][4 quads][MR] of 8 columns
+  // [panel * 8][MT][4 quads][MR] of 8 columns.  Lanes that write a row's next 8 columns would
+  // meet in a bank: 16 rows lie turned by the columns' number.
+  u32x4* sh_x = reinterpret_cast<u32x4*>(sh);
+  const auto place = [](int m, int at) { return MR == 16 ? (m + at) % 8 + (m & 8) : m; };
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int col = lane & 15, quad = lane >> 4;
@@ -136,6 +139,7 @@ __global__ __launch_bounds__(64 * W) void q4_linear_kernel(Q4Args a) {
   for (int t = 0; t < MT; ++t)
 #pragma unroll
     for (int i = 0; i < Y; ++i) y[t][i] = 0.f;
+  const int x_at[2] = {place(min(col, MR - 1), quad), place(min(col, MR - 1), 4 + quad)};
   const u32x4 ones = {Nibbles<T>::kOnes, Nibbles<T>::kOnes, Nibbles<T>::kOnes, Nibbles<T>::kOnes};
   const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
   uint32_t base = Nibbles<T>::kBase;
@@ -169,7 +173,7 @@ __global__ __launch_bounds__(64 * W) void q4_linear_kernel(Q4Args a) {
         for (int g = 0; g < S; ++g) xs[g] = p[g] = zero;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          const u32x4 x = sh_x[(((8 * at + 4 * h + j) * MT + t) * 4 + quad) * MR + min(col, MR - 1)];
+          const u32x4 x = sh_x[(((8 * at + 4 * h + j) * MT + t) * 4 + quad) * MR + x_at[j % 2]];
           xs[j * S / 4] = Elem<T>::mfma16(as_vec8<T>(x), as_vec8<T>(ones), xs[j * S / 4]);
           p[j * S / 4] = Elem<T>::mfma16(as_vec8<T>(x), as_vec8<T>(wide[j]), p[j * S / 4]);
         }
@@ -190,12 +194,13 @@ __global__ __launch_bounds__(64 * W) void q4_linear_kernel(Q4Args a) {
     const int p1 = min(pairs, p0 + a.panel);
     if (p0 > 0) __syncthreads();
     for (int e = tid; e < (p1 - p0) * (32 * M); e += 64 * W) {
-      const int m = e % MR, q = e / MR % 4, t = e / (MR * 4) % MT, block = e / (MR * 4 * MT);
-      const int k = 256 * p0 + 32 * block + 8 * q;
+      // (8 lanes read 128 bytes of a row)
+      const int m = e / 8 % MR, t = e / (8 * MR) % MT, at = e / (8 * MR * MT) * 8 + e % 8;
+      const int k = 256 * p0 + 8 * at;
       u32x4 v = {0, 0, 0, 0};
       if (EVEN || k < a.k)
         v = reorder(load16(a.x + static_cast<int64_t>(min(m0 + 16 * t + m, a.rows - 1)) * a.x_rs + k));
-      sh_x[e] = v;
+      sh_x[((at / 4 * MT + t) * 4 + at % 4) * MR + place(m, at)] = v;
     }
     __syncthreads();
     // the wave's first pair of the panel is in st[0] already

@@ -117,6 +117,9 @@ template <typename T, int S, int M, bool EVEN>
 __global__ __launch_bounds__(64 * W) void q4_linear_kernel(Q4Args a) {
   constexpr int MT = (M + 15) / 16;  // tiles of rows of x,
   constexpr int MR = M < 16 ? M : 16;  // of so many rows,
+  // of x in flight in a thread (19456 x 2560, 12 rows: 1 17.7, 5 16.5, 10, whose registers leave
+  // three waves a SIMD, 19.1 us)
+  constexpr int LOADS = M < 16 ? 1 : 5;
   constexpr int Y = M < 4 ? M : 4;   // of which rows 4 quad .. + Y - 1 in a lane
   extern __shared__ __attribute__((aligned(16))) char sh[];
   // [panel * 8][MT][4 quads][MR] of 8 columns.  Lanes that write a row's next 8 columns would
@@ -193,14 +196,24 @@ __global__ __launch_bounds__(64 * W) void q4_linear_kernel(Q4Args a) {
   for (int p0 = 0; p0 < pairs; p0 += a.panel) {
     const int p1 = min(pairs, p0 + a.panel);
     if (p0 > 0) __syncthreads();
-    for (int e = tid; e < (p1 - p0) * (32 * M); e += 64 * W) {
-      // (8 lanes read 128 bytes of a row)
-      const int m = e / 8 % MR, t = e / (8 * MR) % MT, at = e / (8 * MR * MT) * 8 + e % 8;
-      const int k = 256 * p0 + 8 * at;
-      u32x4 v = {0, 0, 0, 0};
-      if (EVEN || k < a.k)
-        v = reorder(load16(a.x + static_cast<int64_t>(min(m0 + 16 * t + m, a.rows - 1)) * a.x_rs + k));
-      sh_x[((at / 4 * MT + t) * 4 + at % 4) * MR + place(m, at)] = v;
+    for (int e0 = tid; e0 < (p1 - p0) * (32 * M); e0 += 64 * W * LOADS) {
+      u32x4 v[LOADS];
+#pragma unroll
+      for (int i = 0; i < LOADS; ++i) {
+        // (8 lanes read 128 bytes of a row)
+        const int e = e0 + i * 64 * W;
+        const int m = e / 8 % MR, t = e / (8 * MR) % MT, at = e / (8 * MR * MT) * 8 + e % 8;
+        const int k = 256 * p0 + 8 * at;
+        v[i] = u32x4{0, 0, 0, 0};
+        if (e < (p1 - p0) * (32 * M) && (EVEN || k < a.k))
+          v[i] = load16(a.x + static_cast<int64_t>(min(m0 + 16 * t + m, a.rows - 1)) * a.x_rs + k);
+      }
+#pragma unroll
+      for (int i = 0; i < LOADS; ++i) {
+        const int e = e0 + i * 64 * W;
+        const int m = e / 8 % MR, t = e / (8 * MR) % MT, at = e / (8 * MR * MT) * 8 + e % 8;
+        if (e < (p1 - p0) * (32 * M)) sh_x[((at / 4 * MT + t) * 4 + at % 4) * MR + place(m, at)] = reorder(v[i]);
+      }
     }
     __syncthreads();
     // the wave's first pair of the panel is in st[0] already
@@ -235,22 +248,31 @@ __global__ __launch_bounds__(64 * W) void q4_linear_kernel(Q4Args a) {
   }
 }
 
-constexpr int kPanelBytes = 81920;  // of x in LDS at most: two workgroups fit a CU
+constexpr int kPanelBytes = 81920;  // of x in LDS at most where two workgroups share a CU
 
 template <typename T, int S, int M>
 void launch(Q4Args a, hipStream_t s) {
   constexpr int kSum = W * ((M + 15) / 16) * (M < 4 ? M : 4) * 256;
   const int tiles = (a.n + 15) / 16, many = (a.rows + M - 1) / M;
-  // A workgroup reads M rows of x and 16 wn rows of weights, so wn pays in x's
-  // reads and costs in workgroups.  Microseconds for wn = 1 / 2 / 4 / 8: 19456 x 2560
-  // one row 10.4 / 10.3 / 11.5 / 12.9, 12 rows (groups of 32) 23.6 / 19.7 / 17.9 / 19.0, 64 rows
-  // 66.7 / 44.2 / 35.6 / 31.7; 151936 x 2560 one row 61.5 / 48.5 / 46.1 / 51.0, 3 rows 86 / 65 / 56 /
-  // 49.5; 9728 x 2560 4 rows 10.7 / 9.9 / 9.1 / 14.0; 6144 x 2560 one row 5.9 / 6.6 / 8.1 / 12.4, 32
-  // rows 15.9 / 13.2 / 15.3 / 22.0; 2560 x 9728 one row 8.4 / 12.6 / 20.5 / 39.7.
-  const int least = M == 1 ? 8 * cu_count() : M == 16 ? cu_count() : cu_count() / 2;
+  // A workgroup reads M rows of x and 16 wn rows of weights, so wn pays in x's reads
+  // and costs in workgroups.  Microseconds for wn = 1 / 2 / 4 / 8, one row: 19456 x 2560 10.4 /
+  // 10.3 / 11.5 / 12.9, 151936 x 2560 61.5 / 48.5 / 46.1 / 51.0, 6144 x 2560 5.9 / 6.6 / 8.1 / 12.4; 3
+  // rows: 151936 x 2560 86 / 65 / 56 / 49.5; 4 rows: 9728 x 2560 10.7 / 9.9 / 9.1 / 14.0.
+  // From 5 rows on x fills the LDS, and a workgroup alone on its CU has twice as much of it:
+  // the fewest that make the workgroups no more than the CUs, but two a CU rather than
+  // all waves with rows of their own.  wn = 1 / 2, 16 rows: 6144 x 2560 8.6 / 7.8, 4096 x 4096
+  // 8.5 / 10.1; 2 / 4: 10240 x 5120 19.2 / 16.7; 4 / 8: 19456 x 2560, 12 rows 16.4 / 17.4.
+  const auto grid_of = [&](int wn) { return (tiles + wn - 1) / wn * many; };
   a.wn = 1;
-  while (a.wn < W && tiles / (2 * a.wn) * many >= least) a.wn *= 2;
-  const int pairs = (a.k + 255) / 256, most = kPanelBytes / (512 * M);
+  if (M < 16) {
+    const int least = M == 1 ? 8 * cu_count() : cu_count() / 2;
+    while (a.wn < W && tiles / (2 * a.wn) * many >= least) a.wn *= 2;
+  } else {
+    while (a.wn < W && grid_of(a.wn) > (a.wn == 4 ? 2 : 1) * cu_count()) a.wn *= 2;
+  }
+  const int pairs = (a.k + 255) / 256;
+  const bool alone = grid_of(a.wn) <= cu_count();
+  const int most = (alone ? 2 : 1) * kPanelBytes / (512 * M);
   a.panel = pairs < most ? pairs : most;
   const int bytes = a.panel * 512 * M > kSum ? a.panel * 512 * M : kSum;
   const dim3 grid((tiles + a.wn - 1) / a.wn, many);

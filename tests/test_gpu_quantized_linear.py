@@ -69,6 +69,23 @@ def test_column_counts(cuda, group, cols, out):
         _check(cuda, torch.randn((rows, cols), generator=gen).to(BF16), weights, F32)
 
 
+@pytest.mark.parametrize("group,cols", [(32, 2592), (64, 5184), (128, 5376), (64, 10304), (128, 20608)])
+@pytest.mark.parametrize("rows", [4, 5, 16, 19, 64])
+def test_rows_of_several_panels(cuda, group, cols, rows):
+    """More columns of x than lie in LDS at a time, the last panel short or of a part of a step."""
+    gen = torch.Generator().manual_seed(cols + rows)
+    weights = _weights(gen, 35, cols, group, F16 if rows % 2 else BF16)
+    x = torch.randn((rows, cols), generator=gen).to(weights[1].dtype)
+    _check(cuda, x, weights, F32)
+
+
+@pytest.mark.parametrize("rows", [6, 20])
+def test_panels_of_workgroups_that_share_a_cu(cuda, rows):
+    gen = torch.Generator().manual_seed(rows)
+    weights = _weights(gen, 17003, 2624, 64, BF16)
+    _check(cuda, torch.randn((rows, 2624), generator=gen).to(BF16), weights)
+
+
 @pytest.mark.parametrize("rows", [1, 7, 40])
 def test_many_outputs(cuda, rows):
     """Enough outputs for the wide tiles; two calls agree to the bit."""

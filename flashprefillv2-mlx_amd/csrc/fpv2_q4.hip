@@ -23,9 +23,10 @@
 // every wave, it kept the address units busier than the weights did.
 //
 // Measured: 151936 x 2560, groups of 128, 3 rows 50 us (4.2 TB/s); 19456 x 2560, groups of
-// 32, 12 rows of float16 17 us (1.9 TB/s); 2560 x 9728, groups of 64, one row 8.1 us (1.7
-// TB/s: a launch, x, two turns of loads and the sum).  Without gain: two or three
-// pairs in flight (8.8 and 9.6 us for the last), 16 waves, two rows' tiles a wave.
+// 32, 12 rows of float16 15 us (2.1 TB/s); 2560 x 9728, groups of 64, one row 8.1 us (1.7
+// TB/s: a launch, x, two turns of loads and the sum), 16 rows 14, 64 rows 31 us.  Without
+// gain: two or three pairs in flight (8.8 and 9.6 us for one row), 16 waves, two rows'
+// tiles a wave; weights loaded 128 bytes of a row at a time would give 5 %.
 #include "fpv2_common.h"
 #include "fpv2_decode.h"
 

@@ -51,6 +51,7 @@ struct DecodeArgs {
   int64_t q_bs, q_hs, k_ps, k_hs, k_rs, v_ps, v_hs, v_rs, o_bs, o_hs, table_stride;
   int batch, kv_heads, group, item_heads, head_items;  // head_items * item_heads >= group
   int pages, page_size, capacity, length, window, sinks, grid;
+  int join_runs;  // the join's workgroups go by runs, not by items
   uint32_t page_mul, page_shift;  // t / page_size = (umulhi(t, mul) + t) >> shift
   float scale_log2;
 };
@@ -107,6 +108,30 @@ __device__ __forceinline__ int workgroup_of(const DecodeArgs& a, int unit, int t
   return static_cast<int>((static_cast<uint64_t>(unit + 1) * runs - 1) / static_cast<uint32_t>(total));
 }
 
+// The sequence that holds a unit, and its first unit.
+__device__ __forceinline__ int sequence_at(const DecodeArgs& a, int lane, int unit, int* first) {
+  const int items = a.kv_heads * a.head_items;
+  int b = 0, base = 0;
+  for (int b0 = 0; b0 < a.batch; b0 += 64) {
+    int sum = b0 + lane < a.batch ? sequence_of(a, b0 + lane).units() * items : 0;
+#pragma unroll
+    for (int off = 1; off < 64; off <<= 1) {
+      const int up = __shfl_up(sum, off, 64);
+      sum += lane >= off ? up : 0;
+    }
+    const uint64_t past = __ballot(base + sum > unit);
+    if (past != 0) {
+      const int at = __ffsll(static_cast<unsigned long long>(past)) - 1;
+      b = b0 + at;
+      base += at > 0 ? __shfl(sum, at - 1, 64) : 0;
+      break;
+    }
+    base += __shfl(sum, 63, 64);
+  }
+  *first = __builtin_amdgcn_readfirstlane(base);
+  return __builtin_amdgcn_readfirstlane(b);
+}
+
 template <int NW>
 struct Words { uint32_t w[NW]; };
 
@@ -151,27 +176,8 @@ __global__ __launch_bounds__(256, 2) void decode_attn_kernel(DecodeArgs a) {
   const int lo = first_of(a, blockIdx.x, total), hi = first_of(a, blockIdx.x + 1, total);
   if (lo >= hi) return;
 
-  // the sequence that holds block lo: base is its first block
-  int b = 0, base = 0;
-  for (int b0 = 0; b0 < a.batch; b0 += 64) {
-    int sum = b0 + lane < a.batch ? sequence_of(a, b0 + lane).units() * items : 0;
-#pragma unroll
-    for (int off = 1; off < 64; off <<= 1) {
-      const int up = __shfl_up(sum, off, 64);
-      sum += lane >= off ? up : 0;
-    }
-    const uint64_t past = __ballot(base + sum > lo);
-    if (past != 0) {
-      const int at = __ffsll(static_cast<unsigned long long>(past)) - 1;
-      b = b0 + at;
-      base += at > 0 ? __shfl(sum, at - 1, 64) : 0;
-      break;
-    }
-    base += __shfl(sum, 63, 64);
-  }
-  b = __builtin_amdgcn_readfirstlane(b);
-  base = __builtin_amdgcn_readfirstlane(base);
-
+  int base;
+  int b = sequence_at(a, lane, lo, &base);
   Sequence s = sequence_of(a, b);
   for (int cur = lo, end; cur < hi; cur = end) {
     const int units = s.units();
@@ -343,8 +349,9 @@ __global__ __launch_bounds__(256, 2) void decode_attn_kernel(DecodeArgs a) {
 }
 
 // Joins the partials of an item that several workgroups shared: one workgroup
-// per (item, query head, DS of the dims).  First the weights of all partials,
-// then their sum, 16 bytes of a partial a thread.
+// per (item, query head, DS of the dims), or where there are more items than runs,
+// per (run, ..) for the item that goes on in the next one.  First the weights of
+// all partials, then their sum, 16 bytes of a partial a thread.
 template <typename T, int D, int DS>
 __global__ __launch_bounds__(256) void decode_join_kernel(DecodeArgs a) {
   constexpr int kLanes = DS / 4, kSlots = 256 / kLanes;  // partials at a time
@@ -356,14 +363,21 @@ __global__ __launch_bounds__(256) void decode_join_kernel(DecodeArgs a) {
   const int items = a.kv_heads * a.head_items;
   const int d0 = blockIdx.x % kParts * DS, h = blockIdx.x / kParts % a.item_heads;
   const int at = blockIdx.x / kParts / a.item_heads;
-  const int b = at / items, item = at - b * items;
+  int b = at / items, item = at - b * items, before;
+  const int total = wave_total(a, lane, b, &before) * items;
+  int base = before * items;
+  if (a.join_runs) {
+    if (at + 1 >= static_cast<int>(runs_of(a, total))) return;
+    const int unit = first_of(a, at + 1, total);
+    b = sequence_at(a, lane, unit, &base);
+    item = (unit - base) / sequence_of(a, b).units();
+  }
   const int kvh = item / a.head_items, h0 = (item - kvh * a.head_items) * a.item_heads;
   if (h0 + h >= a.group) return;
-  int before;
-  const int total = wave_total(a, lane, b, &before) * items;
   const Sequence s = sequence_of(a, b);
-  const int start = before * items + item * s.units();
+  const int start = base + item * s.units();
   const int w0 = workgroup_of(a, start + kItemUnits, total);
+  if (a.join_runs && w0 != at) return;  // not in the run, or another run's item
   const int n = workgroup_of(a, start + s.units() - 1, total) - w0 + 1;
   if (n == 1) return;  // written by its workgroup
   // a workgroup's first item is in its slot 0, its last in slot 1
@@ -468,7 +482,10 @@ int launch(const DecodeArgs& a, bool join, hipStream_t s) {
     // An item of many partials is joined by several workgroups.  One item of 512
     // partials, 8 heads: the call 27.4 us by whole heads / 24.8 by 32 dims at D =
     // 128, 41.8 / 35.1 at D = 256; 8 items of 64 partials: the join 5.7 / 6.1.
-    const unsigned items = static_cast<unsigned>(a.batch) * a.kv_heads * a.head_items;
+    // With more items than runs most have one workgroup, and there is a join for a run at
+    // most: 512 sequences of 64 keys, 32 / 8 heads of D = 64: the join 36 us by items, @@
+    // by runs; 64 sequences of 8 items 3.9 by items.
+    const unsigned items = a.join_runs ? a.grid - 1 : static_cast<unsigned>(a.batch) * a.kv_heads * a.head_items;
     if (a.grid >= 128u * items)
       hipLaunchKernelGGL((decode_join_kernel<T, D, 32>), dim3(items * a.item_heads * (D / 32)), dim3(256), 0, s, a);
     else
@@ -560,6 +577,7 @@ extern "C" int fpv2_decode_attention(const void* q, const void* k_pages, const v
                                                                                   : a.capacity);
   a.sinks = static_cast<int>(p.sink_tokens < a.capacity ? p.sink_tokens : a.capacity);
   a.grid = plan.grid;
+  a.join_runs = p.batch * p.kv_heads * plan.head_items > plan.grid;
   uint32_t shift = 0;
   while ((1ull << shift) < static_cast<uint64_t>(p.page_size)) ++shift;
   a.page_shift = shift;

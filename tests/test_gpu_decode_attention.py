@@ -96,6 +96,20 @@ def test_ragged_pages(cuda, dtype, dim, heads, hkv):
     assert not got[0].any()
 
 
+@pytest.mark.parametrize("heads,hkv,dim", [(8, 8, 64), (24, 1, 96), (12, 4, 128)])
+@pytest.mark.parametrize("longest", [1, 40, 400])
+def test_more_items_than_workgroups(cuda, heads, hkv, dim, longest):
+    """Hundreds of short sequences: a workgroup has several, and one in two at most."""
+    gen = torch.Generator().manual_seed(heads + longest)
+    batch = 1200 // hkv + 7 if hkv > 1 else 611
+    lengths = torch.randint(0, longest + 1, (batch,), generator=gen).tolist()
+    lengths[3], lengths[-1] = 5 * longest, longest
+    k, v, table = _paged(gen, lengths, hkv, 16, dim, BF16)
+    q = _rand(gen, batch, heads, dim, dtype=BF16) * 2
+    _check(cuda, q, k, v, table, lengths)
+    _check(cuda, q, k, v, table, lengths, window=30, sinks=3)
+
+
 @pytest.mark.parametrize("page", [1, 3, 7, 32, 48, 128, 1000])
 @pytest.mark.parametrize("window,sinks", [(None, 0), (None, 9), (1, 0), (100, 0), (64, 5), (333, 130),
                                           (5000, 5000)])

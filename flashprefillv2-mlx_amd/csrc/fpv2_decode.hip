@@ -76,21 +76,62 @@ __device__ __forceinline__ Sequence sequence_of(const DecodeArgs& a, int b) {
   return s;
 }
 
-// Units of one item of every sequence, and of the ones before sequence `end`.
-__device__ __forceinline__ int wave_total(const DecodeArgs& a, int lane, int end, int* before) {
-  int all = 0, some = 0;
-  for (int b = lane; b < a.batch; b += 64) {
-    const int n = sequence_of(a, b).units();
-    all += n;
-    some += b < end ? n : 0;
-  }
+// Units of one item of a lane's sequences [lane per, ..) and the lanes' before it.
+struct Prefix {
+  int per, upto, total;
+};
+__device__ __forceinline__ int scan_add(int x, int lane) {
 #pragma unroll
-  for (int off = 32; off >= 1; off >>= 1) {
-    all += __shfl_xor(all, off, 64);
-    some += __shfl_xor(some, off, 64);
+  for (int off = 1; off < 64; off <<= 1) {
+    const int up = __shfl_up(x, off, 64);
+    x += lane >= off ? up : 0;
   }
-  *before = some;
-  return all;
+  return x;
+}
+__device__ __forceinline__ Prefix prefix_of(const DecodeArgs& a, int lane) {
+  Prefix p;
+  p.per = (a.batch + 63) / 64;
+  int sum = 0;
+#pragma unroll 4
+  for (int i = 0; i < p.per; ++i) {
+    const int b = lane * p.per + i;
+    sum += b < a.batch ? sequence_of(a, b).units() : 0;
+  }
+  p.upto = scan_add(sum, lane);
+  p.total = __builtin_amdgcn_readlane(p.upto, 63);
+  return p;
+}
+// Units of one item of the sequences before b.
+__device__ __forceinline__ int units_before(const DecodeArgs& a, const Prefix& p, int lane, int b) {
+  const int at = b / p.per;
+  const int base = at > 0 ? __shfl(p.upto, at - 1, 64) : 0;
+  if (p.per == 1) return base;
+  int some = 0;
+  for (int i = at * p.per + lane; i < b; i += 64) some += sequence_of(a, i).units();
+#pragma unroll
+  for (int off = 32; off >= 1; off >>= 1) some += __shfl_xor(some, off, 64);
+  return base + some;
+}
+// The sequence that holds a unit of all items, and its first unit.
+__device__ __forceinline__ int sequence_at(const DecodeArgs& a, const Prefix& p, int lane, int unit, int* first) {
+  const int items = a.kv_heads * a.head_items;
+  const int at = __ffsll(static_cast<unsigned long long>(__ballot(p.upto * items > unit))) - 1;
+  int b = at * p.per, base = at > 0 ? __shfl(p.upto, at - 1, 64) * items : 0;
+  if (p.per > 1) {
+    for (int b0 = b; b0 < a.batch; b0 += 64) {
+      const int sum = scan_add(b0 + lane < a.batch ? sequence_of(a, b0 + lane).units() * items : 0, lane);
+      const uint64_t past = __ballot(base + sum > unit);
+      if (past != 0) {
+        const int l = __ffsll(static_cast<unsigned long long>(past)) - 1;
+        b = b0 + l;
+        base += l > 0 ? __shfl(sum, l - 1, 64) : 0;
+        break;
+      }
+      base += __shfl(sum, 63, 64);
+    }
+  }
+  *first = __builtin_amdgcn_readfirstlane(base);
+  return __builtin_amdgcn_readfirstlane(b);
 }
 
 // The workgroups that have a run: of a tile for each wave at least.
@@ -106,30 +147,6 @@ __device__ __forceinline__ int first_of(const DecodeArgs& a, uint32_t w, int tot
 __device__ __forceinline__ int workgroup_of(const DecodeArgs& a, int unit, int total) {
   const uint32_t runs = runs_of(a, total);
   return static_cast<int>((static_cast<uint64_t>(unit + 1) * runs - 1) / static_cast<uint32_t>(total));
-}
-
-// The sequence that holds a unit, and its first unit.
-__device__ __forceinline__ int sequence_at(const DecodeArgs& a, int lane, int unit, int* first) {
-  const int items = a.kv_heads * a.head_items;
-  int b = 0, base = 0;
-  for (int b0 = 0; b0 < a.batch; b0 += 64) {
-    int sum = b0 + lane < a.batch ? sequence_of(a, b0 + lane).units() * items : 0;
-#pragma unroll
-    for (int off = 1; off < 64; off <<= 1) {
-      const int up = __shfl_up(sum, off, 64);
-      sum += lane >= off ? up : 0;
-    }
-    const uint64_t past = __ballot(base + sum > unit);
-    if (past != 0) {
-      const int at = __ffsll(static_cast<unsigned long long>(past)) - 1;
-      b = b0 + at;
-      base += at > 0 ? __shfl(sum, at - 1, 64) : 0;
-      break;
-    }
-    base += __shfl(sum, 63, 64);
-  }
-  *first = __builtin_amdgcn_readfirstlane(base);
-  return __builtin_amdgcn_readfirstlane(b);
 }
 
 template <int NW>
@@ -170,14 +187,13 @@ __global__ __launch_bounds__(256, 2) void decode_attn_kernel(DecodeArgs a) {
   const int col = lane & 15, quad = lane >> 4;
   const int items = a.kv_heads * a.head_items;
 
-  int before;
-  const int per_item = wave_total(a, lane, 0, &before);
-  const int total = per_item * items;
+  const Prefix prefix = prefix_of(a, lane);
+  const int total = prefix.total * items;
   const int lo = first_of(a, blockIdx.x, total), hi = first_of(a, blockIdx.x + 1, total);
   if (lo >= hi) return;
 
   int base;
-  int b = sequence_at(a, lane, lo, &base);
+  int b = sequence_at(a, prefix, lane, lo, &base);
   Sequence s = sequence_of(a, b);
   for (int cur = lo, end; cur < hi; cur = end) {
     const int units = s.units();
@@ -363,14 +379,18 @@ __global__ __launch_bounds__(256) void decode_join_kernel(DecodeArgs a) {
   const int items = a.kv_heads * a.head_items;
   const int d0 = blockIdx.x % kParts * DS, h = blockIdx.x / kParts % a.item_heads;
   const int at = blockIdx.x / kParts / a.item_heads;
-  int b = at / items, item = at - b * items, before;
-  const int total = wave_total(a, lane, b, &before) * items;
-  int base = before * items;
+  const Prefix prefix = prefix_of(a, lane);
+  const int total = prefix.total * items;
+  int b, item, base;
   if (a.join_runs) {
     if (at + 1 >= static_cast<int>(runs_of(a, total))) return;
     const int unit = first_of(a, at + 1, total);
-    b = sequence_at(a, lane, unit, &base);
+    b = sequence_at(a, prefix, lane, unit, &base);
     item = (unit - base) / sequence_of(a, b).units();
+  } else {
+    b = at / items;
+    item = at - b * items;
+    base = units_before(a, prefix, lane, b) * items;
   }
   const int kvh = item / a.head_items, h0 = (item - kvh * a.head_items) * a.item_heads;
   if (h0 + h >= a.group) return;
@@ -483,7 +503,7 @@ int launch(const DecodeArgs& a, bool join, hipStream_t s) {
     // partials, 8 heads: the call 27.4 us by whole heads / 24.8 by 32 dims at D =
     // 128, 41.8 / 35.1 at D = 256; 8 items of 64 partials: the join 5.7 / 6.1.
     // With more items than runs most have one workgroup, and there is a join for a run at
-    // most: 512 sequences of 64 keys, 32 / 8 heads of D = 64: the join 36 us by items, @@
+    // most: 512 sequences of 64 keys, 32 / 8 heads of D = 64: the join 36 us by items, 12.7
     // by runs; 64 sequences of 8 items 3.9 by items.
     const unsigned items = a.join_runs ? a.grid - 1 : static_cast<unsigned>(a.batch) * a.kv_heads * a.head_items;
     if (a.grid >= 128u * items)

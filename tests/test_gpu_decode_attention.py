@@ -110,6 +110,16 @@ def test_more_items_than_workgroups(cuda, heads, hkv, dim, longest):
     _check(cuda, q, k, v, table, lengths, window=30, sinks=3)
 
 
+@pytest.mark.parametrize("batch", [63, 64, 65, 128, 129, 300])
+def test_batches_past_a_wave(cuda, batch):
+    """More sequences than lanes, fewer items than workgroups, long ones among short ones."""
+    gen = torch.Generator().manual_seed(batch)
+    lengths = torch.randint(0, 300, (batch,), generator=gen).tolist()
+    lengths[0], lengths[batch // 2], lengths[-1], lengths[5] = 2500, 3001, 1999, 0
+    k, v, table = _paged(gen, lengths, 1, 32, 64, F16)
+    _check(cuda, _rand(gen, batch, 5, 64, dtype=F16) * 2, k, v, table, lengths)
+
+
 @pytest.mark.parametrize("page", [1, 3, 7, 32, 48, 128, 1000])
 @pytest.mark.parametrize("window,sinks", [(None, 0), (None, 9), (1, 0), (100, 0), (64, 5), (333, 130),
                                           (5000, 5000)])

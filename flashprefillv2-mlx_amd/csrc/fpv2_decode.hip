@@ -19,7 +19,7 @@
 //
 // Measured (32 / 8 heads, D = 128): one sequence of 131072 keys 92 .. 98 us, 5.5 .. 5.8 TB/s,
 // what plain reads reach; 24 sequences of 61 to 16001 keys in pages of 64 rows 62 us,
-// 4.9 TB/s; 1000 keys 7 us. 16 / 4 heads of D = 256, windows of 4096 keys, 8 sequences: 34 us,
+// 4.9 TB/s; 1000 keys 6.6 us. 16 / 4 heads of D = 256, windows of 4096 keys, 8 sequences: 34 us,
 // 4.1 TB/s. The join takes 5 to 6 us, most of it a launch and three dependent loads.
 // Without gain: tiles of 64 keys, a tile's loads a step ahead (the registers cost a
 // workgroup a CU), more than two workgroups a CU.

@@ -177,6 +177,14 @@ template <typename T, int D>
 __global__ __launch_bounds__(256, 2) void decode_attn_kernel(DecodeArgs a) {
   constexpr int KK = D / 32;  // MFMA steps of a key's dot product
   constexpr int DV = D / 16;  // dims of a lane
+  // Weights are rounded to the storage type for their product with V, as MFMA takes them; the
+  // sum is of the unrounded ones.  float16 has only 2^-14 to 1 at full precision, so there
+  // they are relative to 2^-15 of the tile's own greatest instead of the greatest so far
+  // (a tile 2^-40 and more below it: of 2^-40 of it, so that no float32 sum overflows).
+  // Relative to the greatest, the rest of a sequence 12 to 17 nats below one key lost up to
+  // a quarter of its weight.
+  constexpr bool kByTile = std::is_same<T, f16_t>::value;
+  constexpr float kHeadroom = 15.f, kBelow = 40.f;
   __shared__ float sh_o[4][kMaxHeads][D + 4];
   __shared__ float sh_ml[4][kMaxHeads][2];
   // (at head dim 256 the queries would not fit the registers beside K, V and O)
@@ -228,7 +236,8 @@ __global__ __launch_bounds__(256, 2) void decode_attn_kernel(DecodeArgs a) {
     f32x4 o[DV];
 #pragma unroll
     for (int d = 0; d < DV; ++d) o[d] = f32x4{0.f, 0.f, 0.f, 0.f};
-    float m = neg_inf(), l = 0.f;
+    float m = neg_inf(), l = 0.f;  // the exponent that O and l are relative to
+    float greatest = neg_inf();
 
     const uint16_t* kb = a.k + kvh * a.k_hs;
     const uint16_t* vb = a.v + kvh * a.v_hs;
@@ -293,7 +302,11 @@ __global__ __launch_bounds__(256, 2) void decode_attn_kernel(DecodeArgs a) {
       }
       top = fmaxf(top, __shfl_xor(top, 16, 64));
       top = fmaxf(top, __shfl_xor(top, 32, 64));
-      const float m_new = fmaxf(m, top);
+      float m_new = fmaxf(m, top);
+      if constexpr (kByTile) {
+        greatest = fmaxf(greatest, top);
+        m_new = fmaxf(top, greatest - kBelow) - kHeadroom;
+      }
       // (nothing but -inf so far: weights of zero instead of NaN)
       const float ref = m_new == neg_inf() ? 0.f : m_new;
       const float fix = __builtin_amdgcn_exp2f(m - ref);

@@ -1,0 +1,61 @@
+"""Corners of a decode step's operators on the GPU: scores far below a sequence's
+greatest, infinities beside a rotation, numbers past 64 bits, side streams.
+"""
+
+from __future__ import annotations
+
+import math
+
+import pytest
+import torch
+
+import fpv2
+
+pytestmark = pytest.mark.gpu
+
+BF16, F16 = torch.bfloat16, torch.float16
+
+# Of heads that share their keys: how far the other keys are below the greatest, in nats.
+GAPS = [0.0, 8.0, 12.0, 15.0, 16.875, 17.5, 20.0, 24.0]
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("length,batch,at", [(31, 1, 0), (200, 1, 199), (200, 600, 0), (200, 600, 77),
+                                             (700, 600, 300), (40_000, 1, 0), (40_000, 1, 25_000),
+                                             (40_000, 1, 39_999)])
+def test_keys_far_below_the_greatest(cuda, dtype, dim, length, batch, at):
+    """One key far above the rest whose value is zero, so that the rest are the result; in
+    items of one workgroup (600 sequences of one table row) and of many.
+
+    Tolerance: every weight and the result are off by half a step of the storage type, or
+    of its least normal number, of which a weight's is 2^-29 of the greatest of its 32 keys,
+    so that the 31 keys beside the greatest are off by 2^-40 each.  Scores are sums of three
+    terms of at most 2^5 in float32 times log2 e: off by less than 8 * 2^-19, and the
+    exponential by as much relative to its value; sums of n terms by n 2^-24, which for
+    partial sums of a lane are fewer than 2^11."""
+    gen = torch.Generator().manual_seed(length + at)
+    heads, page = len(GAPS), 64
+    q = torch.zeros((1, heads, dim), dtype=dtype)
+    k = torch.zeros((1, 1, length, dim), dtype=dtype)
+    q[0, :, 0], q[0, :, 5] = torch.tensor(GAPS), 1.0
+    k[0, 0, at, 0] = 1.0
+    k[0, 0, :, 5] = torch.randint(-32, 33, (length,), generator=gen) / 64
+    k[0, 0, at, 5] = 0.5
+    v = (1000 * (0.5 + torch.rand((1, 1, length, dim), generator=gen))).to(dtype)
+    v[0, 0, at] = 0
+    pages = -(-length // page)
+    kp, vp = (torch.zeros((pages * page, dim), dtype=dtype) for _ in "kv")
+    kp[:length], vp[:length] = k[0, 0], v[0, 0]
+    kp, vp = (x.view(pages, page, 1, dim).transpose(1, 2).to(cuda) for x in (kp, vp))
+    table = torch.arange(pages, dtype=torch.int32, device=cuda).expand(batch, pages)
+    got = fpv2.decode_attention(q.expand(batch, heads, dim).to(cuda), kp, vp, table, length, scale=1.0)
+    s = q[0].double() @ k[0, 0].double().T
+    w = torch.softmax(s, 1)
+    want = w @ v[0, 0].double()
+    info = torch.finfo(dtype)
+    top = w.amax(1, keepdim=True)
+    tol = (info.eps / 2 * (2 * want.abs()).clamp(min=info.tiny) + 2.0 ** -12 * want.abs()
+           + (31 * 2.0 ** -40 * 1500 * top if dtype == F16 else 0))
+    err = (got.cpu().double() - want).abs()
+    assert bool((err <= tol).all()), [float(x) for x in (err / tol).amax((0, 2))]

@@ -131,14 +131,24 @@ __global__ __launch_bounds__(256) void rope_pages_kernel(RopePagesArgs a) {
 #pragma unroll
         for (int j = 0; j < 8; ++j) na[j] *= r * wa[j], nb[j] *= r * wb[j];
       }
+      // (a vector behind the rotated ones stays as it is: a product with (1, 0) would make NaN
+      // of what lies beside an infinity)
       if (a.interleaved) {
+        if (ua < 2 * rot) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const float a0 = na[2 * j], a1 = na[2 * j + 1], b0 = nb[2 * j], b1 = nb[2 * j + 1];
-          na[2 * j] = a0 * c[j] - a1 * sn[j];
-          na[2 * j + 1] = a1 * c[j] + a0 * sn[j];
-          nb[2 * j] = b0 * c[4 + j] - b1 * sn[4 + j];
-          nb[2 * j + 1] = b1 * c[4 + j] + b0 * sn[4 + j];
+          for (int j = 0; j < 4; ++j) {
+            const float a0 = na[2 * j], a1 = na[2 * j + 1];
+            na[2 * j] = a0 * c[j] - a1 * sn[j];
+            na[2 * j + 1] = a1 * c[j] + a0 * sn[j];
+          }
+        }
+        if (ub < 2 * rot) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const float b0 = nb[2 * j], b1 = nb[2 * j + 1];
+            nb[2 * j] = b0 * c[4 + j] - b1 * sn[4 + j];
+            nb[2 * j + 1] = b1 * c[4 + j] + b0 * sn[4 + j];
+          }
         }
       } else if (s < rot) {
 #pragma unroll

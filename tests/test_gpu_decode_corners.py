@@ -59,3 +59,28 @@ def test_keys_far_below_the_greatest(cuda, dtype, dim, length, batch, at):
            + (31 * 2.0 ** -40 * 1500 * top if dtype == F16 else 0))
     err = (got.cpu().double() - want).abs()
     assert bool((err <= tol).all()), [float(x) for x in (err / tol).amax((0, 2))]
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("dim,half,tokens", [(96, 24, 3), (128, 8, 2500), (256, 64, 1)])
+def test_dimensions_behind_the_rotation_are_copied(cuda, dtype, interleaved, dim, half, tokens):
+    """Heads without a norm: what is not rotated stays as it is, bit for bit, beside infinities
+    and NaN too."""
+    gen = torch.Generator().manual_seed(dim)
+    heads, hkv, page = 5, 2, 16
+    x = torch.randn((tokens, heads + 2 * hkv, dim), generator=gen).to(dtype)
+    x[:, :, 2 * half + 2] = math.inf
+    x[:, 1::2, 2 * half + 5] = -math.inf
+    x[:, ::2, dim - 1] = math.nan
+    x[:, :, dim - 4] = -0.0
+    angle = torch.rand((50, half), generator=gen) * 6
+    kp, vp = (torch.zeros((-(-tokens // page), hkv, page, dim), dtype=dtype, device=cuda) for _ in "kv")
+    q = fpv2.rope_to_pages(x.view(tokens, -1).to(cuda), None, None, angle.cos().to(cuda),
+                           angle.sin().to(cuda), 7, 0, kp, vp, query_heads=heads, interleaved=interleaved)
+    k = kp.transpose(1, 2).flatten(0, 1)[:tokens]
+    for got, want in ((q.cpu(), x[:, :heads]), (k.cpu(), x[:, heads:heads + hkv])):
+        got, want = got[..., 2 * half:], want[..., 2 * half:]
+        nan = want.isnan()
+        assert torch.equal(got.isnan(), nan)
+        assert torch.equal(got.view(torch.int16)[~nan], want.contiguous().view(torch.int16)[~nan])

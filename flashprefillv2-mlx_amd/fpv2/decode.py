@@ -173,8 +173,11 @@ def decode_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tens
         tensors.append(lengths)
     else:
         uniform = _count(lengths, "lengths")
-    window = 0 if window_tokens is None else _count(window_tokens, "window_tokens", 1)
-    _count(sink_tokens, "sink_tokens")
+    # (numbers past the cache are all of it: none leaves the parameters' 64 bits)
+    keys = width * page_size
+    uniform = min(uniform, keys)
+    window = 0 if window_tokens is None else min(_count(window_tokens, "window_tokens", 1), keys)
+    sinks = min(_count(sink_tokens, "sink_tokens"), keys)
     if out is not None:
         if (out.shape != shape or out.dtype != dtype or out.stride(2) != 1
                 or batch > 1 and out.stride(0) < dim or heads > 1 and out.stride(1) < dim):
@@ -195,7 +198,7 @@ def decode_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tens
     def call(stream):
         params, need = _decode_plan(
             index, batch, heads, kv_heads, dim, pages, page_size, width, table_stride,
-            uniform, window, sink_tokens, dim ** -0.5 if scale is None else scale, *q_strides,
+            uniform, window, sinks, dim ** -0.5 if scale is None else scale, *q_strides,
             *page_strides, out.stride(0), out.stride(1))
         work = torch.empty(need, dtype=torch.uint8, device=out.device) if need > 0 else None
         _lib.check(lib.fpv2_decode_attention(

@@ -84,3 +84,23 @@ def test_dimensions_behind_the_rotation_are_copied(cuda, dtype, interleaved, dim
         nan = want.isnan()
         assert torch.equal(got.isnan(), nan)
         assert torch.equal(got.view(torch.int16)[~nan], want.contiguous().view(torch.int16)[~nan])
+
+
+def _decode_case(cuda, lengths=(700, 90)):
+    gen = torch.Generator().manual_seed(3)
+    k, v = (torch.randn((48, 2, 16, 64), generator=gen).to(BF16).to(cuda) for _ in "kv")
+    q = torch.randn((2, 4, 64), generator=gen).to(BF16).to(cuda)
+    table = torch.arange(48, dtype=torch.int32).expand(2, 48).contiguous().to(cuda)
+    return q, k, v, table, torch.tensor(lengths, dtype=torch.int32, device=cuda)
+
+
+@pytest.mark.parametrize("past", [2 ** 63, 2 ** 64, 2 ** 64 + 5, 2 ** 70 + 17])
+def test_integers_past_64_bits(cuda, past):
+    """Windows, sinks and lengths past any cache are the whole of it."""
+    q, k, v, table, lengths = _decode_case(cuda)
+    want = fpv2.decode_attention(q, k, v, table, lengths)
+    for kwargs in (dict(window_tokens=past), dict(window_tokens=past, sink_tokens=past),
+                   dict(window_tokens=3, sink_tokens=past), dict(sink_tokens=past)):
+        assert torch.equal(fpv2.decode_attention(q, k, v, table, lengths, **kwargs), want)
+    assert torch.equal(fpv2.decode_attention(q, k, v, table, past),
+                       fpv2.decode_attention(q, k, v, table, 768))

@@ -178,6 +178,8 @@ def decode_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tens
     uniform = min(uniform, keys)
     window = 0 if window_tokens is None else min(_count(window_tokens, "window_tokens", 1), keys)
     sinks = min(_count(sink_tokens, "sink_tokens"), keys)
+    # (a number, as it is part of what a plan is kept by)
+    scale = dim ** -0.5 if scale is None else float(scale)
     if out is not None:
         if (out.shape != shape or out.dtype != dtype or out.stride(2) != 1
                 or batch > 1 and out.stride(0) < dim or heads > 1 and out.stride(1) < dim):
@@ -198,7 +200,7 @@ def decode_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tens
     def call(stream):
         params, need = _decode_plan(
             index, batch, heads, kv_heads, dim, pages, page_size, width, table_stride,
-            uniform, window, sinks, dim ** -0.5 if scale is None else scale, *q_strides,
+            uniform, window, sinks, scale, *q_strides,
             *page_strides, out.stride(0), out.stride(1))
         work = torch.empty(need, dtype=torch.uint8, device=out.device) if need > 0 else None
         _lib.check(lib.fpv2_decode_attention(
@@ -301,7 +303,7 @@ def rope_to_pages(qkv: torch.Tensor, q_weight: torch.Tensor | None, k_weight: to
     p = (_rope_params if position_bytes and slot_bytes else _lib.RopePagesParams)(
         tokens, query_heads, kv_heads, dim, half, rows, bool(interleaved), pages, page_size,
         position_bytes, slot_bytes, first_position, first_slot, *qkv_strides, *_row_strides(out),
-        *page_strides, eps)
+        *page_strides, float(eps))
 
     def call(stream):
         _lib.check(lib.fpv2_rope_to_pages(

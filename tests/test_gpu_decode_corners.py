@@ -104,3 +104,24 @@ def test_integers_past_64_bits(cuda, past):
         assert torch.equal(fpv2.decode_attention(q, k, v, table, lengths, **kwargs), want)
     assert torch.equal(fpv2.decode_attention(q, k, v, table, past),
                        fpv2.decode_attention(q, k, v, table, 768))
+
+
+def test_numbers_given_as_tensors_are_read_in_each_call(cuda):
+    """A scale or eps in a tensor of one element that changes between two calls."""
+    q, k, v, table, lengths = _decode_case(cuda)
+    scale = torch.tensor(0.125)
+    for x in (0.125, 0.5, 0.25):
+        scale.fill_(x)
+        assert torch.equal(fpv2.decode_attention(q, k, v, table, lengths, scale=scale),
+                           fpv2.decode_attention(q, k, v, table, lengths, scale=x))
+    ones, eps = torch.ones(64, dtype=BF16, device=cuda), torch.tensor(1e-6)
+    angle = torch.rand((9, 32), device=cuda)
+    at = torch.arange(2, device=cuda)
+
+    def rope(e):
+        return fpv2.rope_to_pages(q.flatten(1).repeat(1, 2), ones, ones, angle, angle, at, at, k, v,
+                                  query_heads=4, eps=e)
+
+    for x in (1e-6, 0.5, 3.0):
+        eps.fill_(x)
+        assert torch.equal(rope(eps), rope(float(eps)))

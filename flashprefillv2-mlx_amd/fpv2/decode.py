@@ -113,11 +113,11 @@ def _page_strides(k_pages: torch.Tensor, v_pages: torch.Tensor):
 
 @lru_cache(maxsize=256)
 def _decode_plan(index: int, *fields):
-    """A call's parameters and the bytes of workspace that it needs on device
-    ``index`` (the current one)."""
+    """A call's parameters but for an integer length, which grows from token to token,
+    and the bytes of workspace that it needs on device ``index`` (the current one)."""
     params = _lib.DecodeParams(*fields)
     need = _lib.load().fpv2_decode_attention_workspace_bytes(ctypes.byref(params))
-    return ctypes.byref(params), need
+    return params, ctypes.byref(params), need
 
 
 def decode_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
@@ -198,14 +198,17 @@ def decode_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tens
     lib = _lib.load()
 
     def call(stream):
-        params, need = _decode_plan(
-            index, batch, heads, kv_heads, dim, pages, page_size, width, table_stride,
-            uniform, window, sinks, scale, *q_strides,
-            *page_strides, out.stride(0), out.stride(1))
+        params, ref, need = _decode_plan(
+            index, batch, heads, kv_heads, dim, pages, page_size, width, table_stride, 0, window,
+            sinks, scale, *q_strides, *page_strides, out.stride(0), out.stride(1))
+        if lengths_ptr is None:
+            params = _lib.DecodeParams.from_buffer_copy(params)
+            params.length = uniform
+            ref = ctypes.byref(params)
         work = torch.empty(need, dtype=torch.uint8, device=out.device) if need > 0 else None
         _lib.check(lib.fpv2_decode_attention(
             q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), table_ptr, lengths_ptr,
-            out.data_ptr(), _lib.dtype_code(dtype), params, _lib.ptr(work), max(need, 0), stream),
+            out.data_ptr(), _lib.dtype_code(dtype), ref, _lib.ptr(work), max(need, 0), stream),
             "decode_attention")
 
     _on_device(index, call)

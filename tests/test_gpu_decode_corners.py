@@ -125,3 +125,16 @@ def test_numbers_given_as_tensors_are_read_in_each_call(cuda):
     for x in (1e-6, 0.5, 3.0):
         eps.fill_(x)
         assert torch.equal(rope(eps), rope(float(eps)))
+
+
+def test_growing_lengths_share_a_plan(cuda):
+    """An integer length is no part of what is kept for calls of one form."""
+    from fpv2.decode import _decode_plan
+    q, k, v, table, _ = _decode_case(cuda)
+    fpv2.decode_attention(q, k, v, table, 1)
+    size = _decode_plan.cache_info().currsize
+    got = [fpv2.decode_attention(q, k, v, table, n) for n in range(2, 60)]
+    assert _decode_plan.cache_info().currsize == size
+    for n, x in zip(range(2, 60), got):
+        both = torch.full((2,), n, dtype=torch.int32, device=cuda)
+        assert torch.equal(x, fpv2.decode_attention(q, k, v, table, both))

@@ -386,7 +386,9 @@ class ChunkedPrefillRunner:
         """Append one token (an integer tensor of one element on the model's device)
         to the prefilled sequence; returns the logits of its position (float32
         ``[vocab]``).  Exact attention over the whole cache in both modes; reads the
-        4-bit weights of a quantized model."""
+        4-bit weights of a quantized model.  A token outside the vocabulary, as
+        ``sample_tokens``' -1 for a row of nothing, has logits of NaN, and as it is in the
+        caches, so has every later one until ``reset``."""
         m, s = self.model, self.model.shape
         if self.attention == "sdpa":
             raise ValueError("decode goes on over the caches of 'fpv2' or 'dense'")
@@ -407,7 +409,10 @@ class ChunkedPrefillRunner:
                 return F.linear(x, m.layers[li][name])
             return quantized_linear(x, *m.packed[li][name])
 
-        x, delta = m.embed[token.reshape(1)], None
+        # (the token is known on the device only: what is no row of the table is NaN)
+        token = token.reshape(1).to(m.embed.device, torch.int64)
+        row = token.clamp(0, m.embed.shape[0] - 1)
+        x, delta = torch.where((row == token)[:, None], m.embed[row], math.nan), None
         for li, (p, cache) in enumerate(zip(m.layers, self.caches)):
             h = _add_rms_norm(x, delta, p["attn_norm"], s.rms_eps)
             k_pages, v_pages = cache.pages()
@@ -427,7 +432,8 @@ class ChunkedPrefillRunner:
                  temperature: float = 1.0, top_k: int = 0, top_p: float = 1.0,
                  min_p: float = 0.0, uniform: torch.Tensor | None = None) -> torch.Tensor:
         """Prefill the prompt in ``chunk``-token pieces, then sample ``new_tokens``
-        tokens (``sample_tokens``'s settings); returns them as int64 ``[new_tokens]``.
+        tokens (``sample_tokens``'s settings); returns them as int64 ``[new_tokens]``,
+        -1 from the first position on whose logits are nothing but -inf or NaN.
         ``uniform``: the float32 random numbers ``[new_tokens]`` of the tokens (by
         default from torch's generator of the model's device)."""
         if isinstance(new_tokens, bool) or not isinstance(new_tokens, int) or new_tokens <= 0:

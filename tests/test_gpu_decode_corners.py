@@ -10,6 +10,7 @@ import pytest
 import torch
 
 import fpv2
+from fpv2.prefill_harness import ChunkedPrefillRunner, DecoderShape, RandomDecoder
 
 pytestmark = pytest.mark.gpu
 
@@ -138,3 +139,45 @@ def test_growing_lengths_share_a_plan(cuda):
     for n, x in zip(range(2, 60), got):
         both = torch.full((2,), n, dtype=torch.int32, device=cuda)
         assert torch.equal(x, fpv2.decode_attention(q, k, v, table, both))
+
+
+SHAPE = DecoderShape(layers=2, hidden=256, query_heads=8, kv_heads=2, head_dim=64,
+                     intermediate=512, vocab=1000)
+
+
+@pytest.mark.parametrize("quantized", [False, True])
+@pytest.mark.parametrize("token", [-1, -1000, 1000, 2 ** 40])
+def test_a_token_outside_the_vocabulary_has_no_logits(cuda, quantized, token):
+    model = RandomDecoder(SHAPE, device=cuda, seed=1)
+    if quantized:
+        model.quantize(32)
+    runner = ChunkedPrefillRunner(model, 64)
+    prompt = torch.arange(20, device=cuda)
+    runner.prefill(prompt, 64)
+    want = runner.decode(torch.tensor([999], device=cuda))
+    runner.reset()
+    runner.prefill(prompt, 64)
+    assert torch.equal(runner.decode(torch.tensor(999, dtype=torch.int32, device=cuda)), want)
+    assert bool(want.isfinite().all())
+    bad = runner.decode(torch.tensor([token], device=cuda))
+    assert bool(bad.isnan().all())
+    after = runner.decode(torch.tensor([5], device=cuda))  # attends to it
+    assert int(fpv2.sample_tokens(after[None], torch.zeros(1, device=cuda))) == -1
+
+
+def test_generate_ends_with_the_first_row_of_nothing(cuda):
+    """A row without a token: all tokens after it are -1 as well."""
+    runner = ChunkedPrefillRunner(RandomDecoder(SHAPE, device=cuda, seed=2), 64)
+    prompt = torch.arange(20, device=cuda)
+    free = runner.generate(prompt, 64, 6, temperature=0.0)
+    assert bool((free >= 0).all())
+    runner.reset()
+    step, calls = runner.decode, []
+
+    def decode(token):
+        logits = step(token)
+        calls.append(int(token))
+        return torch.full_like(logits, -math.inf) if len(calls) == 2 else logits
+
+    runner.decode = decode
+    assert runner.generate(prompt, 64, 6, temperature=0.0).tolist() == free[:2].tolist() + [-1] * 4

@@ -84,6 +84,57 @@ def _row_strides(t: torch.Tensor):
     return strides
 
 
+def _reaches(base: int, spans: list, low: int, high: int) -> bool:
+    """Whether ``base`` and a whole number of strides of each of ``spans`` ``[(stride, least,
+    most)]`` can add up to a number in ``(low, high)``.  (A search over the strides from the
+    greatest on, cut off where the rest cannot reach; layouts that nest take a few
+    steps, and one that takes thousands counts as reaching.)"""
+    spans = sorted((x for x in spans if x[0] > 0), reverse=True)
+    rest = [(0, 0)]
+    for s, a, b in reversed(spans):
+        rest.append((rest[-1][0] + s * a, rest[-1][1] + s * b))
+    rest.reverse()  # of spans[i:]
+    budget = 4096
+
+    def search(i, at):
+        nonlocal budget
+        budget -= 1
+        if budget < 0:
+            return True
+        if i == len(spans):
+            return low < at < high
+        s, a, b = spans[i]
+        below, above = rest[i + 1]
+        first = max(a, -((at + above - low - 1) // s))
+        last = min(b, (high - 1 - at - below) // s)
+        return any(search(i + 1, at + s * n) for n in range(first, last + 1))
+
+    return search(0, base)
+
+
+@lru_cache(maxsize=256)
+def _rows_overlap(shape, strides) -> bool:
+    """Whether two rows (of contiguous last dimensions) of a tensor share memory."""
+    if 0 in shape:
+        return False
+    width = shape[-1]
+    dims = sorted(((s, n) for n, s in zip(shape[:-1], strides) if n > 1), reverse=True)
+    extent = width
+    for s, n in reversed(dims):
+        if s < extent:
+            break
+        extent += s * (n - 1)
+    else:
+        return False  # each dimension steps over all of the next one
+    # two rows whose first difference (in this order) is in dimension i
+    return any(_reaches(s, [(s, 0, n - 2)] + [(r, 1 - m, m - 1) for r, m in dims[i + 1:]], -width, width)
+               for i, (s, n) in enumerate(dims))
+
+
+def _overlaps_itself(t: torch.Tensor) -> bool:
+    return not t.is_contiguous() and _rows_overlap(t.shape, t.stride())
+
+
 def _pages(k_pages: torch.Tensor, v_pages: torch.Tensor):
     """The caches' shape and strides."""
     if k_pages.ndim != 4 or v_pages.ndim != 4:
@@ -182,7 +233,7 @@ def decode_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tens
     scale = dim ** -0.5 if scale is None else float(scale)
     if out is not None:
         if (out.shape != shape or out.dtype != dtype or out.stride(2) != 1
-                or batch > 1 and out.stride(0) < dim or heads > 1 and out.stride(1) < dim):
+                or _overlaps_itself(out)):
             raise ValueError("out must be [batch, query heads, head dim] of q's dtype with a "
                              "contiguous last dimension and no overlap")
         tensors.append(out)
@@ -264,9 +315,9 @@ def rope_to_pages(qkv: torch.Tensor, q_weight: torch.Tensor | None, k_weight: to
     if kv_heads == 0 or qkv.shape[1] != (query_heads + 2 * kv_heads) * dim:
         raise ValueError("qkv rows must hold the query, key and value heads")
     page_strides = _page_strides(k_pages, v_pages)
-    if min(page_strides) < dim and any(
-            n > 1 and s < dim for n, s in zip((pages, kv_heads, page_size) * 2, page_strides)):
-        raise ValueError("the caches' rows overlap")
+    for t in (k_pages, v_pages):
+        if _overlaps_itself(t):
+            raise ValueError("the caches' rows overlap")
     for name, t in (("q_weight", q_weight), ("k_weight", k_weight)):
         if t is not None and (t.shape != (dim,) or t.dtype != qkv.dtype or t.data_ptr() & 15
                               or not t.is_contiguous()):
@@ -289,8 +340,8 @@ def rope_to_pages(qkv: torch.Tensor, q_weight: torch.Tensor | None, k_weight: to
         if t is not None:
             tensors.append(t)
     if out is not None and (out.shape != (tokens, query_heads, dim) or out.dtype != qkv.dtype
-                            or _row_strides(out) is None or tokens > 1 and out.stride(0) < dim
-                            or query_heads > 1 and out.stride(1) < dim):
+                            or _row_strides(out) is None
+                            or _overlaps_itself(out)):
         raise ValueError("out must be [tokens, query heads, head dim] of qkv's dtype with 16-byte "
                          "aligned rows")
     index = _device(tensors)

@@ -1,0 +1,89 @@
+"""Corners of what a decode step's operators refuse (no GPU needed): destinations whose
+rows share memory, tangents, weights of odd layouts."""
+
+from __future__ import annotations
+
+import random
+
+import pytest
+import torch
+
+import fpv2
+from fpv2 import decode
+
+BF16 = torch.bfloat16
+
+
+def _strided(shape, strides):
+    size = 1 + sum((n - 1) * s for n, s in zip(shape, strides))
+    return torch.zeros(size, dtype=BF16).as_strided(shape, strides)
+
+
+def _addresses(t):
+    """Element numbers of a tensor's storage, of every element."""
+    at = torch.tensor([t.storage_offset()])
+    for n, s in zip(t.shape, t.stride()):
+        at = (at[:, None] + s * torch.arange(n)).flatten()
+    return at
+
+
+def test_rows_that_share_memory_are_found():
+    """Against all addresses, over small shapes of strides that nest, interleave and overlap."""
+    rng = random.Random(1)
+    found = 0
+    for _ in range(4000):
+        shape = [rng.choice([1, 1, 2, 3, 5]) for _ in range(rng.choice([1, 2, 3]))] + [rng.choice([1, 4, 8])]
+        strides = [rng.choice([0, 1, 2, 3, 4, 5, 8, 9, 12, 16, 24, 40, 41, 120]) for _ in shape[:-1]] + [1]
+        t = _strided(shape, strides)
+        at = _addresses(t)
+        want = len(at.unique()) < len(at)
+        assert decode._overlaps_itself(t) == want, (shape, strides)
+        found += want
+    assert 500 < found < 3500
+
+
+def _shared(t):
+    at = _addresses(t)
+    return len(at.unique()) < len(at)
+
+
+def _calls(**change):
+    """Calls that get as far as to ask for a ROCm device, if nothing is refused."""
+    pages = [torch.zeros(3, 2, 16, 64, dtype=BF16) for _ in "kv"]
+    attention = dict(q=torch.zeros(2, 8, 64, dtype=BF16), k_pages=pages[0], v_pages=pages[1],
+                     page_table=None, lengths=3)
+    rope = dict(qkv=torch.zeros(2, 12 * 64, dtype=BF16), q_weight=None, k_weight=None,
+                cos=torch.zeros(9, 32), sin=torch.zeros(9, 32), positions=0, slots=0,
+                k_pages=pages[0], v_pages=pages[1], query_heads=8)
+    return [(fpv2.decode_attention, {**attention, **change}), (fpv2.rope_to_pages, {**rope, **change})]
+
+
+@pytest.mark.parametrize("strides,shared", [
+    ((64, 64), True), ((128, 72), True), ((512, 8), True), ((448, 64), True), ((64, 72), True),
+    ((0, 64), True), ((512, 0), True), ((64, 128), False), ((512, 64), False), ((1000, 72), False),
+    ((192, 128), False), ((160, 128), True), ((64, 1024), False)])
+def test_destinations_of_one_row_for_two_are_refused(strides, shared):
+    """Two heads, or heads of two sequences, in one place."""
+    out = _strided((2, 8, 64), (*strides, 1))
+    assert _shared(out) == shared
+    for call, kwargs in _calls(out=out):
+        with pytest.raises(ValueError if shared else RuntimeError,
+                           match="out must be" if shared else "ROCm"):
+            call(**kwargs)
+
+
+@pytest.mark.parametrize("strides,shared", [
+    ((64, 64, 64), True), ((1024, 64, 64), True), ((2048, 512, 64), True), ((1024, 2048, 72), True),
+    ((64, 1024, 128), True), ((2048, 1024, 56), True), ((2048, 0, 64), True), ((2048, 64, 128), False),
+    ((64, 4096, 192), False), ((2304, 1152, 72), False), ((1024, 3072, 64), False)])
+def test_caches_of_one_row_for_two_are_refused(strides, shared):
+    """Two pages, heads or tokens in one place; the attention only reads them."""
+    pages = _strided((3, 2, 16, 64), (*strides, 1))
+    assert _shared(pages) == shared
+    for name in ("k_pages", "v_pages"):
+        (read, read_args), (write, write_args) = _calls(**{name: pages})
+        with pytest.raises(ValueError if shared else RuntimeError,
+                           match="overlap" if shared else "ROCm"):
+            write(**write_args)
+        with pytest.raises(RuntimeError, match="ROCm"):
+            read(**read_args)

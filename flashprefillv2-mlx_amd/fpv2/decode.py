@@ -135,6 +135,39 @@ def _overlaps_itself(t: torch.Tensor) -> bool:
     return not t.is_contiguous() and _rows_overlap(t.shape, t.stride())
 
 
+@lru_cache(maxsize=256)
+def _extent(shape, strides) -> int:
+    """Elements from a tensor's first to behind its last."""
+    return 0 if 0 in shape else 1 + sum(s * (n - 1) for s, n in zip(strides, shape))
+
+
+@lru_cache(maxsize=256)
+def _rows_meet(distance: int, *layouts) -> bool:
+    """Whether two tensors ``(bytes of an element, shape, strides)`` have a byte in common, the
+    first of which starts ``distance`` bytes behind the second."""
+    spans: dict = {}
+    widths = []
+    for sign, (size, shape, strides) in zip((1, -1), layouts):
+        dims = [(s * size, n) for s, n in zip(strides, shape) if n > 1]
+        widths.append(dims.pop()[1] * size if dims and shape[-1] > 1 and strides[-1] == 1 else size)
+        for s, n in dims:
+            least, most = spans.get(s, (0, 0))
+            spans[s] = (least, most + n - 1) if sign > 0 else (least - n + 1, most)
+    return _reaches(distance, [(s, *x) for s, x in spans.items()], -widths[0], widths[1])
+
+
+def _share_memory(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether two tensors of one device have a byte in common."""
+    distance = a.data_ptr() - b.data_ptr()
+    size, other, layout, other_layout = a.element_size(), b.element_size(), a.stride(), b.stride()
+    if (distance >= other * _extent(b.shape, other_layout)
+            or -distance >= size * _extent(a.shape, layout)):
+        return False
+    if a.numel() == 0 or b.numel() == 0:
+        return False
+    return _rows_meet(distance, (size, a.shape, layout), (other, b.shape, other_layout))
+
+
 def _pages(k_pages: torch.Tensor, v_pages: torch.Tensor):
     """The caches' shape and strides."""
     if k_pages.ndim != 4 or v_pages.ndim != 4:
@@ -160,6 +193,15 @@ def _page_strides(k_pages: torch.Tensor, v_pages: torch.Tensor):
     if k is None or v is None:
         raise ValueError("the caches' rows must be contiguous and 16-byte aligned")
     return *k, *v
+
+
+@lru_cache(maxsize=256)
+def _page_layout(pages, heads, rows, dim, *strides):
+    """Whether rows of a cache share memory, and the bytes that each of them spans."""
+    shape = (pages, heads, rows, dim)
+    k, v = (*strides[:3], 1), (*strides[3:], 1)
+    return (_rows_overlap(shape, k) or _rows_overlap(shape, v), 2 * _extent(shape, k),
+            2 * _extent(shape, v))
 
 
 @lru_cache(maxsize=256)
@@ -315,9 +357,10 @@ def rope_to_pages(qkv: torch.Tensor, q_weight: torch.Tensor | None, k_weight: to
     if kv_heads == 0 or qkv.shape[1] != (query_heads + 2 * kv_heads) * dim:
         raise ValueError("qkv rows must hold the query, key and value heads")
     page_strides = _page_strides(k_pages, v_pages)
-    for t in (k_pages, v_pages):
-        if _overlaps_itself(t):
-            raise ValueError("the caches' rows overlap")
+    overlap, k_bytes, v_bytes = _page_layout(pages, kv_heads, page_size, dim, *page_strides)
+    if overlap or (-v_bytes < v_pages.data_ptr() - k_pages.data_ptr() < k_bytes
+                   and _share_memory(k_pages, v_pages)):
+        raise ValueError("the caches' rows overlap")
     for name, t in (("q_weight", q_weight), ("k_weight", k_weight)):
         if t is not None and (t.shape != (dim,) or t.dtype != qkv.dtype or t.data_ptr() & 15
                               or not t.is_contiguous()):

@@ -87,3 +87,44 @@ def test_caches_of_one_row_for_two_are_refused(strides, shared):
             write(**write_args)
         with pytest.raises(RuntimeError, match="ROCm"):
             read(**read_args)
+
+
+def test_shared_memory_is_found():
+    """Against all bytes, over pairs of small views of one storage and of two types."""
+    rng = random.Random(2)
+    store = torch.zeros(4096, dtype=torch.uint8)
+    found = 0
+    for _ in range(4000):
+        pair, taken = [], []
+        for _ in "ab":
+            size = rng.choice([2, 4])
+            shape = [rng.choice([1, 2, 3, 5]) for _ in range(rng.choice([1, 2]))] + [rng.choice([1, 4, 8])]
+            strides = [rng.choice([0, 1, 2, 3, 4, 8, 12, 16, 24, 32, 48, 60]) for _ in shape[:-1]]
+            strides.append(rng.choice([1, 1, 1, 1, 2]))
+            typed = store.view(BF16 if size == 2 else torch.float32)
+            t = typed.as_strided(shape, strides, rng.choice([0, 3, 8, 16, 40, 61, 200, 400]) * 4 // size)
+            pair.append(t)
+            at = _addresses(t) * size
+            taken.append({int(x) + i for x in at for i in range(size)})
+        want = not taken[0].isdisjoint(taken[1])
+        assert decode._share_memory(*pair) == want, [(t.shape, t.stride(), t.storage_offset()) for t in pair]
+        found += want
+    assert 500 < found < 3500
+
+
+def test_keys_and_values_in_one_place_are_refused():
+    pool = torch.zeros(6, 2, 16, 128, dtype=BF16)
+    flat = pool.view(-1)
+    shape = (3, 2, 16, 64)
+    fine = [(pool[:3, ..., :64], pool[:3, ..., 64:]), (pool[::2, ..., :64], pool[1::2, ..., :64]),
+            (pool[:3, :, :, 64:], pool[3:, :, :, 64:]),
+            # K of whole pages, V with the heads inside the rows, page by page
+            (flat.as_strided(shape, (4096, 1024, 64, 1)), flat[2048:].as_strided(shape, (4096, 64, 128, 1)))]
+    bad = [(pool[:3, ..., :64], pool[:3, ..., :64]), (pool[:3, ..., :64], pool[:3, ..., 32:96]),
+           (pool[:3, ..., :64], pool[2:5, ..., :64]),
+           (flat.as_strided(shape, (4096, 1024, 64, 1)), flat[2040:].as_strided(shape, (4096, 64, 128, 1)))]
+    for pairs, error, message in ((fine, RuntimeError, "ROCm"), (bad, ValueError, "overlap")):
+        for k, v in pairs + [(v, k) for k, v in pairs]:
+            (_, _), (rope, args) = _calls(k_pages=k, v_pages=v)
+            with pytest.raises(error, match=message):
+                rope(**args)

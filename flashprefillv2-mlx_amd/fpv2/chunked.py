@@ -53,7 +53,7 @@ from dataclasses import replace
 import torch
 
 from fpv2 import _lib
-from fpv2.decode import _device as check_device, decode_attention
+from fpv2.decode import _check_apart, _device as check_device, _in_place, decode_attention
 from fpv2.kernel import SUPPORTED_HEAD_DIMS, _launch_attention
 from fpv2.patch import (SelectedBlockCounter, _causal_block_count, _effective_config, _geometry,
                         _pool_into, _request_config, _select_attend)
@@ -339,8 +339,8 @@ class ChunkedPrefill:
 
         The reference leaves single tokens to the original attention
         (``fpv2/patch.py:177-205``: fewer queries than a tile).  ``out``: optional
-        ``[Hq, 1, D]`` destination.  The new rows are pooled when a later ``attend``
-        or ``step`` needs them."""
+        ``[Hq, 1, D]`` destination, ``q`` itself or apart from it and the cache.  The
+        new rows are pooled when a later ``attend`` or ``step`` needs them."""
         q3 = self._three_d(q, "q")
         if q3.shape != (self.query_heads, 1, self.head_dim) or q3.dtype != self.dtype:
             raise ValueError("q must be [query_heads, 1, head_dim] of the cache's geometry and dtype")
@@ -352,6 +352,8 @@ class ChunkedPrefill:
                                 or self.query_heads > 1 and out.stride(0) < self.head_dim):
             raise ValueError("out must be [query_heads, 1, head_dim] of q's dtype with contiguous "
                              "rows and no overlap")
+        if out is not None:
+            _check_apart(out, *(q3, self.k, self.v)[_in_place(out, q3):])
         check_device([x for x in (q3, self.k, k, v, out) if x is not None])
         if k is not None:
             k, v = self._rows(k, v)

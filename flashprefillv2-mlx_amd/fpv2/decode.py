@@ -168,6 +168,22 @@ def _share_memory(a: torch.Tensor, b: torch.Tensor) -> bool:
     return _rows_meet(distance, (size, a.shape, layout), (other, b.shape, other_layout))
 
 
+def _in_place(out: torch.Tensor, t: torch.Tensor) -> bool:
+    """Whether ``out`` is ``t``, element for element."""
+    return out.data_ptr() == t.data_ptr() and all(
+        n == 1 or a == b for n, a, b in zip(out.shape, out.stride(), t.stride()))
+
+
+def _check_apart(out: torch.Tensor, *operands) -> None:
+    first = out.data_ptr()
+    end = first + out.element_size() * _extent(out.shape, out.stride())
+    for t in operands:
+        at = t.data_ptr()
+        if (at < end and first < at + t.element_size() * _extent(t.shape, t.stride())
+                and _share_memory(out, t)):
+            raise ValueError("out must not share memory with what the call reads or writes beside it")
+
+
 def _pages(k_pages: torch.Tensor, v_pages: torch.Tensor):
     """The caches' shape and strides."""
     if k_pages.ndim != 4 or v_pages.ndim != 4:
@@ -227,7 +243,7 @@ def decode_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tens
     int32 ``[B]``, or one integer for all: the keys of each sequence, the new
     token's among them.  With ``window_tokens`` only the last that many keys
     and the first ``sink_tokens`` are visible.  Returns ``[B, Hq, D]`` (``out``
-    where given, any strides with ``D`` contiguous).
+    where given, any strides with ``D`` contiguous; ``q`` itself, or apart from all operands).
 
     Lengths and page ids are read on the device: they are clipped to what the
     table and the pages hold, and a sequence of length 0 gives zeros.  Rows
@@ -278,6 +294,7 @@ def decode_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tens
                 or _overlaps_itself(out)):
             raise ValueError("out must be [batch, query heads, head dim] of q's dtype with a "
                              "contiguous last dimension and no overlap")
+        _check_apart(out, *tensors[_in_place(out, q):3])
         tensors.append(out)
     index = _device(tensors)
     if out is None:
@@ -339,7 +356,8 @@ def rope_to_pages(qkv: torch.Tensor, q_weight: torch.Tensor | None, k_weight: to
     a token whose slot lies outside the pages (say -1) is padding and is not
     written.  ``positions`` and ``slots`` are int32 or int64 ``[T]``, or an
     integer: the first token's, the others following.  Returns the query
-    heads ``[T, Hq, D]`` (``out`` where given).
+    heads ``[T, Hq, D]`` (``out`` where given: the query heads of ``qkv`` themselves, or apart
+    from all operands).
 
     Everything is computed in float32 and rounded once.  Positions are clipped
     to the tables.  Slots must be distinct: of two tokens with one slot,
@@ -379,7 +397,7 @@ def rope_to_pages(qkv: torch.Tensor, q_weight: torch.Tensor | None, k_weight: to
     positions, position_bytes, first_position = _index(positions, "positions", tokens)
     slots, slot_bytes, first_slot = _index(slots, "slots", tokens)
     tensors = [qkv, k_pages, v_pages, cos, sin]
-    for t in (q_weight, k_weight, positions, slots, out):
+    for t in (q_weight, k_weight, positions, slots):
         if t is not None:
             tensors.append(t)
     if out is not None and (out.shape != (tokens, query_heads, dim) or out.dtype != qkv.dtype
@@ -387,6 +405,11 @@ def rope_to_pages(qkv: torch.Tensor, q_weight: torch.Tensor | None, k_weight: to
                             or _overlaps_itself(out)):
         raise ValueError("out must be [tokens, query heads, head dim] of qkv's dtype with 16-byte "
                          "aligned rows")
+    if out is not None:
+        here = (out.data_ptr() == qkv.data_ptr() and (tokens <= 1 or out.stride(0) == qkv.stride(0))
+                and (query_heads == 1 or out.stride(1) == dim))
+        _check_apart(out, *tensors[here:3])
+        tensors.append(out)
     index = _device(tensors)
     if out is None:
         out = torch.empty((tokens, query_heads, dim), dtype=qkv.dtype, device=qkv.device)
@@ -475,10 +498,10 @@ def quantized_linear(x: torch.Tensor, packed: torch.Tensor, scales: torch.Tensor
     ``x`` ``[..., K]`` in float16 or bfloat16, ``scales``/``biases`` of the same
     dtype; returns ``[..., N]`` in that dtype or, with ``out_dtype``, in float32.
     ``out``: optional ``[M, N]`` destination (``x`` ``[M, K]``) with contiguous
-    rows.  Products and sums are in float32 with the weights exact; ``x`` must be
-    below 1e34 (an infinite value gives NaN).  Made for the few rows of a decode
-    step: the weights are read once for every 32 rows, so a large prompt is better
-    served by a product with ``dequantize_weight``'s result."""
+    rows, apart from all operands.  Products and sums are in float32 with the weights
+    exact; ``x`` must be below 1e34 (an infinite value gives NaN).  Made for the few
+    rows of a decode step: the weights are read once for every 32 rows, so a large
+    prompt is better served by a product with ``dequantize_weight``'s result."""
     if x.ndim < 1 or x.dtype not in _HALF:
         raise ValueError("x must be [..., in] in float16 or bfloat16")
     group = _group_size(packed, scales, biases)
@@ -504,6 +527,7 @@ def quantized_linear(x: torch.Tensor, packed: torch.Tensor, scales: torch.Tensor
                 or n > 1 and out.stride(1) != 1 or m > 1 and out.stride(0) < n):
             raise ValueError("out must be [rows, out] of out_dtype with contiguous rows, x [rows, in]")
         out_stride = out.stride(0) if m > 1 else n
+        _check_apart(out, x, packed, scales, biases)
         tensors.append(out)
     index = _device(tensors)
     if out is None:

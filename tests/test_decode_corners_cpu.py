@@ -128,3 +128,37 @@ def test_keys_and_values_in_one_place_are_refused():
             (_, _), (rope, args) = _calls(k_pages=k, v_pages=v)
             with pytest.raises(error, match=message):
                 rope(**args)
+
+
+def test_out_in_the_memory_of_other_operands_is_refused():
+    """But for the queries' own place, a destination is apart from what the call reads and writes."""
+    (attention, args), (rope, rope_args) = _calls()
+    pool = torch.zeros(4 * 12 * 64 + 8, dtype=BF16)
+    q, qkv = pool[:1024].view(2, 8, 64), pool[:2 * 12 * 64].view(2, 12 * 64)
+    heads = qkv[:, :512].unflatten(1, (8, 64))
+    wide = torch.zeros(2, 8, 2, 64, dtype=BF16)
+    for out, fine in ((q, True), (pool[1024:2048].view(2, 8, 64), True),
+                      (pool[8:1032].view(2, 8, 64), False)):
+        with pytest.raises(RuntimeError if fine else ValueError, match="ROCm" if fine else "share memory"):
+            attention(**{**args, "q": q, "out": out})
+    swapped = pool[:1024].as_strided((2, 8, 64), (64, 128, 1))  # q's memory in another order
+    for bad in (dict(q=q, out=swapped), dict(out=args["k_pages"][0, 0, :16].view(2, 8, 64)),
+                dict(out=args["v_pages"][1].view(2, -1)[:, :512].unflatten(1, (8, 64)))):
+        with pytest.raises(ValueError, match="share memory"):
+            attention(**{**args, **bad})
+    for out, fine in ((heads, True), (wide[:, :, 0], True), (q, False),
+                      (qkv[:, 256:768].unflatten(1, (8, 64)), False), (pool[1024:2048].view(2, 8, 64), False),
+                      (pool[1536:2560].view(2, 8, 64), True)):
+        with pytest.raises(RuntimeError if fine else ValueError, match="ROCm" if fine else "share memory"):
+            rope(**{**rope_args, "qkv": qkv, "out": out})
+    for name in ("k_pages", "v_pages"):
+        with pytest.raises(ValueError, match="share memory"):
+            rope(**{**rope_args, "out": rope_args[name][1].view(2, -1)[:, :512].unflatten(1, (8, 64))})
+    weights = fpv2.quantize_weight(torch.zeros(128, 128, dtype=BF16))
+    x = torch.zeros(6, 128, dtype=BF16)
+    for out, fine in ((torch.zeros(3, 128, dtype=BF16), True), (x[3:], True), (x[:3], False),
+                      (x[2:5], False), (weights[0].view(BF16).view(-1)[:384].view(3, 128), False),
+                      (weights[1].view(-1)[:128].view(1, 128), False)):
+        rows = x[:out.shape[0]]
+        with pytest.raises(RuntimeError if fine else ValueError, match="ROCm" if fine else "share memory"):
+            fpv2.quantized_linear(rows, *weights, out=out)

@@ -10,6 +10,7 @@ import pytest
 import torch
 
 import fpv2
+from fpv2 import ChunkedPrefill
 from fpv2.prefill_harness import ChunkedPrefillRunner, DecoderShape, RandomDecoder
 
 pytestmark = pytest.mark.gpu
@@ -181,3 +182,51 @@ def test_generate_ends_with_the_first_row_of_nothing(cuda):
 
     runner.decode = decode
     assert runner.generate(prompt, 64, 6, temperature=0.0).tolist() == free[:2].tolist() + [-1] * 4
+
+
+@pytest.mark.parametrize("heads,hkv", [(8, 2), (40, 1)])
+@pytest.mark.parametrize("dim", [64, 256])
+@pytest.mark.parametrize("batch,length", [(1, 9000), (3, 1), (700, 90)])
+def test_attention_in_the_queries_place(cuda, heads, hkv, dim, batch, length):
+    """``out`` may be ``q``: items of one workgroup, of many, and of more heads than a tile."""
+    gen = torch.Generator(device=cuda).manual_seed(length)
+    q = torch.randn((batch, heads, dim), generator=gen, device=cuda).to(BF16)
+    k, v = (torch.randn((40, hkv, 256, dim), generator=gen, device=cuda).to(BF16) for _ in "kv")
+    table = torch.randint(0, 40, (batch, 36), generator=gen, device=cuda, dtype=torch.int32)
+    want = fpv2.decode_attention(q, k, v, table, length)
+    assert fpv2.decode_attention(q, k, v, table, length, out=q) is q
+    assert torch.equal(q, want)
+
+
+@pytest.mark.parametrize("tokens", [1, 9, 2500])
+@pytest.mark.parametrize("interleaved", [False, True])
+def test_rotation_in_the_projections_place(cuda, tokens, interleaved):
+    """``out`` may be the query heads of the rows themselves."""
+    gen = torch.Generator(device=cuda).manual_seed(tokens)
+    qkv = torch.randn((tokens, 12 * 128), generator=gen, device=cuda).to(BF16)
+    weight = torch.rand(128, generator=gen, device=cuda).to(BF16)
+    angle = torch.rand((tokens, 32), generator=gen, device=cuda)
+    pages = [torch.zeros((-(-tokens // 16), 2, 16, 128), dtype=BF16, device=cuda) for _ in "kvkv"]
+
+    def call(kp, vp, out):
+        return fpv2.rope_to_pages(qkv, weight, weight, angle, angle, 0, 0, kp, vp, query_heads=8,
+                                  interleaved=interleaved, out=out)
+
+    rest = qkv[:, 1024:].clone()
+    want = call(*pages[:2], None)
+    got = call(*pages[2:], qkv[:, :1024].unflatten(1, (8, 128)))
+    assert got.data_ptr() == qkv.data_ptr() and torch.equal(got, want)
+    assert torch.equal(pages[0], pages[2]) and torch.equal(pages[1], pages[3])
+    assert torch.equal(qkv[:, 1024:], rest)
+
+
+def test_a_cache_as_destination_is_refused_before_the_append(cuda):
+    cache = ChunkedPrefill(4, 2, 64, 8, device=cuda)
+    q, k = (torch.ones((h, 1, 64), dtype=BF16, device=cuda) for h in (4, 2))
+    for out in (cache.k.view(-1)[:256].view(4, 1, 64), cache.v.view(-1)[512:768].view(4, 1, 64)):
+        with pytest.raises(ValueError, match="share memory"):
+            cache.decode(q, k, k, out=out)
+        assert cache.length == 0
+    want = cache.decode(q, k, k)
+    cache.reset()
+    assert torch.equal(cache.decode(q, k, k, out=q), want) and torch.equal(q[None], want)

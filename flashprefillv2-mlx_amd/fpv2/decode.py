@@ -15,8 +15,9 @@ HIP kernels of the same library (``include/fpv2_decode.h``):
 
 All of them run on the current stream of their tensors' device, whichever
 device is current, allocate from torch's allocator only (so they can be
-captured into a graph) and never synchronise.  None has a backward: tensors
-that require a gradient are refused while gradients are recorded.
+captured into a graph) and never synchronise.  None has a derivative: tensors
+that require a gradient are refused while gradients are recorded, and ones with a
+forward-mode tangent always.
 """
 
 from __future__ import annotations
@@ -25,6 +26,7 @@ import ctypes
 from functools import lru_cache
 
 import torch
+from torch.autograd import forward_ad
 
 from fpv2 import _lib
 from fpv2.kernel import SUPPORTED_HEAD_DIMS
@@ -36,6 +38,10 @@ def _device(tensors) -> int:
     """The index of the one ROCm device that all tensors are on; raises where there is
     none, or where a gradient would be lost.  (These calls take microseconds on
     the device, so the checks are made in few steps.)"""
+    if forward_ad._current_level >= 0 and any(
+            forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise RuntimeError("the decode operators have no derivative: their inputs must not "
+                           "carry tangents")
     index = tensors[0].get_device()
     if index >= 0:
         for t in tensors:

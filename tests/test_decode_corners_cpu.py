@@ -162,3 +162,23 @@ def test_out_in_the_memory_of_other_operands_is_refused():
         rows = x[:out.shape[0]]
         with pytest.raises(RuntimeError if fine else ValueError, match="ROCm" if fine else "share memory"):
             fpv2.quantized_linear(rows, *weights, out=out)
+
+
+def test_tangents_are_refused():
+    """They would be lost without a word, under no_grad too."""
+    weights = fpv2.quantize_weight(torch.zeros(128, 128, dtype=BF16))
+    (attention, args), (rope, rope_args) = _calls()
+    calls = [(attention, args, "q"), (attention, args, "v_pages"), (rope, rope_args, "qkv"),
+             (rope, {**rope_args, "k_weight": torch.ones(64, dtype=BF16)}, "k_weight"),
+             (fpv2.quantized_linear, dict(x=torch.zeros(3, 128, dtype=BF16), packed=weights[0],
+                                          scales=weights[1], biases=weights[2]), "x"),
+             (fpv2.sample_tokens, dict(logits=torch.zeros(3, 50), uniform=torch.zeros(3)), "logits")]
+    with torch.autograd.forward_ad.dual_level():
+        for call, kwargs, name in calls:
+            with pytest.raises(RuntimeError, match="ROCm"):
+                call(**kwargs)  # a level alone is nothing to refuse
+            dual = torch.autograd.forward_ad.make_dual(kwargs[name], torch.ones_like(kwargs[name]))
+            with pytest.raises(RuntimeError, match="tangents"):
+                call(**{**kwargs, name: dual})
+            with torch.no_grad(), pytest.raises(RuntimeError, match="tangents"):
+                call(**{**kwargs, name: dual})

@@ -479,9 +479,9 @@ def dequantize_weight(packed: torch.Tensor, scales: torch.Tensor, biases: torch.
     group = _group_size(packed, scales, biases)
     n = packed.shape[0]
     shifts = torch.arange(0, 32, 4, dtype=torch.int32, device=packed.device)
-    q = ((packed.view(torch.int32)[..., None] >> shifts) & 15).view(n, -1, group)
+    q = ((packed.view(torch.int32)[..., None] >> shifts) & 15).reshape(n, scales.shape[1], group)
     w = q * scales.float()[..., None] + biases.float()[..., None]
-    return w.view(n, -1).to(scales.dtype if dtype is None else dtype)
+    return w.reshape(n, packed.shape[1] * 8).to(scales.dtype if dtype is None else dtype)
 
 
 def _group_size(packed, scales, biases) -> int:

@@ -182,3 +182,19 @@ def test_tangents_are_refused():
                 call(**{**kwargs, name: dual})
             with torch.no_grad(), pytest.raises(RuntimeError, match="tangents"):
                 call(**{**kwargs, name: dual})
+
+
+@pytest.mark.parametrize("rows,group", [(0, 64), (1, 32), (10, 128)])
+def test_weights_of_any_layout_are_read_back(rows, group):
+    """No rows, rows in columns, every other row or column."""
+    gen = torch.Generator().manual_seed(rows)
+    w = torch.randn((rows, 256), generator=gen)
+    packed, scales, biases = fpv2.quantize_weight(w, group_size=group)
+    want = fpv2.dequantize_weight(packed, scales, biases)
+    assert want.shape == (rows, 256) and want.is_contiguous()
+    for layout in (lambda t: t.t().contiguous().t(), lambda t: t.repeat_interleave(2, 1)[:, ::2],
+                   lambda t: t.repeat_interleave(2, 0)[::2]):
+        again = fpv2.dequantize_weight(*(layout(t) for t in (packed, scales, biases)))
+        assert torch.equal(again, want)
+        parts = fpv2.quantize_weight(layout(w), group_size=group)
+        assert all(torch.equal(a, b) and a.is_contiguous() for a, b in zip(parts, (packed, scales, biases)))

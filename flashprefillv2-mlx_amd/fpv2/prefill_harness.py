@@ -37,8 +37,8 @@ import torch.nn.functional as F
 
 from fpv2 import _lib
 from fpv2.chunked import ChunkedPrefill
-from fpv2.decode import (_settings, decode_attention, dequantize_weight, quantize_weight, quantized_linear,
-                         rope_to_pages, sample_tokens)
+from fpv2.decode import (GROUP_SIZES, _settings, decode_attention, dequantize_weight,
+                         quantize_weight, quantized_linear, rope_to_pages, sample_tokens)
 from fpv2.selection import FPV2Config
 
 
@@ -209,13 +209,19 @@ class RandomDecoder:
         Decode steps then read the packed weights; the dense ones, which the
         prefill's products read, become the packed weights' values rounded to
         the model's dtype."""
+        names = ("qkv", "o", "gate_up", "down")
+        # (no weight is cut before all are known to have whole groups)
+        for w in [self.embed, *(layer[name] for layer in self.layers for name in names)]:
+            if group_size not in GROUP_SIZES or w.shape[1] % group_size:
+                raise ValueError(f"group_size must be one of {GROUP_SIZES} and divide the "
+                                 "columns of every weight")
+
         def cut(w):
             packed = quantize_weight(w, group_size=group_size)
             w.copy_(dequantize_weight(*packed))
             return packed
 
-        self.packed = [{name: cut(layer[name]) for name in ("qkv", "o", "gate_up", "down")}
-                       for layer in self.layers]
+        self.packed = [{name: cut(layer[name]) for name in names} for layer in self.layers]
         self.packed_embed = cut(self.embed)
 
     def parameters(self) -> int:

@@ -198,3 +198,17 @@ def test_weights_of_any_layout_are_read_back(rows, group):
         assert torch.equal(again, want)
         parts = fpv2.quantize_weight(layout(w), group_size=group)
         assert all(torch.equal(a, b) and a.is_contiguous() for a, b in zip(parts, (packed, scales, biases)))
+
+
+@pytest.mark.parametrize("group,intermediate", [(64, 288), (128, 448), (48, 288), (32, 272)])
+def test_a_model_is_cut_to_4_bits_as_a_whole_or_not_at_all(group, intermediate):
+    """Groups that the last projection's columns do not hold leave the first ones as they were."""
+    from fpv2.prefill_harness import DecoderShape, RandomDecoder
+    model = RandomDecoder(DecoderShape(layers=2, hidden=256, query_heads=8, kv_heads=2, head_dim=64,
+                                       intermediate=intermediate, vocab=100), device="cpu")
+    before = [{name: t.clone() for name, t in layer.items()} for layer in model.layers]
+    with pytest.raises(ValueError, match="group_size"):
+        model.quantize(group)
+    assert model.packed is None and model.packed_embed is None
+    for layer, old in zip(model.layers, before):
+        assert all(torch.equal(layer[name], old[name]) for name in old)

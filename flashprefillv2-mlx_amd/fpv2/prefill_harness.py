@@ -37,8 +37,9 @@ import torch.nn.functional as F
 
 from fpv2 import _lib
 from fpv2.chunked import ChunkedPrefill
-from fpv2.decode import (GROUP_SIZES, _settings, decode_attention, dequantize_weight,
-                         quantize_weight, quantized_linear, rope_to_pages, sample_tokens)
+from fpv2.decode import (GROUP_SIZES, MAX_VOCAB, _device as check_device, _settings,
+                         decode_attention, dequantize_weight, quantize_weight, quantized_linear,
+                         rope_to_pages, sample_tokens)
 from fpv2.selection import FPV2Config
 
 
@@ -447,7 +448,12 @@ class ChunkedPrefillRunner:
         # (what could be refused is looked at before the prompt is prefilled)
         if self.attention == "sdpa":
             raise ValueError("generate goes on over the caches of 'fpv2' or 'dense'")
-        _settings(temperature, top_k, top_p, min_p, 1)
+        settings = [rows for rows, _ in _settings(temperature, top_k, top_p, min_p, 1)
+                    if rows is not None]
+        if self.model.embed.shape[0] > MAX_VOCAB:
+            raise ValueError(f"the vocabulary must have 1 to {MAX_VOCAB} tokens")
+        if tokens.numel() == 0 or chunk <= 0:
+            raise ValueError("generate needs a prompt and a positive chunk")
         if any(cache.length for cache in self.caches):
             raise ValueError("generate starts from empty caches: call reset() first")
         if tokens.numel() + new_tokens - 1 > self.capacity:
@@ -457,6 +463,7 @@ class ChunkedPrefillRunner:
         elif (uniform.shape != (new_tokens,) or uniform.dtype != torch.float32
               or uniform.device != self.model.embed.device):
             raise ValueError("uniform must be float32 [new_tokens] on the model's device")
+        check_device([uniform, *settings])
         logits = self.prefill(tokens, chunk)
         out = []
         for i in range(new_tokens):

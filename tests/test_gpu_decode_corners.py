@@ -230,3 +230,25 @@ def test_a_cache_as_destination_is_refused_before_the_append(cuda):
     want = cache.decode(q, k, k)
     cache.reset()
     assert torch.equal(cache.decode(q, k, k, out=q), want) and torch.equal(q[None], want)
+
+
+def test_generate_refuses_before_the_prefill(cuda):
+    """What the sampling of the first token would refuse is refused with empty caches."""
+    runner = ChunkedPrefillRunner(RandomDecoder(SHAPE, device=cuda, seed=2), 64)
+    prompt = torch.arange(20, device=cuda)
+    for error, bad in ((RuntimeError, dict(temperature=torch.ones(1))),
+                       (RuntimeError, dict(top_k=torch.ones(1, dtype=torch.int32))),
+                       (RuntimeError, dict(uniform=torch.rand(2, device=cuda).requires_grad_())),
+                       (RuntimeError, dict(top_p=torch.ones(1, device=cuda, requires_grad=True))),
+                       (ValueError, dict(chunk=0)), (ValueError, dict(chunk=-3)),
+                       (ValueError, dict(tokens=prompt[:0]))):
+        with pytest.raises(error):
+            runner.generate(**{"tokens": prompt, "chunk": 64, "new_tokens": 2, **bad})
+        assert all(cache.length == 0 for cache in runner.caches)
+    assert runner.generate(prompt, 64, 2).shape == (2,)
+    wide = DecoderShape(layers=1, hidden=64, query_heads=2, kv_heads=1, head_dim=64,
+                        intermediate=64, vocab=(1 << 19) + 1)
+    runner = ChunkedPrefillRunner(RandomDecoder(wide, device=cuda, seed=2), 64)
+    with pytest.raises(ValueError, match="vocabulary"):
+        runner.generate(prompt, 64, 2)
+    assert runner.caches[0].length == 0

@@ -252,3 +252,47 @@ def test_generate_refuses_before_the_prefill(cuda):
     with pytest.raises(ValueError, match="vocabulary"):
         runner.generate(prompt, 64, 2)
     assert runner.caches[0].length == 0
+
+
+def _late(tensor):
+    """A copy of a tensor that is there only after a while, on the current stream."""
+    late = torch.zeros_like(tensor)
+    torch.cuda._sleep(20_000_000)
+    late.copy_(tensor)
+    return late
+
+
+def test_every_operator_runs_on_the_current_stream(cuda):
+    """The input of a call on a side stream comes late: a launch elsewhere reads zeros."""
+    gen = torch.Generator().manual_seed(4)
+    weights = [t.to(cuda) for t in fpv2.quantize_weight(torch.randn((2560, 1024), generator=gen).to(BF16))]
+    x = torch.randn((6, 1024), generator=gen).to(BF16).to(cuda)
+    logits = torch.randn((3, 40_009), generator=gen).to(cuda)
+    short = logits[:, :300].contiguous()
+    u = torch.rand(3, generator=gen).to(cuda)
+    qkv = torch.randn((5, 8 * 64), generator=gen).to(BF16).to(cuda)
+    angle = torch.rand((9, 32), generator=gen).to(cuda)
+    pages = [torch.zeros((2, 2, 16, 64), dtype=BF16, device=cuda) for _ in "kv"]
+
+    def rope(rows):
+        q = fpv2.rope_to_pages(rows, None, None, angle, angle, 2, 3, *pages, query_heads=4)
+        return [q, *(p.clone() for p in pages)]
+
+    cases = [(x, lambda t: [fpv2.quantized_linear(t, *weights)]),
+             (x[:1], lambda t: [fpv2.quantized_linear(t, *weights, out_dtype=torch.float32)]),
+             (qkv, rope)]
+    for rows in (logits, short):
+        for kwargs in (dict(), dict(temperature=0.0), dict(top_k=60, top_p=0.9), dict(top_p=0.9),
+                       dict(min_p=0.1)):
+            cases.append((rows, lambda t, kwargs=kwargs: list(
+                fpv2.sample_tokens(t, u, return_logprobs=True, **kwargs))))
+    side = torch.cuda.Stream()
+    for tensor, call in cases:
+        want = call(tensor)
+        for page in pages:
+            page.zero_()
+        torch.cuda.synchronize()
+        with torch.cuda.stream(side):
+            got = call(_late(tensor))
+        side.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, want))

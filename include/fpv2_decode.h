@@ -14,6 +14,9 @@
  * allocation, no host synchronisation, FPV2_OK or a negative fpv2_status with
  * fpv2_last_error() set.  Lengths, page ids, positions and slots are read on
  * the device; the ones out of range are clipped or skipped as stated.
+ * Outputs are apart from one another and from all inputs, and no two of an output's
+ * rows share memory (not checked here); only the queries' result may be the queries
+ * themselves (`out` of the attention, `q_out` in the rows of `qkv`), element for element.
  */
 #ifndef FPV2_DECODE_H_
 #define FPV2_DECODE_H_
@@ -51,6 +54,8 @@ typedef struct fpv2_decode_params {
  * page_table[b][t / page_size] (int32; without page_table of page b).  Page ids
  * are clipped to [0, pages) and lengths to [0, table_width * page_size]; a
  * sequence of length 0 gives zeros.  Rows behind a length are not used.
+ * The weights are rounded to the inputs' type for their product with v (f16: relative
+ * to 2^-15 of the greatest of 32 keys), their sum is not; everything else is float32.
  * bf16 or f16; the strides of q, k and v multiples of 8 and their pointers
  * 16-byte aligned.  workspace: fpv2_decode_attention_workspace_bytes bytes for
  * the current device (0: none), 16-byte aligned, not kept between calls; calls

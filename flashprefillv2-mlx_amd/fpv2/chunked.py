@@ -347,6 +347,7 @@ class ChunkedPrefill:
         if (k is None) != (v is None):
             raise ValueError("k and v are given together")
         # (all that could be refused is looked at before the token is appended)
+        scale = self.head_dim ** -0.5 if scale is None else float(scale)
         if out is not None and (out.shape != q3.shape or out.dtype != self.dtype
                                 or out.stride(2) != 1
                                 or self.query_heads > 1 and out.stride(0) < self.head_dim):

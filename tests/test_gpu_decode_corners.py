@@ -296,3 +296,14 @@ def test_every_operator_runs_on_the_current_stream(cuda):
             got = call(_late(tensor))
         side.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_a_scale_that_is_no_number_leaves_the_cache(cuda):
+    cache = ChunkedPrefill(4, 2, 64, 8, device=cuda)
+    q, k = (torch.ones((h, 1, 64), dtype=BF16, device=cuda) for h in (4, 2))
+    for bad in ("wide", [0.1], torch.ones(2)):
+        with pytest.raises((TypeError, ValueError, RuntimeError)):
+            cache.decode(q, k, k, scale=bad)
+        assert cache.length == 0
+    cache.decode(q, k, k, scale=0.5)
+    assert cache.length == 1

@@ -420,20 +420,25 @@ class ChunkedPrefillRunner:
         token = token.reshape(1).to(m.embed.device, torch.int64)
         row = token.clamp(0, m.embed.shape[0] - 1)
         x, delta = torch.where((row == token)[:, None], m.embed[row], math.nan), None
-        for li, (p, cache) in enumerate(zip(m.layers, self.caches)):
-            h = _add_rms_norm(x, delta, p["attn_norm"], s.rms_eps)
-            k_pages, v_pages = cache.pages()
-            cache.reserve(1)
-            q = rope_to_pages(linear(h, li, "qkv"), p["q_norm"], p["k_norm"], *self._tables,
-                              position, position, k_pages, v_pages, query_heads=s.query_heads,
-                              eps=s.rms_eps)
-            attn = decode_attention(q, k_pages, v_pages, None, cache.length)
-            h = _add_rms_norm(x, linear(attn.view(1, -1), li, "o"), p["mlp_norm"], s.rms_eps)
-            delta = linear(_silu_mul(linear(h, li, "gate_up"), s.intermediate), li, "down")
-        if m.packed_embed is None:
-            return self._head(x, delta)
-        last = _add_rms_norm(x, delta, m.final_norm, s.rms_eps)
-        return quantized_linear(last, *m.packed_embed, out_dtype=torch.float32)[0]
+        try:
+            for li, (p, cache) in enumerate(zip(m.layers, self.caches)):
+                h = _add_rms_norm(x, delta, p["attn_norm"], s.rms_eps)
+                k_pages, v_pages = cache.pages()
+                cache.reserve(1)
+                q = rope_to_pages(linear(h, li, "qkv"), p["q_norm"], p["k_norm"], *self._tables,
+                                  position, position, k_pages, v_pages, query_heads=s.query_heads,
+                                  eps=s.rms_eps)
+                attn = decode_attention(q, k_pages, v_pages, None, cache.length)
+                h = _add_rms_norm(x, linear(attn.view(1, -1), li, "o"), p["mlp_norm"], s.rms_eps)
+                delta = linear(_silu_mul(linear(h, li, "gate_up"), s.intermediate), li, "down")
+            if m.packed_embed is None:
+                return self._head(x, delta)
+            last = _add_rms_norm(x, delta, m.final_norm, s.rms_eps)
+            return quantized_linear(last, *m.packed_embed, out_dtype=torch.float32)[0]
+        except BaseException:
+            for cache in self.caches:  # (rows behind a cache's length are never used)
+                cache.length = position
+            raise
 
     def generate(self, tokens: torch.Tensor, chunk: int, new_tokens: int, *,
                  temperature: float = 1.0, top_k: int = 0, top_p: float = 1.0,

@@ -75,7 +75,7 @@ def test_destinations_of_one_row_for_two_are_refused(strides, shared):
 @pytest.mark.parametrize("strides,shared", [
     ((64, 64, 64), True), ((1024, 64, 64), True), ((2048, 512, 64), True), ((1024, 2048, 72), True),
     ((64, 1024, 128), True), ((2048, 1024, 56), True), ((2048, 0, 64), True), ((2048, 64, 128), False),
-    ((64, 4096, 192), False), ((2304, 1152, 72), False), ((1024, 3072, 64), False)])
+    ((64, 4096, 192), False), ((2304, 1152, 72), False), ((1024, 4096, 64), False)])
 def test_caches_of_one_row_for_two_are_refused(strides, shared):
     """Two pages, heads or tokens in one place; the attention only reads them."""
     pages = _strided((3, 2, 16, 64), (*strides, 1))
@@ -133,7 +133,7 @@ def test_keys_and_values_in_one_place_are_refused():
 def test_out_in_the_memory_of_other_operands_is_refused():
     """But for the queries' own place, a destination is apart from what the call reads and writes."""
     (attention, args), (rope, rope_args) = _calls()
-    pool = torch.zeros(4 * 12 * 64 + 8, dtype=BF16)
+    pool = torch.zeros(3200, dtype=BF16)
     q, qkv = pool[:1024].view(2, 8, 64), pool[:2 * 12 * 64].view(2, 12 * 64)
     heads = qkv[:, :512].unflatten(1, (8, 64))
     wide = torch.zeros(2, 8, 2, 64, dtype=BF16)

@@ -307,3 +307,25 @@ def test_a_scale_that_is_no_number_leaves_the_cache(cuda):
         assert cache.length == 0
     cache.decode(q, k, k, scale=0.5)
     assert cache.length == 1
+
+
+def test_a_step_that_fails_takes_its_token_back(cuda):
+    """A refusal inside a later layer leaves every layer's cache as it was."""
+    model = RandomDecoder(SHAPE, device=cuda, seed=3)
+    runner = ChunkedPrefillRunner(model, 64)
+    prompt, token = torch.arange(20, device=cuda), torch.tensor([7], device=cuda)
+    runner.prefill(prompt, 64)
+    want = runner.decode(token)
+    runner.reset()
+    runner.prefill(prompt, 64)
+    model.layers[1]["qkv"].requires_grad_()
+    with pytest.raises(RuntimeError, match="no backward"):
+        runner.decode(token)
+    assert [cache.length for cache in runner.caches] == [20, 20]
+    with torch.no_grad():
+        model.final_norm, norm = model.final_norm.float(), model.final_norm
+        with pytest.raises(ValueError, match="weight"):
+            runner.decode(token)
+        assert [cache.length for cache in runner.caches] == [20, 20]
+        model.final_norm = norm
+        assert torch.equal(runner.decode(token), want)

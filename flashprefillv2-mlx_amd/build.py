@@ -23,7 +23,8 @@ INCLUDE = ROOT / "include"
 OUT = HERE / "fpv2" / "libfpv2_hip.so"
 SOURCES = ["fpv2_abi.cpp", "fpv2_pool.hip", "fpv2_select.hip", "fpv2_attention.hip",
            "fpv2_decoder.hip", "fpv2_decode.hip", "fpv2_rope_pages.hip", "fpv2_q4.hip",
-           "fpv2_sample.hip"]
+           "fpv2_sample.hip", "fpv2_shared_prefix.hip", "fpv2_cache8.hip", "fpv2_decode_q8.hip",
+           "fpv2_logprobs.hip"]
 ARCH = "gfx950"
 
 

@@ -8,8 +8,13 @@ selection front end (``FPV2Config``/``pool_blocks``/``block_scores_and_select``/
 layer's chunked prefill over a growing KV cache with incremental pooling.
 ``fpv2.decode`` holds the operators of the decode step that follows:
 ``decode_attention``, ``rope_to_pages``, ``quantized_linear``, ``sample_tokens``.
+``fpv2.batch`` holds the ones of serving a batch: ``shared_prefix_attention``,
+``quantize_to_pages``, ``dequantize_pages``, ``quantized_decode_attention``,
+``token_logprobs``.
 """
 
+from fpv2.batch import (TokenLogprobs, dequantize_pages, quantize_to_pages,
+                        quantized_decode_attention, shared_prefix_attention, token_logprobs)
 from fpv2.chunked import ChunkedPrefill
 from fpv2.decode import (decode_attention, dequantize_weight, quantize_weight, quantized_linear,
                          rope_to_pages, sample_tokens)
@@ -19,18 +24,24 @@ from fpv2.selection import FPV2Config, block_scores_and_select, density, pool_bl
 __all__ = [
     "ChunkedPrefill",
     "FPV2Config",
+    "TokenLogprobs",
     "block_scores_and_select",
     "block_sparsity",
     "decode_attention",
     "density",
+    "dequantize_pages",
     "dequantize_weight",
     "disable",
     "enable",
     "fpv2_sdpa",
     "is_enabled",
     "pool_blocks",
+    "quantize_to_pages",
     "quantize_weight",
+    "quantized_decode_attention",
     "quantized_linear",
     "rope_to_pages",
     "sample_tokens",
+    "shared_prefix_attention",
+    "token_logprobs",
 ]

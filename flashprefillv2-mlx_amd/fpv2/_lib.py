@@ -1,5 +1,5 @@
 """ctypes binding of ``libfpv2_hip.so`` (C ABI declared in ``include/fpv2.h``,
-``include/fpv2_decoder.h`` and ``include/fpv2_decode.h``).
+``include/fpv2_decoder.h``, ``include/fpv2_decode.h`` and ``include/fpv2_batch.h``).
 
 The library is built in-tree by ``flashprefillv2-mlx_amd/build.py``.  There is
 no fallback: if the library is missing or a tensor is not on a ROCm device,
@@ -60,6 +60,15 @@ EXPORTED_SYMBOLS = (
     "fpv2_quantized_linear",
     "fpv2_sample_tokens_workspace_bytes",
     "fpv2_sample_tokens",
+    # serving a batch (fpv2_batch.h)
+    "fpv2_shared_prefix_attention_workspace_bytes",
+    "fpv2_shared_prefix_attention",
+    "fpv2_quantize_to_pages",
+    "fpv2_dequantize_pages",
+    "fpv2_quantized_decode_attention_workspace_bytes",
+    "fpv2_quantized_decode_attention",
+    "fpv2_token_logprobs_workspace_bytes",
+    "fpv2_token_logprobs",
 )
 
 
@@ -175,6 +184,58 @@ class SampleParams(ctypes.Structure):
     ]
 
 
+class SharedPrefixParams(ctypes.Structure):
+    """``fpv2_shared_prefix_params`` (field order and types as in fpv2_batch.h)."""
+
+    _fields_ = [("own", DecodeParams)] + [(name, ctypes.c_int64) for name in (
+        "prefix_pages", "prefix_page_size", "prefix_table_width", "prefix_length",
+        "pk_page_stride", "pk_head_stride", "pk_row_stride", "pv_page_stride", "pv_head_stride",
+        "pv_row_stride")]
+
+
+_SCALE_STRIDES = [(name, ctypes.c_int64) for name in (
+    "ks_page_stride", "ks_head_stride", "ks_row_stride", "vs_page_stride", "vs_head_stride",
+    "vs_row_stride")]
+
+
+class CodePages(ctypes.Structure):
+    """``fpv2_code_pages`` (field order and types as in fpv2_batch.h)."""
+
+    _fields_ = [(name, ctypes.c_int64) for name in (
+        "kv_heads", "head_dim", "pages", "page_size", "k_page_stride", "k_head_stride",
+        "k_row_stride", "v_page_stride", "v_head_stride", "v_row_stride")] + _SCALE_STRIDES
+
+
+class QuantizeParams(ctypes.Structure):
+    """``fpv2_quantize_params`` (field order and types as in fpv2_batch.h)."""
+
+    _fields_ = [("cache", CodePages)] + [(name, ctypes.c_int64) for name in (
+        "tokens", "slot_bytes", "first_slot", "k_token_stride", "k_head_stride",
+        "v_token_stride", "v_head_stride")]
+
+
+class DequantizeParams(ctypes.Structure):
+    """``fpv2_dequantize_params`` (field order and types as in fpv2_batch.h)."""
+
+    _fields_ = [("cache", CodePages)] + [(name, ctypes.c_int64) for name in (
+        "batch", "table_width", "table_stride", "length", "tokens", "zero_rest",
+        "k_batch_stride", "k_head_stride", "k_row_stride", "v_batch_stride", "v_head_stride",
+        "v_row_stride")]
+
+
+class QuantizedDecodeParams(ctypes.Structure):
+    """``fpv2_quantized_decode_params`` (field order and types as in fpv2_batch.h)."""
+
+    _fields_ = [("attention", DecodeParams)] + _SCALE_STRIDES
+
+
+class LogprobsParams(ctypes.Structure):
+    """``fpv2_logprobs_params`` (field order and types as in fpv2_batch.h)."""
+
+    _fields_ = [(name, ctypes.c_int64) for name in (
+        "rows", "vocab", "logits_stride", "token_bytes", "top")]
+
+
 _lib = None
 
 
@@ -247,6 +308,26 @@ def _declare(lib: ctypes.CDLL) -> None:
     lib.fpv2_sample_tokens_workspace_bytes.argtypes = [ctypes.POINTER(SampleParams)]
     lib.fpv2_quantized_linear.restype = ctypes.c_int
     lib.fpv2_quantized_linear.argtypes = [vp] * 5 + [i32, i32] + [i64] * 8 + [vp]
+    lib.fpv2_shared_prefix_attention_workspace_bytes.restype = i64
+    lib.fpv2_shared_prefix_attention_workspace_bytes.argtypes = [ctypes.POINTER(SharedPrefixParams)]
+    lib.fpv2_shared_prefix_attention.restype = ctypes.c_int
+    lib.fpv2_shared_prefix_attention.argtypes = [vp] * 10 + [i32, ctypes.POINTER(SharedPrefixParams),
+                                                             vp, i64, vp]
+    lib.fpv2_quantize_to_pages.restype = ctypes.c_int
+    lib.fpv2_quantize_to_pages.argtypes = [vp] * 7 + [i32, ctypes.POINTER(QuantizeParams), vp]
+    lib.fpv2_dequantize_pages.restype = ctypes.c_int
+    lib.fpv2_dequantize_pages.argtypes = [vp] * 8 + [i32, ctypes.POINTER(DequantizeParams), vp]
+    lib.fpv2_quantized_decode_attention_workspace_bytes.restype = i64
+    lib.fpv2_quantized_decode_attention_workspace_bytes.argtypes = [
+        ctypes.POINTER(QuantizedDecodeParams)]
+    lib.fpv2_quantized_decode_attention.restype = ctypes.c_int
+    lib.fpv2_quantized_decode_attention.argtypes = [vp] * 8 + [
+        i32, ctypes.POINTER(QuantizedDecodeParams), vp, i64, vp]
+    lib.fpv2_token_logprobs_workspace_bytes.restype = i64
+    lib.fpv2_token_logprobs_workspace_bytes.argtypes = [ctypes.POINTER(LogprobsParams)]
+    lib.fpv2_token_logprobs.restype = ctypes.c_int
+    lib.fpv2_token_logprobs.argtypes = [vp, vp, i32, ctypes.POINTER(LogprobsParams)] + [vp] * 5 + [
+        i64, vp]
 
 
 def load(path: str | os.PathLike | None = None) -> ctypes.CDLL:

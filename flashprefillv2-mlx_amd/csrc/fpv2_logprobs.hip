@@ -7,8 +7,11 @@
 //   t' = f (t + (R - R') s), s' = f s, f = 2^(R - R').
 // e is one fused multiply-add, so neither large logits nor R's own rounding cost bits.
 //
-// The alternatives: each wave keeps its greatest logits in order, one a lane, and
-// inserts the ones above its last.  Bound by reading the logits.
+// The alternatives: a logit and its token are one 64-bit key, whose order is theirs.  A
+// wave collects the keys above a floor in 64 slots and, when these are full, sorts them
+// and keeps the first.  The floor of its first logits is the greatest number that enough
+// lanes' maxima reach, so that few more than the wanted ones are collected at all.
+// Bound by reading the logits.
 #include "fpv2_batch.h"
 #include "fpv2_common.h"
 
@@ -27,8 +30,8 @@ struct LogArgs {
   float* entropy;
   int64_t* top_tokens;
   float* top_logprobs;
-  f32x4* parts;  // [rows][chunks] {R, s, t, -}
-  u32x2* lists;  // [rows][chunks][top] {bits of the logit, index}
+  f32x4* parts;     // [rows][chunks] {R, s, t, -}
+  uint64_t* lists;  // [rows][chunks][top] keys
   int64_t stride;
   int rows, vocab, top, chunks, token_bytes;
 };
@@ -69,35 +72,93 @@ __device__ __forceinline__ Sums join(Sums a, Sums b) {
   return {r, a.s + b.s, a.t + b.t};
 }
 
-// A wave's greatest logits so far, in order, equal ones by index: one a lane.
-struct List {
-  float x;
-  int at;
-  float last_x;  // of the last lane: what is not above it does not enter
-  int last_at;
-  __device__ __forceinline__ void clear() {
-    x = last_x = neg_inf();
-    at = last_at = 0x7fffffff;
+// Keys: greater logits first, equal ones (0 and -0 too) by token; 0: none.
+__device__ __forceinline__ uint32_t ordered(float x) {
+  const uint32_t b = __float_as_uint(x + 0.f);
+  return b ^ (static_cast<int32_t>(b) < 0 ? 0xffffffffu : 0x80000000u);
+}
+__device__ __forceinline__ float logit_of(uint64_t key) {
+  const uint32_t s = static_cast<uint32_t>(key >> 32);
+  return __uint_as_float(s ^ (s & 0x80000000u ? 0x80000000u : 0xffffffffu));
+}
+__device__ __forceinline__ int token_of(uint64_t key) { return static_cast<int>(~static_cast<uint32_t>(key)); }
+__device__ __forceinline__ uint64_t key_of(float x, uint32_t token) {
+  return x > neg_inf() ? static_cast<uint64_t>(ordered(x)) << 32 | static_cast<uint32_t>(~token) : 0;
+}
+
+// The wave's keys from the greatest on, one a lane.  HALVES: where the first 32 fall and
+// the rest rise, the last steps alone.
+template <bool HALVES>
+__device__ __forceinline__ uint64_t sorted(uint64_t key, int lane) {
+#pragma unroll
+  for (int size = HALVES ? 64 : 2; size <= 64; size *= 2)
+#pragma unroll
+    for (int step = size / 2; step >= 1; step /= 2) {
+      const uint64_t other = __shfl_xor(key, step, 64);
+      const bool first = (lane & step) == 0, falling = (lane & size) == 0 || size == 64;
+      key = (key > other) == (first == falling) ? key : other;
+    }
+  return key;
+}
+
+// A wave's greatest keys.
+struct Best {
+  uint64_t* slots;  // 64 of the wave's LDS
+  int top, count;
+  uint64_t floor;   // keys above it enter
+  float floor_x;    // which are of this logit or greater ones
+  __device__ __forceinline__ void start(uint64_t* lds, int wanted) {
+    slots = lds;
+    top = wanted;
+    count = 0;
+    floor = 0;
+    floor_x = neg_inf();
   }
-  __device__ __forceinline__ bool enters(float cx, int c) const {
-    return cx > last_x || (cx == last_x && c < last_at);
+  __device__ __forceinline__ void raise(uint64_t to) {
+    floor = to;
+    floor_x = logit_of(to + 1);  // (to is of the same logit, or just below all keys of the next)
   }
-  // all lanes with (cx, c) that enter, one after the other
-  __device__ __forceinline__ void insert(float cx, int c, bool live, int lane, int top) {
-    uint64_t mask = __ballot(live && cx > neg_inf() && enters(cx, c));
+  // The floor under a wave's first keys, from each lane's greatest (its high word, 0: none).
+  __device__ __forceinline__ void first_floor(uint32_t most) {
+    uint32_t at = 0;
+#pragma unroll
+    for (int bit = 31; bit >= 8; --bit) {
+      const uint32_t to = at | 1u << bit;
+      if (__popcll(__ballot(most >= to)) >= top) at = to;
+    }
+    if (at != 0) raise((static_cast<uint64_t>(at) << 32) - 1);
+  }
+  // All slots in order, the first ones kept; returns the lane's.
+  __device__ __forceinline__ uint64_t settle(int lane) {
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    uint64_t key = sorted<false>(lane < count ? slots[lane] : 0, lane);
+    key = lane < top ? key : 0;
+    slots[lane] = key;
+    count = __popcll(__ballot(key != 0));
+    if (count == top) {
+      const uint32_t high = __builtin_amdgcn_readlane(static_cast<uint32_t>(key >> 32), top - 1);
+      const uint32_t low = __builtin_amdgcn_readlane(static_cast<uint32_t>(key), top - 1);
+      floor = static_cast<uint64_t>(high) << 32 | low;
+      floor_x = logit_of(floor);
+    }
+    return key;
+  }
+  __device__ __forceinline__ void add(uint64_t key, int lane) {
+    uint64_t mask = __ballot(key > floor);
     while (mask != 0) {
-      const int from = __builtin_ctzll(mask);
-      const float nx = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(cx), from));
-      const int n = __builtin_amdgcn_readlane(c, from);
-      const int before = __popcll(__ballot(lane < top && (x > nx || (x == nx && at < n))));
-      const float up_x = __shfl_up(x, 1, 64);
-      const int up = __shfl_up(at, 1, 64);
-      x = lane == before ? nx : lane > before ? up_x : x;
-      at = lane == before ? n : lane > before ? up : at;
-      last_x = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(x), top - 1));
-      last_at = __builtin_amdgcn_readlane(at, top - 1);
-      mask &= mask - 1;
-      mask &= __ballot(enters(cx, c));
+      const int room = 64 - count;
+      const int before = __builtin_amdgcn_mbcnt_hi(mask >> 32, __builtin_amdgcn_mbcnt_lo(mask, 0));
+      const bool mine = mask >> lane & 1;
+      if (mine && before < room) slots[count + before] = key;
+      const int n = __popcll(mask);
+      if (n <= room) {
+        count += n;
+        return;
+      }
+      count = 64;
+      settle(lane);
+      mask = __ballot(mine && before >= room && key > floor);
     }
   }
 };
@@ -112,16 +173,22 @@ __device__ __forceinline__ Sums join_all(Sums a, Sums* sh, int tid) {
   return join(join(sh[0], sh[1]), join(sh[2], sh[3]));
 }
 
-// The lists of a workgroup's waves in its first one's (sh: [4][FPV2_MAX_TOP]).
-__device__ __forceinline__ void join_lists(List& list, u32x2 (*sh)[FPV2_MAX_TOP], int tid, int top) {
+// The greatest keys of a workgroup's waves, in the first one's lanes.
+__device__ __forceinline__ uint64_t join_best(Best& best, uint64_t (*sh)[64], int tid) {
   const int lane = tid & 63, wave = tid >> 6;
-  if (lane < top) sh[wave][lane] = u32x2{__float_as_uint(list.x), static_cast<uint32_t>(list.at)};
-  __syncthreads();
-  if (wave != 0) return;
-  for (int w = 1; w < 4; ++w) {
-    const u32x2 c = sh[w][lane % FPV2_MAX_TOP];
-    list.insert(__uint_as_float(c[0]), static_cast<int>(c[1]), lane < top, lane, top);
+  uint64_t key = best.settle(lane);
+#pragma unroll
+  for (int with = 1; with <= 2; with *= 2) {
+    __syncthreads();
+    if (wave % (2 * with) == 0) {
+      // (32 keys of each at most, the other's from its last on)
+      key = lane < 32 ? key : sh[wave + with][63 - lane];
+      key = sorted<true>(key, lane);
+      key = lane < best.top ? key : 0;
+      sh[wave][lane] = key;
+    }
   }
+  return key;
 }
 
 // (rounding could leave a sure token 2^-24 above 0)
@@ -130,7 +197,7 @@ __device__ __forceinline__ float log_share(float x, float r, float norm) {
 }
 
 template <typename T>
-__device__ __forceinline__ void write_row(const LogArgs& a, int row, Sums s, const List& list, int tid) {
+__device__ __forceinline__ void write_row(const LogArgs& a, int row, Sums s, uint64_t key, int tid) {
   const float norm = log2f(s.s);
   const bool none = s.r == neg_inf();
   if (tid == 0) {
@@ -144,10 +211,9 @@ __device__ __forceinline__ void write_row(const LogArgs& a, int row, Sums s, con
     a.entropy[row] = none ? 0.f : fmaxf((norm - s.t / s.s) * kLn2, 0.f);
   }
   if (tid < a.top) {
-    const bool some = list.x > neg_inf();
-    a.top_tokens[static_cast<int64_t>(row) * a.top + tid] = some ? list.at : -1;
+    a.top_tokens[static_cast<int64_t>(row) * a.top + tid] = key != 0 ? token_of(key) : -1;
     a.top_logprobs[static_cast<int64_t>(row) * a.top + tid] =
-        some ? log_share(clamped(list.x), s.r, norm) : neg_inf();
+        key != 0 ? log_share(clamped(logit_of(key)), s.r, norm) : neg_inf();
   }
 }
 
@@ -157,7 +223,7 @@ __global__ __launch_bounds__(256) void logprobs_kernel(LogArgs a) {
   typedef typename Logit<T>::raw raw;
   constexpr int kPer = Logit<T>::kPer, kEach = kVecs * kPer;
   __shared__ Sums sh_s[4];
-  __shared__ u32x2 sh_l[4][FPV2_MAX_TOP];
+  __shared__ uint64_t sh_l[TOP ? 4 : 1][64];
   const int tid = threadIdx.x, lane = tid & 63;
   const int row = blockIdx.x / a.chunks, chunk = blockIdx.x - row * a.chunks;
   const raw* const p = static_cast<const raw*>(a.logits) + row * a.stride;
@@ -167,8 +233,8 @@ __global__ __launch_bounds__(256) void logprobs_kernel(LogArgs a) {
   const int first = static_cast<int>(static_cast<int64_t>(vecs) * chunk / a.chunks);
   const int last = static_cast<int>(static_cast<int64_t>(vecs) * (chunk + 1) / a.chunks);
   Sums s = {neg_inf(), 0.f, 0.f};
-  List list;
-  list.clear();
+  Best best;
+  if constexpr (TOP) best.start(sh_l[tid >> 6], a.top);
   for (int v0 = first; v0 < last; v0 += 256 * kVecs) {
     float x[kEach];
 #pragma unroll
@@ -188,10 +254,12 @@ __global__ __launch_bounds__(256) void logprobs_kernel(LogArgs a) {
 #pragma unroll
     for (int j = 0; j < kEach; ++j) most = fmaxf(most, x[j]);
     if constexpr (TOP) {
-      if (__any(most >= list.last_x)) {
+      if (v0 == first) best.first_floor(most > neg_inf() ? ordered(most) : 0);
+      if (__any(most >= best.floor_x)) {
 #pragma unroll
         for (int j = 0; j < kEach; ++j)
-          list.insert(x[j], (v0 + 256 * (j / kPer) + tid) * kPer - skew + j % kPer, true, lane, a.top);
+          if (__any(x[j] >= best.floor_x))
+            best.add(key_of(x[j], (v0 + 256 * (j / kPer) + tid) * kPer - skew + j % kPer), lane);
       }
     }
     if (__builtin_fabsf(most) > kHuge && most != neg_inf()) {
@@ -209,41 +277,50 @@ __global__ __launch_bounds__(256) void logprobs_kernel(LogArgs a) {
     }
   }
   s = join_all(s, sh_s, tid);
-  if constexpr (TOP) join_lists(list, sh_l, tid, a.top);
+  uint64_t key = 0;
+  if constexpr (TOP) key = join_best(best, sh_l, tid);
   if (a.chunks == 1) {
-    write_row<T>(a, row, s, list, tid);
+    write_row<T>(a, row, s, key, tid);
     return;
   }
   const int64_t at = static_cast<int64_t>(row) * a.chunks + chunk;
   if (tid == 0) a.parts[at] = f32x4{s.r, s.s, s.t, 0.f};
-  if (TOP && tid < a.top) a.lists[at * a.top + tid] = u32x2{__float_as_uint(list.x), static_cast<uint32_t>(list.at)};
+  if (TOP && tid < a.top) a.lists[at * a.top + tid] = key;
 }
 
 // Joins a row's chunks: one workgroup a row.
 template <typename T, bool TOP>
 __global__ __launch_bounds__(256) void logprobs_join_kernel(LogArgs a) {
   __shared__ Sums sh_s[4];
-  __shared__ u32x2 sh_l[4][FPV2_MAX_TOP];
+  __shared__ uint64_t sh_l[TOP ? 4 : 1][64];
   const int tid = threadIdx.x, lane = tid & 63, row = blockIdx.x;
   const int64_t base = static_cast<int64_t>(row) * a.chunks;
+  uint64_t key = 0;
+  if constexpr (TOP) {
+    Best best;
+    best.start(sh_l[tid >> 6], a.top);
+    const int n = a.chunks * a.top;
+    for (int i0 = 0; i0 < n; i0 += 256 * kVecs) {
+      uint64_t keys[kVecs], most = 0;
+#pragma unroll
+      for (int i = 0; i < kVecs; ++i) {
+        const int at = i0 + 256 * i + tid;
+        keys[i] = at < n ? a.lists[base * a.top + at] : 0;
+        most = keys[i] > most ? keys[i] : most;
+      }
+      if (i0 == 0) best.first_floor(static_cast<uint32_t>(most >> 32));
+#pragma unroll
+      for (int i = 0; i < kVecs; ++i) best.add(keys[i], lane);
+    }
+    key = join_best(best, sh_l, tid);
+  }
   Sums s = {neg_inf(), 0.f, 0.f};
   for (int i = tid; i < a.chunks; i += 256) {
     const f32x4 part = a.parts[base + i];
     s = join(s, Sums{part[0], part[1], part[2]});
   }
   s = join_all(s, sh_s, tid);
-  List list;
-  list.clear();
-  if constexpr (TOP) {
-    const int n = a.chunks * a.top;
-    for (int i0 = 0; i0 < n; i0 += 256) {
-      const int i = i0 + tid;
-      const u32x2 c = i < n ? a.lists[base * a.top + i] : u32x2{0xff800000u, 0u};
-      list.insert(__uint_as_float(c[0]), static_cast<int>(c[1]), i < n, lane, a.top);
-    }
-    join_lists(list, sh_l, tid, a.top);
-  }
-  write_row<T>(a, row, s, list, tid);
+  write_row<T>(a, row, s, key, tid);
 }
 
 // Workgroups of a row: as many as fill the chip, of 1024 16-byte vectors at least.
@@ -331,7 +408,7 @@ extern "C" int fpv2_token_logprobs(const void* logits, const void* tokens, int d
   a.token_bytes = static_cast<int>(p.token_bytes);
   a.chunks = chunks_of(p, dtype);
   a.parts = static_cast<f32x4*>(workspace);
-  a.lists = reinterpret_cast<u32x2*>(a.parts + p.rows * a.chunks);
+  a.lists = reinterpret_cast<uint64_t*>(a.parts + p.rows * a.chunks);
   const hipStream_t s = static_cast<hipStream_t>(stream);
   return dtype == FPV2_F32    ? launch_top<float>(a, s)
          : dtype == FPV2_BF16 ? launch_top<bf16_t>(a, s)

@@ -18,7 +18,8 @@
 namespace fpv2 {
 namespace {
 
-constexpr int kMaxSplits = 512;
+constexpr int kMaxSplits = 512;  // parts of the prefix
+constexpr int kMaxOwn = 512;     // workgroups of the own keys
 
 struct PrefixArgs {
   const uint16_t* q;
@@ -40,10 +41,91 @@ __device__ __forceinline__ int prefix_length(const PrefixArgs& a) {
   return min(max(n, 0), a.capacity);
 }
 
-// A column's weights are relative to a reference.  bfloat16: one that moves only when a
-// score exceeds it by 2^kLag, so that most tiles rescale nothing (weights reach 2^kLag).
-// float16, which has only 2^-14 to 1 at full precision: by tile, as in the decode attention.
-constexpr float kLag = 8.f, kHeadroom = 15.f, kBelow = 40.f;
+// A column's weights are 2^(x - m), x = scale log2(e) q.k, with a reference m that moves when
+// it has to, so that most tiles rescale nothing.
+//   bfloat16: where a weight exceeds 2^kLag, to the greatest score.
+//   float16, which has only 2^-14 to 2^16: where a weight would exceed 2^kMost or the
+// tile's greatest is below 2^kLeast, to 2^-12 of the tile's greatest score (or 2^-40 of the
+// greatest so far, so that no float32 sum overflows).  So weights down to 2^-19 of their
+// tile's greatest keep their bits, whatever lies above that tile, and smaller ones are off by
+// 2^-30 of it.  (2^-15 instead of 2^-12: most tiles have a column that exceeds it, 128
+// sequences of an 8191-key prefix 41 us instead of @.)
+constexpr float kLag = 8.f, kMost = 15.9f, kLeast = 5.f, kHeadroom = 12.f, kBelow = 40.f;
+constexpr float kNone = -3e38f;  // the reference before any score: below all of them
+
+// The maximum of a column's four lanes, in each of them.
+__device__ __forceinline__ float column_max(float x) {
+  const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  x = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+  const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
+
+// A tile's exponents of 16 rows from its scores (of 32 keys the ones before `live`, counted
+// from the lane's first); O, l and m of the rows are moved where they have to be.
+struct Exponents {
+  float y[8];
+};
+template <typename T, int DT>
+__device__ __forceinline__ Exponents relate(const f32x4 (&sc)[2], float scale, int live, float& m, float& l,
+                                            float& greatest, f32x4 (&o)[DT]) {
+  constexpr bool kHalf = std::is_same<T, f16_t>::value;
+  const bool cut = live < 32;
+  Exponents e;
+  float top = neg_inf();
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    e.y[j] = __builtin_fmaf(sc[j / 4][j % 4], scale, -m);
+    if (cut && 16 * (j / 4) + j % 4 >= live) e.y[j] = neg_inf();
+    top = fmaxf(top, e.y[j]);
+  }
+  bool move;
+  if constexpr (kHalf) {
+    const uint64_t some = __ballot(top >= kLeast);
+    const uint32_t any = static_cast<uint32_t>(some) | static_cast<uint32_t>(some >> 32);
+    move = ((any | any >> 16) & 0xffffu) != 0xffffu || __any(top > kMost);
+  } else {
+    move = __any(top > kLag);
+  }
+  if (move) {
+    top = neg_inf();
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      e.y[j] = sc[j / 4][j % 4] * scale;
+      if (cut && 16 * (j / 4) + j % 4 >= live) e.y[j] = neg_inf();
+      top = fmaxf(top, e.y[j]);
+    }
+    top = column_max(top);
+    float to = m;
+    if constexpr (kHalf) {
+      greatest = fmaxf(greatest, top);
+      if ((top > m + kMost || top < m + kLeast) && greatest > neg_inf())
+        to = fmaxf(top, greatest - kBelow) - kHeadroom;
+    } else {
+      to = top > m + kLag ? top : m;
+    }
+    const float fix = __builtin_amdgcn_exp2f(m - to);
+    m = to;
+    l *= fix;
+#pragma unroll
+    for (int d = 0; d < DT; ++d) o[d] *= fix;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) e.y[j] -= to;
+  }
+  return e;
+}
+// Their weights, as the B operand of the product with V, and l's share.
+template <typename T>
+__device__ __forceinline__ u32x4 weigh(const Exponents& e, float& l) {
+  u32x4 pf;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const float a = __builtin_amdgcn_exp2f(e.y[2 * j]), b = __builtin_amdgcn_exp2f(e.y[2 * j + 1]);
+    pf[j] = pack2<T>(a, b);
+    l += a + b;
+  }
+  return pf;
+}
 
 // A page of the prefix (as the table has it) and a row in it.  In scalar registers where t
 // is: a vector load would have to wait for all that were issued before it.
@@ -60,6 +142,16 @@ __device__ __forceinline__ At prefix_at(const PrefixArgs& a, int t) {
 __device__ __forceinline__ int64_t page_of(const PrefixArgs& a, int id) { return min(max(id, 0), a.pages - 1); }
 // Loads stay in the order that they are written in.
 __device__ __forceinline__ void in_order() { asm volatile("" ::: "memory"); }
+
+// A row's queries as the B operand of the scores, negated where the scale is negative.
+template <int KK>
+__device__ __forceinline__ void load_queries(const PrefixArgs& a, int kvh, int row, bool live, int quad, u32x4 (&qf)[KK]) {
+  const int b = row / a.group, g = row - b * a.group;
+  const uint16_t* p = a.q + b * a.q_bs + (kvh * a.group + g) * a.q_hs + 8 * quad;
+  const uint32_t sign = a.scale_log2 < 0.f ? 0x80008000u : 0u;
+#pragma unroll
+  for (int kk = 0; kk < KK; ++kk) qf[kk] = live ? load16(p + 32 * kk) ^ sign : u32x4{0, 0, 0, 0};
+}
 
 // A wave's 32 keys: K as the A operands of the scores, V as 8 rows' dims of a lane.
 template <int D>
@@ -92,20 +184,16 @@ __device__ __forceinline__ Words<NW> buf_load_words(rsrc_t r, uint32_t off, uint
 // HALVES: 16 keys from a multiple of 16 on lie in one page (or there is no table): their
 // addresses are the wave's, a lane's offsets do not change, and a descriptor of the rows
 // up to the prefix's end reads zeros behind it.
+// At most 16 rows: one tile of MFMA; the workgroup's waves take 32 keys each, as they lie.
 template <typename T, int D, bool HALVES>
 __global__ __launch_bounds__(256, D > 128 ? 1 : 2) void prefix_few_kernel(PrefixArgs a) {
-  constexpr int KK = D / 32, DV = D / 16, CT = 1, ROWS = 16 * CT;
-  constexpr bool kByTile = std::is_same<T, f16_t>::value;
+  constexpr int KK = D / 32, DV = D / 16;
   __shared__ float sh_o[4][16][D + 4];
   __shared__ float sh_ml[4][16][2];
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int col = lane & 15, quad = lane >> 4;
-  // A unit is a part of a KV head's keys; its row tiles' workgroups are 8 apart, so
-  // that they share an XCD's L2.
-  const int unit = blockIdx.x % 8 + 8 * (blockIdx.x / (8 * a.row_tiles));
-  const int rt = blockIdx.x / 8 % a.row_tiles;
-  if (unit >= a.kv_heads * a.splits) return;
+  const int unit = blockIdx.x;
   const int split = unit / a.kv_heads, kvh = unit - split * a.kv_heads;
   const int n = __builtin_amdgcn_readfirstlane(prefix_length(a));
   const int tiles = (n + kTileKeys - 1) / kTileKeys;
@@ -160,70 +248,25 @@ __global__ __launch_bounds__(256, D > 128 ? 1 : 2) void prefix_few_kernel(Prefix
     }
   };
 
-  u32x4 qf[CT][KK];
+  const float scale = fmaxf(__builtin_fabsf(a.scale_log2), 1e-30f);
+  u32x4 qf[KK];
+  load_queries<KK>(a, kvh, col, col < a.rows, quad, qf);
+  f32x4 o[DV];
+  float m = kNone, l = 0.f, greatest = neg_inf();
 #pragma unroll
-  for (int c = 0; c < CT; ++c) {
-    const int at = rt * ROWS + 16 * c + col;
-    const int b = at / a.group, g = at - b * a.group;
-    const uint16_t* p = a.q + b * a.q_bs + (kvh * a.group + g) * a.q_hs + 8 * quad;
-#pragma unroll
-    for (int kk = 0; kk < KK; ++kk) qf[c][kk] = at < a.rows ? load16(p + 32 * kk) : u32x4{0, 0, 0, 0};
-  }
-  f32x4 o[CT][DV];
-  float m[CT], l[CT], greatest[CT];
-#pragma unroll
-  for (int c = 0; c < CT; ++c) {
-    m[c] = greatest[c] = neg_inf();
-    l[c] = 0.f;
-#pragma unroll
-    for (int d = 0; d < DV; ++d) o[c][d] = f32x4{0.f, 0.f, 0.f, 0.f};
-  }
+  for (int d = 0; d < DV; ++d) o[d] = f32x4{0.f, 0.f, 0.f, 0.f};
 
   const auto multiply = [&](Tile<D>& y, int u0) {
-    const bool cut = u0 + kTileKeys > n;
-    u32x4 pf[CT];
+    f32x4 sc[2];
 #pragma unroll
-    for (int c = 0; c < CT; ++c) {
-      f32x4 sc[2];
+    for (int t = 0; t < 2; ++t) {
+      sc[t] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int t = 0; t < 2; ++t) {
-        sc[t] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int kk = 0; kk < KK; ++kk)
-          sc[t] = Elem<T>::mfma16(as_vec8<T>(y.k[t][kk]), as_vec8<T>(qf[c][kk]), sc[t]);
-      }
-      float x[8], top = neg_inf();
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        x[j] = sc[j / 4][j % 4] * a.scale_log2;
-        if (cut && u0 + 16 * (j / 4) + 4 * quad + j % 4 >= n) x[j] = neg_inf();
-        top = fmaxf(top, x[j]);
-      }
-      if (kByTile || __any(top > m[c] + kLag)) {
-        top = fmaxf(top, __shfl_xor(top, 16, 64));
-        top = fmaxf(top, __shfl_xor(top, 32, 64));
-        float to = top > m[c] + kLag ? top : m[c];
-        if constexpr (kByTile) {
-          greatest[c] = fmaxf(greatest[c], top);
-          to = fmaxf(top, greatest[c] - kBelow) - kHeadroom;
-        }
-        const float fix = __builtin_amdgcn_exp2f(m[c] - (to == neg_inf() ? 0.f : to));
-        m[c] = to;
-        l[c] *= fix;
-#pragma unroll
-        for (int d = 0; d < DV; ++d) o[c][d] *= fix;
-      }
-      // (nothing but -inf so far: weights of zero instead of NaN)
-      const float ref = m[c] == neg_inf() ? 0.f : m[c];
-#pragma unroll
-      for (int j = 0; j < 8; ++j) x[j] = __builtin_amdgcn_exp2f(x[j] - ref);
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        pf[c][j] = pack2<T>(x[2 * j], x[2 * j + 1]);
-        l[c] += x[2 * j] + x[2 * j + 1];
-      }
+      for (int kk = 0; kk < KK; ++kk) sc[t] = Elem<T>::mfma16(as_vec8<T>(y.k[t][kk]), as_vec8<T>(qf[kk]), sc[t]);
     }
-    if (!HALVES && cut) {
+    const u32x4 pf = weigh<T>(
+        relate<T>(sc, scale, n - u0 < kTileKeys ? n - u0 - 4 * quad : kTileKeys, m, l, greatest, o), l);
+    if (!HALVES && u0 + kTileKeys > n) {
       // (a zero weight would make NaN of what an unused row may hold)
 #pragma unroll
       for (int j = 0; j < 8; ++j)
@@ -239,8 +282,7 @@ __global__ __launch_bounds__(256, D > 128 ? 1 : 2) void prefix_few_kernel(Prefix
       for (int j = 0; j < 4; ++j)
         vt[j] = __builtin_amdgcn_perm(y.v[2 * j + 1].w[d / 2], y.v[2 * j].w[d / 2],
                                       d % 2 ? 0x07060302u : 0x05040100u);
-#pragma unroll
-      for (int c = 0; c < CT; ++c) o[c][d] = Elem<T>::mfma16(as_vec8<T>(vt), as_vec8<T>(pf[c]), o[c][d]);
+      o[d] = Elem<T>::mfma16(as_vec8<T>(vt), as_vec8<T>(pf), o[d]);
     }
   };
 
@@ -264,60 +306,56 @@ __global__ __launch_bounds__(256, D > 128 ? 1 : 2) void prefix_few_kernel(Prefix
     }
   }
 
-  // join the four waves, 16 rows at a time
+  // join the four waves
+  l += __shfl_xor(l, 16, 64);
+  l += __shfl_xor(l, 32, 64);
+  if (quad == 0) {
+    sh_ml[wave][col][0] = m;
+    sh_ml[wave][col][1] = l;
+  }
 #pragma unroll
-  for (int c = 0; c < CT; ++c) {
-    l[c] += __shfl_xor(l[c], 16, 64);
-    l[c] += __shfl_xor(l[c], 32, 64);
-    if (c > 0) __syncthreads();
-    if (quad == 0) {
-      sh_ml[wave][col][0] = m[c];
-      sh_ml[wave][col][1] = l[c];
+  for (int i = 0; i < 4; ++i)
+#pragma unroll
+    for (int d = 0; d < DV; ++d) sh_o[wave][col][(4 * quad + i) * DV + d] = o[d][i];
+  __syncthreads();
+  for (int e = tid; e < a.rows * D; e += 256) {
+    const int r = e / D, d = e % D;
+    float top = neg_inf();
+#pragma unroll
+    for (int w = 0; w < 4; ++w) top = fmaxf(top, sh_ml[w][r][0]);
+    float sum = 0.f, den = 0.f;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      // (a wave without keys has sum 0 and O 0)
+      const float f = __builtin_amdgcn_exp2f(sh_ml[w][r][0] - top);
+      sum += f * sh_o[w][r][d];
+      den += f * sh_ml[w][r][1];
     }
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-#pragma unroll
-      for (int d = 0; d < DV; ++d) sh_o[wave][col][(4 * quad + i) * DV + d] = o[c][d][i];
-    __syncthreads();
-    const int r0 = rt * ROWS + 16 * c;
-    for (int e = tid; e < 16 * D; e += 256) {
-      const int r = e / D, d = e % D;
-      if (r0 + r >= a.rows) break;
-      float top = neg_inf();
-#pragma unroll
-      for (int w = 0; w < 4; ++w) top = fmaxf(top, sh_ml[w][r][0]);
-      const float ref = top == neg_inf() ? 0.f : top;
-      float sum = 0.f, den = 0.f;
-#pragma unroll
-      for (int w = 0; w < 4; ++w) {
-        // (a wave without keys has max -inf, sum 0 and O 0)
-        const float f = __builtin_amdgcn_exp2f(sh_ml[w][r][0] - ref);
-        sum += f * sh_o[w][r][d];
-        den += f * sh_ml[w][r][1];
-      }
-      const int64_t at = static_cast<int64_t>(unit) * a.rows + r0 + r;
-      a.part_o[at * D + d] = sum;
-      if (d == 0) {
-        a.part_ml[at * 2] = top;
-        a.part_ml[at * 2 + 1] = den;
-      }
+    const int64_t at = static_cast<int64_t>(unit) * a.rows + r;
+    a.part_o[at * D + d] = sum;
+    if (d == 0) {
+      a.part_ml[at * 2] = top;
+      a.part_ml[at * 2 + 1] = den;
     }
   }
 }
 
-
-// More rows than a tile of MFMA: the workgroup's waves, 32 rows each, share the keys
-// through LDS.  A stage is 32 keys' K and V, rows of a power of two of bytes whose 16-byte
+// More rows than a tile of MFMA: the workgroup's waves, 32 rows each (16 at head dim 256,
+// whose rows are twice as long), share the keys through LDS.  A stage is 32 keys' K and V, rows of a power of two of bytes whose 16-byte
 // chunks are permuted so that neither the reads of K (16 keys' chunks) nor the transposing
-// reads of V (8 keys, 32 bytes each) meet in a bank.  Two stages in LDS, kAhead more on
-// their way in registers: 16 bytes a load, a few loads a thread and stage.
+// reads of V (8 keys, 32 bytes each) meet in a bank.  Three stages in LDS, two more on
+// their way in registers.  Each wave loads some keys' K or V: one page, one descriptor a
+// stage.
 template <int D>
 struct Stage {
   static constexpr int kRow = D <= 64 ? 128 : D <= 128 ? 256 : 512;  // bytes of a row in LDS
   static constexpr int kMatrix = kTileKeys * kRow;
-  static constexpr int kChunks = D / 8;                              // 16-byte chunks of a row
-  static constexpr int kLoads = (kTileKeys * kChunks + 255) / 256;   // a thread's, of K and of V each
-  static constexpr int kSpan = D <= 96 ? 32 : 16;                    // keys of a load, in one page
+  static constexpr int kChunks = D / 8;             // 16-byte chunks of a row
+  static constexpr int kWaves = D > 128 ? 8 : 4;
+  static constexpr int kTiles = D > 128 ? 1 : 2;    // 16-row tiles of a wave
+  static constexpr int kKeys = 2 * kTileKeys / kWaves;    // of a wave's loads
+  static constexpr int kLoads = kKeys * kChunks / 64;     // of a lane
+  static constexpr int kAhead = 2;                  // stages on their way
   static __device__ __forceinline__ int k_mask(int row) { return kRow >= 256 ? row & 15 : row >> 1 & 7; }
   static __device__ __forceinline__ int v_mask(int row) { return (kRow >= 256 ? row & 7 : row >> 1 & 3) << 1; }
 };
@@ -328,14 +366,12 @@ typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
 // its loads from memory (as __syncthreads() does).
 __device__ __forceinline__ void barrier_lds() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 
-// SPANS: the keys of a load lie in one page (or there is no table): their addresses are the
-// wave's, and a descriptor of the rows up to the prefix's end reads zeros behind it.
-template <typename T, int D, bool SPANS>
-__global__ __launch_bounds__(256, D > 128 ? 1 : 2) void prefix_many_kernel(PrefixArgs a) {
+// HALVES: as above.
+template <typename T, int D, bool HALVES>
+__global__ __launch_bounds__(64 * Stage<D>::kWaves, D > 128 ? 1 : 2) void prefix_many_kernel(PrefixArgs a) {
   using S = Stage<D>;
-  constexpr int KK = D / 32, DT = D / 16, CT = 2, L = S::kLoads, kAhead = 2;
-  constexpr bool kByTile = std::is_same<T, f16_t>::value;
-  __shared__ alignas(1024) uint8_t sh[2][2][S::kMatrix];
+  constexpr int KK = D / 32, DT = D / 16, CT = S::kTiles, L = S::kLoads, R = 3, G = S::kAhead;
+  __shared__ alignas(1024) uint8_t sh[R][2 * S::kMatrix];
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int col = lane & 15, quad = lane >> 4;
@@ -349,159 +385,122 @@ __global__ __launch_bounds__(256, D > 128 ? 1 : 2) void prefix_many_kernel(Prefi
   const int tiles = (n + kTileKeys - 1) / kTileKeys;
   const int first = static_cast<int>(static_cast<int64_t>(tiles) * split / a.splits);
   const int last = static_cast<int>(static_cast<int64_t>(tiles) * (split + 1) / a.splits);
-  const int r0 = rt * a.tile_rows + 32 * wave;                    // this wave's rows
+  const int r0 = rt * a.tile_rows + 16 * CT * wave;  // this wave's rows
   const int r_end = min(a.rows, (rt + 1) * a.tile_rows);
 
-  const uint16_t* kb = a.k + kvh * a.k_hs;
-  const uint16_t* vb = a.v + kvh * a.v_hs;
-  // a thread's loads: chunk at[i] of the stage, row at[i] / kChunks of it
-  int key[L], part[L], k_to[L], v_to[L];
+  // this wave's loads: some keys' K or V of a stage, chunk lane + 64 i of their rows
+  const bool is_v = wave >= S::kWaves / 2;
+  const int key0 = S::kKeys * (wave % (S::kWaves / 2));
+  const uint16_t* const base = is_v ? a.v + kvh * a.v_hs : a.k + kvh * a.k_hs;
+  const int64_t ps = is_v ? a.v_ps : a.k_ps, rs = is_v ? a.v_rs : a.k_rs;
+  int key[L], part[L];
+  uint32_t from[L], to[L];
 #pragma unroll
   for (int i = 0; i < L; ++i) {
-    const int c = tid + 256 * i;
+    const int c = lane + 64 * i;
     key[i] = c / S::kChunks;
     part[i] = c - key[i] * S::kChunks;
-    k_to[i] = key[i] * S::kRow + (part[i] ^ S::k_mask(key[i])) * 16;
-    v_to[i] = key[i] * S::kRow + (part[i] ^ S::v_mask(key[i])) * 16;
+    from[i] = (key[i] * static_cast<uint32_t>(rs) + 8 * part[i]) * 2;
+    const int row = key0 + key[i];
+    to[i] = (is_v ? S::kMatrix : 0) + row * S::kRow + (part[i] ^ (is_v ? S::v_mask(row) : S::k_mask(row))) * 16;
   }
-  const auto in_stage = [&](int i) { return kTileKeys * S::kChunks % 256 == 0 || key[i] < kTileKeys; };
-  constexpr int kSpans = SPANS && S::kSpan == 16 ? 2 : 1;
-  constexpr int kPer = 256 / S::kChunks;  // keys of a thread's load and the next
-  At from[SPANS ? kSpans : L];  // of a coming stage's spans, or the thread's loads
-  const auto look_up = [&](int tile) {
-    const int u0 = tile * kTileKeys;
-    if constexpr (SPANS) {
-#pragma unroll
-      for (int i = 0; i < kSpans; ++i) from[i] = prefix_at(a, u0 + 16 * i < n ? u0 + 16 * i : 0);
+  At here;           // HALVES: of a coming stage's keys
+  At there[L];       // else: of the lane's loads
+  const auto look_up = [&](int tile) __attribute__((always_inline)) {
+    const int u0 = tile * kTileKeys + key0;
+    if constexpr (HALVES) {
+      here = prefix_at(a, u0 < n ? u0 : 0);
     } else {
 #pragma unroll
       for (int i = 0; i < L; ++i) {
-        const uint32_t t = min(u0 + min(key[i], kTileKeys - 1), n - 1);
+        const uint32_t t = min(u0 + key[i], n - 1);
         const uint32_t page = (__umulhi(t, a.page_mul) + t) >> a.page_shift;
-        from[i] = {a.table != nullptr ? a.table[page] : 0, static_cast<int>(t - page * a.page_size)};
+        there[i] = {a.table != nullptr ? a.table[page] : 0, static_cast<int>(t - page * a.page_size)};
       }
     }
   };
   struct Regs {
-    u32x4 k[L], v[L];
+    u32x4 x[L];
   };
-  const auto load = [&](Regs& x, int tile) {
+  const auto load = [&](Regs& r, int tile) __attribute__((always_inline)) {
+    if constexpr (HALVES) {
+      const int live = min(n - tile * kTileKeys - key0, S::kKeys);  // (0 and less: zeros)
+      const rsrc_t src = make_rsrc(base + page_of(a, here.id) * ps + here.row * rs,
+                                   live > 0 ? ((live - 1) * static_cast<int>(rs) + D) * 2 : 0);
+#pragma unroll
+      for (int i = 0; i < L; ++i) r.x[i] = buf_load16(src, from[i]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < L; ++i)
+        r.x[i] = load16(base + page_of(a, there[i].id) * ps + there[i].row * rs + 8 * part[i]);
+    }
+    in_order();
+  };
+  const auto store = [&](const Regs& r, int tile, auto buffer) __attribute__((always_inline)) {
 #pragma unroll
     for (int i = 0; i < L; ++i) {
-      if constexpr (SPANS) {
-        constexpr bool kBoth = kSpans == 2;
-        const int s = kBoth ? i * kPer / 16 : 0;  // the load's span
-        const int live = min(n - tile * kTileKeys - 16 * s, kTileKeys);  // (0 and less: zeros)
-        const rsrc_t kr = make_rsrc(kb + page_of(a, from[s].id) * a.k_ps + from[s].row * a.k_rs,
-                                    live > 0 ? ((live - 1) * a.k_rs + D) * 2 : 0);
-        const rsrc_t vr = make_rsrc(vb + page_of(a, from[s].id) * a.v_ps + from[s].row * a.v_rs,
-                                    live > 0 ? ((live - 1) * a.v_rs + D) * 2 : 0);
-        const uint32_t in = key[i] - 16 * s;
-        x.k[i] = buf_load16(kr, in_stage(i) ? (in * static_cast<uint32_t>(a.k_rs) + 8 * part[i]) * 2 : kOOB);
-        in_order();
-        x.v[i] = buf_load16(vr, in_stage(i) ? (in * static_cast<uint32_t>(a.v_rs) + 8 * part[i]) * 2 : kOOB);
-        in_order();
-      } else {
-        x.k[i] = load16(kb + page_of(a, from[i].id) * a.k_ps + from[i].row * a.k_rs + 8 * part[i]);
-        in_order();
-        x.v[i] = load16(vb + page_of(a, from[i].id) * a.v_ps + from[i].row * a.v_rs + 8 * part[i]);
-        in_order();
-      }
+      // (a zero weight would make NaN of what an unused row may hold)
+      const bool live = HALVES || tile * kTileKeys + key0 + key[i] < n;
+      store16(&sh[decltype(buffer)::value][to[i]], live ? r.x[i] : u32x4{0, 0, 0, 0});
     }
   };
-  const auto store = [&](const Regs& x, int tile) {
-    uint8_t* const at = &sh[tile & 1][0][0];
-#pragma unroll
-    for (int i = 0; i < L; ++i)
-      if (in_stage(i)) {
-        store16(at + k_to[i], x.k[i]);
-        // (a zero weight would make NaN of what an unused row may hold)
-        const bool live = SPANS || tile * kTileKeys + key[i] < n;
-        store16(at + S::kMatrix + v_to[i], live ? x.v[i] : u32x4{0, 0, 0, 0});
-      }
-  };
 
+  const float scale = fmaxf(__builtin_fabsf(a.scale_log2), 1e-30f);
   u32x4 qf[CT][KK];
-#pragma unroll
-  for (int c = 0; c < CT; ++c) {
-    const int at = r0 + 16 * c + col;
-    const int b = at / a.group, g = at - b * a.group;
-    const uint16_t* p = a.q + b * a.q_bs + (kvh * a.group + g) * a.q_hs + 8 * quad;
-#pragma unroll
-    for (int kk = 0; kk < KK; ++kk) qf[c][kk] = at < r_end ? load16(p + 32 * kk) : u32x4{0, 0, 0, 0};
-  }
   f32x4 o[CT][DT];
   float m[CT], l[CT], greatest[CT];
 #pragma unroll
   for (int c = 0; c < CT; ++c) {
-    m[c] = greatest[c] = neg_inf();
+    load_queries<KK>(a, kvh, r0 + 16 * c + col, r0 + 16 * c + col < r_end, quad, qf[c]);
+    m[c] = kNone;
+    greatest[c] = neg_inf();
     l[c] = 0.f;
 #pragma unroll
     for (int d = 0; d < DT; ++d) o[c][d] = f32x4{0.f, 0.f, 0.f, 0.f};
   }
-  // this lane's reads: K row col's chunk, V rows 4 quad + col / 4's 8 bytes
+  // this lane's reads: of K row col's chunks, of V 8 bytes of row 4 quad + col / 4 (16 rows on
+  // the masks are the same)
   const int v_row = 4 * quad + col / 4;
+  uint32_t k_at[KK], v_at[DT];
+#pragma unroll
+  for (int kk = 0; kk < KK; ++kk) k_at[kk] = col * S::kRow + ((4 * kk + quad) ^ S::k_mask(col)) * 16;
+#pragma unroll
+  for (int d = 0; d < DT; ++d)
+    v_at[d] = lds_addr(&sh[0][0]) + S::kMatrix + v_row * S::kRow + ((2 * d + (col % 4) / 2) ^ S::v_mask(v_row)) * 16 + col % 2 * 8;
 
-  const auto multiply = [&](int tile) {
-    const uint8_t* const ks = &sh[tile & 1][0][0];
-    const uint8_t* const vs = ks + S::kMatrix;
-    f32x4 sc[CT][2];
+  f32x4 sc[CT][2];  // a tile's scores
+  const auto score = [&](auto buffer) __attribute__((always_inline)) {
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
 #pragma unroll
       for (int c = 0; c < CT; ++c) sc[c][t] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int kk = 0; kk < KK; ++kk) {
-        const u32x4 kf = load16(ks + (16 * t + col) * S::kRow + ((4 * kk + quad) ^ S::k_mask(16 * t + col)) * 16);
+        const u32x4 kf = load16(&sh[decltype(buffer)::value][16 * t * S::kRow + k_at[kk]]);
 #pragma unroll
         for (int c = 0; c < CT; ++c) sc[c][t] = Elem<T>::mfma16(as_vec8<T>(kf), as_vec8<T>(qf[c][kk]), sc[c][t]);
       }
     }
-    const int u0 = tile * kTileKeys;
-    const bool cut = u0 + kTileKeys > n;
+  };
+  // A tile's weights and their product with V beside the scores of the next one: matrix
+  // instructions of the one while the other's exponentials are computed.
+  const auto multiply = [&](int tile, auto buffer, auto next) __attribute__((always_inline)) {
+    const int left = n - tile * kTileKeys;
+    Exponents e[CT];
+#pragma unroll
+    for (int c = 0; c < CT; ++c)
+      e[c] = relate<T>(sc[c], scale, left < kTileKeys ? left - 4 * quad : kTileKeys, m[c], l[c], greatest[c], o[c]);
+    score(next);
     u32x4 pf[CT];
 #pragma unroll
-    for (int c = 0; c < CT; ++c) {
-      float x[8], top = neg_inf();
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        x[j] = sc[c][j / 4][j % 4] * a.scale_log2;
-        if (cut && u0 + 16 * (j / 4) + 4 * quad + j % 4 >= n) x[j] = neg_inf();
-        top = fmaxf(top, x[j]);
-      }
-      if (kByTile || __any(top > m[c] + kLag)) {
-        top = fmaxf(top, __shfl_xor(top, 16, 64));
-        top = fmaxf(top, __shfl_xor(top, 32, 64));
-        float to = top > m[c] + kLag ? top : m[c];
-        if constexpr (kByTile) {
-          greatest[c] = fmaxf(greatest[c], top);
-          to = fmaxf(top, greatest[c] - kBelow) - kHeadroom;
-        }
-        const float fix = __builtin_amdgcn_exp2f(m[c] - (to == neg_inf() ? 0.f : to));
-        m[c] = to;
-        l[c] *= fix;
-#pragma unroll
-        for (int d = 0; d < DT; ++d) o[c][d] *= fix;
-      }
-      // (nothing but -inf so far: weights of zero instead of NaN)
-      const float ref = m[c] == neg_inf() ? 0.f : m[c];
-#pragma unroll
-      for (int j = 0; j < 8; ++j) x[j] = __builtin_amdgcn_exp2f(x[j] - ref);
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        pf[c][j] = pack2<T>(x[2 * j], x[2 * j + 1]);
-        l[c] += x[2 * j] + x[2 * j + 1];
-      }
-    }
+    for (int c = 0; c < CT; ++c) pf[c] = weigh<T>(e[c], l[c]);
 #pragma unroll
     for (int d = 0; d < DT; ++d) {
       u32x4 vt;  // dim d of the lane's 8 keys
 #pragma unroll
       for (int t = 0; t < 2; ++t) {
-        const int row = 16 * t + v_row;
-        const uint8_t* p = vs + row * S::kRow + ((2 * d + (col % 4) / 2) ^ S::v_mask(row)) * 16 + col % 2 * 8;
-        const s16x4 w = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-            reinterpret_cast<lds_s16x4*>(static_cast<uintptr_t>(lds_addr(p))));
+        const s16x4 w = __builtin_amdgcn_ds_read_tr16_b64_v4i16(reinterpret_cast<lds_s16x4*>(
+            static_cast<uintptr_t>(v_at[d] + decltype(buffer)::value * 2 * S::kMatrix + 16 * t * S::kRow)));
         const u32x2 words = __builtin_bit_cast(u32x2, w);
         vt[2 * t] = words[0];
         vt[2 * t + 1] = words[1];
@@ -511,30 +510,35 @@ __global__ __launch_bounds__(256, D > 128 ? 1 : 2) void prefix_many_kernel(Prefi
     }
   };
 
-  const bool rows_here = r0 < r_end;
-  // (Stages behind the last one are loaded too, SPANS: as zeros, else the last key again; so
+  // (Stages behind the last one are loaded too, HALVES: as zeros, else the last key again; so
   // that it is known at each store how many loads were issued since its own.)
   if (first < last) {
-    Regs even, odd;  // stages first + 1, + 3 .. and + 2, + 4 ..
+    const bool rows_here = r0 < r_end;
+    Regs regs[G];  // stage first + i, + i + G .. in regs[i % G]
     look_up(first);
-    load(even, first);
-    look_up(first + 1);
-    store(even, first);
-    load(even, first + 1);
-    look_up(first + 2);
-    load(odd, first + 2);
-    look_up(first + 3);
-    for (int at = first; at < last; at += 2) {
-      const auto step = [&](Regs& next, int tile) {
-        barrier_lds();  // the stage is written, and the other one read
-        store(next, tile + 1);
-        load(next, tile + 1 + kAhead);
-        look_up(tile + 2 + kAhead);
-        if (rows_here && tile < last) multiply(tile);
-      };
-      step(even, at);
-      step(odd, at + 1);
-    }
+    StaticFor<0, G>::run([&](auto i) {
+      load(regs[i], first + i);
+      look_up(first + i + 1);
+    });
+    StaticFor<0, 2>::run([&](auto i) {
+      store(regs[i % G], first + i, i);
+      load(regs[i % G], first + i + G);
+      look_up(first + i + 1 + G);
+    });
+    barrier_lds();
+    if (rows_here) score(std::integral_constant<int, 0>{});
+    for (int at = first; at < last; at += R * G)
+      StaticFor<0, R * G>::run([&](auto i) __attribute__((always_inline)) {
+        // (R = 3: the next stage is written, and the one before this one read)
+        constexpr std::integral_constant<int, i % R> kThis{};
+        constexpr std::integral_constant<int, (i + 1) % R> kNext{};
+        constexpr std::integral_constant<int, (i + 2) % R> kAfter{};
+        barrier_lds();
+        store(regs[(i + 2) % G], at + i + 2, kAfter);
+        load(regs[(i + 2) % G], at + i + 2 + G);
+        look_up(at + i + 3 + G);
+        if (rows_here && at + i < last) multiply(at + i, kThis, kNext);
+      });
   }
 
   // (each row is one wave's)
@@ -554,17 +558,19 @@ __global__ __launch_bounds__(256, D > 128 ? 1 : 2) void prefix_many_kernel(Prefi
   }
 }
 
-// Joins a query head's partials of the prefix and of its sequence's own keys: first
-// the weights of all partials, then their sum, 16 bytes of a partial a thread.
-template <typename T, int D>
+// Joins a query head's partials of the prefix and of its sequence's own keys: WAVES waves
+// a head, each of which finds the maximum and the sum of all partials; then their share of
+// the partials' O, 16 bytes a lane.
+template <typename T, int D, int WAVES>
 __global__ __launch_bounds__(256) void shared_join_kernel(PrefixArgs p, DecodeArgs a) {
-  constexpr int kLanes = D / 4, kSlots = 256 / kLanes;  // partials at a time
-  __shared__ float sh_f[kMaxSplits + kMaxGrid];
-  __shared__ float sh_r[4];
-  __shared__ f32x4 sh_o[kSlots][kLanes];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  constexpr int kLanes = D / 4, kAtOnce = 64 / kLanes, kHeads = 4 / WAVES;
+  __shared__ f32x4 sh_o[4][kAtOnce][kLanes];
+  __shared__ float sh_f[4][kMaxSplits + kMaxOwn];
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int items = a.kv_heads * a.head_items, heads = a.kv_heads * a.group;
-  const int b = blockIdx.x / heads, head = blockIdx.x - b * heads;
+  const int at = min(static_cast<int>(blockIdx.x) * kHeads + wave / WAVES, a.batch * heads - 1);
+  const int b = at / heads, head = at - b * heads;
   const int kvh = head / a.group, g = head - kvh * a.group;
   const int item = kvh * a.head_items + g / a.item_heads, h = g % a.item_heads;
   const Prefix prefix = prefix_of(a, lane);
@@ -585,44 +591,48 @@ __global__ __launch_bounds__(256) void shared_join_kernel(PrefixArgs p, DecodeAr
                                   : 2 * static_cast<int64_t>(w0 + i) + (i == 0 ? in_last : 0);
     return slot * a.item_heads + h;
   };
+  typedef float f32x2 __attribute__((ext_vector_type(2)));
+  const auto ml_of = [&](int i) {
+    return *reinterpret_cast<const f32x2*>((i < p.splits ? p.part_ml : a.part_ml) + row_of(i) * 2);
+  };
   float top = neg_inf();
-  for (int i = tid; i < n; i += 256) {
-    const float m = (i < p.splits ? p.part_ml : a.part_ml)[row_of(i) * 2];
-    sh_f[i] = m;
+  for (int i = lane; i < n; i += 64) {
+    const float m = ml_of(i)[0];
+    sh_f[wave][i] = m;
     top = fmaxf(top, m);
   }
 #pragma unroll
   for (int off = 32; off >= 1; off >>= 1) top = fmaxf(top, __shfl_xor(top, off, 64));
-  if (lane == 0) sh_r[wave] = top;
-  __syncthreads();
-  top = fmaxf(fmaxf(sh_r[0], sh_r[1]), fmaxf(sh_r[2], sh_r[3]));
   const float ref = top == neg_inf() ? 0.f : top;
-  __syncthreads();
   float den = 0.f;
-  for (int i = tid; i < n; i += 256) {
-    const float f = __builtin_amdgcn_exp2f(sh_f[i] - ref);
-    sh_f[i] = f;
-    den += f * (i < p.splits ? p.part_ml : a.part_ml)[row_of(i) * 2 + 1];
+  for (int i = lane; i < n; i += 64) {
+    const float f = __builtin_amdgcn_exp2f(sh_f[wave][i] - ref);
+    sh_f[wave][i] = f;
+    den += f * ml_of(i)[1];
   }
 #pragma unroll
   for (int off = 32; off >= 1; off >>= 1) den += __shfl_xor(den, off, 64);
-  if (lane == 0) sh_r[wave] = den;
-  __syncthreads();
-  den = (sh_r[0] + sh_r[1]) + (sh_r[2] + sh_r[3]);
+  // (its own wave's LDS)
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
   f32x4 o = {0.f, 0.f, 0.f, 0.f};
-  const int slot = tid / kLanes, e = tid % kLanes;
-  if (slot < kSlots) {
-#pragma unroll 4
-    for (int i = slot; i < n; i += kSlots)
-      o += sh_f[i] * *reinterpret_cast<const f32x4*>((i < p.splits ? p.part_o : a.part_o) + row_of(i) * D + 4 * e);
-    sh_o[slot][e] = o;
+  const int slot = lane / kLanes, e = lane % kLanes;
+  if (slot < kAtOnce) {
+#pragma unroll 8
+    for (int i = wave % WAVES * kAtOnce + slot; i < n; i += WAVES * kAtOnce)
+      o += sh_f[wave][i] *
+           *reinterpret_cast<const f32x4*>((i < p.splits ? p.part_o : a.part_o) + row_of(i) * D + 4 * e);
+    sh_o[wave][slot][e] = o;
   }
   __syncthreads();
-  if (tid < kLanes) {
+  if (wave % WAVES == 0 && lane < kLanes) {
+    o = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int i = 1; i < kSlots; ++i) o += sh_o[i][tid];
+    for (int w = 0; w < WAVES; ++w)
+#pragma unroll
+      for (int i = 0; i < kAtOnce; ++i) o += sh_o[wave + w][i][lane];
     const bool none = s.n == 0 && prefix_length(p) == 0;
-    uint16_t* out = a.out + b * a.o_bs + head * a.o_hs + 4 * tid;
+    uint16_t* out = a.out + b * a.o_bs + head * a.o_hs + 4 * lane;
 #pragma unroll
     for (int j = 0; j < 4; ++j) out[j] = Elem<T>::from_float(none ? 0.f : o[j] / den);
   }
@@ -637,6 +647,7 @@ struct SharedPlan {
 SharedPlan shared_plan(const fpv2_shared_prefix_params& p) {
   SharedPlan plan;
   plan.own = decode_plan(p.own);
+  if (plan.own.grid > kMaxOwn) plan.own.grid = kMaxOwn;
   const int64_t rows = p.own.batch * (p.own.query_heads / p.own.kv_heads);
   // tiles of at most 128 rows, all alike, of whole waves
   plan.row_tiles = static_cast<int>((rows + 127) / 128);
@@ -645,7 +656,7 @@ SharedPlan shared_plan(const fpv2_shared_prefix_params& p) {
   const int64_t tiles = (p.prefix_table_width * p.prefix_page_size + kTileKeys - 1) / kTileKeys;
   const int64_t per = p.own.head_dim > 128 ? 1 : 2;
   int64_t splits = per * cu_count() / (p.own.kv_heads * (plan.row_tiles > 0 ? plan.row_tiles : 1));
-  const int64_t most = (tiles + 2 * kWaves - 1) / (2 * kWaves);
+  const int64_t most = (tiles + kWaves - 1) / kWaves;
   splits = splits < most ? splits : most;
   splits = splits < kMaxSplits ? splits : kMaxSplits;
   plan.splits = static_cast<int>(splits > 1 ? splits : 1);
@@ -677,24 +688,25 @@ int64_t shared_bytes(const fpv2_shared_prefix_params& p, const SharedPlan& plan)
 
 template <typename T, int D>
 int launch(const PrefixArgs& p, const DecodeArgs& a, hipStream_t s) {
-  const unsigned units = (static_cast<unsigned>(p.kv_heads) * p.splits + 7) / 8 * 8;
-  const dim3 grid(units * p.row_tiles);
-  const bool few = p.rows <= 16;
-  // (offsets within a stage are 32 bits)
-  const bool spans = (p.table == nullptr || p.page_size % (few ? 16 : Stage<D>::kSpan) == 0) &&
-                     p.k_rs < (1 << 24) && p.v_rs < (1 << 24);
-  if (few && spans)
-    hipLaunchKernelGGL((prefix_few_kernel<T, D, true>), grid, dim3(256), 0, s, p);
-  else if (few)
-    hipLaunchKernelGGL((prefix_few_kernel<T, D, false>), grid, dim3(256), 0, s, p);
-  else if (spans)
-    hipLaunchKernelGGL((prefix_many_kernel<T, D, true>), grid, dim3(256), 0, s, p);
+  const unsigned units = static_cast<unsigned>(p.kv_heads) * p.splits;
+  const dim3 few(units), many((units + 7) / 8 * 8 * p.row_tiles);
+  // (offsets within 16 rows are 32 bits)
+  const bool halves = (p.table == nullptr || p.page_size % 16 == 0) && p.k_rs < (1 << 25) && p.v_rs < (1 << 25);
+  if (p.rows <= 16 && halves)
+    hipLaunchKernelGGL((prefix_few_kernel<T, D, true>), few, dim3(256), 0, s, p);
+  else if (p.rows <= 16)
+    hipLaunchKernelGGL((prefix_few_kernel<T, D, false>), few, dim3(256), 0, s, p);
+  else if (halves)
+    hipLaunchKernelGGL((prefix_many_kernel<T, D, true>), many, dim3(64 * Stage<D>::kWaves), 0, s, p);
   else
-    hipLaunchKernelGGL((prefix_many_kernel<T, D, false>), grid, dim3(256), 0, s, p);
+    hipLaunchKernelGGL((prefix_many_kernel<T, D, false>), many, dim3(64 * Stage<D>::kWaves), 0, s, p);
   if (const int rc = check_launch("prefix_many_kernel")) return rc;
   hipLaunchKernelGGL((decode_attn_kernel<T, D, true>), dim3(a.grid), dim3(256), 0, s, a);
-  hipLaunchKernelGGL((shared_join_kernel<T, D>), dim3(static_cast<unsigned>(a.batch) * a.kv_heads * a.group),
-                     dim3(256), 0, s, p, a);
+  const unsigned heads = static_cast<unsigned>(a.batch) * a.kv_heads * a.group;
+  if (heads < 1024)
+    hipLaunchKernelGGL((shared_join_kernel<T, D, 4>), dim3(heads), dim3(256), 0, s, p, a);
+  else
+    hipLaunchKernelGGL((shared_join_kernel<T, D, 1>), dim3((heads + 3) / 4), dim3(256), 0, s, p, a);
   return check_launch("shared_join_kernel");
 }
 

@@ -175,9 +175,19 @@ __device__ __forceinline__ Words<NW> load_words(const uint16_t* p) {
   return r;
 }
 
-// KEEP: items that one workgroup covers leave their partial too, behind the runs' slots.
+template <int D>
+struct DecodeShared {
+  // (at head dim 256 the queries would not fit the registers beside K, V and O)
+  static constexpr bool kLdsQ = D > 128;
+  float o[4][kMaxHeads][D + 4];
+  float ml[4][kMaxHeads][2];
+  u32x4 q[kLdsQ ? 2 * D : 1];
+};
+
+// A workgroup of 256 threads.  KEEP: items that one workgroup covers leave their partial
+// too, behind the runs' slots.
 template <typename T, int D, bool KEEP>
-__global__ __launch_bounds__(256, 2) void decode_attn_kernel(DecodeArgs a) {
+__device__ __forceinline__ void decode_attn(const DecodeArgs& a, int block, DecodeShared<D>& sh) {
   constexpr int KK = D / 32;  // MFMA steps of a key's dot product
   constexpr int DV = D / 16;  // dims of a lane
   // Weights are rounded to the storage type for their product with V, as MFMA takes them; the
@@ -188,11 +198,10 @@ __global__ __launch_bounds__(256, 2) void decode_attn_kernel(DecodeArgs a) {
   // a quarter of its weight.
   constexpr bool kByTile = std::is_same<T, f16_t>::value;
   constexpr float kHeadroom = 15.f, kBelow = 40.f;
-  __shared__ float sh_o[4][kMaxHeads][D + 4];
-  __shared__ float sh_ml[4][kMaxHeads][2];
-  // (at head dim 256 the queries would not fit the registers beside K, V and O)
-  constexpr bool kLdsQ = D > 128;
-  __shared__ u32x4 sh_q[kLdsQ ? 64 * KK : 1];
+  constexpr bool kLdsQ = DecodeShared<D>::kLdsQ;
+  auto& sh_o = sh.o;
+  auto& sh_ml = sh.ml;
+  auto& sh_q = sh.q;
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int col = lane & 15, quad = lane >> 4;
@@ -200,7 +209,7 @@ __global__ __launch_bounds__(256, 2) void decode_attn_kernel(DecodeArgs a) {
 
   const Prefix prefix = prefix_of(a, lane);
   const int total = prefix.total * items;
-  const int lo = first_of(a, blockIdx.x, total), hi = first_of(a, blockIdx.x + 1, total);
+  const int lo = first_of(a, block, total), hi = first_of(a, block + 1, total);
   if (lo >= hi) return;
 
   int base;
@@ -351,7 +360,7 @@ __global__ __launch_bounds__(256, 2) void decode_attn_kernel(DecodeArgs a) {
     __syncthreads();
     const bool whole = first == 0 && last == s_now.tiles;
     const int64_t slot = KEEP && whole ? 2 * static_cast<int64_t>(a.grid) + static_cast<int64_t>(b_now) * items + item
-                                       : 2 * static_cast<int64_t>(blockIdx.x) + (cur == lo ? 0 : 1);
+                                       : 2 * static_cast<int64_t>(block) + (cur == lo ? 0 : 1);
     for (int e = tid; e < heads * D; e += 256) {
       const int h = e / D, d = e % D;
       float top = neg_inf();
@@ -379,6 +388,12 @@ __global__ __launch_bounds__(256, 2) void decode_attn_kernel(DecodeArgs a) {
     }
     __syncthreads();
   }
+}
+
+template <typename T, int D, bool KEEP>
+__global__ __launch_bounds__(256, 2) void decode_attn_kernel(DecodeArgs a) {
+  __shared__ DecodeShared<D> sh;
+  decode_attn<T, D, KEEP>(a, blockIdx.x, sh);
 }
 
 // Joins the partials of an item that several workgroups shared: one workgroup

@@ -6,8 +6,8 @@
 //
 // The sums split over t: partials (O, max, sum) of parts of the keys are joined as
 //   O = sum_i exp(m_i - m) O_i, l = sum_i exp(m_i - m) l_i, m = max_i m_i.
-// Three launches: the prefix (here), the own keys (decode_attn_kernel, all items left
-// as partials), and the join.
+// Two launches: workgroups of the own keys (decode_attn, all items left as partials) and of
+// the prefix, then the join.
 //
 // Prefix: the rows of a KV head are the batch's query heads of it, packed; a workgroup
 // takes a tile of them and a part of the prefix's keys.  Its waves take 32 keys each on
@@ -185,15 +185,20 @@ __device__ __forceinline__ Words<NW> buf_load_words(rsrc_t r, uint32_t off, uint
 // addresses are the wave's, a lane's offsets do not change, and a descriptor of the rows
 // up to the prefix's end reads zeros behind it.
 // At most 16 rows: one tile of MFMA; the workgroup's waves take 32 keys each, as they lie.
+template <int D>
+struct FewShared {
+  float o[4][16][D + 4];
+  float ml[4][16][2];
+};
 template <typename T, int D, bool HALVES>
-__global__ __launch_bounds__(256, D > 128 ? 1 : 2) void prefix_few_kernel(PrefixArgs a) {
+__device__ __forceinline__ void prefix_few(const PrefixArgs& a, int block, FewShared<D>& sh) {
   constexpr int KK = D / 32, DV = D / 16;
-  __shared__ float sh_o[4][16][D + 4];
-  __shared__ float sh_ml[4][16][2];
+  auto& sh_o = sh.o;
+  auto& sh_ml = sh.ml;
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int col = lane & 15, quad = lane >> 4;
-  const int unit = blockIdx.x;
+  const int unit = block;
   const int split = unit / a.kv_heads, kvh = unit - split * a.kv_heads;
   const int n = __builtin_amdgcn_readfirstlane(prefix_length(a));
   const int tiles = (n + kTileKeys - 1) / kTileKeys;
@@ -340,6 +345,18 @@ __global__ __launch_bounds__(256, D > 128 ? 1 : 2) void prefix_few_kernel(Prefix
   }
 }
 
+template <typename T, int D, bool HALVES>
+__global__ __launch_bounds__(256, D > 128 ? 1 : 2) void prefix_few_kernel(PrefixArgs p, DecodeArgs a) {
+  __shared__ union {
+    FewShared<D> few;
+    DecodeShared<D> own;
+  } sh;
+  if (static_cast<int>(blockIdx.x) < a.grid)
+    decode_attn<T, D, true>(a, blockIdx.x, sh.own);
+  else
+    prefix_few<T, D, HALVES>(p, blockIdx.x - a.grid, sh.few);
+}
+
 // More rows than a tile of MFMA: the workgroup's waves, 32 rows each (16 at head dim 256,
 // whose rows are twice as long), share the keys through LDS.  A stage is 32 keys' K and V, rows of a power of two of bytes whose 16-byte
 // chunks are permuted so that neither the reads of K (16 keys' chunks) nor the transposing
@@ -368,17 +385,16 @@ __device__ __forceinline__ void barrier_lds() { asm volatile("s_waitcnt lgkmcnt(
 
 // HALVES: as above.
 template <typename T, int D, bool HALVES>
-__global__ __launch_bounds__(64 * Stage<D>::kWaves, D > 128 ? 1 : 2) void prefix_many_kernel(PrefixArgs a) {
+__device__ __forceinline__ void prefix_many(const PrefixArgs& a, int block, uint8_t (&sh)[3][2 * Stage<D>::kMatrix]) {
   using S = Stage<D>;
   constexpr int KK = D / 32, DT = D / 16, CT = S::kTiles, L = S::kLoads, R = 3, G = S::kAhead;
-  __shared__ alignas(1024) uint8_t sh[R][2 * S::kMatrix];
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int col = lane & 15, quad = lane >> 4;
   // A unit is a part of a KV head's keys; its row tiles' workgroups are 8 apart, so
   // that they share an XCD's L2.
-  const int unit = blockIdx.x % 8 + 8 * (blockIdx.x / (8 * a.row_tiles));
-  const int rt = blockIdx.x / 8 % a.row_tiles;
+  const int unit = block % 8 + 8 * (block / (8 * a.row_tiles));
+  const int rt = block / 8 % a.row_tiles;
   if (unit >= a.kv_heads * a.splits) return;
   const int split = unit / a.kv_heads, kvh = unit - split * a.kv_heads;
   const int n = __builtin_amdgcn_readfirstlane(prefix_length(a));
@@ -558,6 +574,20 @@ __global__ __launch_bounds__(64 * Stage<D>::kWaves, D > 128 ? 1 : 2) void prefix
   }
 }
 
+template <typename T, int D, bool HALVES>
+__global__ __launch_bounds__(64 * Stage<D>::kWaves, D > 128 ? 1 : 2) void prefix_many_kernel(PrefixArgs p, DecodeArgs a) {
+  __shared__ union {
+    alignas(1024) uint8_t ring[3][2 * Stage<D>::kMatrix];
+    DecodeShared<D> own;
+  } sh;
+  // (workgroups of more threads than the own keys' have a launch of their own for these)
+  if (Stage<D>::kWaves == 4 && static_cast<int>(blockIdx.x) < a.grid) {
+    if constexpr (Stage<D>::kWaves == 4) decode_attn<T, D, true>(a, blockIdx.x, sh.own);
+  } else {
+    prefix_many<T, D, HALVES>(p, blockIdx.x - (Stage<D>::kWaves == 4 ? a.grid : 0), sh.ring);
+  }
+}
+
 // Joins a query head's partials of the prefix and of its sequence's own keys: WAVES waves
 // a head, each of which finds the maximum and the sum of all partials; then their share of
 // the partials' O, 16 bytes a lane.
@@ -648,6 +678,7 @@ SharedPlan shared_plan(const fpv2_shared_prefix_params& p) {
   SharedPlan plan;
   plan.own = decode_plan(p.own);
   if (plan.own.grid > kMaxOwn) plan.own.grid = kMaxOwn;
+  plan.own.grid = (plan.own.grid + 7) / 8 * 8;  // (the prefix's workgroups keep their XCDs)
   const int64_t rows = p.own.batch * (p.own.query_heads / p.own.kv_heads);
   // tiles of at most 128 rows, all alike, of whole waves
   plan.row_tiles = static_cast<int>((rows + 127) / 128);
@@ -689,19 +720,21 @@ int64_t shared_bytes(const fpv2_shared_prefix_params& p, const SharedPlan& plan)
 template <typename T, int D>
 int launch(const PrefixArgs& p, const DecodeArgs& a, hipStream_t s) {
   const unsigned units = static_cast<unsigned>(p.kv_heads) * p.splits;
-  const dim3 few(units), many((units + 7) / 8 * 8 * p.row_tiles);
+  constexpr int kThreads = 64 * Stage<D>::kWaves;
+  const dim3 few(a.grid + units), many((kThreads == 256 ? a.grid : 0) + (units + 7) / 8 * 8 * p.row_tiles);
   // (offsets within 16 rows are 32 bits)
   const bool halves = (p.table == nullptr || p.page_size % 16 == 0) && p.k_rs < (1 << 25) && p.v_rs < (1 << 25);
   if (p.rows <= 16 && halves)
-    hipLaunchKernelGGL((prefix_few_kernel<T, D, true>), few, dim3(256), 0, s, p);
+    hipLaunchKernelGGL((prefix_few_kernel<T, D, true>), few, dim3(256), 0, s, p, a);
   else if (p.rows <= 16)
-    hipLaunchKernelGGL((prefix_few_kernel<T, D, false>), few, dim3(256), 0, s, p);
+    hipLaunchKernelGGL((prefix_few_kernel<T, D, false>), few, dim3(256), 0, s, p, a);
   else if (halves)
-    hipLaunchKernelGGL((prefix_many_kernel<T, D, true>), many, dim3(64 * Stage<D>::kWaves), 0, s, p);
+    hipLaunchKernelGGL((prefix_many_kernel<T, D, true>), many, dim3(kThreads), 0, s, p, a);
   else
-    hipLaunchKernelGGL((prefix_many_kernel<T, D, false>), many, dim3(64 * Stage<D>::kWaves), 0, s, p);
+    hipLaunchKernelGGL((prefix_many_kernel<T, D, false>), many, dim3(kThreads), 0, s, p, a);
+  if constexpr (kThreads != 256)
+    if (p.rows > 16) hipLaunchKernelGGL((decode_attn_kernel<T, D, true>), dim3(a.grid), dim3(256), 0, s, a);
   if (const int rc = check_launch("prefix_many_kernel")) return rc;
-  hipLaunchKernelGGL((decode_attn_kernel<T, D, true>), dim3(a.grid), dim3(256), 0, s, a);
   const unsigned heads = static_cast<unsigned>(a.batch) * a.kv_heads * a.group;
   if (heads < 1024)
     hipLaunchKernelGGL((shared_join_kernel<T, D, 4>), dim3(heads), dim3(256), 0, s, p, a);

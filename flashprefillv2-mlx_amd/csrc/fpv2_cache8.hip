@@ -17,6 +17,7 @@ namespace fpv2 {
 namespace {
 
 typedef int i32x2 __attribute__((ext_vector_type(2)));
+typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
 
 struct QuantArgs {
   const uint16_t* x[2];   // k, v
@@ -26,65 +27,83 @@ struct QuantArgs {
   int64_t x_ts[2], x_hs[2];
   int64_t c_ps[2], c_hs[2], c_rs[2];
   int64_t s_ps[2], s_hs[2], s_rs[2];
-  int64_t first_slot, pages, page_size, rows;  // rows: tokens * kv_heads
-  int slot_bytes, kv_heads;
+  int64_t first_slot, slot_count, page_size;
+  int slot_bytes, kv_heads, tokens;
+  uint32_t page_mul, page_shift;  // slot / page_size = (umulhi(slot, mul) + slot) >> shift
 };
 
-// One group of lanes a row, 8 values a lane.
-template <typename T, int D>
+constexpr int kMaxBlocks = 1 << 18;  // of a launch; more work is done in turns
+
+// A group of lanes a row, 8 values a lane; HEADS rows of a token, with as many loads in flight.
+template <typename T, int D, int HEADS>
 __global__ __launch_bounds__(256) void quantize_kernel(QuantArgs a) {
   constexpr int kLanes = D / 8 <= 8 ? 8 : D / 8 <= 16 ? 16 : 32;
+  constexpr uint32_t kInf = std::is_same<T, bf16_t>::value ? 0x7f80u : 0x7c00u;
   const int tid = threadIdx.x, at = tid % kLanes;
-  const int64_t row = static_cast<int64_t>(blockIdx.x) * (256 / kLanes) + tid / kLanes;
-  const int side = blockIdx.y;
-  const bool live = row < a.rows && 8 * at < D;
-  const int64_t t = row / a.kv_heads;
-  const int h = static_cast<int>(row - t * a.kv_heads);
-  u32x4 w = {0, 0, 0, 0};
-  int64_t slot = -1;
-  if (live) {
-    w = load16(a.x[side] + t * a.x_ts[side] + h * a.x_hs[side] + 8 * at);
-    slot = a.slot_bytes == 8   ? static_cast<const int64_t*>(a.slots)[t]
-           : a.slot_bytes == 4 ? static_cast<const int32_t*>(a.slots)[t]
-                               : a.first_slot + t;
-  }
-  float x[8], top = 0.f;
-  uint32_t bad = 0;
+  const int side = blockIdx.y, chunks = (a.kv_heads + HEADS - 1) / HEADS;
+  const uint32_t groups = static_cast<uint32_t>(a.tokens) * chunks;
+  for (uint32_t g = blockIdx.x * (256 / kLanes) + tid / kLanes; g < groups; g += gridDim.x * (256 / kLanes)) {
+    const int64_t t = g / chunks;
+    const int h0 = static_cast<int>(g - static_cast<uint32_t>(t) * chunks) * HEADS;
+    u32x4 w[HEADS];
 #pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    x[j] = Elem<T>::to_float(static_cast<uint16_t>(w[j / 2] >> (16 * (j % 2))));
-    const float size = __builtin_fabsf(x[j]);
-    bad |= !(size <= 3.402823466e38f);
-    top = fmaxf(top, size);
-  }
+    for (int i = 0; i < HEADS; ++i)
+      w[i] = 8 * at < D && h0 + i < a.kv_heads
+                 ? load16(a.x[side] + t * a.x_ts[side] + (h0 + i) * a.x_hs[side] + 8 * at)
+                 : u32x4{0, 0, 0, 0};
+    const int64_t slot = a.slot_bytes == 8   ? static_cast<const int64_t*>(a.slots)[t]
+                         : a.slot_bytes == 4 ? static_cast<const int32_t*>(a.slots)[t]
+                                             : a.first_slot + t;
+    const bool live = slot >= 0 && slot < a.slot_count && 8 * at < D;
+    int64_t page, r;
+    if (a.slot_count <= 0x7fffffff) {
+      const uint32_t s = live ? static_cast<uint32_t>(slot) : 0;
+      page = (__umulhi(s, a.page_mul) + s) >> a.page_shift;
+      r = s - static_cast<uint32_t>(page) * static_cast<uint32_t>(a.page_size);
+    } else {
+      page = live ? slot / a.page_size : 0;
+      r = live ? slot - page * a.page_size : 0;
+    }
+    int8_t* const codes = a.codes[side] + page * a.c_ps[side] + r * a.c_rs[side] + 8 * at;
+    float* const scales = a.scales[side] + page * a.s_ps[side] + r * a.s_rs[side];
 #pragma unroll
-  for (int off = kLanes / 2; off >= 1; off >>= 1) {
-    top = fmaxf(top, __shfl_xor(top, off, 64));
-    bad |= __shfl_xor(bad, off, 64);
-  }
-  if (!live || slot < 0 || slot >= a.pages * a.page_size) return;
-  // (the quotients are the same for rows of tiny or huge values times a power of two)
-  const float up = top < 0x1p-64f ? 0x1p64f : top > 0x1p64f ? 0x1p-64f : 1.f;
-  const float most = top * up;
-  const float y = 1.f / most;
-  uint32_t code[8];
+    for (int i = 0; i < HEADS; ++i) {
+      // the greatest magnitude, as the bits of the type: two at a time
+      u16x2 two = {0, 0};
 #pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    const float n = 127.f * (x[j] * up);
-    float q = n * y;
-    q = __builtin_fmaf(__builtin_fmaf(-q, most, n), y, q);
-    code[j] = top == 0.f || bad ? 0 : static_cast<uint32_t>(static_cast<int>(__builtin_rintf(q)));
-  }
-  i32x2 out;
+      for (int j = 0; j < 4; ++j)
+        two = __builtin_elementwise_max(two, __builtin_bit_cast(u16x2, w[i][j] & 0x7fff7fffu));
+      uint32_t bits = max(static_cast<uint32_t>(two[0]), static_cast<uint32_t>(two[1]));
 #pragma unroll
-  for (int i = 0; i < 2; ++i)
-    out[i] = static_cast<int>((code[4 * i] & 255) | (code[4 * i + 1] & 255) << 8 | (code[4 * i + 2] & 255) << 16 |
-                              code[4 * i + 3] << 24);
-  const int64_t page = slot / a.page_size, r = slot - page * a.page_size;
-  *reinterpret_cast<i32x2*>(a.codes[side] + page * a.c_ps[side] + h * a.c_hs[side] + r * a.c_rs[side] + 8 * at) = out;
-  if (at == 0)
-    a.scales[side][page * a.s_ps[side] + h * a.s_hs[side] + r * a.s_rs[side]] =
-        bad ? __builtin_nanf("") : top / 127.f;
+      for (int off = kLanes / 2; off >= 1; off >>= 1) bits = max(bits, static_cast<uint32_t>(__shfl_xor(bits, off, 64)));
+      const bool bad = bits >= kInf;
+      const float top = Elem<T>::to_float(static_cast<uint16_t>(bits));
+      // (the quotients are the same for rows of tiny or huge values times a power of two)
+      const float up = top < 0x1p-64f ? 0x1p64f : top > 0x1p64f ? 0x1p-64f : 1.f;
+      const float most = top * up, factor = 127.f * up;
+      const float y = top > 0.f ? 1.f / most : 0.f;
+      uint32_t code[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const float n = Elem<T>::to_float(static_cast<uint16_t>(w[i][j / 2] >> (16 * (j % 2)))) * factor;
+        float q = n * y;
+        q = __builtin_fmaf(__builtin_fmaf(-q, most, n), y, q);
+        // (the sum is rounded to a whole number, whose two's complement is in its low bits)
+        code[j] = __float_as_uint(q + 0x1.8p23f);
+      }
+      i32x2 out;
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        const uint32_t low = __builtin_amdgcn_perm(code[4 * k + 1], code[4 * k], 0x0c0c0400u);
+        const uint32_t high = __builtin_amdgcn_perm(code[4 * k + 3], code[4 * k + 2], 0x04000c0cu);
+        out[k] = bad ? 0 : static_cast<int>(low | high);
+      }
+      if (live && h0 + i < a.kv_heads) {
+        *reinterpret_cast<i32x2*>(codes + (h0 + i) * a.c_hs[side]) = out;
+        if (at == 0) scales[(h0 + i) * a.s_hs[side]] = bad ? __builtin_nanf("") : top / 127.f;
+      }
+    }
+  }
 }
 
 struct ReadArgs {
@@ -98,42 +117,61 @@ struct ReadArgs {
   int64_t o_bs[2], o_hs[2], o_rs[2];
   int64_t table_stride;
   int kv_heads, pages, page_size, capacity, length, tokens, zero_rest;
+  uint32_t page_mul, page_shift;  // t / page_size = (umulhi(t, mul) + t) >> shift
 };
 
-// 16 values a lane, a row's chunks next to one another; blocks: (tokens, sequence * head, side).
-template <typename T, int D>
+// 8 values a lane, a row's chunks next to one another, TURNS of them in flight; blocks:
+// (tokens, sequence * head, side).  More than one: the stores go past the caches.
+template <typename T, int D, int TURNS>
 __global__ __launch_bounds__(256) void dequantize_kernel(ReadArgs a) {
-  constexpr int kChunks = D / 16;
-  const int64_t e = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
-  const int64_t t = e / kChunks;
-  const int c = static_cast<int>(e - t * kChunks), side = blockIdx.z;
+  constexpr int kChunks = D / 8;
+  const int side = blockIdx.z;
   const int b = blockIdx.y / a.kv_heads, h = blockIdx.y - b * a.kv_heads;
-  if (t >= a.tokens) return;
   int len = a.lengths != nullptr ? a.lengths[b] : a.length;
   len = min(max(len, 0), a.capacity);
-  uint16_t* out = a.out[side] + b * a.o_bs[side] + h * a.o_hs[side] + t * a.o_rs[side] + 16 * c;
-  if (t >= len) {
-    if (a.zero_rest) {
-      store16(out, u32x4{0, 0, 0, 0});
-      store16(out + 8, u32x4{0, 0, 0, 0});
-    }
-    return;
-  }
-  const int at = static_cast<int>(t) / a.page_size, r = static_cast<int>(t) - at * a.page_size;
-  const int id = a.table != nullptr ? a.table[b * a.table_stride + at] : b;
-  const int64_t page = min(max(id, 0), a.pages - 1);
-  const u32x4 w = load16(a.codes[side] + page * a.c_ps[side] + h * a.c_hs[side] + r * a.c_rs[side] + 16 * c);
-  const float scale = a.scales[side][page * a.s_ps[side] + h * a.s_hs[side] + r * a.s_rs[side]];
+  const uint32_t end = static_cast<uint32_t>(a.zero_rest ? a.tokens : min(a.tokens, len));
+  uint16_t* const base = a.out[side] + b * a.o_bs[side] + h * a.o_hs[side];
+  const int8_t* const codes = a.codes[side] + h * a.c_hs[side];
+  const float* const scales = a.scales[side] + h * a.s_hs[side];
+  const int64_t count = static_cast<int64_t>(end) * kChunks;
+  for (int64_t e0 = static_cast<int64_t>(blockIdx.x) * (256 * TURNS) + threadIdx.x; e0 < count;
+       e0 += static_cast<int64_t>(gridDim.x) * (256 * TURNS)) {
+    u32x2 w[TURNS];
+    float scale[TURNS];
 #pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    u32x4 v;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int word = static_cast<int>(w[2 * i + j / 2]) >> (16 * (j % 2));
-      v[j] = pack2<T>(static_cast<float>(static_cast<int8_t>(word)) * scale,
-                      static_cast<float>(static_cast<int8_t>(word >> 8)) * scale);
+    for (int i = 0; i < TURNS; ++i) {
+      const uint32_t t = static_cast<uint32_t>((e0 + 256 * i) / kChunks);
+      const int c = static_cast<int>(e0 + 256 * i - static_cast<int64_t>(t) * kChunks);
+      w[i] = u32x2{0, 0};
+      scale[i] = 0.f;
+      if (t < end && t < static_cast<uint32_t>(len)) {
+        const uint32_t at = (__umulhi(t, a.page_mul) + t) >> a.page_shift;
+        const int64_t r = t - at * static_cast<uint32_t>(a.page_size);
+        const int id = a.table != nullptr ? a.table[b * a.table_stride + at] : b;
+        const int64_t page = min(max(id, 0), a.pages - 1);
+        w[i] = *reinterpret_cast<const u32x2*>(codes + page * a.c_ps[side] + r * a.c_rs[side] + 8 * c);
+        scale[i] = scales[page * a.s_ps[side] + r * a.s_rs[side]];
+      }
     }
-    store16(out + 8 * i, v);
+#pragma unroll
+    for (int i = 0; i < TURNS; ++i) {
+      const uint32_t t = static_cast<uint32_t>((e0 + 256 * i) / kChunks);
+      const int c = static_cast<int>(e0 + 256 * i - static_cast<int64_t>(t) * kChunks);
+      u32x4 v;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int word = static_cast<int>(w[i][j / 2]) >> (16 * (j % 2));
+        v[j] = pack2<T>(static_cast<float>(static_cast<int8_t>(word)) * scale[i],
+                        static_cast<float>(static_cast<int8_t>(word >> 8)) * scale[i]);
+      }
+      u32x4* const out = reinterpret_cast<u32x4*>(base + t * a.o_rs[side] + 8 * c);
+      if (t < end) {
+        if constexpr (TURNS > 1)
+          __builtin_nontemporal_store(v, out);
+        else
+          *out = v;
+      }
+    }
   }
 }
 
@@ -155,6 +193,14 @@ int check_cache(const char* name, const fpv2_code_pages& c) {
   return FPV2_OK;
 }
 
+// t / page_size = (umulhi(t, mul) + t) >> shift for t below 2^31.
+void page_division(int64_t page_size, uint32_t* mul, uint32_t* shift) {
+  uint32_t s = 0;
+  while ((1ull << s) < static_cast<uint64_t>(page_size)) ++s;
+  *shift = s;
+  *mul = static_cast<uint32_t>((((1ull << s) - page_size) << 32) / page_size + 1);
+}
+
 bool a16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
 template <typename A>
@@ -165,29 +211,46 @@ void set_cache(A* a, const fpv2_code_pages& c) {
   a->s_ps[1] = c.vs_page_stride, a->s_hs[1] = c.vs_head_stride, a->s_rs[1] = c.vs_row_stride;
 }
 
-template <typename T, int D>
+template <typename T, int D, int HEADS>
 int launch_quantize(const QuantArgs& a, hipStream_t s) {
   constexpr int kRows = 256 / (D / 8 <= 8 ? 8 : D / 8 <= 16 ? 16 : 32);
-  hipLaunchKernelGGL((quantize_kernel<T, D>), dim3(static_cast<unsigned>((a.rows + kRows - 1) / kRows), 2), dim3(256),
-                     0, s, a);
+  const int64_t blocks = (static_cast<int64_t>(a.tokens) * ((a.kv_heads + HEADS - 1) / HEADS) + kRows - 1) / kRows;
+  hipLaunchKernelGGL((quantize_kernel<T, D, HEADS>),
+                     dim3(static_cast<unsigned>(blocks < kMaxBlocks ? blocks : kMaxBlocks), 2), dim3(256), 0, s, a);
   return check_launch("quantize_kernel");
 }
 
+// Many rows: several of a token in turn.
+template <typename T, int D>
+int launch_rows(const QuantArgs& a, hipStream_t s) {
+  return a.kv_heads > 1 && static_cast<int64_t>(a.tokens) * a.kv_heads >= 1 << 14 ? launch_quantize<T, D, 4>(a, s)
+                                                                                   : launch_quantize<T, D, 1>(a, s);
+}
+
+template <typename T, int D, int TURNS>
+int launch_turns(const ReadArgs& a, int batch, hipStream_t s) {
+  const int64_t blocks = (static_cast<int64_t>(a.tokens) * (D / 8) + 256 * TURNS - 1) / (256 * TURNS);
+  hipLaunchKernelGGL((dequantize_kernel<T, D, TURNS>),
+                     dim3(static_cast<unsigned>(blocks < kMaxBlocks ? blocks : kMaxBlocks),
+                          static_cast<unsigned>(batch) * a.kv_heads, 2),
+                     dim3(256), 0, s, a);
+  return check_launch("dequantize_kernel");
+}
+
+// Results that no cache holds (2^25 bytes and more of K and of V each).
 template <typename T, int D>
 int launch_dequantize(const ReadArgs& a, int batch, hipStream_t s) {
-  const int64_t blocks = (static_cast<int64_t>(a.tokens) * (D / 16) + 255) / 256;
-  hipLaunchKernelGGL((dequantize_kernel<T, D>),
-                     dim3(static_cast<unsigned>(blocks), static_cast<unsigned>(batch) * a.kv_heads, 2), dim3(256), 0, s, a);
-  return check_launch("dequantize_kernel");
+  return static_cast<int64_t>(a.tokens) * batch * a.kv_heads * D >= 1 << 24 ? launch_turns<T, D, 4>(a, batch, s)
+                                                                            : launch_turns<T, D, 1>(a, batch, s);
 }
 
 template <typename T>
 int quantize_dim(const QuantArgs& a, int64_t dim, hipStream_t s) {
   switch (dim) {
-    case 64: return launch_quantize<T, 64>(a, s);
-    case 96: return launch_quantize<T, 96>(a, s);
-    case 128: return launch_quantize<T, 128>(a, s);
-    default: return launch_quantize<T, 256>(a, s);
+    case 64: return launch_rows<T, 64>(a, s);
+    case 96: return launch_rows<T, 96>(a, s);
+    case 128: return launch_rows<T, 128>(a, s);
+    default: return launch_rows<T, 256>(a, s);
   }
 }
 
@@ -214,8 +277,8 @@ extern "C" int fpv2_quantize_to_pages(const void* k, const void* v, const void* 
   if (const int rc = check_cache(name, p.cache)) return rc;
   if (dtype != FPV2_BF16 && dtype != FPV2_F16)
     return fail(FPV2_ERR_UNSUPPORTED, "%s: dtype must be bf16 or f16", name);
-  if (p.tokens < 0 || p.tokens > 0x7fffffff / p.cache.kv_heads)
-    return fail(FPV2_ERR_ARGUMENT, "%s: tokens * kv_heads must be 0 to 2^31 - 1", name);
+  if (p.tokens < 0 || p.tokens > 0x3fffffff / p.cache.kv_heads)
+    return fail(FPV2_ERR_ARGUMENT, "%s: tokens * kv_heads must be 0 to 2^30 - 1", name);
   if (p.slot_bytes != 0 && p.slot_bytes != 4 && p.slot_bytes != 8)
     return fail(FPV2_ERR_ARGUMENT, "%s: slot_bytes must be 0, 4 or 8", name);
   const int64_t strides[] = {p.k_token_stride, p.k_head_stride, p.v_token_stride, p.v_head_stride};
@@ -237,9 +300,10 @@ extern "C" int fpv2_quantize_to_pages(const void* k, const void* v, const void* 
   a.x_ts[0] = p.k_token_stride, a.x_hs[0] = p.k_head_stride;
   a.x_ts[1] = p.v_token_stride, a.x_hs[1] = p.v_head_stride;
   a.first_slot = p.first_slot;
-  a.pages = p.cache.pages;
+  a.slot_count = p.cache.pages * p.cache.page_size;
   a.page_size = p.cache.page_size;
-  a.rows = p.tokens * p.cache.kv_heads;
+  page_division(p.cache.page_size, &a.page_mul, &a.page_shift);
+  a.tokens = static_cast<int>(p.tokens);
   a.slot_bytes = static_cast<int>(p.slot_bytes);
   a.kv_heads = static_cast<int>(p.cache.kv_heads);
   const hipStream_t s = static_cast<hipStream_t>(stream);
@@ -288,6 +352,7 @@ extern "C" int fpv2_dequantize_pages(const void* k_codes, const float* k_scales,
   a.kv_heads = static_cast<int>(p.cache.kv_heads);
   a.pages = static_cast<int>(p.cache.pages);
   a.page_size = static_cast<int>(p.cache.page_size);
+  page_division(p.cache.page_size, &a.page_mul, &a.page_shift);
   a.capacity = static_cast<int>(p.table_width * p.cache.page_size);
   a.length = static_cast<int>(p.length < a.capacity ? p.length : a.capacity);
   a.tokens = static_cast<int>(p.tokens);

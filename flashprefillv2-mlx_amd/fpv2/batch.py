@@ -29,7 +29,7 @@ import torch
 from fpv2 import _lib
 from fpv2.decode import (_HALF, MAX_VOCAB, _check_apart, _count, _device, _extent, _in_place, _index,
                          _on_device, _overlaps_itself, _page_strides, _pages, _row_strides,
-                         _rows_overlap, _share_memory)
+                         _rows_meet, _rows_overlap, _share_memory)
 from fpv2.kernel import SUPPORTED_HEAD_DIMS
 
 
@@ -169,45 +169,75 @@ def shared_prefix_attention(q: torch.Tensor, prefix_k: torch.Tensor, prefix_v: t
     return out
 
 
-def _code_pages(k_codes, k_scales, v_codes, v_scales):
-    """The shape ``(P, Hkv, page_size, D)`` of a cache of codes and all its strides."""
-    shape = k_codes.shape
-    for name, codes, scales in (("k", k_codes, k_scales), ("v", v_codes, v_scales)):
-        if codes.ndim != 4 or codes.dtype != torch.int8:
-            raise ValueError(f"{name}_codes must be int8 [pages, KV heads, page size, head dim]")
-        if codes.shape != shape:
-            raise ValueError("k_codes and v_codes must have the same shape")
-        if scales.shape != shape[:3] or scales.dtype != torch.float32:
-            raise ValueError(f"{name}_scales must be float32 [pages, KV heads, page size]")
-        if codes.data_ptr() % 16 or codes.stride(3) != 1 or any(
-                s % 16 for s, n in zip(codes.stride()[:3], shape) if n > 1):
-            raise ValueError("the codes' rows must be contiguous and 16-byte aligned")
+class _Codes(NamedTuple):
+    """A cache of codes as the calls need it."""
+
+    shape: tuple     # (P, Hkv, page_size, D)
+    strides: tuple   # of k_codes' and v_codes' first three dimensions
+    scales: tuple    # of k_scales and v_scales
+    bytes: tuple     # from each tensor's first byte to behind its last
+    overlap: bool    # whether rows share memory
+
+
+@lru_cache(maxsize=256)
+def _codes_layout(shape, k_strides, v_strides, ks_strides, vs_strides, *distances) -> _Codes:
+    """Of codes ``shape`` and their scales, the latter three tensors ``distances`` bytes behind the
+    first one."""
     if 0 in shape[:3]:
         raise ValueError("the caches must hold at least one row")
     if shape[3] not in SUPPORTED_HEAD_DIMS:
         raise ValueError(f"head dimension must be one of {SUPPORTED_HEAD_DIMS}")
-    strides = []
-    for codes in (k_codes, v_codes):
-        strides += [s if n > 1 else 0 for s, n in zip(codes.stride()[:3], shape)]
-    return shape, tuple(strides), (*k_scales.stride(), *v_scales.stride())
+    layouts = []  # (bytes of an element, shape, strides) of k_codes, v_codes, k_scales, v_scales
+    for strides in (k_strides, v_strides):
+        if strides[3] != 1 or any(s % 16 for s, n in zip(strides, shape[:3]) if n > 1):
+            raise ValueError("the codes' rows must be contiguous and 16-byte aligned")
+        layouts.append((1, shape, strides))
+    layouts += [(4, (*shape[:3], 1), (*strides, 1)) for strides in (ks_strides, vs_strides)]
+    overlap = any(_rows_overlap(n, s) for _, n, s in layouts)
+    extents = tuple(size * _extent(n, s) for size, n, s in layouts)
+    at = (0, *distances)
+    for i, a in enumerate(layouts):
+        for j, b in enumerate(layouts[:i]):
+            if -extents[i] < at[i] - at[j] < extents[j]:
+                overlap = overlap or _rows_meet(at[i] - at[j], a, b)
+    codes = [s if n > 1 else 0 for strides in (k_strides, v_strides) for s, n in zip(strides, shape[:3])]
+    return _Codes(shape, tuple(codes), (*ks_strides, *vs_strides), extents, overlap)
+
+
+def _code_pages(k_codes, k_scales, v_codes, v_scales) -> _Codes:
+    shape = k_codes.shape
+    if (k_codes.dtype != torch.int8 or v_codes.dtype != torch.int8 or len(shape) != 4
+            or v_codes.shape != shape or k_scales.dtype != torch.float32
+            or v_scales.dtype != torch.float32 or k_scales.shape != shape[:3]
+            or v_scales.shape != shape[:3]):
+        for name, codes, scales in (("k", k_codes, k_scales), ("v", v_codes, v_scales)):
+            if codes.ndim != 4 or codes.dtype != torch.int8:
+                raise ValueError(f"{name}_codes must be int8 [pages, KV heads, page size, head dim]")
+            if codes.shape != shape:
+                raise ValueError("k_codes and v_codes must have the same shape")
+            if scales.shape != shape[:3] or scales.dtype != torch.float32:
+                raise ValueError(f"{name}_scales must be float32 [pages, KV heads, page size]")
+    first, second = k_codes.data_ptr(), v_codes.data_ptr()
+    if (first | second) & 15:
+        raise ValueError("the codes' rows must be contiguous and 16-byte aligned")
+    return _codes_layout(shape, k_codes.stride(), v_codes.stride(), k_scales.stride(), v_scales.stride(),
+                         second - first, k_scales.data_ptr() - first, v_scales.data_ptr() - first)
 
 
 @lru_cache(maxsize=256)
-def _codes_overlap(shape, strides, scale_strides) -> bool:
-    """Whether two rows of a cache share memory."""
-    return any(_rows_overlap(shape, (*strides[i:i + 3], 1))
-               or _rows_overlap((*shape[:3], 1), (*scale_strides[i:i + 3], 1)) for i in (0, 3))
+def _write_params(codes: _Codes, *fields):
+    params = _lib.QuantizeParams(
+        _lib.CodePages(codes.shape[1], codes.shape[3], codes.shape[0], codes.shape[2], *codes.strides,
+                       *codes.scales), *fields)
+    return params, ctypes.byref(params)
 
 
-def _spans_meet(tensors) -> bool:
-    """Whether any two of the tensors share memory."""
-    spans = sorted((t.data_ptr(), t.data_ptr() + t.element_size() * _extent(t.shape, t.stride()), i)
-                   for i, t in enumerate(tensors))
-    end, meet = 0, False
-    for first, last, _ in spans:
-        meet |= first < end
-        end = max(end, last)
-    return meet and any(_share_memory(a, b) for i, a in enumerate(tensors) for b in tensors[:i])
+@lru_cache(maxsize=256)
+def _read_params(codes: _Codes, *fields):
+    params = _lib.DequantizeParams(
+        _lib.CodePages(codes.shape[1], codes.shape[3], codes.shape[0], codes.shape[2], *codes.strides,
+                       *codes.scales), *fields)
+    return params, ctypes.byref(params)
 
 
 def quantize_to_pages(k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor | int,
@@ -227,43 +257,56 @@ def quantize_to_pages(k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor | in
 
     A row with an infinity or a NaN reads back as NaN, a row of zeros as zeros.
     """
-    shape, strides, scale_strides = _code_pages(k_codes, k_scales, v_codes, v_scales)
-    pages, kv_heads, page_size, dim = shape
-    for name, x in (("k", k), ("v", v)):
-        if x.ndim != 3 or x.shape[1:] != (kv_heads, dim) or x.shape != k.shape:
-            raise ValueError(f"{name} must be [tokens, KV heads, head dim] of the caches' geometry")
-        if x.dtype not in _HALF or x.dtype != k.dtype:
-            raise ValueError("k and v must share float16 or bfloat16 dtype")
-    tokens = k.shape[0]
-    if _codes_overlap(shape, strides, scale_strides) or _spans_meet((k_codes, k_scales, v_codes, v_scales)):
+    codes = _code_pages(k_codes, k_scales, v_codes, v_scales)
+    _, kv_heads, _, dim = codes.shape
+    shape, dtype = k.shape, k.dtype
+    if (len(shape) != 3 or v.shape != shape or shape[1] != kv_heads or shape[2] != dim
+            or dtype not in _HALF or v.dtype != dtype):
+        for name, x in (("k", k), ("v", v)):
+            if x.ndim != 3 or x.shape[1:] != (kv_heads, dim) or x.shape != shape:
+                raise ValueError(f"{name} must be [tokens, KV heads, head dim] of the caches' geometry")
+        raise ValueError("k and v must share float16 or bfloat16 dtype")
+    tokens = shape[0]
+    if codes.overlap:
         raise ValueError("the caches' rows overlap")
     slots, slot_bytes, first_slot = _index(slots, "slots", tokens)
-    tensors = [k, v, k_codes, k_scales, v_codes, v_scales]
+    tensors = [k, v, k_codes, v_codes, k_scales, v_scales]
     if slots is not None:
         tensors.append(slots)
-    for cache in tensors[2:6]:
-        for x in (k, v, slots):
-            if x is not None and _share_memory(cache, x):
+    # (what is read lies apart from what is written)
+    firsts = [x.data_ptr() for x in tensors]
+    for x, first in zip(tensors, firsts):
+        if x is k_codes:
+            break
+        end = first + 2 * _extent(shape, x.stride())
+        for cache, at, size in zip(tensors[2:6], firsts[2:6], codes.bytes):
+            if first < at + size and at < end and _share_memory(cache, x):
+                raise ValueError("the caches must not share memory with what the call reads")
+    if slots is not None:
+        first, end = firsts[6], firsts[6] + slot_bytes * tokens
+        for cache, at, size in zip(tensors[2:6], firsts[2:6], codes.bytes):
+            if first < at + size and at < end and _share_memory(cache, slots):
                 raise ValueError("the caches must not share memory with what the call reads")
     index = _device(tensors)
-    rows = []
-    for x in (k, v):
-        if _row_strides(x) is None:
-            x = x.clone(memory_format=torch.contiguous_format)
-        rows.append((x, _row_strides(x)))
     if tokens == 0:
         return
-    (k, k_strides), (v, v_strides) = rows
-    lib = _lib.load()
-    params = _lib.QuantizeParams(
-        _lib.CodePages(kv_heads, dim, pages, page_size, *strides, *scale_strides), tokens,
-        slot_bytes, first_slot, *k_strides, *v_strides)
+    k_strides, v_strides = _row_strides(k), _row_strides(v)
+    if k_strides is None:
+        k = k.clone(memory_format=torch.contiguous_format)
+        k_strides = _row_strides(k)
+    if v_strides is None:
+        v = v.clone(memory_format=torch.contiguous_format)
+        v_strides = _row_strides(v)
+    params, ref = _write_params(codes, tokens, slot_bytes, 0, *k_strides, *v_strides)
+    if first_slot:
+        params = _lib.QuantizeParams.from_buffer_copy(params)
+        params.first_slot = first_slot
+        ref = ctypes.byref(params)
 
     def call(stream):
-        _lib.check(lib.fpv2_quantize_to_pages(
-            k.data_ptr(), v.data_ptr(), _lib.ptr(slots), k_codes.data_ptr(), k_scales.data_ptr(),
-            v_codes.data_ptr(), v_scales.data_ptr(), _lib.dtype_code(k.dtype),
-            ctypes.byref(params), stream), "quantize_to_pages")
+        _lib.check(_lib.load().fpv2_quantize_to_pages(
+            k.data_ptr(), v.data_ptr(), None if slots is None else firsts[6], firsts[2], firsts[4],
+            firsts[3], firsts[5], _lib.dtype_code(dtype), ref, stream), "quantize_to_pages")
 
     _on_device(index, call)
 
@@ -283,8 +326,8 @@ def dequantize_pages(k_codes: torch.Tensor, k_scales: torch.Tensor, v_codes: tor
     of destinations with 16-byte aligned rows, apart from one another and from all operands:
     the caches of a ``ChunkedPrefill`` that goes on are ``out=cp.pages()``.
     """
-    shape, strides, scale_strides = _code_pages(k_codes, k_scales, v_codes, v_scales)
-    pages, kv_heads, page_size, dim = shape
+    codes = _code_pages(k_codes, k_scales, v_codes, v_scales)
+    pages, kv_heads, page_size, dim = codes.shape
     width, table_stride = 1, 0
     if page_table is not None:
         batch = page_table.shape[0] if page_table.ndim == 2 else -1
@@ -320,16 +363,18 @@ def dequantize_pages(k_codes: torch.Tensor, k_scales: torch.Tensor, v_codes: tor
                     for _ in "kv")
     if batch == 0 or tokens == 0:
         return out
-    lib = _lib.load()
-    params = _lib.DequantizeParams(
-        _lib.CodePages(kv_heads, dim, pages, page_size, *strides, *scale_strides), batch, width,
-        table_stride, length, tokens, zero_rest, *_row_strides(out[0]), *_row_strides(out[1]))
+    params, ref = _read_params(codes, batch, width, table_stride, 0, tokens, zero_rest,
+                               *_row_strides(out[0]), *_row_strides(out[1]))
+    if length:
+        params = _lib.DequantizeParams.from_buffer_copy(params)
+        params.length = length
+        ref = ctypes.byref(params)
 
     def call(stream):
-        _lib.check(lib.fpv2_dequantize_pages(
+        _lib.check(_lib.load().fpv2_dequantize_pages(
             k_codes.data_ptr(), k_scales.data_ptr(), v_codes.data_ptr(), v_scales.data_ptr(),
             _lib.ptr(page_table), _lib.ptr(lengths), out[0].data_ptr(), out[1].data_ptr(),
-            _lib.dtype_code(dtype), ctypes.byref(params), stream), "dequantize_pages")
+            _lib.dtype_code(dtype), ref, stream), "dequantize_pages")
 
     _on_device(index, call)
     return out
@@ -356,8 +401,8 @@ def quantized_decode_attention(q: torch.Tensor, k_codes: torch.Tensor, k_scales:
     codes are exact in the products; a query's values below 2^-14 of its greatest one are
     rounded to 2^-25 of it, the weights times the values' scales to float16 of 11 bits.
     """
-    shape, strides, scale_strides = _code_pages(k_codes, k_scales, v_codes, v_scales)
-    pages, kv_heads, page_size, page_dim = shape
+    codes = _code_pages(k_codes, k_scales, v_codes, v_scales)
+    pages, kv_heads, page_size, page_dim = codes.shape
     batch, heads, dim = _queries(q, kv_heads, page_dim)
     if q.dtype not in _HALF:
         raise ValueError("q must be float16 or bfloat16")
@@ -392,7 +437,7 @@ def quantized_decode_attention(q: torch.Tensor, k_codes: torch.Tensor, k_scales:
     def call(stream):
         params, ref, need = _quantized_plan(
             index, (batch, heads, kv_heads, dim, pages, page_size, width, table_stride, 0, window, sinks,
-                    scale, *q_strides, *strides, out.stride(0), out.stride(1)), *scale_strides)
+                    scale, *q_strides, *codes.strides, out.stride(0), out.stride(1)), *codes.scales)
         if lengths is None:
             params = _lib.QuantizedDecodeParams.from_buffer_copy(params)
             params.attention.length = length
@@ -420,6 +465,14 @@ class TokenLogprobs(NamedTuple):
     top_logprobs: torch.Tensor  # float32 [N, top]
 
 
+@lru_cache(maxsize=256)
+def _logprobs_plan(index: int, *fields):
+    """A call's parameters and the bytes of workspace that it needs on device ``index`` (the
+    current one)."""
+    ref = ctypes.byref(_lib.LogprobsParams(*fields))
+    return ref, _lib.load().fpv2_token_logprobs_workspace_bytes(ref)
+
+
 def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, *, top: int = 0) -> TokenLogprobs:
     """Log probabilities of ``tokens`` ``[N]`` (int32 or int64), one for each row of ``logits``
     ``[N, V]``, the entropies of the rows' distributions and their ``top`` most likely
@@ -445,23 +498,20 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, *, top: int = 0) 
     if vocab > 1 and logits.stride(1) != 1:
         logits = logits.contiguous()
     device = logits.device
-    sums = torch.empty((2, rows), dtype=torch.float32, device=device)
-    res = TokenLogprobs(sums[0], sums[1], torch.empty((rows, top), dtype=torch.int64, device=device),
+    res = TokenLogprobs(*(torch.empty(rows, dtype=torch.float32, device=device) for _ in range(2)),
+                        torch.empty((rows, top), dtype=torch.int64, device=device),
                         torch.empty((rows, top), dtype=torch.float32, device=device))
     if rows == 0:
         return res
-    lib = _lib.load()
-    params = _lib.LogprobsParams(rows, vocab, logits.stride(0) if rows > 1 else 0,
-                                 tokens.element_size(), top)
 
     def call(stream):
-        need = lib.fpv2_token_logprobs_workspace_bytes(ctypes.byref(params))
+        ref, need = _logprobs_plan(index, rows, vocab, logits.stride(0) if rows > 1 else 0,
+                                   tokens.element_size(), top)
         work = torch.empty(need, dtype=torch.uint8, device=device) if need > 0 else None
-        _lib.check(lib.fpv2_token_logprobs(
-            logits.data_ptr(), tokens.data_ptr(), _lib.dtype_code(logits.dtype),
-            ctypes.byref(params), res.logprobs.data_ptr(), res.entropy.data_ptr(),
-            res.top_tokens.data_ptr(), res.top_logprobs.data_ptr(), _lib.ptr(work), max(need, 0),
-            stream), "token_logprobs")
+        _lib.check(_lib.load().fpv2_token_logprobs(
+            logits.data_ptr(), tokens.data_ptr(), _lib.dtype_code(logits.dtype), ref,
+            res.logprobs.data_ptr(), res.entropy.data_ptr(), res.top_tokens.data_ptr(),
+            res.top_logprobs.data_ptr(), _lib.ptr(work), max(need, 0), stream), "token_logprobs")
 
     _on_device(index, call)
     return res

@@ -7,7 +7,7 @@ namespace {
 
 template <typename T, int D>
 int launch(const DecodeArgs& a, bool join, hipStream_t s) {
-  hipLaunchKernelGGL((decode_attn_kernel<T, D, false>), dim3(a.grid), dim3(256), 0, s, a);
+  hipLaunchKernelGGL((decode_attn_kernel<T, D>), dim3(a.grid), dim3(256), 0, s, a);
   if (join) launch_join<T, D>(a, s);
   return check_launch("decode_attn_kernel");
 }

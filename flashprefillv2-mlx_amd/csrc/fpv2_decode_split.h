@@ -184,9 +184,8 @@ struct DecodeShared {
   u32x4 q[kLdsQ ? 2 * D : 1];
 };
 
-// A workgroup of 256 threads.  KEEP: items that one workgroup covers leave their partial
-// too, behind the runs' slots.
-template <typename T, int D, bool KEEP>
+// A workgroup of 256 threads.
+template <typename T, int D>
 __device__ __forceinline__ void decode_attn(const DecodeArgs& a, int block, DecodeShared<D>& sh) {
   constexpr int KK = D / 32;  // MFMA steps of a key's dot product
   constexpr int DV = D / 16;  // dims of a lane
@@ -359,8 +358,7 @@ __device__ __forceinline__ void decode_attn(const DecodeArgs& a, int block, Deco
     }
     __syncthreads();
     const bool whole = first == 0 && last == s_now.tiles;
-    const int64_t slot = KEEP && whole ? 2 * static_cast<int64_t>(a.grid) + static_cast<int64_t>(b_now) * items + item
-                                       : 2 * static_cast<int64_t>(block) + (cur == lo ? 0 : 1);
+    const int64_t slot = 2 * static_cast<int64_t>(block) + (cur == lo ? 0 : 1);
     for (int e = tid; e < heads * D; e += 256) {
       const int h = e / D, d = e % D;
       float top = neg_inf();
@@ -375,7 +373,7 @@ __device__ __forceinline__ void decode_attn(const DecodeArgs& a, int block, Deco
         sum += f * sh_o[w][h][d];
         den += f * sh_ml[w][h][1];
       }
-      if (!KEEP && whole) {
+      if (whole) {
         const float r = s_now.n == 0 ? 0.f : sum / den;
         a.out[b_now * a.o_bs + (kvh * a.group + h0 + h) * a.o_hs + d] = Elem<T>::from_float(r);
       } else {
@@ -390,10 +388,10 @@ __device__ __forceinline__ void decode_attn(const DecodeArgs& a, int block, Deco
   }
 }
 
-template <typename T, int D, bool KEEP>
+template <typename T, int D>
 __global__ __launch_bounds__(256, 2) void decode_attn_kernel(DecodeArgs a) {
   __shared__ DecodeShared<D> sh;
-  decode_attn<T, D, KEEP>(a, blockIdx.x, sh);
+  decode_attn<T, D>(a, blockIdx.x, sh);
 }
 
 // Joins the partials of an item that several workgroups shared: one workgroup

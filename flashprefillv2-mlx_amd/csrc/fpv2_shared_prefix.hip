@@ -6,8 +6,7 @@
 //
 // The sums split over t: partials (O, max, sum) of parts of the keys are joined as
 //   O = sum_i exp(m_i - m) O_i, l = sum_i exp(m_i - m) l_i, m = max_i m_i.
-// Two launches: workgroups of the own keys (decode_attn, all items left as partials) and of
-// the prefix, then the join.
+// Two launches: workgroups of the own keys and of the prefix, then the join.
 //
 // Prefix: the rows of a KV head are the batch's query heads of it, packed; a workgroup
 // takes a tile of them and a part of the prefix's keys.  Its waves take 32 keys each on
@@ -19,7 +18,7 @@ namespace fpv2 {
 namespace {
 
 constexpr int kMaxSplits = 512;  // parts of the prefix
-constexpr int kMaxOwn = 512;     // workgroups of the own keys
+constexpr int kMaxRuns = 2048;   // waves of the own keys
 
 struct PrefixArgs {
   const uint16_t* q;
@@ -31,6 +30,7 @@ struct PrefixArgs {
   float* part_ml;          // [splits][kv_heads][rows][2]
   int64_t q_bs, q_hs, k_ps, k_hs, k_rs, v_ps, v_hs, v_rs;
   int kv_heads, group, rows, row_tiles, tile_rows, splits;  // rows: batch * group
+  int own_blocks;  // workgroups of the own keys, before the prefix's
   int pages, page_size, capacity, length;
   uint32_t page_mul, page_shift;
   float scale_log2;
@@ -184,6 +184,131 @@ __device__ __forceinline__ Words<NW> buf_load_words(rsrc_t r, uint32_t off, uint
 // HALVES: 16 keys from a multiple of 16 on lie in one page (or there is no table): their
 // addresses are the wave's, a lane's offsets do not change, and a descriptor of the rows
 // up to the prefix's end reads zeros behind it.
+// Own keys: the decode attention's schedule (fpv2_decode_split.h) with runs of waves instead of
+// workgroups, as they are short: a wave takes its items' tiles one after the other and
+// leaves a partial of each, a whole item's behind the runs' slots.
+template <typename T, int D>
+__device__ __forceinline__ void own_attn(const DecodeArgs& a, int run) {
+  constexpr int KK = D / 32, DV = D / 16;
+  constexpr int kEarly = D > 128 ? 0 : 8;  // values whose loads do not wait for the scores
+  const int lane = threadIdx.x & 63, col = lane & 15, quad = lane >> 4;
+  const int items = a.kv_heads * a.head_items;
+  const Prefix prefix = prefix_of(a, lane);
+  const int total = prefix.total * items;
+  const int lo = first_of(a, run, total), hi = first_of(a, run + 1, total);
+  if (lo >= hi) return;
+  int base;
+  int b = sequence_at(a, prefix, lane, lo, &base);
+  Sequence s = sequence_of(a, b);
+  for (int cur = lo, end; cur < hi; cur = end) {
+    const int units = s.units();
+    const int item = (cur - base) / units;
+    const int item_start = base + item * units;
+    end = min(hi, item_start + units);
+    // tiles [first, last) of the item; the run may start or end among the other units
+    const int first = max(0, cur - item_start - kItemUnits), last = end - item_start - kItemUnits;
+    const int b_now = b;
+    const Sequence s_now = s;
+    if (end < hi && end == base + items * units) {
+      base = end;
+      s = sequence_of(a, ++b);
+    }
+    if (last <= first) continue;
+    const int kvh = item / a.head_items;
+    const int h0 = (item - kvh * a.head_items) * a.item_heads;
+    const int heads = min(a.item_heads, a.group - h0);
+    const int head = kvh * a.group + h0 + col;
+    const uint32_t sign = a.scale_log2 < 0.f ? 0x80008000u : 0u;
+    const float scale = fmaxf(__builtin_fabsf(a.scale_log2), 1e-30f);
+    u32x4 qf[KK];
+#pragma unroll
+    for (int kk = 0; kk < KK; ++kk)
+      qf[kk] = col < heads ? load16(a.q + b_now * a.q_bs + head * a.q_hs + 32 * kk + 8 * quad) ^ sign : u32x4{0, 0, 0, 0};
+    f32x4 o[DV];
+    float m = kNone, l = 0.f, greatest = neg_inf();
+#pragma unroll
+    for (int d = 0; d < DV; ++d) o[d] = f32x4{0.f, 0.f, 0.f, 0.f};
+
+    const uint16_t* kb = a.k + kvh * a.k_hs;
+    const uint16_t* vb = a.v + kvh * a.v_hs;
+    const int32_t* table = a.table != nullptr ? a.table + b_now * a.table_stride : nullptr;
+    // lane i (and i + 32) looks up the row of the tile's key i
+    int row = 0, page = 0;
+    const auto look_up = [&](int u0) {
+      const uint32_t t = min(u0 + (lane & 31), s_now.n - 1);
+      const uint32_t at = (__umulhi(t, a.page_mul) + t) >> a.page_shift;
+      row = t - at * a.page_size;
+      const int id = table != nullptr ? table[at] : b_now;
+      page = min(max(id, 0), a.pages - 1);
+    };
+    const int u_end = min(s_now.n, last * kTileKeys);
+    if (first * kTileKeys < u_end) look_up(first * kTileKeys);
+    for (int u0 = first * kTileKeys; u0 < u_end; u0 += kTileKeys) {
+      const int64_t koff = page * a.k_ps + row * a.k_rs;
+      const int64_t voff = page * a.v_ps + row * a.v_rs;
+      u32x4 kf[2][KK];
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        const uint16_t* p = kb + __shfl(koff, 16 * t + col, 64) + 8 * quad;
+#pragma unroll
+        for (int kk = 0; kk < KK; ++kk) kf[t][kk] = load16(p + 32 * kk);
+      }
+      Words<DV / 2> vf[8];
+      const auto load_v = [&](int j) {
+        return load_words<DV / 2>(vb + __shfl(voff, 16 * (j / 4) + 4 * quad + j % 4, 64) + DV * col);
+      };
+#pragma unroll
+      for (int j = 0; j < kEarly; ++j) vf[j] = load_v(j);
+      if (u0 + kTileKeys < u_end) look_up(u0 + kTileKeys);
+      f32x4 sc[2];
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        sc[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int kk = 0; kk < KK; ++kk) sc[t] = Elem<T>::mfma16(as_vec8<T>(kf[t][kk]), as_vec8<T>(qf[kk]), sc[t]);
+      }
+#pragma unroll
+      for (int j = kEarly; j < 8; ++j) vf[j] = load_v(j);
+      const int left = s_now.n - u0;
+      const u32x4 pf =
+          weigh<T>(relate<T>(sc, scale, left < kTileKeys ? left - 4 * quad : kTileKeys, m, l, greatest, o), l);
+      if (left < kTileKeys) {
+        // (a zero weight would make NaN of what an unused row may hold)
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          if (16 * (j / 4) + 4 * quad + j % 4 >= left) {
+#pragma unroll
+            for (int w = 0; w < DV / 2; ++w) vf[j].w[w] = 0;
+          }
+      }
+#pragma unroll
+      for (int d = 0; d < DV; ++d) {
+        u32x4 vt;  // dim d of the lane's 8 keys
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          vt[j] = __builtin_amdgcn_perm(vf[2 * j + 1].w[d / 2], vf[2 * j].w[d / 2], d % 2 ? 0x07060302u : 0x05040100u);
+        o[d] = Elem<T>::mfma16(as_vec8<T>(vt), as_vec8<T>(pf), o[d]);
+      }
+    }
+    l += __shfl_xor(l, 16, 64);
+    l += __shfl_xor(l, 32, 64);
+    const bool whole = first == 0 && last == s_now.tiles;
+    const int64_t slot = whole ? 2 * static_cast<int64_t>(a.grid) + static_cast<int64_t>(b_now) * items + item
+                               : 2 * static_cast<int64_t>(run) + (cur == lo ? 0 : 1);
+    if (col < heads) {
+      const int64_t at = slot * a.item_heads + col;
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int d = 0; d < DV; ++d) a.part_o[at * D + (4 * quad + i) * DV + d] = o[d][i];
+      if (quad == 0) {
+        a.part_ml[at * 2] = m;
+        a.part_ml[at * 2 + 1] = l;
+      }
+    }
+  }
+}
+
 // At most 16 rows: one tile of MFMA; the workgroup's waves take 32 keys each, as they lie.
 template <int D>
 struct FewShared {
@@ -347,22 +472,20 @@ __device__ __forceinline__ void prefix_few(const PrefixArgs& a, int block, FewSh
 
 template <typename T, int D, bool HALVES>
 __global__ __launch_bounds__(256, D > 128 ? 1 : 2) void prefix_few_kernel(PrefixArgs p, DecodeArgs a) {
-  __shared__ union {
-    FewShared<D> few;
-    DecodeShared<D> own;
-  } sh;
-  if (static_cast<int>(blockIdx.x) < a.grid)
-    decode_attn<T, D, true>(a, blockIdx.x, sh.own);
+  __shared__ FewShared<D> sh;
+  const int block = static_cast<int>(blockIdx.x) - p.own_blocks;
+  if (block < 0)
+    own_attn<T, D>(a, blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6));
   else
-    prefix_few<T, D, HALVES>(p, blockIdx.x - a.grid, sh.few);
+    prefix_few<T, D, HALVES>(p, block, sh);
 }
 
-// More rows than a tile of MFMA: the workgroup's waves, 32 rows each (16 at head dim 256,
-// whose rows are twice as long), share the keys through LDS.  A stage is 32 keys' K and V, rows of a power of two of bytes whose 16-byte
-// chunks are permuted so that neither the reads of K (16 keys' chunks) nor the transposing
-// reads of V (8 keys, 32 bytes each) meet in a bank.  Three stages in LDS, two more on
-// their way in registers.  Each wave loads some keys' K or V: one page, one descriptor a
-// stage.
+// More rows than a tile of MFMA: the workgroup's waves, 32 rows each (at head dim 256, whose
+// rows are twice as long, 8 waves of 16 rows), share the keys through LDS.  A stage is 32
+// keys' K and V, rows of a power of two of bytes whose 16-byte chunks are permuted so that
+// neither the reads of K (16 keys' chunks) nor the transposing reads of V (8 keys, 32 bytes
+// each) meet in a bank.  Three stages in LDS, two more on their way in registers.  Each wave
+// loads some keys' K or V: one page, one descriptor a stage.
 template <int D>
 struct Stage {
   static constexpr int kRow = D <= 64 ? 128 : D <= 128 ? 256 : 512;  // bytes of a row in LDS
@@ -401,6 +524,8 @@ __device__ __forceinline__ void prefix_many(const PrefixArgs& a, int block, uint
   const int tiles = (n + kTileKeys - 1) / kTileKeys;
   const int first = static_cast<int>(static_cast<int64_t>(tiles) * split / a.splits);
   const int last = static_cast<int>(static_cast<int64_t>(tiles) * (split + 1) / a.splits);
+  const int steps = last - first;
+  const auto tile_of = [&](int step) { return first + step; };
   const int r0 = rt * a.tile_rows + 16 * CT * wave;  // this wave's rows
   const int r_end = min(a.rows, (rt + 1) * a.tile_rows);
 
@@ -530,62 +655,76 @@ __device__ __forceinline__ void prefix_many(const PrefixArgs& a, int block, uint
   // that it is known at each store how many loads were issued since its own.)
   if (first < last) {
     const bool rows_here = r0 < r_end;
-    Regs regs[G];  // stage first + i, + i + G .. in regs[i % G]
-    look_up(first);
+    Regs regs[G];  // stage i, i + G .. in regs[i % G]
+    look_up(tile_of(0));
     StaticFor<0, G>::run([&](auto i) {
-      load(regs[i], first + i);
-      look_up(first + i + 1);
+      load(regs[i], tile_of(i));
+      look_up(tile_of(i + 1));
     });
     StaticFor<0, 2>::run([&](auto i) {
-      store(regs[i % G], first + i, i);
-      load(regs[i % G], first + i + G);
-      look_up(first + i + 1 + G);
+      store(regs[i % G], tile_of(i), i);
+      load(regs[i % G], tile_of(i + G));
+      look_up(tile_of(i + 1 + G));
     });
     barrier_lds();
     if (rows_here) score(std::integral_constant<int, 0>{});
-    for (int at = first; at < last; at += R * G)
+    for (int at = 0; at < steps; at += R * G)
       StaticFor<0, R * G>::run([&](auto i) __attribute__((always_inline)) {
         // (R = 3: the next stage is written, and the one before this one read)
         constexpr std::integral_constant<int, i % R> kThis{};
         constexpr std::integral_constant<int, (i + 1) % R> kNext{};
         constexpr std::integral_constant<int, (i + 2) % R> kAfter{};
         barrier_lds();
-        store(regs[(i + 2) % G], at + i + 2, kAfter);
-        load(regs[(i + 2) % G], at + i + 2 + G);
-        look_up(at + i + 3 + G);
-        if (rows_here && at + i < last) multiply(at + i, kThis, kNext);
+        store(regs[(i + 2) % G], tile_of(at + i + 2), kAfter);
+        load(regs[(i + 2) % G], tile_of(at + i + 2 + G));
+        look_up(tile_of(at + i + 3 + G));
+        if (rows_here && tile_of(at + i) < last) multiply(tile_of(at + i), kThis, kNext);
       });
   }
 
-  // (each row is one wave's)
+  // The sums, each row one wave's: through its part of the ring, so that a store is of whole
+  // rows.
+  constexpr int kWide = D < 128 ? D : 128, kPad = kWide + 4;  // dims at a time
+  static_assert(sizeof(sh) >= S::kWaves * 16 * kPad * 4, "16 rows of every wave fit the ring");
+  float* const mine = reinterpret_cast<float*>(&sh[0][0]) + wave * 16 * kPad;
+  barrier_lds();
 #pragma unroll
   for (int c = 0; c < CT; ++c) {
     l[c] += __shfl_xor(l[c], 16, 64);
     l[c] += __shfl_xor(l[c], 32, 64);
-    const int row = r0 + 16 * c + col;
-    if (row >= r_end) continue;
-    const int64_t at = static_cast<int64_t>(unit) * a.rows + row;
+    const int row0 = r0 + 16 * c;
+    const int64_t at = static_cast<int64_t>(unit) * a.rows + row0;
 #pragma unroll
-    for (int d = 0; d < DT; ++d) *reinterpret_cast<f32x4*>(a.part_o + at * D + 16 * d + 4 * quad) = o[c][d];
-    if (quad == 0) {
-      a.part_ml[at * 2] = m[c];
-      a.part_ml[at * 2 + 1] = l[c];
+    for (int d0 = 0; d0 < D; d0 += kWide) {
+#pragma unroll
+      for (int d = 0; d < kWide / 16; ++d)
+        *reinterpret_cast<f32x4*>(mine + col * kPad + 16 * d + 4 * quad) = o[c][d0 / 16 + d];
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      __builtin_amdgcn_wave_barrier();
+#pragma unroll
+      for (int i = 0; i < 16 * kWide / 4 / 64; ++i) {
+        const int e = lane + 64 * i, row = e / (kWide / 4), part = e - row * (kWide / 4);
+        if (row0 + row < r_end)
+          *reinterpret_cast<f32x4*>(a.part_o + (at + row) * D + d0 + 4 * part) =
+              *reinterpret_cast<const f32x4*>(mine + row * kPad + 4 * part);
+      }
+      __builtin_amdgcn_wave_barrier();
+    }
+    if (quad == 0 && row0 + col < r_end) {
+      a.part_ml[(at + col) * 2] = m[c];
+      a.part_ml[(at + col) * 2 + 1] = l[c];
     }
   }
 }
 
 template <typename T, int D, bool HALVES>
 __global__ __launch_bounds__(64 * Stage<D>::kWaves, D > 128 ? 1 : 2) void prefix_many_kernel(PrefixArgs p, DecodeArgs a) {
-  __shared__ union {
-    alignas(1024) uint8_t ring[3][2 * Stage<D>::kMatrix];
-    DecodeShared<D> own;
-  } sh;
-  // (workgroups of more threads than the own keys' have a launch of their own for these)
-  if (Stage<D>::kWaves == 4 && static_cast<int>(blockIdx.x) < a.grid) {
-    if constexpr (Stage<D>::kWaves == 4) decode_attn<T, D, true>(a, blockIdx.x, sh.own);
-  } else {
-    prefix_many<T, D, HALVES>(p, blockIdx.x - (Stage<D>::kWaves == 4 ? a.grid : 0), sh.ring);
-  }
+  __shared__ alignas(1024) uint8_t ring[3][2 * Stage<D>::kMatrix];
+  const int block = static_cast<int>(blockIdx.x) - p.own_blocks;
+  if (block < 0)
+    own_attn<T, D>(a, blockIdx.x * Stage<D>::kWaves + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6));
+  else
+    prefix_many<T, D, HALVES>(p, block, ring);
 }
 
 // Joins a query head's partials of the prefix and of its sequence's own keys: WAVES waves
@@ -595,7 +734,8 @@ template <typename T, int D, int WAVES>
 __global__ __launch_bounds__(256) void shared_join_kernel(PrefixArgs p, DecodeArgs a) {
   constexpr int kLanes = D / 4, kAtOnce = 64 / kLanes, kHeads = 4 / WAVES;
   __shared__ f32x4 sh_o[4][kAtOnce][kLanes];
-  __shared__ float sh_f[4][kMaxSplits + kMaxOwn];
+  constexpr int kFactors = 512;  // partials whose weights are in LDS at a time
+  __shared__ float sh_f[4][kFactors];
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int items = a.kv_heads * a.head_items, heads = a.kv_heads * a.group;
@@ -614,7 +754,7 @@ __global__ __launch_bounds__(256) void shared_join_kernel(PrefixArgs p, DecodeAr
   const int n = p.splits + own;
   // the partials' rows: the prefix's parts, then the own keys' (one workgroup's whole item
   // lies behind the runs' slots)
-  const auto row_of = [&](int i) -> int64_t {
+  const auto row_of = [&](int i) __attribute__((always_inline)) -> int64_t {
     if (i < p.splits) return (static_cast<int64_t>(i) * p.kv_heads + kvh) * p.rows + b * p.group + g;
     i -= p.splits;
     const int64_t slot = own == 1 ? 2 * static_cast<int64_t>(a.grid) + static_cast<int64_t>(b) * items + item
@@ -622,38 +762,39 @@ __global__ __launch_bounds__(256) void shared_join_kernel(PrefixArgs p, DecodeAr
     return slot * a.item_heads + h;
   };
   typedef float f32x2 __attribute__((ext_vector_type(2)));
-  const auto ml_of = [&](int i) {
+  const auto ml_of = [&](int i) __attribute__((always_inline)) {
     return *reinterpret_cast<const f32x2*>((i < p.splits ? p.part_ml : a.part_ml) + row_of(i) * 2);
   };
   float top = neg_inf();
-  for (int i = lane; i < n; i += 64) {
-    const float m = ml_of(i)[0];
-    sh_f[wave][i] = m;
-    top = fmaxf(top, m);
-  }
+  for (int i = lane; i < n; i += 64) top = fmaxf(top, ml_of(i)[0]);
 #pragma unroll
   for (int off = 32; off >= 1; off >>= 1) top = fmaxf(top, __shfl_xor(top, off, 64));
   const float ref = top == neg_inf() ? 0.f : top;
   float den = 0.f;
-  for (int i = lane; i < n; i += 64) {
-    const float f = __builtin_amdgcn_exp2f(sh_f[wave][i] - ref);
-    sh_f[wave][i] = f;
-    den += f * ml_of(i)[1];
-  }
-#pragma unroll
-  for (int off = 32; off >= 1; off >>= 1) den += __shfl_xor(den, off, 64);
-  // (its own wave's LDS)
-  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-  __builtin_amdgcn_wave_barrier();
   f32x4 o = {0.f, 0.f, 0.f, 0.f};
   const int slot = lane / kLanes, e = lane % kLanes;
-  if (slot < kAtOnce) {
+  for (int i0 = 0; i0 < n; i0 += kFactors) {
+    const int upto = min(n, i0 + kFactors);
+    for (int i = i0 + lane; i < upto; i += 64) {
+      const f32x2 ml = ml_of(i);
+      const float f = __builtin_amdgcn_exp2f(ml[0] - ref);
+      sh_f[wave][i - i0] = f;
+      den += f * ml[1];
+    }
+    // (its own wave's LDS)
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    if (slot < kAtOnce) {
 #pragma unroll 8
-    for (int i = wave % WAVES * kAtOnce + slot; i < n; i += WAVES * kAtOnce)
-      o += sh_f[wave][i] *
-           *reinterpret_cast<const f32x4*>((i < p.splits ? p.part_o : a.part_o) + row_of(i) * D + 4 * e);
-    sh_o[wave][slot][e] = o;
+      for (int i = i0 + wave % WAVES * kAtOnce + slot; i < upto; i += WAVES * kAtOnce)
+        o += sh_f[wave][i - i0] *
+             *reinterpret_cast<const f32x4*>((i < p.splits ? p.part_o : a.part_o) + row_of(i) * D + 4 * e);
+    }
+    __builtin_amdgcn_wave_barrier();
   }
+  if (slot < kAtOnce) sh_o[wave][slot][e] = o;
+#pragma unroll
+  for (int off = 32; off >= 1; off >>= 1) den += __shfl_xor(den, off, 64);
   __syncthreads();
   if (wave % WAVES == 0 && lane < kLanes) {
     o = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -677,14 +818,17 @@ struct SharedPlan {
 SharedPlan shared_plan(const fpv2_shared_prefix_params& p) {
   SharedPlan plan;
   plan.own = decode_plan(p.own);
-  if (plan.own.grid > kMaxOwn) plan.own.grid = kMaxOwn;
-  plan.own.grid = (plan.own.grid + 7) / 8 * 8;  // (the prefix's workgroups keep their XCDs)
+  // runs of waves: two for each SIMD
+  const int64_t units = p.own.batch * p.own.kv_heads * plan.own.head_items * (plan.own.most_tiles + kItemUnits);
+  const int64_t runs = (units + kWaves - 1) / kWaves, most_runs = 8 * static_cast<int64_t>(cu_count());
+  plan.own.grid = static_cast<int>(runs < most_runs ? runs : most_runs < kMaxRuns ? most_runs : kMaxRuns);
   const int64_t rows = p.own.batch * (p.own.query_heads / p.own.kv_heads);
   // tiles of at most 128 rows, all alike, of whole waves
   plan.row_tiles = static_cast<int>((rows + 127) / 128);
   plan.tile_rows = rows <= 16 ? 16 : static_cast<int>((rows + 32 * plan.row_tiles - 1) / (32 * plan.row_tiles) * 32);
   if (plan.row_tiles > 0) plan.row_tiles = static_cast<int>((rows + plan.tile_rows - 1) / plan.tile_rows);
   const int64_t tiles = (p.prefix_table_width * p.prefix_page_size + kTileKeys - 1) / kTileKeys;
+  // (workgroups a CU)
   const int64_t per = p.own.head_dim > 128 ? 1 : 2;
   int64_t splits = per * cu_count() / (p.own.kv_heads * (plan.row_tiles > 0 ? plan.row_tiles : 1));
   const int64_t most = (tiles + kWaves - 1) / kWaves;
@@ -720,8 +864,7 @@ int64_t shared_bytes(const fpv2_shared_prefix_params& p, const SharedPlan& plan)
 template <typename T, int D>
 int launch(const PrefixArgs& p, const DecodeArgs& a, hipStream_t s) {
   const unsigned units = static_cast<unsigned>(p.kv_heads) * p.splits;
-  constexpr int kThreads = 64 * Stage<D>::kWaves;
-  const dim3 few(a.grid + units), many((kThreads == 256 ? a.grid : 0) + (units + 7) / 8 * 8 * p.row_tiles);
+  const dim3 few(p.own_blocks + units), many(p.own_blocks + (units + 7) / 8 * 8 * p.row_tiles);
   // (offsets within 16 rows are 32 bits)
   const bool halves = (p.table == nullptr || p.page_size % 16 == 0) && p.k_rs < (1 << 25) && p.v_rs < (1 << 25);
   if (p.rows <= 16 && halves)
@@ -729,11 +872,9 @@ int launch(const PrefixArgs& p, const DecodeArgs& a, hipStream_t s) {
   else if (p.rows <= 16)
     hipLaunchKernelGGL((prefix_few_kernel<T, D, false>), few, dim3(256), 0, s, p, a);
   else if (halves)
-    hipLaunchKernelGGL((prefix_many_kernel<T, D, true>), many, dim3(kThreads), 0, s, p, a);
+    hipLaunchKernelGGL((prefix_many_kernel<T, D, true>), many, dim3(64 * Stage<D>::kWaves), 0, s, p, a);
   else
-    hipLaunchKernelGGL((prefix_many_kernel<T, D, false>), many, dim3(kThreads), 0, s, p, a);
-  if constexpr (kThreads != 256)
-    if (p.rows > 16) hipLaunchKernelGGL((decode_attn_kernel<T, D, true>), dim3(a.grid), dim3(256), 0, s, a);
+    hipLaunchKernelGGL((prefix_many_kernel<T, D, false>), many, dim3(64 * Stage<D>::kWaves), 0, s, p, a);
   if (const int rc = check_launch("prefix_many_kernel")) return rc;
   const unsigned heads = static_cast<unsigned>(a.batch) * a.kv_heads * a.group;
   if (heads < 1024)
@@ -832,6 +973,9 @@ extern "C" int fpv2_shared_prefix_attention(const void* q, const void* prefix_k,
   x.row_tiles = plan.row_tiles;
   x.tile_rows = plan.tile_rows;
   x.splits = plan.splits;
+  // (of 4 or 8 waves; a multiple of 8, so that the prefix's workgroups keep their XCDs)
+  const int waves = x.rows > 16 && p.own.head_dim > 128 ? 8 : 4;
+  x.own_blocks = (plan.own.grid + 8 * waves - 1) / (8 * waves) * 8;
   x.pages = static_cast<int>(p.prefix_pages);
   x.page_size = static_cast<int>(p.prefix_page_size);
   x.capacity = static_cast<int>(p.prefix_table_width * p.prefix_page_size);

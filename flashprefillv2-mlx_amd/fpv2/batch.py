@@ -275,18 +275,17 @@ def quantize_to_pages(k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor | in
         tensors.append(slots)
     # (what is read lies apart from what is written)
     firsts = [x.data_ptr() for x in tensors]
-    for x, first in zip(tensors, firsts):
+    _, _, a, b, c, d = firsts[:6]
+    size = codes.bytes
+    a_end, b_end, c_end, d_end = a + size[0], b + size[1], c + size[2], d + size[3]
+    for x in tensors if slots is None else (k, v, slots):
         if x is k_codes:
             break
-        end = first + 2 * _extent(shape, x.stride())
-        for cache, at, size in zip(tensors[2:6], firsts[2:6], codes.bytes):
-            if first < at + size and at < end and _share_memory(cache, x):
-                raise ValueError("the caches must not share memory with what the call reads")
-    if slots is not None:
-        first, end = firsts[6], firsts[6] + slot_bytes * tokens
-        for cache, at, size in zip(tensors[2:6], firsts[2:6], codes.bytes):
-            if first < at + size and at < end and _share_memory(cache, slots):
-                raise ValueError("the caches must not share memory with what the call reads")
+        first = x.data_ptr()
+        end = first + x.element_size() * _extent(x.shape, x.stride())
+        if ((first < a_end and a < end or first < b_end and b < end or first < c_end and c < end
+                or first < d_end and d < end) and any(_share_memory(cache, x) for cache in tensors[2:6])):
+            raise ValueError("the caches must not share memory with what the call reads")
     index = _device(tensors)
     if tokens == 0:
         return
@@ -339,7 +338,11 @@ def dequantize_pages(k_codes: torch.Tensor, k_scales: torch.Tensor, v_codes: tor
     if page_table is None and pages < batch:
         raise ValueError("without a page_table every sequence needs a page")
     lengths, length = _lengths(lengths, batch, width * page_size)
-    tensors = [x for x in (k_codes, k_scales, v_codes, v_scales, page_table, lengths) if x is not None]
+    tensors = [k_codes, k_scales, v_codes, v_scales]
+    if page_table is not None:
+        tensors.append(page_table)
+    if lengths is not None:
+        tensors.append(lengths)
     if out is None:
         tokens = width * page_size if tokens is None else _count(tokens, "tokens")
         dtype = torch.bfloat16 if dtype is None else dtype
@@ -359,12 +362,14 @@ def dequantize_pages(k_codes: torch.Tensor, k_scales: torch.Tensor, v_codes: tor
     index = _device(tensors)
     zero_rest = out is None
     if out is None:
-        out = tuple(torch.empty((batch, kv_heads, tokens, dim), dtype=dtype, device=k_codes.device)
-                    for _ in "kv")
+        shape, device = (batch, kv_heads, tokens, dim), k_codes.device
+        out = (torch.empty(shape, dtype=dtype, device=device), torch.empty(shape, dtype=dtype, device=device))
+        strides = 2 * (kv_heads * tokens * dim, tokens * dim, dim)
+    else:
+        strides = (*_row_strides(out[0]), *_row_strides(out[1]))
     if batch == 0 or tokens == 0:
         return out
-    params, ref = _read_params(codes, batch, width, table_stride, 0, tokens, zero_rest,
-                               *_row_strides(out[0]), *_row_strides(out[1]))
+    params, ref = _read_params(codes, batch, width, table_stride, 0, tokens, zero_rest, *strides)
     if length:
         params = _lib.DequantizeParams.from_buffer_copy(params)
         params.length = length

@@ -21,7 +21,9 @@ and storing bf16.
 
 ``ChunkedPrefillRunner.decode`` goes on token by token over the prefill's caches
 and ``generate`` samples the tokens (``fpv2.decode``; the reference leaves both to
-mlx-lm, ``fpv2/generate.py:97-130``).  With ``RandomDecoder.quantize`` the decode
+mlx-lm, ``fpv2/generate.py:97-130``).  ``generate_many`` samples several
+continuations of one prompt at once, whose keys stay in the prefill's caches, and
+``score`` gives the log probabilities of a text's own tokens (``fpv2.batch``).  With ``RandomDecoder.quantize`` the decode
 steps read 4-bit weights, as the reference's MLX models do, and the prefill, which
 is bound by arithmetic, the dense weights of the same values.
 """
@@ -36,6 +38,7 @@ import torch
 import torch.nn.functional as F
 
 from fpv2 import _lib
+from fpv2.batch import shared_prefix_attention, token_logprobs
 from fpv2.chunked import ChunkedPrefill
 from fpv2.decode import (GROUP_SIZES, MAX_VOCAB, _device as check_device, _settings,
                          decode_attention, dequantize_weight, quantize_weight, quantized_linear,
@@ -355,9 +358,9 @@ class ChunkedPrefillRunner:
         act = _silu_mul(F.linear(h, p["gate_up"]), s.intermediate)
         return x, F.linear(act, p["down"])
 
-    def prefill(self, tokens: torch.Tensor, chunk: int) -> torch.Tensor:
-        """Run the prompt in ``chunk``-token pieces; returns the logits of the
-        last position (float32 ``[vocab]``)."""
+    def _chunks(self, tokens: torch.Tensor, chunk: int):
+        """Runs the prompt in ``chunk``-token pieces; yields each one's residual stream
+        ``(x, delta)`` and the position behind it."""
         m = self.model
         n = tokens.numel()
         if n > self.capacity:
@@ -368,7 +371,6 @@ class ChunkedPrefillRunner:
             # the dense tail applies on the chunk that reaches it
             for cache in self.caches:
                 cache.total_tokens = n
-        x = delta = None
         for start in range(0, n, chunk):
             end = min(start + chunk, n)
             pos = torch.arange(start, end, device=m.device)
@@ -376,6 +378,14 @@ class ChunkedPrefillRunner:
             x, delta = m.embed[tokens[start:end]], None
             for li in range(m.shape.layers):
                 x, delta = self._layer(li, x, delta, cos, sin)
+            yield x, delta, end
+
+    def prefill(self, tokens: torch.Tensor, chunk: int) -> torch.Tensor:
+        """Run the prompt in ``chunk``-token pieces; returns the logits of the
+        last position (float32 ``[vocab]``)."""
+        x = delta = None
+        for x, delta, _ in self._chunks(tokens, chunk):
+            pass
         return self._head(x[-1:], delta[-1:])
 
     def _head(self, x: torch.Tensor, delta: torch.Tensor) -> torch.Tensor:
@@ -388,6 +398,56 @@ class ChunkedPrefillRunner:
             # (rows that the kernel does not read in place, or a graph to keep)
             return F.linear(last, w).float()[0]
         return _row_logits(last[0], w)
+
+    def _angles(self, positions: int) -> tuple:
+        """cos / sin ``[positions or more, head_dim / 2]`` of a decode step's rotation."""
+        if self._tables is None or self._tables[0].shape[0] < positions:
+            pos = torch.arange(max(positions, self.capacity), device=self.model.device)
+            half = self.model.shape.head_dim // 2
+            self._tables = tuple(t[:, :half].contiguous() for t in rope_tables(self.model.shape, pos))
+        return self._tables
+
+    def _linear(self, x: torch.Tensor, li: int, name: str) -> torch.Tensor:
+        """A decode step's projection, with 4-bit weights where the model has them."""
+        m = self.model
+        if m.packed is None:
+            return F.linear(x, m.layers[li][name])
+        return quantized_linear(x, *m.packed[li][name])
+
+    def _embed(self, tokens: torch.Tensor) -> torch.Tensor:
+        """Rows of the table for int64 ``tokens`` (known on the device only: what is no row
+        of it is NaN)."""
+        embed = self.model.embed
+        row = tokens.clamp(0, embed.shape[0] - 1)
+        return torch.where((row == tokens)[:, None], embed[row], math.nan)
+
+    def _logits(self, last: torch.Tensor, dense: bool) -> torch.Tensor:
+        """float32 logits ``[rows, vocab]`` of normalised rows, by the dense head or, where the
+        model has one, the 4-bit one."""
+        m = self.model
+        if not dense and m.packed_embed is not None:
+            return quantized_linear(last, *m.packed_embed, out_dtype=torch.float32)
+        return torch.mm(last, m.embed.t(), out_dtype=torch.float32)
+
+    def score(self, tokens: torch.Tensor, chunk: int) -> torch.Tensor:
+        """Log probabilities (float32 ``[n - 1]``) of a text's tokens after its first one, each
+        given the ones before it: the text is prefilled in ``chunk``-token pieces, whose
+        attention is the runner's, into the caches, which have to be empty.  Tokens as in
+        ``prefill`` (of the vocabulary); a text of one token has no score."""
+        m, n = self.model, tokens.numel()
+        if tokens.ndim != 1 or n == 0 or chunk <= 0:
+            raise ValueError("score needs a text [tokens] and a positive chunk")
+        if any(cache.length for cache in self.caches):
+            raise ValueError("score starts from empty caches: call reset() first")
+        out, rows = [], 512  # rows whose logits are held at a time
+        for x, delta, end in self._chunks(tokens, chunk):
+            last = _add_rms_norm(x, delta, m.final_norm, m.shape.rms_eps)
+            start = end - last.shape[0]
+            for a in range(start, min(end, n - 1), rows):
+                b = min(a + rows, end, n - 1)
+                logits = self._logits(last[a - start:b - start], dense=True)
+                out.append(token_logprobs(logits, tokens[a + 1:b + 1].contiguous()).logprobs)
+        return torch.cat(out) if out else torch.empty(0, device=m.device)
 
     def decode(self, token: torch.Tensor) -> torch.Tensor:
         """Append one token (an integer tensor of one element on the model's device)
@@ -406,26 +466,15 @@ class ChunkedPrefillRunner:
             raise ValueError("decode needs a prefilled prompt")
         if position >= self.capacity:
             raise ValueError("the KV cache capacity is exceeded")
-        if self._tables is None:
-            pos = torch.arange(self.capacity, device=m.device)
-            half = s.head_dim // 2
-            self._tables = tuple(t[:, :half].contiguous() for t in rope_tables(s, pos))
-
-        def linear(x, li, name):
-            if m.packed is None:
-                return F.linear(x, m.layers[li][name])
-            return quantized_linear(x, *m.packed[li][name])
-
-        # (the token is known on the device only: what is no row of the table is NaN)
-        token = token.reshape(1).to(m.embed.device, torch.int64)
-        row = token.clamp(0, m.embed.shape[0] - 1)
-        x, delta = torch.where((row == token)[:, None], m.embed[row], math.nan), None
+        tables = self._angles(self.capacity)
+        linear = self._linear
+        x, delta = self._embed(token.reshape(1).to(m.embed.device, torch.int64)), None
         try:
             for li, (p, cache) in enumerate(zip(m.layers, self.caches)):
                 h = _add_rms_norm(x, delta, p["attn_norm"], s.rms_eps)
                 k_pages, v_pages = cache.pages()
                 cache.reserve(1)
-                q = rope_to_pages(linear(h, li, "qkv"), p["q_norm"], p["k_norm"], *self._tables,
+                q = rope_to_pages(linear(h, li, "qkv"), p["q_norm"], p["k_norm"], *tables,
                                   position, position, k_pages, v_pages, query_heads=s.query_heads,
                                   eps=s.rms_eps)
                 attn = decode_attention(q, k_pages, v_pages, None, cache.length)
@@ -477,6 +526,71 @@ class ChunkedPrefillRunner:
             out.append(sample_tokens(logits[None], uniform[i:i + 1], temperature=temperature,
                                      top_k=top_k, top_p=top_p, min_p=min_p))
         return torch.cat(out)
+
+
+    def generate_many(self, tokens: torch.Tensor, chunk: int, new_tokens: int, samples: int, *,
+                      temperature: float = 1.0, top_k: int = 0, top_p: float = 1.0,
+                      min_p: float = 0.0, uniform: torch.Tensor | None = None):
+        """``samples`` continuations of one prompt at once: int64 tokens ``[samples,
+        new_tokens]`` and the model's float32 log probabilities of them (without
+        temperature and filters: their sums rank the continuations).
+
+        The prompt is prefilled as in ``generate`` and its keys stay in the runner's
+        caches, where each step reads them once for all samples
+        (``fpv2.shared_prefix_attention``); the new tokens' keys are in pages of the call's
+        own, so that the caches hold the prompt alone afterwards.  Settings as in
+        ``generate`` (tensors: one for each sample); ``uniform`` float32 ``[samples,
+        new_tokens]``.  A sample goes on with -1 and -inf after a row of nothing."""
+        m, s = self.model, self.model.shape
+        for value, name in ((new_tokens, "new_tokens"), (samples, "samples")):
+            if isinstance(value, bool) or not isinstance(value, int) or value <= 0:
+                raise ValueError(f"{name} must be a positive integer")
+        # (what could be refused is looked at before the prompt is prefilled)
+        if self.attention == "sdpa":
+            raise ValueError("generate_many goes on over the caches of 'fpv2' or 'dense'")
+        settings = [rows for rows, _ in _settings(temperature, top_k, top_p, min_p, samples)
+                    if rows is not None]
+        if m.embed.shape[0] > MAX_VOCAB:
+            raise ValueError(f"the vocabulary must have 1 to {MAX_VOCAB} tokens")
+        if tokens.numel() == 0 or chunk <= 0:
+            raise ValueError("generate_many needs a prompt and a positive chunk")
+        if any(cache.length for cache in self.caches):
+            raise ValueError("generate_many starts from empty caches: call reset() first")
+        if uniform is None:
+            uniform = torch.rand((samples, new_tokens), device=m.device)
+        elif (uniform.shape != (samples, new_tokens) or uniform.dtype != torch.float32
+              or uniform.device != m.embed.device):
+            raise ValueError("uniform must be float32 [samples, new_tokens] on the model's device")
+        check_device([uniform, *settings])
+        uniform = uniform.t().contiguous()
+        n = tokens.numel()
+        logits = self.prefill(tokens, chunk).expand(samples, -1)
+        own = [[torch.empty((samples, s.kv_heads, new_tokens, s.head_dim), dtype=m.dtype, device=m.device)
+                for _ in "kv"] for _ in m.layers]
+        tables = self._angles(n + new_tokens)
+        slots = torch.arange(samples, device=m.device) * new_tokens
+        out, logprobs = [], []
+        for i in range(new_tokens):
+            if i > 0:
+                logits = self._step_many(out[-1], n, i - 1, own, tables, slots)
+            out.append(sample_tokens(logits, uniform[i], temperature=temperature, top_k=top_k, top_p=top_p,
+                                     min_p=min_p))
+            logprobs.append(token_logprobs(logits, out[-1]).logprobs)
+        return torch.stack(out, 1), torch.stack(logprobs, 1)
+
+    def _step_many(self, tokens, n, i, own, tables, slots) -> torch.Tensor:
+        """The logits after each sample's ``i``-th new token, of a prompt of ``n``."""
+        m, s = self.model, self.model.shape
+        x, delta = self._embed(tokens), None
+        positions, slots = torch.full_like(tokens, n + i), slots + i
+        for li, (p, cache, pages) in enumerate(zip(m.layers, self.caches, own)):
+            h = _add_rms_norm(x, delta, p["attn_norm"], s.rms_eps)
+            q = rope_to_pages(self._linear(h, li, "qkv"), p["q_norm"], p["k_norm"], *tables, positions,
+                              slots, *pages, query_heads=s.query_heads, eps=s.rms_eps)
+            attn = shared_prefix_attention(q, *cache.pages(), None, n, *pages, None, i + 1)
+            h = _add_rms_norm(x, self._linear(attn.view(len(tokens), -1), li, "o"), p["mlp_norm"], s.rms_eps)
+            delta = self._linear(_silu_mul(self._linear(h, li, "gate_up"), s.intermediate), li, "down")
+        return self._logits(_add_rms_norm(x, delta, m.final_norm, s.rms_eps), dense=False)
 
 
 def measure(shape: DecoderShape, *, tokens: int, chunk: int, alpha: float, device,

@@ -9,7 +9,10 @@
 // codes (x = a / 2 is) means 127 x / a is so exactly, so the quotients have to be rounded
 // correctly: with y = 1 / a rounded, q = n y, q + (n - q a) y is (a is not all ones).
 //
-// Both are bound by memory: 3 bytes a value.
+// Both are bound by memory, 3 bytes a value.  8 heads of D = 128: 32768 tokens written in 35 us, read
+// in 31 (201 MB, 5.8 and 6.6 TB/s, where the caches hold some of it), 131072 tokens 165 and 164 (4.9 TB/s);
+// a few tokens 3.1 and 3.3, a launch.  The greatest magnitude by pairs of bits instead of
+// floats, and the codes by one sum: 97 us to 71 where 24 sequences' prompts are written.
 #include "fpv2_batch.h"
 #include "fpv2_common.h"
 
@@ -220,7 +223,8 @@ int launch_quantize(const QuantArgs& a, hipStream_t s) {
   return check_launch("quantize_kernel");
 }
 
-// Many rows: several of a token in turn.
+// Many rows: several of a token in turn.  8 heads of D = 128, four rows in turn / one: 512 tokens 4.7 / 3.7
+// us, 2048 (2^14 rows) 5.6 / 5.8, 32768 35 / 41, 131072 165 / 185.
 template <typename T, int D>
 int launch_rows(const QuantArgs& a, hipStream_t s) {
   return a.kv_heads > 1 && static_cast<int64_t>(a.tokens) * a.kv_heads >= 1 << 14 ? launch_quantize<T, D, 4>(a, s)
@@ -237,10 +241,12 @@ int launch_turns(const ReadArgs& a, int batch, hipStream_t s) {
   return check_launch("dequantize_kernel");
 }
 
-// Results that no cache holds (2^25 bytes and more of K and of V each).
+// Results of which few stay in the L2s (2^23 bytes and more of K and of V each).  8 heads of
+// D = 128, four turns / one: 512 tokens 4.4 / 3.6 us, 2048 5.3 / 5.5, 4096 (2^22 values) 5.9 / 7.8,
+// 32768 31 / 38, 131072 164 / 229.
 template <typename T, int D>
 int launch_dequantize(const ReadArgs& a, int batch, hipStream_t s) {
-  return static_cast<int64_t>(a.tokens) * batch * a.kv_heads * D >= 1 << 24 ? launch_turns<T, D, 4>(a, batch, s)
+  return static_cast<int64_t>(a.tokens) * batch * a.kv_heads * D >= 1 << 22 ? launch_turns<T, D, 4>(a, batch, s)
                                                                             : launch_turns<T, D, 1>(a, batch, s);
 }
 

@@ -15,6 +15,12 @@
 //   float16 relative to 2^-15 of the tile's greatest such weight (a tile 2^-40 and more
 //   below the greatest so far: of 2^-40 of that one), so that neither the scores' range nor
 //   the values' sizes cost bits.  The sum of the p_t is of unrounded ones.
+//
+// Measured (32 / 8 heads, D = 128): one sequence of 131072 keys 56 us, 4.9 TB/s of codes and scales,
+// where 16-bit keys take 95; 32 sequences of 61 to 16001 keys 47; 1000 keys 7.5 us.  A byte costs
+// four times the instructions of the 16-bit attention's, which fill what the reads leave.
+// Without gain: loads a tile ahead (58.6 us), three and four workgroups a CU (58, 65); codes with
+// their offset of 128 taken off the sums afterwards (55 us, but sums that cancel lose bits).
 #include "fpv2_batch.h"
 #include "fpv2_decode_split.h"
 

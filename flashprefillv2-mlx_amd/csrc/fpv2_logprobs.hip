@@ -11,7 +11,9 @@
 // wave collects the keys above a floor in 64 slots and, when these are full, sorts them
 // and keeps the first.  The floor of its first logits is the greatest number that enough
 // lanes' maxima reach, so that few more than the wanted ones are collected at all.
-// Bound by reading the logits.
+// Bound by reading the logits: 1536 bfloat16 rows of 151936 84 us, 5.5 TB/s; few rows by two launches
+// and their chains: one float32 row of 151936 with 20 alternatives 8.8 + 5.4 us (34.7 + 21 with the
+// keys collected from none on), 160 float16 rows of 50001 with 5 15.0 + 5.7.
 #include "fpv2_batch.h"
 #include "fpv2_common.h"
 

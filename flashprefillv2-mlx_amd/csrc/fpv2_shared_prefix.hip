@@ -9,8 +9,21 @@
 // Two launches: workgroups of the own keys and of the prefix, then the join.
 //
 // Prefix: the rows of a KV head are the batch's query heads of it, packed; a workgroup
-// takes a tile of them and a part of the prefix's keys.  Its waves take 32 keys each on
-// MFMA, as the decode attention does, for all rows of the tile.
+// takes a tile of them and a part of the prefix's keys, on MFMA: S^T = K Q^T and O^T += V^T P^T,
+// so that a lane's scores are its operand of the second product as they are.  Up to 16 rows
+// are one tile of MFMA and the reads of the keys bound it: its waves take 32 keys each straight
+// from memory, as the decode attention does.  Of more rows each key serves several waves, which
+// share it through LDS; MFMA, the exponentials beside it and the partials bound that.
+//
+// Measured (bfloat16, 32 / 8 heads, D = 128, 16 own keys a sequence): a prefix of 131072 keys,
+// 4 sequences 99 us, 5.4 TB/s; 32768 keys, 4 sequences 29 us, 40 sequences 52 us; 8192
+// keys, 128 sequences 38 us.  With the length the time grows by 6.1 TB/s of keys at 8
+// sequences, 3.8 TB/s at 40, 864 TFLOP/s at 128; the rest of a call is a launch, 0.5 us for each
+// MB of partials (10 to 33), some 10 us where the own keys are hundreds a sequence, and the
+// join's 5.5 to 10 us.
+// Without gain: workgroups of 8 waves in two groups of keys that join in LDS (half the partials,
+// but a barrier of 8 waves: 128 sequences 3 us more), three stages in registers on their way,
+// partials past the caches (1.5 us less here, 1.5 more in the join).
 #include "fpv2_batch.h"
 #include "fpv2_decode_split.h"
 
@@ -49,7 +62,7 @@ __device__ __forceinline__ int prefix_length(const PrefixArgs& a) {
 // greatest so far, so that no float32 sum overflows).  So weights down to 2^-19 of their
 // tile's greatest keep their bits, whatever lies above that tile, and smaller ones are off by
 // 2^-30 of it.  (2^-15 instead of 2^-12: most tiles have a column that exceeds it, 128
-// sequences of an 8191-key prefix 41 us instead of @.)
+// sequences of an 8191-key prefix 41 us instead of 38.)
 constexpr float kLag = 8.f, kMost = 15.9f, kLeast = 5.f, kHeadroom = 12.f, kBelow = 40.f;
 constexpr float kNone = -3e38f;  // the reference before any score: below all of them
 
@@ -160,33 +173,11 @@ struct Tile {
   Words<D / 32> v[8];
 };
 
-template <int NW>
-__device__ __forceinline__ Words<NW> buf_load_words(rsrc_t r, uint32_t off, uint32_t base) {
-  Words<NW> x;
-  if constexpr (NW % 4 == 0) {
-#pragma unroll
-    for (int i = 0; i < NW / 4; ++i) {
-      const u32x4 w = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(r, off + 16 * i, base, 0));
-#pragma unroll
-      for (int j = 0; j < 4; ++j) x.w[4 * i + j] = w[j];
-    }
-  } else if constexpr (NW == 2) {
-    const u32x2 w = __builtin_bit_cast(u32x2, __builtin_amdgcn_raw_buffer_load_b64(r, off, base, 0));
-    x.w[0] = w[0];
-    x.w[1] = w[1];
-  } else {
-#pragma unroll
-    for (int i = 0; i < NW; ++i) x.w[i] = __builtin_amdgcn_raw_buffer_load_b32(r, off + 4 * i, base, 0);
-  }
-  return x;
-}
-
-// HALVES: 16 keys from a multiple of 16 on lie in one page (or there is no table): their
-// addresses are the wave's, a lane's offsets do not change, and a descriptor of the rows
-// up to the prefix's end reads zeros behind it.
 // Own keys: the decode attention's schedule (fpv2_decode_split.h) with runs of waves instead of
 // workgroups, as they are short: a wave takes its items' tiles one after the other and
-// leaves a partial of each, a whole item's behind the runs' slots.
+// leaves a partial of each, a whole item's behind the runs' slots.  (By workgroups whose waves
+// join in LDS: 128 sequences of an 8191-key prefix 52 us, by waves 50; 40 of 32768 keys 64 and 65; at head
+// dim 256, where the prefix's workgroups have 8 waves, a launch of their own, 28 + 13 us, and 43 in one.)
 template <typename T, int D>
 __device__ __forceinline__ void own_attn(const DecodeArgs& a, int run) {
   constexpr int KK = D / 32, DV = D / 16;
@@ -315,7 +306,7 @@ struct FewShared {
   float o[4][16][D + 4];
   float ml[4][16][2];
 };
-template <typename T, int D, bool HALVES>
+template <typename T, int D>
 __device__ __forceinline__ void prefix_few(const PrefixArgs& a, int block, FewShared<D>& sh) {
   constexpr int KK = D / 32, DV = D / 16;
   auto& sh_o = sh.o;
@@ -332,50 +323,26 @@ __device__ __forceinline__ void prefix_few(const PrefixArgs& a, int block, FewSh
 
   const uint16_t* kb = a.k + kvh * a.k_hs;
   const uint16_t* vb = a.v + kvh * a.v_hs;
-  const uint32_t k_lane = (col * static_cast<uint32_t>(a.k_rs) + 8 * quad) * 2;
-  const uint32_t v_lane = (4 * quad * static_cast<uint32_t>(a.v_rs) + DV * col) * 2;
-  At half[2];  // HALVES: of the next tile's first and 17th key
-  int row = 0, page = 0;  // else: lane i's (and i + 32's) of its key i
+  int row = 0, page = 0;  // lane i's (and i + 32's) of the next tile's key i
   const auto look_up = [&](int u0) {
-    if constexpr (HALVES) {
-#pragma unroll
-      for (int t = 0; t < 2; ++t) half[t] = prefix_at(a, u0 + 16 * t < n ? u0 + 16 * t : 0);
-    } else {
-      const uint32_t t = min(u0 + (lane & 31), n - 1);
-      const uint32_t at = (__umulhi(t, a.page_mul) + t) >> a.page_shift;
-      row = t - at * a.page_size;
-      const int id = a.table != nullptr ? a.table[at] : 0;
-      page = min(max(id, 0), a.pages - 1);
-    }
+    const uint32_t t = min(u0 + (lane & 31), n - 1);
+    const uint32_t at = (__umulhi(t, a.page_mul) + t) >> a.page_shift;
+    row = t - at * a.page_size;
+    const int id = a.table != nullptr ? a.table[at] : 0;
+    page = min(max(id, 0), a.pages - 1);
   };
-  const auto load = [&](Tile<D>& x, int u0) {
-    if constexpr (HALVES) {
+  const auto load = [&](Tile<D>& x) {
+    const int64_t koff = page * a.k_ps + row * a.k_rs;
+    const int64_t voff = page * a.v_ps + row * a.v_rs;
 #pragma unroll
-      for (int t = 0; t < 2; ++t) {
-        const int live = min(n - u0 - 16 * t, 16);  // (0 and less: zeros)
-        const rsrc_t kr = make_rsrc(kb + page_of(a, half[t].id) * a.k_ps + half[t].row * a.k_rs,
-                                    live > 0 ? ((live - 1) * a.k_rs + D) * 2 : 0);
-        const rsrc_t vr = make_rsrc(vb + page_of(a, half[t].id) * a.v_ps + half[t].row * a.v_rs,
-                                    live > 0 ? ((live - 1) * a.v_rs + D) * 2 : 0);
+    for (int t = 0; t < 2; ++t) {
+      const uint16_t* p = kb + __shfl(koff, 16 * t + col, 64) + 8 * quad;
 #pragma unroll
-        for (int kk = 0; kk < KK; ++kk) x.k[t][kk] = buf_load16(kr, k_lane + 64 * kk);
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-          x.v[4 * t + j] = buf_load_words<DV / 2>(vr, v_lane, j * static_cast<uint32_t>(a.v_rs) * 2);
-      }
-    } else {
-      const int64_t koff = page * a.k_ps + row * a.k_rs;
-      const int64_t voff = page * a.v_ps + row * a.v_rs;
-#pragma unroll
-      for (int t = 0; t < 2; ++t) {
-        const uint16_t* p = kb + __shfl(koff, 16 * t + col, 64) + 8 * quad;
-#pragma unroll
-        for (int kk = 0; kk < KK; ++kk) x.k[t][kk] = load16(p + 32 * kk);
-      }
-#pragma unroll
-      for (int j = 0; j < 8; ++j)
-        x.v[j] = load_words<DV / 2>(vb + __shfl(voff, 16 * (j / 4) + 4 * quad + j % 4, 64) + DV * col);
+      for (int kk = 0; kk < KK; ++kk) x.k[t][kk] = load16(p + 32 * kk);
     }
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      x.v[j] = load_words<DV / 2>(vb + __shfl(voff, 16 * (j / 4) + 4 * quad + j % 4, 64) + DV * col);
   };
 
   const float scale = fmaxf(__builtin_fabsf(a.scale_log2), 1e-30f);
@@ -396,7 +363,7 @@ __device__ __forceinline__ void prefix_few(const PrefixArgs& a, int block, FewSh
     }
     const u32x4 pf = weigh<T>(
         relate<T>(sc, scale, n - u0 < kTileKeys ? n - u0 - 4 * quad : kTileKeys, m, l, greatest, o), l);
-    if (!HALVES && u0 + kTileKeys > n) {
+    if (u0 + kTileKeys > n) {
       // (a zero weight would make NaN of what an unused row may hold)
 #pragma unroll
       for (int j = 0; j < 8; ++j)
@@ -417,20 +384,20 @@ __device__ __forceinline__ void prefix_few(const PrefixArgs& a, int block, FewSh
   };
 
   // A tile's loads are a tile ahead of its products, and its pages one more.  (Tiles behind
-  // the last one are loaded too, HALVES: as zeros, else the last key again; so that it is
-  // known at each product how many loads were issued since its own.)
+  // the last one are loaded too, as the last key again, so that it is known at each product
+  // how many loads were issued since its own.)
   int u0 = (first + wave) * kTileKeys;
   const int u_end = min(n, last * kTileKeys);
   if (u0 < u_end) {
     Tile<D> even, odd;
     look_up(u0);
-    load(even, u0);
+    load(even);
     look_up(u0 + kStepKeys);
     for (; u0 < u_end; u0 += 2 * kStepKeys) {
-      load(odd, u0 + kStepKeys);
+      load(odd);
       look_up(u0 + 2 * kStepKeys);
       multiply(even, u0);
-      load(even, u0 + 2 * kStepKeys);
+      load(even);
       look_up(u0 + 3 * kStepKeys);
       if (u0 + kStepKeys < u_end) multiply(odd, u0 + kStepKeys);
     }
@@ -470,14 +437,14 @@ __device__ __forceinline__ void prefix_few(const PrefixArgs& a, int block, FewSh
   }
 }
 
-template <typename T, int D, bool HALVES>
+template <typename T, int D>
 __global__ __launch_bounds__(256, D > 128 ? 1 : 2) void prefix_few_kernel(PrefixArgs p, DecodeArgs a) {
   __shared__ FewShared<D> sh;
   const int block = static_cast<int>(blockIdx.x) - p.own_blocks;
   if (block < 0)
     own_attn<T, D>(a, blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6));
   else
-    prefix_few<T, D, HALVES>(p, block, sh);
+    prefix_few<T, D>(p, block, sh);
 }
 
 // More rows than a tile of MFMA: the workgroup's waves, 32 rows each (at head dim 256, whose
@@ -506,7 +473,11 @@ typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
 // its loads from memory (as __syncthreads() does).
 __device__ __forceinline__ void barrier_lds() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 
-// HALVES: as above.
+// HALVES: 16 keys from a multiple of 16 on lie in one page (or there is no table): their
+// addresses are the wave's, a lane's offsets do not change, and a descriptor of the rows
+// up to the prefix's end reads zeros behind it.  128 sequences, 8192 keys: 37.3 us, with each
+// lane's own page and row 42.6; 40 sequences, 32768 keys in pages of 64: 52 and 77.  (Up to 16
+// rows the same either way, so that has the lanes' own alone.)
 template <typename T, int D, bool HALVES>
 __device__ __forceinline__ void prefix_many(const PrefixArgs& a, int block, uint8_t (&sh)[3][2 * Stage<D>::kMatrix]) {
   using S = Stage<D>;
@@ -867,17 +838,22 @@ int launch(const PrefixArgs& p, const DecodeArgs& a, hipStream_t s) {
   const dim3 few(p.own_blocks + units), many(p.own_blocks + (units + 7) / 8 * 8 * p.row_tiles);
   // (offsets within 16 rows are 32 bits)
   const bool halves = (p.table == nullptr || p.page_size % 16 == 0) && p.k_rs < (1 << 25) && p.v_rs < (1 << 25);
-  if (p.rows <= 16 && halves)
-    hipLaunchKernelGGL((prefix_few_kernel<T, D, true>), few, dim3(256), 0, s, p, a);
-  else if (p.rows <= 16)
-    hipLaunchKernelGGL((prefix_few_kernel<T, D, false>), few, dim3(256), 0, s, p, a);
+  // (16 rows: 32768 keys 29 us by few, 35 by many; 131072 keys, one sequence 96 and 105; 1000 keys 7.6
+  // and 9.4)
+  if (p.rows <= 16)
+    hipLaunchKernelGGL((prefix_few_kernel<T, D>), few, dim3(256), 0, s, p, a);
   else if (halves)
     hipLaunchKernelGGL((prefix_many_kernel<T, D, true>), many, dim3(64 * Stage<D>::kWaves), 0, s, p, a);
   else
     hipLaunchKernelGGL((prefix_many_kernel<T, D, false>), many, dim3(64 * Stage<D>::kWaves), 0, s, p, a);
-  if (const int rc = check_launch("prefix_many_kernel")) return rc;
+  if (const int rc = check_launch("prefix_kernel")) return rc;
   const unsigned heads = static_cast<unsigned>(a.batch) * a.kv_heads * a.group;
-  if (heads < 1024)
+  // Few heads of many partials have four waves each.  64 partials: 192 heads 6.6 us by four waves, 9.2
+  // by one; 512 heads 7.7 and 9.4; 768 heads 9.4 either way; 1536 heads 9.8 and 8.6.  32 partials and less:
+  // the same up to 768 heads (6.2 .. 7.2), 1536 heads 9.9 and 8.5.  A wave takes 64 / (D / 4) partials at a
+  // time: 32 of D = 256, 128 heads 6.5 and 8.9.
+  constexpr int kAtOnce = 64 / (D / 4);
+  if (heads < 1024 && p.splits + a.grid / (a.batch * a.kv_heads * a.head_items) > 24 * kAtOnce)
     hipLaunchKernelGGL((shared_join_kernel<T, D, 4>), dim3(heads), dim3(256), 0, s, p, a);
   else
     hipLaunchKernelGGL((shared_join_kernel<T, D, 1>), dim3((heads + 3) / 4), dim3(256), 0, s, p, a);

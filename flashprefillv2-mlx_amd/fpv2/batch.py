@@ -321,7 +321,7 @@ def dequantize_pages(k_codes: torch.Tensor, k_scales: torch.Tensor, v_codes: tor
     ``decode_attention`` (``None`` and an integer: sequence ``b`` is page ``b``, for all
     pages, or for ``out``'s batch).  ``tokens`` rows of each sequence are read (by default as many
     as its pages hold), code times scale rounded once to ``dtype`` (bfloat16 by default, or
-    ``out``'s).  Rows behind a sequence's length are zeros, or left as they are in ``out``, a pair
+    ``out``'s); sequences times heads are at most 65535.  Rows behind a sequence's length are zeros, or left as they are in ``out``, a pair
     of destinations with 16-byte aligned rows, apart from one another and from all operands:
     the caches of a ``ChunkedPrefill`` that goes on are ``out=cp.pages()``.
     """
@@ -404,7 +404,8 @@ def quantized_decode_attention(q: torch.Tensor, k_codes: torch.Tensor, k_scales:
 
     The cache as in ``quantize_to_pages``, all else as in ``decode_attention``.  The
     codes are exact in the products; a query's values below 2^-14 of its greatest one are
-    rounded to 2^-25 of it, the weights times the values' scales to float16 of 11 bits.
+    rounded to 2^-25 of it, the weights times the values' scales to float16 of 11 bits (products
+    below 2^-111, where the greatest score's weight is 1, may count as 0).
     """
     codes = _code_pages(k_codes, k_scales, v_codes, v_scales)
     pages, kv_heads, page_size, page_dim = codes.shape

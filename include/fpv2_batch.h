@@ -36,8 +36,9 @@ typedef struct fpv2_shared_prefix_params {
  * t % prefix_page_size of page prefix_table[t / prefix_page_size] (int32; without
  * prefix_table of page 0); a sequence's own tokens as in fpv2_decode_attention.
  * Page ids and lengths are clipped as there; a sequence with no keys at all gives
- * zeros.  Weights are rounded to the inputs' type for their product with v (f16:
- * relative to 2^-15 of the greatest of 32 keys), their sum is not.  The prefix's
+ * zeros.  Weights are rounded to the inputs' type for their product with v, their sum is
+ * not (f16: weights down to 2^-19 of the greatest of their 32 keys to 11 bits, smaller ones
+ * to 2^-30 of it).  At most 2^24 - 1 query heads of the batch.  The prefix's
  * strides are multiples of 8 and its pointers 16-byte aligned; its pages may be of
  * the sequences' own pool.  workspace: fpv2_shared_prefix_attention_workspace_bytes
  * bytes, 16-byte aligned, not kept between calls; calls that share one on
@@ -103,7 +104,7 @@ typedef struct fpv2_dequantize_params {
  * k_out[b][h][t][j] = codes[j] scale of token t of sequence b, t < min(length, tokens),
  * rounded once to bf16 or f16; likewise v_out.  Tokens, page ids and lengths as in
  * fpv2_decode_attention.  The results' strides are multiples of 8, their pointers
- * 16-byte aligned.
+ * 16-byte aligned; batch * kv_heads is at most 65535.
  */
 int fpv2_dequantize_pages(const void* k_codes, const float* k_scales, const void* v_codes,
                           const float* v_scales, const int32_t* page_table,
@@ -120,9 +121,10 @@ typedef struct fpv2_quantized_decode_params {
 /*
  * fpv2_decode_attention over the values codes[j] scale.  The codes are whole numbers and
  * exact in the products; the queries are multiplied as float16 of 11 bits, relative to a
- * power of two by their greatest, a key's scale in float32 with its score; a value's scale with its weight, which is
- * then rounded to float16, relative to 2^-15 of the greatest such product of 32 keys.  The codes'
- * strides are multiples of 16, their pointers 16-byte aligned.
+ * power of two by their greatest, a key's scale in float32 with its score; a value's scale
+ * with its weight, which is then rounded to float16, relative to 2^-15 of the greatest such
+ * product of 32 keys.  Products below 2^-111, where the greatest score's weight is 1, may
+ * count as 0.  The codes' strides are multiples of 16, their pointers 16-byte aligned.
  */
 int64_t fpv2_quantized_decode_attention_workspace_bytes(const fpv2_quantized_decode_params* params);
 int fpv2_quantized_decode_attention(const void* q, const void* k_codes, const float* k_scales,

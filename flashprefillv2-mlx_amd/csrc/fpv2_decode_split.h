@@ -143,8 +143,8 @@ __device__ __forceinline__ uint32_t runs_of(const DecodeArgs& a, int total) {
 // The first unit of a workgroup's run (runs differ by a unit at most), and the
 // workgroup that has a unit.
 __device__ __forceinline__ int first_of(const DecodeArgs& a, uint32_t w, int total) {
-  const uint32_t runs = runs_of(a, total);
-  return static_cast<int>(static_cast<uint64_t>(min(w, runs)) * static_cast<uint32_t>(total) / runs);
+  const uint32_t runs = runs_of(a, total), per = static_cast<uint32_t>(total) / runs, i = min(w, runs);
+  return static_cast<int>(i * per + i * (static_cast<uint32_t>(total) - per * runs) / runs);  // i total / runs
 }
 __device__ __forceinline__ int workgroup_of(const DecodeArgs& a, int unit, int total) {
   const uint32_t runs = runs_of(a, total);

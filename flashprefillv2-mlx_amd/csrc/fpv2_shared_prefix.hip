@@ -15,23 +15,24 @@
 // from memory, as the decode attention does.  Of more rows each key serves several waves, which
 // share it through LDS; MFMA, the exponentials beside it and the partials bound that.
 //
-// Measured (bfloat16, 32 / 8 heads, D = 128, 16 own keys a sequence): a prefix of 131072 keys,
-// 4 sequences 99 us, 5.4 TB/s; 32768 keys, 4 sequences 29 us, 40 sequences 52 us; 8192
-// keys, 128 sequences 38 us.  With the length the time grows by 6.1 TB/s of keys at 8
-// sequences, 3.8 TB/s at 40, 864 TFLOP/s at 128; the rest of a call is a launch, 0.5 us for each
-// MB of partials (10 to 33), some 10 us where the own keys are hundreds a sequence, and the
-// join's 5.5 to 10 us.
+// Measured (32 / 8 heads, D = 128; caches that change from call to call): 40 sequences of 20 to 700 own
+// keys after 32768 in pages of 64, bfloat16, 58 us + the join's 8; 128 of 5 to 300 after 8191, float16,
+// 44 + 10; 64 of up to 32 after 32768 61 + 10.5; 16 / 4 heads of D = 256, 21 of 9 to 1500 after 20011, 40 + 8.
+// Up to 16 rows 4 sequences after 32768 keys 34 + 8, one after 131072 93 + 7.5 (5.7 TB/s).  A launch takes
+// some 5 us of these, and each MB of partials (10 to 33 of them) half a microsecond.
 // Without gain: workgroups of 8 waves in two groups of keys that join in LDS (half the partials,
-// but a barrier of 8 waves: 128 sequences 3 us more), three stages in registers on their way,
-// partials past the caches (1.5 us less here, 1.5 more in the join).
+// but a barrier of 8 waves in each step), partials past the caches (1.5 us less here, 1.5 more in
+// the join).
 #include "fpv2_batch.h"
 #include "fpv2_decode_split.h"
 
 namespace fpv2 {
 namespace {
 
-constexpr int kMaxSplits = 512;  // parts of the prefix
-constexpr int kMaxRuns = 2048;   // waves of the own keys
+// What a tile of own keys costs a wave beside what one of the prefix, of more than 16 rows, costs
+// each wave of its workgroup: measured best of 1 to 8, at head dim 256 (kOwnWide) of 1 to 20.
+constexpr float kOwnTile = 2.f, kOwnWide = 8.f;
+constexpr int kLong = 24;
 
 struct PrefixArgs {
   const uint16_t* q;
@@ -42,16 +43,77 @@ struct PrefixArgs {
   float* part_o;           // [splits][kv_heads][rows][D]
   float* part_ml;          // [splits][kv_heads][rows][2]
   int64_t q_bs, q_hs, k_ps, k_hs, k_rs, v_ps, v_hs, v_rs;
-  int kv_heads, group, rows, row_tiles, tile_rows, splits;  // rows: batch * group
-  int own_blocks;  // workgroups of the own keys, before the prefix's
+  int kv_heads, group, rows, row_tiles, tile_rows;  // rows: batch * group
+  int cus, roomy, most_splits, most_own;  // most_own: workgroups of the own keys
   int pages, page_size, capacity, length;
   uint32_t page_mul, page_shift;
   float scale_log2;
 };
 
+// The launch's first argument, read again: what the workgroups' two kinds of work, and their starts
+// and ends, hold of their arguments would not fit the scalar registers together, and the loop over the keys
+// would fetch the rest of it from lanes of vector registers.
+typedef const __attribute__((address_space(4))) PrefixArgs ScalarArgs;
+__device__ __forceinline__ ScalarArgs& again() {
+  uintptr_t p = reinterpret_cast<uintptr_t>(__builtin_amdgcn_kernarg_segment_ptr());
+  asm volatile("" : "+s"(p));
+  return *reinterpret_cast<ScalarArgs*>(p);
+}
+
 __device__ __forceinline__ int prefix_length(const PrefixArgs& a) {
   const int n = a.lengths != nullptr ? *a.lengths : a.length;
   return min(max(n, 0), a.capacity);
+}
+
+// What the launch's workgroups do: the first own_blocks the own keys, by waves; then the parts
+// of the prefix.
+struct Division {
+  int own_blocks, splits;
+};
+// The waves of a workgroup.
+template <int D>
+__host__ __device__ __forceinline__ int waves_of(int64_t rows) { return D > 128 && rows > 16 ? 8 : 4; }
+
+// The workgroups that run at once are shared out by the work, which the lengths on the device say,
+// so that both kinds take equally long, side by side: the own keys wait for memory, the prefix for
+// MFMA, and no workgroup waits for another's place.  Against the own keys first, in as many waves as
+// they have tiles for, and then the prefix: 40 sequences after 32768 keys 66 to 58 us, 128 after 8191
+// 50 to 44, 8 after 16384 31 to 23, 64 of up to 2000 after 4096 37 to 33.
+// - A few own keys (a 32nd of the work and less) before many of the prefix (kLong tiles a workgroup)
+//   come first all the same: to round the parts down to what they leave costs more (64 sequences after
+//   32768 keys 65 us beside, 61 before; 8 after 16384, 8 tiles a workgroup, 23 and 31).
+// - The prefix has a second workgroup on a CU where each of one has more than 8 tiles of more than 16
+//   rows (31 sequences after 8192 keys, 8 tiles: 20 us by one, 21 by two and the join 7 and 10;
+//   64 after 8192, 16 tiles: 31 and 26).
+// - Where all that the caches can hold has room at once (roomy), the prefix's workgroups need not
+//   know the own keys' lengths: 4 sequences after 1000 keys 1 us less.
+// n: the prefix's length; units: of all own items, 8 of each item's beside its tiles (counted as 2
+// here).  (Nothing to contract in it: both launches divide alike.)
+template <int D>
+__device__ __forceinline__ Division divide(const PrefixArgs& p, const DecodeArgs& a, int n, int units) {
+#pragma clang fp contract(off)
+  const bool few = p.rows <= 16;
+  const int tiles = (n + kTileKeys - 1) / kTileKeys, waves = waves_of<D>(p.rows);
+  const int each = p.kv_heads * p.row_tiles;  // workgroups of a part
+  const int most = max(min((tiles + kWaves - 1) / kWaves, p.most_splits), 1);
+  if (p.roomy) return {p.most_own, most};
+  const float all = static_cast<float>(tiles) * static_cast<float>(each);
+  const int slots = D <= 128 ? 2 * p.cus : p.cus;
+  const int mine = units - (kItemUnits - 2) * a.batch * a.kv_heads * a.head_items;
+  const float own = static_cast<float>(mine) * (few ? 1.f : D > 128 ? kOwnWide : kOwnTile);
+  const float pre = few ? all : all * static_cast<float>(waves);
+  // (the parts that then follow on them take all workgroups)
+  const bool before = !few && D <= 128 && all >= static_cast<float>(kLong * slots) && 32.f * mine < pre;
+  const int share = before ? slots : min(static_cast<int>(static_cast<float>(slots) * pre * __builtin_amdgcn_rcpf(own + pre)),
+                        few || all <= static_cast<float>(8 * p.cus) ? min(p.cus, slots - 8) : slots - 8);
+  // (half a workgroup off a whole number: the quotient's floor)
+  const int quotient = static_cast<int>((static_cast<float>(share) + 0.5f) *
+                                        __builtin_amdgcn_rcpf(static_cast<float>(each)));
+  const int splits = min(max(quotient, 1), most);
+  const int need = ((units / kWaves + waves) / waves + 7) / 8 * 8;
+  const int blocks = before ? need : min(max(slots - splits * each, slots - share) / 8 * 8, need);
+  // (known to be the wave's, and all that follows from them)
+  return {__builtin_amdgcn_readfirstlane(min(blocks, p.most_own)), __builtin_amdgcn_readfirstlane(splits)};
 }
 
 // A column's weights are 2^(x - m), x = scale log2(e) q.k, with a reference m that moves when
@@ -146,19 +208,19 @@ struct At {
   int id, row;
 };
 __device__ const int32_t kPageZero = 0;
-__device__ __forceinline__ At prefix_at(const PrefixArgs& a, int t) {
+__device__ __forceinline__ At prefix_at(ScalarArgs& a, int t) {
   typedef const __attribute__((address_space(4))) int32_t* scalar_ptr;
   const uint32_t page = (__umulhi(static_cast<uint32_t>(t), a.page_mul) + t) >> a.page_shift;
   const int32_t* p = a.table != nullptr ? a.table + page : &kPageZero;
   return {*reinterpret_cast<scalar_ptr>(reinterpret_cast<uintptr_t>(p)), t - static_cast<int>(page) * a.page_size};
 }
-__device__ __forceinline__ int64_t page_of(const PrefixArgs& a, int id) { return min(max(id, 0), a.pages - 1); }
+__device__ __forceinline__ int64_t page_of(ScalarArgs& a, int id) { return min(max(id, 0), a.pages - 1); }
 // Loads stay in the order that they are written in.
 __device__ __forceinline__ void in_order() { asm volatile("" ::: "memory"); }
 
 // A row's queries as the B operand of the scores, negated where the scale is negative.
 template <int KK>
-__device__ __forceinline__ void load_queries(const PrefixArgs& a, int kvh, int row, bool live, int quad, u32x4 (&qf)[KK]) {
+__device__ __forceinline__ void load_queries(ScalarArgs& a, int kvh, int row, bool live, int quad, u32x4 (&qf)[KK]) {
   const int b = row / a.group, g = row - b * a.group;
   const uint16_t* p = a.q + b * a.q_bs + (kvh * a.group + g) * a.q_hs + 8 * quad;
   const uint32_t sign = a.scale_log2 < 0.f ? 0x80008000u : 0u;
@@ -173,18 +235,136 @@ struct Tile {
   Words<D / 32> v[8];
 };
 
+// A KV head's keys of one table, tile after tile.
+struct Keys {
+  const uint16_t* k;
+  const uint16_t* v;
+  const int32_t* table;
+  int64_t k_ps, k_rs, v_ps, v_rs;
+  int page, pages, page_size, n;  // page: of all keys where there is no table
+  uint32_t page_mul, page_shift;
+};
+// 16 rows' sums over a wave's keys: the tiles at u0, u0 + STEP .. before u_end.  AHEAD: with a tile's
+// loads on their way beside another's products (own keys, of a few tiles each, take as long
+// without, whose K and V share registers).
+template <int D>
+struct Rows {
+  u32x4 q[D / 32];
+  f32x4 o[D / 16];
+  float scale, m, l, greatest;
+};
+template <int D>
+__device__ __forceinline__ void start_rows(Rows<D>& r, float scale_log2) {
+  r.scale = fmaxf(__builtin_fabsf(scale_log2), 1e-30f);
+  r.m = kNone;
+  r.l = 0.f;
+  r.greatest = neg_inf();
+#pragma unroll
+  for (int d = 0; d < D / 16; ++d) r.o[d] = f32x4{0.f, 0.f, 0.f, 0.f};
+}
+template <typename T, int D, int STEP, bool AHEAD>
+__device__ __forceinline__ void walk(const Keys& a, int u0, int u_end, int lane, Rows<D>& r) {
+  constexpr int KK = D / 32, DV = D / 16;
+  const int col = lane & 15, quad = lane >> 4;
+  int row = 0, page = 0;  // lane i's (and i + 32's) of the next tile's key i
+  const auto look_up = [&](int u) {
+    const uint32_t t = min(u + (lane & 31), a.n - 1);
+    const uint32_t at = (__umulhi(t, a.page_mul) + t) >> a.page_shift;
+    row = t - at * a.page_size;
+    const int id = a.table != nullptr ? a.table[at] : a.page;
+    page = min(max(id, 0), a.pages - 1);
+  };
+  const auto load_k = [&](Tile<D>& x) {
+    const int64_t koff = page * a.k_ps + row * a.k_rs;
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      const uint16_t* p = a.k + __shfl(koff, 16 * t + col, 64) + 8 * quad;
+#pragma unroll
+      for (int kk = 0; kk < KK; ++kk) x.k[t][kk] = load16(p + 32 * kk);
+    }
+  };
+  const auto load_v = [&](Tile<D>& x, int64_t voff) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      x.v[j] = load_words<DV / 2>(a.v + __shfl(voff, 16 * (j / 4) + 4 * quad + j % 4, 64) + DV * col);
+  };
+  const auto score = [&](const Tile<D>& y, f32x4 (&sc)[2]) {
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      sc[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int kk = 0; kk < KK; ++kk) sc[t] = Elem<T>::mfma16(as_vec8<T>(y.k[t][kk]), as_vec8<T>(r.q[kk]), sc[t]);
+    }
+  };
+  const auto multiply = [&](Tile<D>& y, const f32x4 (&sc)[2], int u) {
+    const int left = a.n - u;
+    const u32x4 pf = weigh<T>(
+        relate<T>(sc, r.scale, left < kTileKeys ? left - 4 * quad : kTileKeys, r.m, r.l, r.greatest, r.o), r.l);
+    if (left < kTileKeys) {
+      // (a zero weight would make NaN of what an unused row may hold)
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (16 * (j / 4) + 4 * quad + j % 4 >= left) {
+#pragma unroll
+          for (int w = 0; w < DV / 2; ++w) y.v[j].w[w] = 0;
+        }
+    }
+#pragma unroll
+    for (int d = 0; d < DV; ++d) {
+      u32x4 vt;  // dim d of the lane's 8 keys
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        vt[j] = __builtin_amdgcn_perm(y.v[2 * j + 1].w[d / 2], y.v[2 * j].w[d / 2],
+                                      d % 2 ? 0x07060302u : 0x05040100u);
+      r.o[d] = Elem<T>::mfma16(as_vec8<T>(vt), as_vec8<T>(pf), r.o[d]);
+    }
+  };
+  if (u0 >= u_end) return;
+  look_up(u0);
+  if constexpr (AHEAD) {
+    // A tile's loads are a tile ahead of its products, and its pages one more.  (Tiles behind
+    // the last one are loaded too, as the last key again, so that it is known at each product
+    // how many loads were issued since its own.)
+    Tile<D> even, odd;
+    const auto load = [&](Tile<D>& x, int next) {
+      load_k(x);
+      load_v(x, page * a.v_ps + row * a.v_rs);
+      look_up(next);
+    };
+    const auto both = [&](Tile<D>& x, int u) {
+      f32x4 sc[2];
+      score(x, sc);
+      multiply(x, sc, u);
+    };
+    load(even, u0 + STEP);
+    for (; u0 < u_end; u0 += 2 * STEP) {
+      load(odd, u0 + 2 * STEP);
+      both(even, u0);
+      load(even, u0 + 3 * STEP);
+      if (u0 + STEP < u_end) both(odd, u0 + STEP);
+    }
+  } else {
+    for (; u0 < u_end; u0 += STEP) {
+      Tile<D> x;
+      load_k(x);
+      const int64_t voff = page * a.v_ps + row * a.v_rs;
+      look_up(u0 + STEP);
+      f32x4 sc[2];
+      score(x, sc);
+      load_v(x, voff);
+      multiply(x, sc, u0);
+    }
+  }
+}
+
 // Own keys: the decode attention's schedule (fpv2_decode_split.h) with runs of waves instead of
 // workgroups, as they are short: a wave takes its items' tiles one after the other and
-// leaves a partial of each, a whole item's behind the runs' slots.  (By workgroups whose waves
-// join in LDS: 128 sequences of an 8191-key prefix 52 us, by waves 50; 40 of 32768 keys 64 and 65; at head
-// dim 256, where the prefix's workgroups have 8 waves, a launch of their own, 28 + 13 us, and 43 in one.)
+// leaves a partial of each, a whole item's behind the runs' slots.
 template <typename T, int D>
-__device__ __forceinline__ void own_attn(const DecodeArgs& a, int run) {
-  constexpr int KK = D / 32, DV = D / 16;
-  constexpr int kEarly = D > 128 ? 0 : 8;  // values whose loads do not wait for the scores
+__device__ __forceinline__ void own_attn(const DecodeArgs& a, const Prefix& prefix, int run, int whole_slots) {
+  constexpr int DV = D / 16;
   const int lane = threadIdx.x & 63, col = lane & 15, quad = lane >> 4;
   const int items = a.kv_heads * a.head_items;
-  const Prefix prefix = prefix_of(a, lane);
   const int total = prefix.total * items;
   const int lo = first_of(a, run, total), hi = first_of(a, run + 1, total);
   if (lo >= hi) return;
@@ -209,92 +389,31 @@ __device__ __forceinline__ void own_attn(const DecodeArgs& a, int run) {
     const int h0 = (item - kvh * a.head_items) * a.item_heads;
     const int heads = min(a.item_heads, a.group - h0);
     const int head = kvh * a.group + h0 + col;
+    Rows<D> r;
     const uint32_t sign = a.scale_log2 < 0.f ? 0x80008000u : 0u;
-    const float scale = fmaxf(__builtin_fabsf(a.scale_log2), 1e-30f);
-    u32x4 qf[KK];
 #pragma unroll
-    for (int kk = 0; kk < KK; ++kk)
-      qf[kk] = col < heads ? load16(a.q + b_now * a.q_bs + head * a.q_hs + 32 * kk + 8 * quad) ^ sign : u32x4{0, 0, 0, 0};
-    f32x4 o[DV];
-    float m = kNone, l = 0.f, greatest = neg_inf();
-#pragma unroll
-    for (int d = 0; d < DV; ++d) o[d] = f32x4{0.f, 0.f, 0.f, 0.f};
-
-    const uint16_t* kb = a.k + kvh * a.k_hs;
-    const uint16_t* vb = a.v + kvh * a.v_hs;
-    const int32_t* table = a.table != nullptr ? a.table + b_now * a.table_stride : nullptr;
-    // lane i (and i + 32) looks up the row of the tile's key i
-    int row = 0, page = 0;
-    const auto look_up = [&](int u0) {
-      const uint32_t t = min(u0 + (lane & 31), s_now.n - 1);
-      const uint32_t at = (__umulhi(t, a.page_mul) + t) >> a.page_shift;
-      row = t - at * a.page_size;
-      const int id = table != nullptr ? table[at] : b_now;
-      page = min(max(id, 0), a.pages - 1);
-    };
-    const int u_end = min(s_now.n, last * kTileKeys);
-    if (first * kTileKeys < u_end) look_up(first * kTileKeys);
-    for (int u0 = first * kTileKeys; u0 < u_end; u0 += kTileKeys) {
-      const int64_t koff = page * a.k_ps + row * a.k_rs;
-      const int64_t voff = page * a.v_ps + row * a.v_rs;
-      u32x4 kf[2][KK];
-#pragma unroll
-      for (int t = 0; t < 2; ++t) {
-        const uint16_t* p = kb + __shfl(koff, 16 * t + col, 64) + 8 * quad;
-#pragma unroll
-        for (int kk = 0; kk < KK; ++kk) kf[t][kk] = load16(p + 32 * kk);
-      }
-      Words<DV / 2> vf[8];
-      const auto load_v = [&](int j) {
-        return load_words<DV / 2>(vb + __shfl(voff, 16 * (j / 4) + 4 * quad + j % 4, 64) + DV * col);
-      };
-#pragma unroll
-      for (int j = 0; j < kEarly; ++j) vf[j] = load_v(j);
-      if (u0 + kTileKeys < u_end) look_up(u0 + kTileKeys);
-      f32x4 sc[2];
-#pragma unroll
-      for (int t = 0; t < 2; ++t) {
-        sc[t] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int kk = 0; kk < KK; ++kk) sc[t] = Elem<T>::mfma16(as_vec8<T>(kf[t][kk]), as_vec8<T>(qf[kk]), sc[t]);
-      }
-#pragma unroll
-      for (int j = kEarly; j < 8; ++j) vf[j] = load_v(j);
-      const int left = s_now.n - u0;
-      const u32x4 pf =
-          weigh<T>(relate<T>(sc, scale, left < kTileKeys ? left - 4 * quad : kTileKeys, m, l, greatest, o), l);
-      if (left < kTileKeys) {
-        // (a zero weight would make NaN of what an unused row may hold)
-#pragma unroll
-        for (int j = 0; j < 8; ++j)
-          if (16 * (j / 4) + 4 * quad + j % 4 >= left) {
-#pragma unroll
-            for (int w = 0; w < DV / 2; ++w) vf[j].w[w] = 0;
-          }
-      }
-#pragma unroll
-      for (int d = 0; d < DV; ++d) {
-        u32x4 vt;  // dim d of the lane's 8 keys
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-          vt[j] = __builtin_amdgcn_perm(vf[2 * j + 1].w[d / 2], vf[2 * j].w[d / 2], d % 2 ? 0x07060302u : 0x05040100u);
-        o[d] = Elem<T>::mfma16(as_vec8<T>(vt), as_vec8<T>(pf), o[d]);
-      }
-    }
-    l += __shfl_xor(l, 16, 64);
-    l += __shfl_xor(l, 32, 64);
+    for (int kk = 0; kk < D / 32; ++kk)
+      r.q[kk] = col < heads ? load16(a.q + b_now * a.q_bs + head * a.q_hs + 32 * kk + 8 * quad) ^ sign
+                            : u32x4{0, 0, 0, 0};
+    start_rows(r, a.scale_log2);
+    walk<T, D, kTileKeys, false>(
+        {a.k + kvh * a.k_hs, a.v + kvh * a.v_hs, a.table != nullptr ? a.table + b_now * a.table_stride : nullptr,
+         a.k_ps, a.k_rs, a.v_ps, a.v_rs, b_now, a.pages, a.page_size, s_now.n, a.page_mul, a.page_shift},
+        first * kTileKeys, min(s_now.n, last * kTileKeys), lane, r);
+    r.l += __shfl_xor(r.l, 16, 64);
+    r.l += __shfl_xor(r.l, 32, 64);
     const bool whole = first == 0 && last == s_now.tiles;
-    const int64_t slot = whole ? 2 * static_cast<int64_t>(a.grid) + static_cast<int64_t>(b_now) * items + item
+    const int64_t slot = whole ? whole_slots + static_cast<int64_t>(b_now) * items + item
                                : 2 * static_cast<int64_t>(run) + (cur == lo ? 0 : 1);
     if (col < heads) {
       const int64_t at = slot * a.item_heads + col;
 #pragma unroll
       for (int i = 0; i < 4; ++i)
 #pragma unroll
-        for (int d = 0; d < DV; ++d) a.part_o[at * D + (4 * quad + i) * DV + d] = o[d][i];
+        for (int d = 0; d < DV; ++d) a.part_o[at * D + (4 * quad + i) * DV + d] = r.o[d][i];
       if (quad == 0) {
-        a.part_ml[at * 2] = m;
-        a.part_ml[at * 2 + 1] = l;
+        a.part_ml[at * 2] = r.m;
+        a.part_ml[at * 2 + 1] = r.l;
       }
     }
   }
@@ -307,128 +426,51 @@ struct FewShared {
   float ml[4][16][2];
 };
 template <typename T, int D>
-__device__ __forceinline__ void prefix_few(const PrefixArgs& a, int block, FewShared<D>& sh) {
-  constexpr int KK = D / 32, DV = D / 16;
+__device__ __forceinline__ void prefix_few(ScalarArgs& a, int n, int splits, int unit, FewShared<D>& sh) {
+  constexpr int DV = D / 16;
   auto& sh_o = sh.o;
   auto& sh_ml = sh.ml;
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int col = lane & 15, quad = lane >> 4;
-  const int unit = block;
+  if (unit >= a.kv_heads * splits) return;
   const int split = unit / a.kv_heads, kvh = unit - split * a.kv_heads;
-  const int n = __builtin_amdgcn_readfirstlane(prefix_length(a));
   const int tiles = (n + kTileKeys - 1) / kTileKeys;
-  const int first = static_cast<int>(static_cast<int64_t>(tiles) * split / a.splits);
-  const int last = static_cast<int>(static_cast<int64_t>(tiles) * (split + 1) / a.splits);
-
-  const uint16_t* kb = a.k + kvh * a.k_hs;
-  const uint16_t* vb = a.v + kvh * a.v_hs;
-  int row = 0, page = 0;  // lane i's (and i + 32's) of the next tile's key i
-  const auto look_up = [&](int u0) {
-    const uint32_t t = min(u0 + (lane & 31), n - 1);
-    const uint32_t at = (__umulhi(t, a.page_mul) + t) >> a.page_shift;
-    row = t - at * a.page_size;
-    const int id = a.table != nullptr ? a.table[at] : 0;
-    page = min(max(id, 0), a.pages - 1);
-  };
-  const auto load = [&](Tile<D>& x) {
-    const int64_t koff = page * a.k_ps + row * a.k_rs;
-    const int64_t voff = page * a.v_ps + row * a.v_rs;
-#pragma unroll
-    for (int t = 0; t < 2; ++t) {
-      const uint16_t* p = kb + __shfl(koff, 16 * t + col, 64) + 8 * quad;
-#pragma unroll
-      for (int kk = 0; kk < KK; ++kk) x.k[t][kk] = load16(p + 32 * kk);
-    }
-#pragma unroll
-    for (int j = 0; j < 8; ++j)
-      x.v[j] = load_words<DV / 2>(vb + __shfl(voff, 16 * (j / 4) + 4 * quad + j % 4, 64) + DV * col);
-  };
-
-  const float scale = fmaxf(__builtin_fabsf(a.scale_log2), 1e-30f);
-  u32x4 qf[KK];
-  load_queries<KK>(a, kvh, col, col < a.rows, quad, qf);
-  f32x4 o[DV];
-  float m = kNone, l = 0.f, greatest = neg_inf();
-#pragma unroll
-  for (int d = 0; d < DV; ++d) o[d] = f32x4{0.f, 0.f, 0.f, 0.f};
-
-  const auto multiply = [&](Tile<D>& y, int u0) {
-    f32x4 sc[2];
-#pragma unroll
-    for (int t = 0; t < 2; ++t) {
-      sc[t] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-      for (int kk = 0; kk < KK; ++kk) sc[t] = Elem<T>::mfma16(as_vec8<T>(y.k[t][kk]), as_vec8<T>(qf[kk]), sc[t]);
-    }
-    const u32x4 pf = weigh<T>(
-        relate<T>(sc, scale, n - u0 < kTileKeys ? n - u0 - 4 * quad : kTileKeys, m, l, greatest, o), l);
-    if (u0 + kTileKeys > n) {
-      // (a zero weight would make NaN of what an unused row may hold)
-#pragma unroll
-      for (int j = 0; j < 8; ++j)
-        if (u0 + 16 * (j / 4) + 4 * quad + j % 4 >= n) {
-#pragma unroll
-          for (int w = 0; w < DV / 2; ++w) y.v[j].w[w] = 0;
-        }
-    }
-#pragma unroll
-    for (int d = 0; d < DV; ++d) {
-      u32x4 vt;  // dim d of the lane's 8 keys
-#pragma unroll
-      for (int j = 0; j < 4; ++j)
-        vt[j] = __builtin_amdgcn_perm(y.v[2 * j + 1].w[d / 2], y.v[2 * j].w[d / 2],
-                                      d % 2 ? 0x07060302u : 0x05040100u);
-      o[d] = Elem<T>::mfma16(as_vec8<T>(vt), as_vec8<T>(pf), o[d]);
-    }
-  };
-
-  // A tile's loads are a tile ahead of its products, and its pages one more.  (Tiles behind
-  // the last one are loaded too, as the last key again, so that it is known at each product
-  // how many loads were issued since its own.)
-  int u0 = (first + wave) * kTileKeys;
-  const int u_end = min(n, last * kTileKeys);
-  if (u0 < u_end) {
-    Tile<D> even, odd;
-    look_up(u0);
-    load(even);
-    look_up(u0 + kStepKeys);
-    for (; u0 < u_end; u0 += 2 * kStepKeys) {
-      load(odd);
-      look_up(u0 + 2 * kStepKeys);
-      multiply(even, u0);
-      load(even);
-      look_up(u0 + 3 * kStepKeys);
-      if (u0 + kStepKeys < u_end) multiply(odd, u0 + kStepKeys);
-    }
-  }
+  const int per = tiles / splits, more = tiles - per * splits;
+  const int first = split * per + min(split, more), last = first + per + (split < more ? 1 : 0);
+  Rows<D> r;
+  load_queries<D / 32>(a, kvh, col, col < a.rows, quad, r.q);
+  start_rows(r, a.scale_log2);
+  walk<T, D, kStepKeys, true>({a.k + kvh * a.k_hs, a.v + kvh * a.v_hs, a.table, a.k_ps, a.k_rs, a.v_ps, a.v_rs, 0,
+                               a.pages, a.page_size, n, a.page_mul, a.page_shift},
+                              (first + wave) * kTileKeys, min(n, last * kTileKeys), lane, r);
 
   // join the four waves
-  l += __shfl_xor(l, 16, 64);
-  l += __shfl_xor(l, 32, 64);
+  r.l += __shfl_xor(r.l, 16, 64);
+  r.l += __shfl_xor(r.l, 32, 64);
   if (quad == 0) {
-    sh_ml[wave][col][0] = m;
-    sh_ml[wave][col][1] = l;
+    sh_ml[wave][col][0] = r.m;
+    sh_ml[wave][col][1] = r.l;
   }
 #pragma unroll
   for (int i = 0; i < 4; ++i)
 #pragma unroll
-    for (int d = 0; d < DV; ++d) sh_o[wave][col][(4 * quad + i) * DV + d] = o[d][i];
+    for (int d = 0; d < DV; ++d) sh_o[wave][col][(4 * quad + i) * DV + d] = r.o[d][i];
   __syncthreads();
   for (int e = tid; e < a.rows * D; e += 256) {
-    const int r = e / D, d = e % D;
+    const int h = e / D, d = e % D;
     float top = neg_inf();
 #pragma unroll
-    for (int w = 0; w < 4; ++w) top = fmaxf(top, sh_ml[w][r][0]);
+    for (int w = 0; w < 4; ++w) top = fmaxf(top, sh_ml[w][h][0]);
     float sum = 0.f, den = 0.f;
 #pragma unroll
     for (int w = 0; w < 4; ++w) {
       // (a wave without keys has sum 0 and O 0)
-      const float f = __builtin_amdgcn_exp2f(sh_ml[w][r][0] - top);
-      sum += f * sh_o[w][r][d];
-      den += f * sh_ml[w][r][1];
+      const float f = __builtin_amdgcn_exp2f(sh_ml[w][h][0] - top);
+      sum += f * sh_o[w][h][d];
+      den += f * sh_ml[w][h][1];
     }
-    const int64_t at = static_cast<int64_t>(unit) * a.rows + r;
+    const int64_t at = static_cast<int64_t>(unit) * a.rows + h;
     a.part_o[at * D + d] = sum;
     if (d == 0) {
       a.part_ml[at * 2] = top;
@@ -440,18 +482,23 @@ __device__ __forceinline__ void prefix_few(const PrefixArgs& a, int block, FewSh
 template <typename T, int D>
 __global__ __launch_bounds__(256, D > 128 ? 1 : 2) void prefix_few_kernel(PrefixArgs p, DecodeArgs a) {
   __shared__ FewShared<D> sh;
-  const int block = static_cast<int>(blockIdx.x) - p.own_blocks;
+  const int n = __builtin_amdgcn_readfirstlane(prefix_length(p));
+  Prefix prefix = {};
+  if (!p.roomy || static_cast<int>(blockIdx.x) < p.most_own) prefix = prefix_of(a, threadIdx.x & 63);
+  const Division by = divide<D>(p, a, n, prefix.total * a.kv_heads * a.head_items);
+  a.grid = 4 * by.own_blocks;
+  const int block = static_cast<int>(blockIdx.x) - by.own_blocks;
   if (block < 0)
-    own_attn<T, D>(a, blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6));
+    own_attn<T, D>(a, prefix, blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), 8 * p.most_own);
   else
-    prefix_few<T, D>(p, block, sh);
+    prefix_few<T, D>(again(), n, by.splits, block, sh);
 }
 
 // More rows than a tile of MFMA: the workgroup's waves, 32 rows each (at head dim 256, whose
 // rows are twice as long, 8 waves of 16 rows), share the keys through LDS.  A stage is 32
 // keys' K and V, rows of a power of two of bytes whose 16-byte chunks are permuted so that
 // neither the reads of K (16 keys' chunks) nor the transposing reads of V (8 keys, 32 bytes
-// each) meet in a bank.  Three stages in LDS, two more on their way in registers.  Each wave
+// each) meet in a bank.  Three stages in LDS, three more on their way in registers.  Each wave
 // loads some keys' K or V: one page, one descriptor a stage.
 template <int D>
 struct Stage {
@@ -462,7 +509,6 @@ struct Stage {
   static constexpr int kTiles = D > 128 ? 1 : 2;    // 16-row tiles of a wave
   static constexpr int kKeys = 2 * kTileKeys / kWaves;    // of a wave's loads
   static constexpr int kLoads = kKeys * kChunks / 64;     // of a lane
-  static constexpr int kAhead = 2;                  // stages on their way
   static __device__ __forceinline__ int k_mask(int row) { return kRow >= 256 ? row & 15 : row >> 1 & 7; }
   static __device__ __forceinline__ int v_mask(int row) { return (kRow >= 256 ? row & 7 : row >> 1 & 3) << 1; }
 };
@@ -475,13 +521,13 @@ __device__ __forceinline__ void barrier_lds() { asm volatile("s_waitcnt lgkmcnt(
 
 // HALVES: 16 keys from a multiple of 16 on lie in one page (or there is no table): their
 // addresses are the wave's, a lane's offsets do not change, and a descriptor of the rows
-// up to the prefix's end reads zeros behind it.  128 sequences, 8192 keys: 37.3 us, with each
-// lane's own page and row 42.6; 40 sequences, 32768 keys in pages of 64: 52 and 77.  (Up to 16
-// rows the same either way, so that has the lanes' own alone.)
+// up to the prefix's end reads zeros behind it.  128 sequences of 16 own keys, 8192 of the prefix:
+// 37.3 us, with each lane's own page and row 42.6; 40 sequences, 32768 in pages of 64: 52 and 77.  (Up to
+// 16 rows the same either way, so that form has the lanes' own alone.)
 template <typename T, int D, bool HALVES>
-__device__ __forceinline__ void prefix_many(const PrefixArgs& a, int block, uint8_t (&sh)[3][2 * Stage<D>::kMatrix]) {
+__device__ __forceinline__ void prefix_many(ScalarArgs& a, int n, int splits, int block, uint8_t (&sh)[3][2 * Stage<D>::kMatrix]) {
   using S = Stage<D>;
-  constexpr int KK = D / 32, DT = D / 16, CT = S::kTiles, L = S::kLoads, R = 3, G = S::kAhead;
+  constexpr int KK = D / 32, DT = D / 16, CT = S::kTiles, L = S::kLoads, R = 3;  // stages
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int col = lane & 15, quad = lane >> 4;
@@ -489,12 +535,11 @@ __device__ __forceinline__ void prefix_many(const PrefixArgs& a, int block, uint
   // that they share an XCD's L2.
   const int unit = block % 8 + 8 * (block / (8 * a.row_tiles));
   const int rt = block / 8 % a.row_tiles;
-  if (unit >= a.kv_heads * a.splits) return;
+  if (unit >= a.kv_heads * splits) return;
   const int split = unit / a.kv_heads, kvh = unit - split * a.kv_heads;
-  const int n = __builtin_amdgcn_readfirstlane(prefix_length(a));
   const int tiles = (n + kTileKeys - 1) / kTileKeys;
-  const int first = static_cast<int>(static_cast<int64_t>(tiles) * split / a.splits);
-  const int last = static_cast<int>(static_cast<int64_t>(tiles) * (split + 1) / a.splits);
+  const int per = tiles / splits, more = tiles - per * splits;
+  const int first = split * per + min(split, more), last = first + per + (split < more ? 1 : 0);
   const int steps = last - first;
   const auto tile_of = [&](int step) { return first + step; };
   const int r0 = rt * a.tile_rows + 16 * CT * wave;  // this wave's rows
@@ -626,29 +671,29 @@ __device__ __forceinline__ void prefix_many(const PrefixArgs& a, int block, uint
   // that it is known at each store how many loads were issued since its own.)
   if (first < last) {
     const bool rows_here = r0 < r_end;
-    Regs regs[G];  // stage i, i + G .. in regs[i % G]
+    Regs regs[R];  // stage i, i + R .. in regs[i % R]
     look_up(tile_of(0));
-    StaticFor<0, G>::run([&](auto i) {
+    StaticFor<0, R>::run([&](auto i) {
       load(regs[i], tile_of(i));
       look_up(tile_of(i + 1));
     });
     StaticFor<0, 2>::run([&](auto i) {
-      store(regs[i % G], tile_of(i), i);
-      load(regs[i % G], tile_of(i + G));
-      look_up(tile_of(i + 1 + G));
+      store(regs[i], tile_of(i), i);
+      load(regs[i], tile_of(i + R));
+      look_up(tile_of(i + 1 + R));
     });
     barrier_lds();
     if (rows_here) score(std::integral_constant<int, 0>{});
-    for (int at = 0; at < steps; at += R * G)
-      StaticFor<0, R * G>::run([&](auto i) __attribute__((always_inline)) {
+    for (int at = 0; at < steps; at += R)
+      StaticFor<0, R>::run([&](auto i) __attribute__((always_inline)) {
         // (R = 3: the next stage is written, and the one before this one read)
-        constexpr std::integral_constant<int, i % R> kThis{};
+        constexpr std::integral_constant<int, i> kThis{};
         constexpr std::integral_constant<int, (i + 1) % R> kNext{};
         constexpr std::integral_constant<int, (i + 2) % R> kAfter{};
         barrier_lds();
-        store(regs[(i + 2) % G], tile_of(at + i + 2), kAfter);
-        load(regs[(i + 2) % G], tile_of(at + i + 2 + G));
-        look_up(tile_of(at + i + 3 + G));
+        store(regs[kAfter], tile_of(at + i + 2), kAfter);
+        load(regs[kAfter], tile_of(at + i + 2 + R));
+        look_up(tile_of(at + i + 3 + R));
         if (rows_here && tile_of(at + i) < last) multiply(tile_of(at + i), kThis, kNext);
       });
   }
@@ -659,12 +704,13 @@ __device__ __forceinline__ void prefix_many(const PrefixArgs& a, int block, uint
   static_assert(sizeof(sh) >= S::kWaves * 16 * kPad * 4, "16 rows of every wave fit the ring");
   float* const mine = reinterpret_cast<float*>(&sh[0][0]) + wave * 16 * kPad;
   barrier_lds();
+  ScalarArgs& z = again();
 #pragma unroll
   for (int c = 0; c < CT; ++c) {
     l[c] += __shfl_xor(l[c], 16, 64);
     l[c] += __shfl_xor(l[c], 32, 64);
     const int row0 = r0 + 16 * c;
-    const int64_t at = static_cast<int64_t>(unit) * a.rows + row0;
+    const int64_t at = static_cast<int64_t>(unit) * z.rows + row0;
 #pragma unroll
     for (int d0 = 0; d0 < D; d0 += kWide) {
 #pragma unroll
@@ -676,14 +722,14 @@ __device__ __forceinline__ void prefix_many(const PrefixArgs& a, int block, uint
       for (int i = 0; i < 16 * kWide / 4 / 64; ++i) {
         const int e = lane + 64 * i, row = e / (kWide / 4), part = e - row * (kWide / 4);
         if (row0 + row < r_end)
-          *reinterpret_cast<f32x4*>(a.part_o + (at + row) * D + d0 + 4 * part) =
+          *reinterpret_cast<f32x4*>(z.part_o + (at + row) * D + d0 + 4 * part) =
               *reinterpret_cast<const f32x4*>(mine + row * kPad + 4 * part);
       }
       __builtin_amdgcn_wave_barrier();
     }
     if (quad == 0 && row0 + col < r_end) {
-      a.part_ml[(at + col) * 2] = m[c];
-      a.part_ml[(at + col) * 2 + 1] = l[c];
+      z.part_ml[(at + col) * 2] = m[c];
+      z.part_ml[(at + col) * 2 + 1] = l[c];
     }
   }
 }
@@ -691,11 +737,18 @@ __device__ __forceinline__ void prefix_many(const PrefixArgs& a, int block, uint
 template <typename T, int D, bool HALVES>
 __global__ __launch_bounds__(64 * Stage<D>::kWaves, D > 128 ? 1 : 2) void prefix_many_kernel(PrefixArgs p, DecodeArgs a) {
   __shared__ alignas(1024) uint8_t ring[3][2 * Stage<D>::kMatrix];
-  const int block = static_cast<int>(blockIdx.x) - p.own_blocks;
+  constexpr int kGroup = Stage<D>::kWaves;
+  const int n = __builtin_amdgcn_readfirstlane(prefix_length(p));
+  Prefix prefix = {};
+  if (!p.roomy || static_cast<int>(blockIdx.x) < p.most_own) prefix = prefix_of(a, threadIdx.x & 63);
+  const Division by = divide<D>(p, a, n, prefix.total * a.kv_heads * a.head_items);
+  a.grid = kGroup * by.own_blocks;
+  const int block = static_cast<int>(blockIdx.x) - by.own_blocks;
   if (block < 0)
-    own_attn<T, D>(a, blockIdx.x * Stage<D>::kWaves + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6));
+    own_attn<T, D>(a, prefix, blockIdx.x * kGroup + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6),
+                             2 * kGroup * p.most_own);
   else
-    prefix_many<T, D, HALVES>(p, block, ring);
+    prefix_many<T, D, HALVES>(again(), n, by.splits, block, ring);
 }
 
 // Joins a query head's partials of the prefix and of its sequence's own keys: WAVES waves
@@ -714,27 +767,31 @@ __global__ __launch_bounds__(256) void shared_join_kernel(PrefixArgs p, DecodeAr
   const int b = at / heads, head = at - b * heads;
   const int kvh = head / a.group, g = head - kvh * a.group;
   const int item = kvh * a.head_items + g / a.item_heads, h = g % a.item_heads;
+  const int of_prefix = prefix_length(p);
   const Prefix prefix = prefix_of(a, lane);
   const int total = prefix.total * items;
+  const Division by = divide<D>(p, a, of_prefix, total);
+  a.grid = waves_of<D>(p.rows) * by.own_blocks;
+  const int whole_slots = 2 * waves_of<D>(p.rows) * p.most_own;
   const int base = units_before(a, prefix, lane, b) * items;
   const Sequence s = sequence_of(a, b);
   const int start = base + item * s.units();
   const int w0 = workgroup_of(a, start + kItemUnits, total);
   const int own = workgroup_of(a, start + s.units() - 1, total) - w0 + 1;
   const int in_last = start > first_of(a, w0, total) ? 1 : 0;
-  const int n = p.splits + own;
+  const int n = by.splits + own;
   // the partials' rows: the prefix's parts, then the own keys' (one workgroup's whole item
   // lies behind the runs' slots)
   const auto row_of = [&](int i) __attribute__((always_inline)) -> int64_t {
-    if (i < p.splits) return (static_cast<int64_t>(i) * p.kv_heads + kvh) * p.rows + b * p.group + g;
-    i -= p.splits;
-    const int64_t slot = own == 1 ? 2 * static_cast<int64_t>(a.grid) + static_cast<int64_t>(b) * items + item
+    if (i < by.splits) return (static_cast<int64_t>(i) * p.kv_heads + kvh) * p.rows + b * p.group + g;
+    i -= by.splits;
+    const int64_t slot = own == 1 ? whole_slots + static_cast<int64_t>(b) * items + item
                                   : 2 * static_cast<int64_t>(w0 + i) + (i == 0 ? in_last : 0);
     return slot * a.item_heads + h;
   };
   typedef float f32x2 __attribute__((ext_vector_type(2)));
   const auto ml_of = [&](int i) __attribute__((always_inline)) {
-    return *reinterpret_cast<const f32x2*>((i < p.splits ? p.part_ml : a.part_ml) + row_of(i) * 2);
+    return *reinterpret_cast<const f32x2*>((i < by.splits ? p.part_ml : a.part_ml) + row_of(i) * 2);
   };
   float top = neg_inf();
   for (int i = lane; i < n; i += 64) top = fmaxf(top, ml_of(i)[0]);
@@ -756,10 +813,19 @@ __global__ __launch_bounds__(256) void shared_join_kernel(PrefixArgs p, DecodeAr
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     __builtin_amdgcn_wave_barrier();
     if (slot < kAtOnce) {
-#pragma unroll 8
-      for (int i = i0 + wave % WAVES * kAtOnce + slot; i < upto; i += WAVES * kAtOnce)
-        o += sh_f[wave][i - i0] *
-             *reinterpret_cast<const f32x4*>((i < p.splits ? p.part_o : a.part_o) + row_of(i) * D + 4 * e);
+      // (8 loads on their way, behind the last partial of this one again)
+      constexpr int kStep = WAVES * kAtOnce;
+      for (int i = i0 + wave % WAVES * kAtOnce + slot; i < upto; i += 8 * kStep) {
+        f32x4 x[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const int at_j = i + j * kStep < upto ? i + j * kStep : i;
+          x[j] = *reinterpret_cast<const f32x4*>((at_j < by.splits ? p.part_o : a.part_o) + row_of(at_j) * D + 4 * e);
+        }
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          if (i + j * kStep < upto) o += sh_f[wave][i + j * kStep - i0] * x[j];
+      }
     }
     __builtin_amdgcn_wave_barrier();
   }
@@ -773,42 +839,55 @@ __global__ __launch_bounds__(256) void shared_join_kernel(PrefixArgs p, DecodeAr
     for (int w = 0; w < WAVES; ++w)
 #pragma unroll
       for (int i = 0; i < kAtOnce; ++i) o += sh_o[wave + w][i][lane];
-    const bool none = s.n == 0 && prefix_length(p) == 0;
+    const bool none = s.n == 0 && of_prefix == 0;
     uint16_t* out = a.out + b * a.o_bs + head * a.o_hs + 4 * lane;
 #pragma unroll
     for (int j = 0; j < 4; ++j) out[j] = Elem<T>::from_float(none ? 0.f : o[j] / den);
   }
 }
 
+// (Own keys have 8 workgroups at least, and multiples of 8.)
+int cus_of() {
+  const int n = cu_count() / 8 * 8;
+  return n > 16 ? n : 16;
+}
+
 struct SharedPlan {
   DecodePlan own;
-  int row_tiles, tile_rows, splits;
+  int row_tiles, tile_rows, most_splits, most_own;
+  int64_t blocks;
+  bool roomy;
   int64_t own_rows, prefix_rows;  // of partials
 };
 
 SharedPlan shared_plan(const fpv2_shared_prefix_params& p) {
   SharedPlan plan;
   plan.own = decode_plan(p.own);
-  // runs of waves: two for each SIMD
-  const int64_t units = p.own.batch * p.own.kv_heads * plan.own.head_items * (plan.own.most_tiles + kItemUnits);
-  const int64_t runs = (units + kWaves - 1) / kWaves, most_runs = 8 * static_cast<int64_t>(cu_count());
-  plan.own.grid = static_cast<int>(runs < most_runs ? runs : most_runs < kMaxRuns ? most_runs : kMaxRuns);
-  const int64_t rows = p.own.batch * (p.own.query_heads / p.own.kv_heads);
-  // tiles of at most 128 rows, all alike, of whole waves
-  plan.row_tiles = static_cast<int>((rows + 127) / 128);
-  plan.tile_rows = rows <= 16 ? 16 : static_cast<int>((rows + 32 * plan.row_tiles - 1) / (32 * plan.row_tiles) * 32);
-  if (plan.row_tiles > 0) plan.row_tiles = static_cast<int>((rows + plan.tile_rows - 1) / plan.tile_rows);
-  const int64_t tiles = (p.prefix_table_width * p.prefix_page_size + kTileKeys - 1) / kTileKeys;
-  // (workgroups a CU)
-  const int64_t per = p.own.head_dim > 128 ? 1 : 2;
-  int64_t splits = per * cu_count() / (p.own.kv_heads * (plan.row_tiles > 0 ? plan.row_tiles : 1));
-  const int64_t most = (tiles + kWaves - 1) / kWaves;
-  splits = splits < most ? splits : most;
-  splits = splits < kMaxSplits ? splits : kMaxSplits;
-  plan.splits = static_cast<int>(splits > 1 ? splits : 1);
+  const int64_t cus = cus_of(), rows = p.own.batch * (p.own.query_heads / p.own.kv_heads);
   const int64_t items = p.own.kv_heads * plan.own.head_items;
-  plan.own_rows = (2LL * plan.own.grid + p.own.batch * items) * plan.own.item_heads;
-  plan.prefix_rows = static_cast<int64_t>(plan.splits) * p.own.kv_heads * rows;
+  // tiles of at most 128 rows, all alike, of whole waves
+  const int64_t most_tiles = (rows + 127) / 128;
+  plan.tile_rows = rows <= 16 ? 16 : static_cast<int>((rows + 32 * most_tiles - 1) / (32 * most_tiles) * 32);
+  plan.row_tiles = rows > 0 ? static_cast<int>((rows + plan.tile_rows - 1) / plan.tile_rows) : 1;
+  // What the division on the device can come to at most.
+  const int64_t slots = (p.own.head_dim > 128 ? 1 : 2) * cus, waves = p.own.head_dim > 128 ? waves_of<256>(rows) : waves_of<128>(rows);
+  const int64_t units = p.own.batch * items * (plan.own.most_tiles + kItemUnits);
+  const int64_t need = ((units / kWaves + waves) / waves + 7) / 8 * 8;
+  plan.most_own = static_cast<int>(need < slots ? need : slots);
+  const int64_t tiles = (p.prefix_table_width * p.prefix_page_size + kTileKeys - 1) / kTileKeys;
+  const int64_t most = (tiles + kWaves - 1) / kWaves;
+  int64_t splits = (rows <= 16 ? cus : slots) / (p.own.kv_heads * plan.row_tiles);
+  splits = splits < most ? splits : most;
+  plan.most_splits = static_cast<int>(splits > 1 ? splits : 1);
+  // (the parts' workgroups begin at multiples of 8, and so do their ends)
+  const int64_t each = p.own.kv_heads * plan.row_tiles, rest = p.own.kv_heads % 8 ? 7 * plan.row_tiles : 0;
+  const int64_t all = plan.most_own + plan.most_splits * each + rest, one = plan.most_own + each + rest;
+  const bool before = rows > 16 && p.own.head_dim <= 128 && tiles * each >= kLong * slots;
+  const int64_t full = slots + rest + (before ? plan.most_own : 0);
+  plan.blocks = all < full ? all : one < full ? full : one;
+  plan.roomy = plan.most_splits * each <= cus && plan.most_own + plan.most_splits * each <= slots;
+  plan.own_rows = (2LL * plan.most_own * waves + p.own.batch * items) * plan.own.item_heads;
+  plan.prefix_rows = static_cast<int64_t>(plan.most_splits) * p.own.kv_heads * rows;
   return plan;
 }
 
@@ -833,27 +912,23 @@ int64_t shared_bytes(const fpv2_shared_prefix_params& p, const SharedPlan& plan)
 }
 
 template <typename T, int D>
-int launch(const PrefixArgs& p, const DecodeArgs& a, hipStream_t s) {
-  const unsigned units = static_cast<unsigned>(p.kv_heads) * p.splits;
-  const dim3 few(p.own_blocks + units), many(p.own_blocks + (units + 7) / 8 * 8 * p.row_tiles);
+int launch(const PrefixArgs& p, const DecodeArgs& a, unsigned blocks, hipStream_t s) {
   // (offsets within 16 rows are 32 bits)
   const bool halves = (p.table == nullptr || p.page_size % 16 == 0) && p.k_rs < (1 << 25) && p.v_rs < (1 << 25);
   // (16 rows: 32768 keys 29 us by few, 35 by many; 131072 keys, one sequence 96 and 105; 1000 keys 7.6
   // and 9.4)
   if (p.rows <= 16)
-    hipLaunchKernelGGL((prefix_few_kernel<T, D>), few, dim3(256), 0, s, p, a);
+    hipLaunchKernelGGL((prefix_few_kernel<T, D>), dim3(blocks), dim3(256), 0, s, p, a);
   else if (halves)
-    hipLaunchKernelGGL((prefix_many_kernel<T, D, true>), many, dim3(64 * Stage<D>::kWaves), 0, s, p, a);
+    hipLaunchKernelGGL((prefix_many_kernel<T, D, true>), dim3(blocks), dim3(64 * Stage<D>::kWaves), 0, s, p, a);
   else
-    hipLaunchKernelGGL((prefix_many_kernel<T, D, false>), many, dim3(64 * Stage<D>::kWaves), 0, s, p, a);
+    hipLaunchKernelGGL((prefix_many_kernel<T, D, false>), dim3(blocks), dim3(64 * Stage<D>::kWaves), 0, s, p, a);
   if (const int rc = check_launch("prefix_kernel")) return rc;
   const unsigned heads = static_cast<unsigned>(a.batch) * a.kv_heads * a.group;
-  // Few heads of many partials have four waves each.  64 partials: 192 heads 6.6 us by four waves, 9.2
-  // by one; 512 heads 7.7 and 9.4; 768 heads 9.4 either way; 1536 heads 9.8 and 8.6.  32 partials and less:
-  // the same up to 768 heads (6.2 .. 7.2), 1536 heads 9.9 and 8.5.  A wave takes 64 / (D / 4) partials at a
-  // time: 32 of D = 256, 128 heads 6.5 and 8.9.
-  constexpr int kAtOnce = 64 / (D / 4);
-  if (heads < 1024 && p.splits + a.grid / (a.batch * a.kv_heads * a.head_items) > 24 * kAtOnce)
+  // Few heads have four waves each.  128 heads of 32 partials 5.6 us by four waves, 7.4 by one; 512 heads
+  // of 62 7.6 and 9.2; 896 heads 9.7 and 9.6; 1536 heads 10.2 and 8.6 (D = 256: 128 heads 6.3 and
+  // 10.1, 640 8.8 and 9.8; D = 64: 5.7 and 7.0, 7.2 and 6.9).
+  if (heads <= 768)
     hipLaunchKernelGGL((shared_join_kernel<T, D, 4>), dim3(heads), dim3(256), 0, s, p, a);
   else
     hipLaunchKernelGGL((shared_join_kernel<T, D, 1>), dim3((heads + 3) / 4), dim3(256), 0, s, p, a);
@@ -861,12 +936,12 @@ int launch(const PrefixArgs& p, const DecodeArgs& a, hipStream_t s) {
 }
 
 template <typename T>
-int launch_dim(const PrefixArgs& p, const DecodeArgs& a, int64_t dim, hipStream_t s) {
+int launch_dim(const PrefixArgs& p, const DecodeArgs& a, int64_t dim, unsigned blocks, hipStream_t s) {
   switch (dim) {
-    case 64: return launch<T, 64>(p, a, s);
-    case 96: return launch<T, 96>(p, a, s);
-    case 128: return launch<T, 128>(p, a, s);
-    default: return launch<T, 256>(p, a, s);
+    case 64: return launch<T, 64>(p, a, blocks, s);
+    case 96: return launch<T, 96>(p, a, blocks, s);
+    case 128: return launch<T, 128>(p, a, blocks, s);
+    default: return launch<T, 256>(p, a, blocks, s);
   }
 }
 
@@ -948,10 +1023,10 @@ extern "C" int fpv2_shared_prefix_attention(const void* q, const void* prefix_k,
   x.rows = a.batch * a.group;
   x.row_tiles = plan.row_tiles;
   x.tile_rows = plan.tile_rows;
-  x.splits = plan.splits;
-  // (of 4 or 8 waves; a multiple of 8, so that the prefix's workgroups keep their XCDs)
-  const int waves = x.rows > 16 && p.own.head_dim > 128 ? 8 : 4;
-  x.own_blocks = (plan.own.grid + 8 * waves - 1) / (8 * waves) * 8;
+  x.roomy = plan.roomy;
+  x.most_splits = plan.most_splits;
+  x.most_own = plan.most_own;
+  x.cus = cus_of();
   x.pages = static_cast<int>(p.prefix_pages);
   x.page_size = static_cast<int>(p.prefix_page_size);
   x.capacity = static_cast<int>(p.prefix_table_width * p.prefix_page_size);
@@ -959,6 +1034,7 @@ extern "C" int fpv2_shared_prefix_attention(const void* q, const void* prefix_k,
   page_division(p.prefix_page_size, &x.page_mul, &x.page_shift);
   x.scale_log2 = a.scale_log2;
   const hipStream_t s = static_cast<hipStream_t>(stream);
-  return dtype == FPV2_BF16 ? launch_dim<bf16_t>(x, a, p.own.head_dim, s)
-                            : launch_dim<f16_t>(x, a, p.own.head_dim, s);
+  const unsigned blocks = static_cast<unsigned>(plan.blocks);
+  return dtype == FPV2_BF16 ? launch_dim<bf16_t>(x, a, p.own.head_dim, blocks, s)
+                            : launch_dim<f16_t>(x, a, p.own.head_dim, blocks, s);
 }

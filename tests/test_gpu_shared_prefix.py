@@ -245,6 +245,46 @@ def test_many_short_own_parts(cuda):
     _check(c, cuda)
 
 
+@pytest.mark.parametrize("lengths", [[9, 1, 0, 33] * 10, [900, 5] * 20], ids=["few", "many"])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_long_prefix_of_many_rows(cuda, dim, lengths):
+    """Own keys before a long prefix's workgroups, and beside them."""
+    _check(_case(4, 25_000, lengths, 32, 8, dim, BF16, 16, 64), cuda)
+
+
+@pytest.mark.parametrize("dim", [64, 256])
+def test_more_rows_than_workgroups(cuda, dim):
+    """Every workgroup's place taken by one part of the prefix."""
+    gen = torch.Generator().manual_seed(5)
+    lengths = torch.randint(0, 40, (2100,), generator=gen).tolist()
+    _check(_case(5, 70, lengths, 32, 8, dim, F16, 16, 16), cuda)
+
+
+@pytest.mark.parametrize("batch,heads,hkv", [(2, 4, 2), (40, 12, 3), (150, 8, 1)])
+@pytest.mark.parametrize("prefix,length", [(0, 0), (3, 1), (0, 600), (5000, 0), (5000, 600), (9000, 3)])
+def test_caches_wider_than_what_they_hold(cuda, batch, heads, hkv, prefix, length):
+    """The launch goes by the caches' size, the work by the lengths on the device."""
+    gen = torch.Generator().manual_seed(6)
+    dim, page = 64, 16
+    k, v = (rand(gen, 700, hkv, page, dim, dtype=BF16) for _ in "kv")
+    c = {"q": rand(gen, batch, heads, dim, dtype=BF16) * 2, "k": k, "v": v, "prefix_k": k, "prefix_v": v,
+         "prefix_table": torch.randint(0, 700, (600,), generator=gen, dtype=torch.int32),
+         "table": torch.randint(0, 700, (batch, 40), generator=gen, dtype=torch.int32),
+         "prefix_length": torch.tensor([prefix], dtype=torch.int32),
+         "lengths": torch.tensor([max(0, length - b % 3) for b in range(batch)], dtype=torch.int32)}
+    rows = [x.transpose(1, 2).reshape(-1, hkv, dim) for x in (k, v)]
+    t = torch.arange(page)
+
+    def held(table, n):
+        at = (table.long()[:, None] * page + t).view(-1)[:n]
+        return [x[at].transpose(0, 1) for x in rows]
+
+    shared = held(c["prefix_table"], prefix)
+    c["dense"] = [[torch.cat(x, 1) for x in zip(shared, held(c["table"][b], int(c["lengths"][b])))]
+                  for b in range(batch)]
+    _check(c, cuda)
+
+
 def test_prefix_past_32_bits(cuda):
     """A contiguous prefix whose last rows lie behind 4 GiB (and 2^31 elements): values of ones
     there, of zeros before, and scores that make only the last rows count."""

@@ -303,6 +303,18 @@ def test_prefix_past_32_bits(cuda):
         assert bool((got == 1).all())
 
 
+@pytest.mark.parametrize("batch", [2, 20])
+def test_rows_far_apart(cuda, batch):
+    """Rows of the prefix whose distance times 16 leaves 31 bits of bytes."""
+    c = _case(7, 39, [5 + b % 7 for b in range(batch)], 4, 1, 64, BF16, 16, 0)
+    far = torch.empty(39 * 2 ** 26 + 128, dtype=BF16, device=cuda)
+    for name, at in (("prefix_k", 0), ("prefix_v", 64)):
+        rows = far.as_strided((1, 1, 39, 64), (0, 0, 2 ** 26, 1), at)
+        rows.copy_(c[name][:, :, :39])
+        c[name] = rows
+    _check(c, cuda)
+
+
 def test_graph_replays_follow_lengths_and_tables(cuda):
     """Two captured calls of different sizes and eager calls between their replays."""
     cases = [_case(9, 600, [90, 40, 0], 8, 2, 64, BF16, 16, 16, fill=0.0),

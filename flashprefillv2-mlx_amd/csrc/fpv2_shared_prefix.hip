@@ -32,7 +32,7 @@ namespace {
 // What a tile of own keys costs a wave beside what one of the prefix, of more than 16 rows, costs
 // each wave of its workgroup: measured best of 1 to 8, at head dim 256 (kOwnWide) of 1 to 20.
 constexpr float kOwnTile = 2.f, kOwnWide = 8.f;
-constexpr int kLong = 24;
+constexpr int kLong = 24, kCoarse = 8;
 
 struct PrefixArgs {
   const uint16_t* q;
@@ -42,6 +42,7 @@ struct PrefixArgs {
   const int32_t* lengths;  // of one
   float* part_o;           // [splits][kv_heads][rows][D]
   float* part_ml;          // [splits][kv_heads][rows][2]
+  int32_t* units;          // [64]: the own keys' Prefix, for the join
   int64_t q_bs, q_hs, k_ps, k_hs, k_rs, v_ps, v_hs, v_rs;
   int kv_heads, group, rows, row_tiles, tile_rows;  // rows: batch * group
   int cus, roomy, most_splits, most_own;  // most_own: workgroups of the own keys
@@ -81,7 +82,9 @@ __host__ __device__ __forceinline__ int waves_of(int64_t rows) { return D > 128 
 // 50 to 44, 8 after 16384 31 to 23, 64 of up to 2000 after 4096 37 to 33.
 // - A few own keys (a 32nd of the work and less) before many of the prefix (kLong tiles a workgroup)
 //   come first all the same: to round the parts down to what they leave costs more (64 sequences after
-//   32768 keys 65 us beside, 61 before; 8 after 16384, 8 tiles a workgroup, 23 and 31).
+//   32768 keys 65 us beside, 61 before; 8 after 16384, 8 tiles a workgroup, 23 and 31).  So they do where
+//   a part has an 8th of the workgroups and more (kCoarse) and that takes longer by the tiles of a
+//   workgroup (512 sequences after 4096 keys 75 beside, 66 before).
 // - The prefix has a second workgroup on a CU where each of one has more than 8 tiles of more than 16
 //   rows (31 sequences after 8192 keys, 8 tiles: 20 us by one, 21 by two and the join 7 and 10;
 //   64 after 8192, 16 tiles: 31 and 26).
@@ -103,15 +106,22 @@ __device__ __forceinline__ Division divide(const PrefixArgs& p, const DecodeArgs
   const float own = static_cast<float>(mine) * (few ? 1.f : D > 128 ? kOwnWide : kOwnTile);
   const float pre = few ? all : all * static_cast<float>(waves);
   // (the parts that then follow on them take all workgroups)
-  const bool before = !few && D <= 128 && all >= static_cast<float>(kLong * slots) && 32.f * mine < pre;
-  const int share = before ? slots : min(static_cast<int>(static_cast<float>(slots) * pre * __builtin_amdgcn_rcpf(own + pre)),
+  const int share = min(static_cast<int>(static_cast<float>(slots) * pre * __builtin_amdgcn_rcpf(own + pre)),
                         few || all <= static_cast<float>(8 * p.cus) ? min(p.cus, slots - 8) : slots - 8);
   // (half a workgroup off a whole number: the quotient's floor)
   const int quotient = static_cast<int>((static_cast<float>(share) + 0.5f) *
                                         __builtin_amdgcn_rcpf(static_cast<float>(each)));
   const int splits = min(max(quotient, 1), most);
   const int need = ((units / kWaves + waves) / waves + 7) / 8 * 8;
-  const int blocks = before ? need : min(max(slots - splits * each, slots - share) / 8 * 8, need);
+  const int blocks = min(max(slots - splits * each, slots - share) / 8 * 8, need);
+  bool before = !few && D <= 128 && all >= static_cast<float>(kLong * slots) && 32.f * mine < pre;
+  if (!few && kCoarse * each >= slots) {
+    const float beside = fmaxf(static_cast<float>(tiles) * __builtin_amdgcn_rcpf(static_cast<float>(splits)),
+                               own * __builtin_amdgcn_rcpf(static_cast<float>(blocks * waves)));
+    const float turns = static_cast<float>(tiles) * __builtin_amdgcn_rcpf(static_cast<float>(most));
+    before = before || turns + own * __builtin_amdgcn_rcpf(static_cast<float>(slots * waves)) + 2.f < beside;
+  }
+  if (before) return {__builtin_amdgcn_readfirstlane(min(need, p.most_own)), __builtin_amdgcn_readfirstlane(most)};
   // (known to be the wave's, and all that follows from them)
   return {__builtin_amdgcn_readfirstlane(min(blocks, p.most_own)), __builtin_amdgcn_readfirstlane(splits)};
 }
@@ -487,6 +497,7 @@ __global__ __launch_bounds__(256, D > 128 ? 1 : 2) void prefix_few_kernel(Prefix
   if (!p.roomy || static_cast<int>(blockIdx.x) < p.most_own) prefix = prefix_of(a, threadIdx.x & 63);
   const Division by = divide<D>(p, a, n, prefix.total * a.kv_heads * a.head_items);
   a.grid = 4 * by.own_blocks;
+  if (blockIdx.x == 0 && threadIdx.x < 64) p.units[threadIdx.x] = prefix.upto;
   const int block = static_cast<int>(blockIdx.x) - by.own_blocks;
   if (block < 0)
     own_attn<T, D>(a, prefix, blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), 8 * p.most_own);
@@ -743,6 +754,7 @@ __global__ __launch_bounds__(64 * Stage<D>::kWaves, D > 128 ? 1 : 2) void prefix
   if (!p.roomy || static_cast<int>(blockIdx.x) < p.most_own) prefix = prefix_of(a, threadIdx.x & 63);
   const Division by = divide<D>(p, a, n, prefix.total * a.kv_heads * a.head_items);
   a.grid = kGroup * by.own_blocks;
+  if (blockIdx.x == 0 && threadIdx.x < 64) p.units[threadIdx.x] = prefix.upto;
   const int block = static_cast<int>(blockIdx.x) - by.own_blocks;
   if (block < 0)
     own_attn<T, D>(a, prefix, blockIdx.x * kGroup + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6),
@@ -768,7 +780,9 @@ __global__ __launch_bounds__(256) void shared_join_kernel(PrefixArgs p, DecodeAr
   const int kvh = head / a.group, g = head - kvh * a.group;
   const int item = kvh * a.head_items + g / a.item_heads, h = g % a.item_heads;
   const int of_prefix = prefix_length(p);
-  const Prefix prefix = prefix_of(a, lane);
+  // (as the first launch had it)
+  const int upto = p.units[lane];
+  const Prefix prefix = {(a.batch + 63) / 64, upto, __builtin_amdgcn_readlane(upto, 63)};
   const int total = prefix.total * items;
   const Division by = divide<D>(p, a, of_prefix, total);
   a.grid = waves_of<D>(p.rows) * by.own_blocks;
@@ -882,7 +896,8 @@ SharedPlan shared_plan(const fpv2_shared_prefix_params& p) {
   // (the parts' workgroups begin at multiples of 8, and so do their ends)
   const int64_t each = p.own.kv_heads * plan.row_tiles, rest = p.own.kv_heads % 8 ? 7 * plan.row_tiles : 0;
   const int64_t all = plan.most_own + plan.most_splits * each + rest, one = plan.most_own + each + rest;
-  const bool before = rows > 16 && p.own.head_dim <= 128 && tiles * each >= kLong * slots;
+  const bool before =
+      rows > 16 && (p.own.head_dim <= 128 && tiles * each >= kLong * slots || kCoarse * each >= slots);
   const int64_t full = slots + rest + (before ? plan.most_own : 0);
   plan.blocks = all < full ? all : one < full ? full : one;
   plan.roomy = plan.most_splits * each <= cus && plan.most_own + plan.most_splits * each <= slots;
@@ -908,7 +923,7 @@ int check_shared(const char* name, const fpv2_shared_prefix_params* p) {
 }
 
 int64_t shared_bytes(const fpv2_shared_prefix_params& p, const SharedPlan& plan) {
-  return p.own.batch == 0 ? 0 : (plan.own_rows + plan.prefix_rows) * (p.own.head_dim + 2) * 4;
+  return p.own.batch == 0 ? 0 : (plan.own_rows + plan.prefix_rows) * (p.own.head_dim + 2) * 4 + 64 * 4;
 }
 
 template <typename T, int D>
@@ -1005,6 +1020,7 @@ extern "C" int fpv2_shared_prefix_attention(const void* q, const void* prefix_k,
   x.part_o = a.part_o + plan.own_rows * p.own.head_dim;
   a.part_ml = x.part_o + plan.prefix_rows * p.own.head_dim;
   x.part_ml = a.part_ml + plan.own_rows * 2;
+  x.units = reinterpret_cast<int32_t*>(x.part_ml + plan.prefix_rows * 2);
   x.q = a.q;
   x.k = static_cast<const uint16_t*>(prefix_k);
   x.v = static_cast<const uint16_t*>(prefix_v);

@@ -151,6 +151,14 @@ __device__ __forceinline__ int workgroup_of(const DecodeArgs& a, int unit, int t
   return static_cast<int>((static_cast<uint64_t>(unit + 1) * runs - 1) / static_cast<uint32_t>(total));
 }
 
+// What a tile's float16 weights are relative to: `headroom` below their greatest exponent, so that this
+// one's weight is 2^headroom.  From 2^24 on not every whole number is a float32 one, and 16 below would be a
+// weight of infinity: there 7 below it, which no rounding makes more than 8.
+__device__ __forceinline__ float below(float greatest, float headroom) {
+  const float to = greatest - headroom;
+  return greatest - to > 15.f ? greatest - 7.f : to;
+}
+
 template <int NW>
 struct Words { uint32_t w[NW]; };
 

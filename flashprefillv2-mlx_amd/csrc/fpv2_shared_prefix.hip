@@ -184,8 +184,9 @@ __device__ __forceinline__ Exponents relate(const f32x4 (&sc)[2], float scale, i
     float to = m;
     if constexpr (kHalf) {
       greatest = fmaxf(greatest, top);
-      if ((top > m + kMost || top < m + kLeast) && greatest > neg_inf())
-        to = fmaxf(top, greatest - kBelow) - kHeadroom;
+      // (by their difference, which is what the weight will be: a sum of m may round to 2^16's)
+      if ((top - m > kMost || top - m < kLeast) && greatest > neg_inf())
+        to = below(fmaxf(top, greatest - kBelow), kHeadroom);
     } else {
       to = top > m + kLag ? top : m;
     }

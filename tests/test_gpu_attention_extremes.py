@@ -1,0 +1,70 @@
+"""Attention of single tokens where scores, scales or values are as great as their types allow,
+against the formula in float64 on the CPU.
+
+Scores here are powers of two and whole numbers of steps beside them, exact in float32, so that
+a weight is 2 to the power of an exact difference whatever the scores' size."""
+
+from __future__ import annotations
+
+import math
+
+import pytest
+import torch
+
+import fpv2
+from batch_cases import BF16, F16
+
+pytestmark = pytest.mark.gpu
+
+LN2 = math.log(2)  # a scale of ln 2: scores are exponents of two
+
+
+def _great_scores(exponent, dtype, dim, heads, n, sign):
+    """Queries ``[heads, dim]``, keys ``[n, dim]`` and the exponents ``[heads, n]``: 2^exponent and
+    whole steps beside it, of 4 or of a float32 number's, which grow (``sign`` 1) or fall (-1) by one from
+    each 128 keys to the next and by one more for a key of each 32."""
+    step = max(4.0, 2.0 ** (exponent - 23))
+    t = torch.arange(n)
+    steps = sign * (t // 128 + (t % 32 == 5).long())
+    q, k = torch.zeros((heads, dim), dtype=dtype), torch.zeros((n, dim), dtype=dtype)
+    q[:, 0], k[:, 0] = 2.0 ** 14, 2.0 ** (exponent - 14)
+    q[:, 3], k[:, 3] = step * (torch.arange(heads) % 3), steps.to(dtype)
+    s = q.double() @ k.double().T
+    assert torch.equal(s, s.float().double())
+    return q, k, s
+
+
+def _great_result(s, v, dtype):
+    """The result and its tolerance: the weights are powers of two, exact where they are 2^-24 of their 32
+    keys' greatest and more, else off by 2^-25 of it; v_exp_f32 by 2^-22, sums of n terms by n 2^-24."""
+    w = torch.exp2(s - s.amax(1, keepdim=True))
+    w = w / w.sum(1, keepdim=True)
+    want, mass = w @ v.double(), w @ v.double().abs()
+    tol = (torch.finfo(dtype).eps / 2 * want.abs() + 2.0 ** -20 * mass
+           + 2 * len(v) * (2.0 ** -24 * mass + 2.0 ** -25 * float(v.abs().max())))
+    return want, tol
+
+
+EXPONENTS = [14, 20, 21, 22, 23, 24, 25, 26, 27, 28]
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("exponent", EXPONENTS)
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("batch", [2, 5])
+def test_shared_prefix_great_scores(cuda, dtype, exponent, dim, batch):
+    """In the prefix, up to 16 rows a KV head and more, and among the own keys."""
+    for sign in (1, -1):
+        n = 600
+        q, k, s = _great_scores(exponent, dtype, dim, 6, n, sign)
+        v = torch.randn((n, dim), generator=torch.Generator().manual_seed(exponent)).to(dtype)
+        want, tol = _great_result(s, v, dtype)
+        kd, vd = k.to(cuda), v.to(cuda)
+        for prefix in (n, 320, 0):
+            own = [x[prefix:].expand(batch, 1, n - prefix, dim).contiguous() if prefix < n
+                   else torch.zeros((batch, 1, 1, dim), dtype=dtype, device=cuda) for x in (kd, vd)]
+            got = fpv2.shared_prefix_attention(
+                q.expand(batch, 6, dim).to(cuda), kd[None, None], vd[None, None], None, prefix, *own, None,
+                n - prefix, scale=LN2)
+            err = (got.cpu().double() - want).abs()
+            assert bool((err <= tol).all()), (sign, prefix, float((err / tol).amax()))

@@ -324,7 +324,7 @@ __device__ __forceinline__ void decode_attn(const DecodeArgs& a, int block, Deco
       float m_new = fmaxf(m, top);
       if constexpr (kByTile) {
         greatest = fmaxf(greatest, top);
-        m_new = fmaxf(top, greatest - kBelow) - kHeadroom;
+        m_new = below(fmaxf(top, greatest - kBelow), kHeadroom);
       }
       // (nothing but -inf so far: weights of zero instead of NaN)
       const float ref = m_new == neg_inf() ? 0.f : m_new;

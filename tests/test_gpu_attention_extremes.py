@@ -12,7 +12,7 @@ import pytest
 import torch
 
 import fpv2
-from batch_cases import BF16, F16
+from batch_cases import BF16, F16, attention, tolerance
 
 pytestmark = pytest.mark.gpu
 
@@ -68,3 +68,18 @@ def test_shared_prefix_great_scores(cuda, dtype, exponent, dim, batch):
                 n - prefix, scale=LN2)
             err = (got.cpu().double() - want).abs()
             assert bool((err <= tol).all()), (sign, prefix, float((err / tol).amax()))
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("exponent", EXPONENTS)
+@pytest.mark.parametrize("dim", [64, 128, 256])
+def test_decode_great_scores(cuda, dtype, exponent, dim):
+    for sign in (1, -1):
+        for n in (1, 600):
+            q, k, s = _great_scores(exponent, dtype, dim, 6, n, sign)
+            v = torch.randn((n, dim), generator=torch.Generator().manual_seed(exponent)).to(dtype)
+            want, tol = _great_result(s, v, dtype)
+            got = fpv2.decode_attention(q[None].to(cuda), k[None, None].to(cuda), v[None, None].to(cuda), None, n,
+                                        scale=LN2)
+            err = (got[0].cpu().double() - want).abs()
+            assert bool((err <= tol).all()), (sign, n, float((err / tol).amax()))

@@ -11,10 +11,11 @@
 //   the queries relative to the power of two of their greatest (bf16's 8 and f16's 11
 //   bits stay whole down to 2^-14 of it, below that they are off by 2^-25 of it);
 //   a key's scale on its score, in float32;
-//   a value's scale on its weight: w_t = p_t vs_t = exp2(x_t + log2 vs_t), rounded to
-//   float16 relative to 2^-15 of the tile's greatest such weight (a tile 2^-40 and more
-//   below the greatest so far: of 2^-40 of that one), so that neither the scores' range nor
-//   the values' sizes cost bits.  The sum of the p_t is of unrounded ones.
+//   a value's scale on its weight: w_t = p_t vs_t = exp2((x_t - m) + log2 vs_t), m the greatest
+//   x so far, rounded to float16 relative to 2^-15 of the tile's greatest such weight (a tile
+//   2^-40 and more below the greatest so far: of 2^-40 of that one), so that neither the scores' range nor
+//   the values' sizes cost bits: the logarithm is added to a difference of exponents, beside whose sizes
+//   (2^17 and more) it would be rounded away.  The sum of the p_t is of unrounded ones.
 //
 // Measured (32 / 8 heads, D = 128): one sequence of 131072 keys 56 us, 4.9 TB/s of codes and scales,
 // where 16-bit keys take 95; 32 sequences of 61 to 16001 keys 47; 1000 keys 7.5 us.  A byte costs
@@ -35,6 +36,7 @@ struct Q8Args {
 };
 
 constexpr float kHeadroom = 15.f, kBelow = 40.f;
+constexpr float kLeast = -150.f;  // weights below are zeros, so that all exponents are small and exact
 
 // Two bytes with the byte of float16's 1024 above each (from words with their top bits
 // turned), less 1152: the codes.
@@ -127,7 +129,7 @@ __global__ __launch_bounds__(256, 2) void decode_q8_kernel(Q8Args args) {
 #pragma unroll
     for (int d = 0; d < DV; ++d) o[d] = f32x4{0.f, 0.f, 0.f, 0.f};
     float m = neg_inf(), l = 0.f;  // the exponent that l is relative to
-    float mo = neg_inf(), greatest = neg_inf();  // and that O is
+    float off = 0.f, greatest = neg_inf();  // and, relative to m, the one that O is, and the greatest so far
 
     const int8_t* kb = k_codes + kvh * a.k_hs;
     const int8_t* vb = v_codes + kvh * a.v_hs;
@@ -190,39 +192,41 @@ __global__ __launch_bounds__(256, 2) void decode_q8_kernel(Q8Args args) {
       }
       const bool cut = u0 + kTileKeys > s_now.n;
       float x[8], y[8], top = neg_inf(), top_o = neg_inf();
+      f32x4 vs[2];
 #pragma unroll
       for (int t = 0; t < 2; ++t) {
         const f32x4 ks = *reinterpret_cast<const f32x4*>(&sh_s[wave][0][16 * t + 4 * quad]);
-        const f32x4 vs = *reinterpret_cast<const f32x4*>(&sh_s[wave][1][16 * t + 4 * quad]);
+        vs[t] = *reinterpret_cast<const f32x4*>(&sh_s[wave][1][16 * t + 4 * quad]);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const int j = 4 * t + i;
           x[j] = sc[t][i] * score_scale * ks[i];
-          y[j] = x[j] + vs[i];
-          if (cut && u0 + 16 * t + 4 * quad + i >= s_now.n) x[j] = y[j] = neg_inf();
+          if (cut && u0 + 16 * t + 4 * quad + i >= s_now.n) x[j] = neg_inf();
           top = fmaxf(top, x[j]);
-          top_o = fmaxf(top_o, y[j]);
         }
       }
       __builtin_amdgcn_wave_barrier();
-      top = fmaxf(top, __shfl_xor(top, 16, 64));
-      top = fmaxf(top, __shfl_xor(top, 32, 64));
-      top_o = fmaxf(top_o, __shfl_xor(top_o, 16, 64));
-      top_o = fmaxf(top_o, __shfl_xor(top_o, 32, 64));
-      top = fmaxf(m, top);
-      greatest = fmaxf(greatest, top_o);
-      top_o = fmaxf(top_o, greatest - kBelow) - kHeadroom;
+      top = fmaxf(m, column_max(top));
       // (nothing but -inf so far: weights of zero instead of NaN)
-      const float ref = top == neg_inf() ? 0.f : top, ref_o = top_o == neg_inf() ? 0.f : top_o;
-      l *= __builtin_amdgcn_exp2f(m - ref);
-      const float fix = __builtin_amdgcn_exp2f(mo - ref_o);
+      const float ref = top == neg_inf() ? 0.f : top, down = m - ref;
       m = top;
-      mo = top_o;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        x[j] -= ref;
+        y[j] = x[j] + vs[j / 4][j % 4];
+        top_o = fmaxf(top_o, y[j]);
+      }
+      top_o = column_max(top_o);
+      greatest = fmaxf(greatest + down, top_o);
+      const float to = fmaxf(fmaxf(top_o, greatest - kBelow), kLeast) - kHeadroom;
+      l *= __builtin_amdgcn_exp2f(down);
+      const float fix = __builtin_amdgcn_exp2f(down + (off - to));
+      off = to;
       u32x4 pf;
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        l += __builtin_amdgcn_exp2f(x[2 * j] - ref) + __builtin_amdgcn_exp2f(x[2 * j + 1] - ref);
-        pf[j] = pack2<f16_t>(__builtin_amdgcn_exp2f(y[2 * j] - ref_o), __builtin_amdgcn_exp2f(y[2 * j + 1] - ref_o));
+        l += __builtin_amdgcn_exp2f(x[2 * j]) + __builtin_amdgcn_exp2f(x[2 * j + 1]);
+        pf[j] = pack2<f16_t>(__builtin_amdgcn_exp2f(y[2 * j] - to), __builtin_amdgcn_exp2f(y[2 * j + 1] - to));
       }
 #pragma unroll
       for (int d = 0; d < DV; ++d) {
@@ -238,7 +242,7 @@ __global__ __launch_bounds__(256, 2) void decode_q8_kernel(Q8Args args) {
     l += __shfl_xor(l, 16, 64);
     l += __shfl_xor(l, 32, 64);
     // O relative to what l is
-    const float fix = mo == neg_inf() ? 0.f : __builtin_amdgcn_exp2f(mo - m);
+    const float fix = __builtin_amdgcn_exp2f(off);
 
     // join the four waves
     if (quad == 0) {

@@ -159,6 +159,14 @@ __device__ __forceinline__ float below(float greatest, float headroom) {
   return greatest - to > 15.f ? greatest - 7.f : to;
 }
 
+// The maximum of a column's four lanes, in each of them.
+__device__ __forceinline__ float column_max(float x) {
+  const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  x = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+  const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
+
 template <int NW>
 struct Words { uint32_t w[NW]; };
 

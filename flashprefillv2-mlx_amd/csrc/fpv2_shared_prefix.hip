@@ -138,14 +138,6 @@ __device__ __forceinline__ Division divide(const PrefixArgs& p, const DecodeArgs
 constexpr float kLag = 8.f, kMost = 15.9f, kLeast = 5.f, kHeadroom = 12.f, kBelow = 40.f;
 constexpr float kNone = -3e38f;  // the reference before any score: below all of them
 
-// The maximum of a column's four lanes, in each of them.
-__device__ __forceinline__ float column_max(float x) {
-  const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-  x = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
-  const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-  return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
-}
-
 // A tile's exponents of 16 rows from its scores (of 32 keys the ones before `live`, counted
 // from the lane's first); O, l and m of the rows are moved where they have to be.
 struct Exponents {

@@ -83,3 +83,41 @@ def test_decode_great_scores(cuda, dtype, exponent, dim):
                                         scale=LN2)
             err = (got[0].cpu().double() - want).abs()
             assert bool((err <= tol).all()), (sign, n, float((err / tol).amax()))
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("exponent", EXPONENTS)
+@pytest.mark.parametrize("dim", [64, 96, 128, 256])
+def test_quantized_decode_great_scores(cuda, dtype, exponent, dim):
+    """The values' scales are of any size beside the scores'.
+
+    Tolerance: weight times scale is rounded once to float16 (half a step of the mass), where it is
+    below 2^-29 of its 32 keys' greatest by 2^-40 of that; the scale's logarithm, of at most 8, is off by 2^-22
+    and the weight's exponent by 2^-20 when it is added; sums as above."""
+    for sign in (1, -1):
+        for n in (1, 600):
+            gen = torch.Generator().manual_seed(exponent)
+            step = max(4.0, 2.0 ** (exponent - 23))
+            t = torch.arange(n)
+            steps = sign * (t // 128 + (t % 32 == 5).long())
+            q = torch.zeros((6, dim), dtype=dtype)
+            k = torch.zeros((n, dim), dtype=torch.int8)
+            ks = torch.full((n,), 2.0 ** (exponent - 20))
+            q[:, 0], k[:, 0] = 2.0 ** 14, 64
+            q[:, 3], k[:, 3] = step * 2.0 ** (20 - exponent) * (torch.arange(6) % 3), steps.to(torch.int8)
+            v = torch.randint(-127, 128, (n, dim), generator=gen).to(torch.int8)
+            vs = 2.0 ** (12 * torch.rand(n, generator=gen) - 6)
+            got = fpv2.quantized_decode_attention(
+                *(x.to(cuda) for x in (q[None], k[None, None], ks[None, None], v[None, None], vs[None, None])),
+                None, n, scale=LN2)
+            s = q.double() @ (k.double() * ks.double()[:, None]).T
+            assert torch.equal(s, s.float().double())
+            value = v.double() * vs.double()[:, None]
+            w = torch.exp2(s - s.amax(1, keepdim=True))
+            w = w / w.sum(1, keepdim=True)
+            want, mass = w @ value, w @ value.abs()
+            greatest = (w * vs.double()).amax(1, keepdim=True)
+            tol = (torch.finfo(dtype).eps / 2 * want.abs() + (2.0 ** -11 + 2.0 ** -19) * mass
+                   + 2 * n * (2.0 ** -24 * mass + 2.0 ** -40 * 127 * greatest))
+            err = (got[0].cpu().double() - want).abs()
+            assert bool((err <= tol).all()), (sign, n, float((err / tol).amax()))

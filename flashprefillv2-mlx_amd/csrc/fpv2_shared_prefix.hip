@@ -258,7 +258,7 @@ struct Rows {
 };
 template <int D>
 __device__ __forceinline__ void start_rows(Rows<D>& r, float scale_log2) {
-  r.scale = fmaxf(__builtin_fabsf(scale_log2), 1e-30f);
+  r.scale = __builtin_fabsf(scale_log2);
   r.m = kNone;
   r.l = 0.f;
   r.greatest = neg_inf();
@@ -606,7 +606,7 @@ __device__ __forceinline__ void prefix_many(ScalarArgs& a, int n, int splits, in
     }
   };
 
-  const float scale = fmaxf(__builtin_fabsf(a.scale_log2), 1e-30f);
+  const float scale = __builtin_fabsf(a.scale_log2);
   u32x4 qf[CT][KK];
   f32x4 o[CT][DT];
   float m[CT], l[CT], greatest[CT];

@@ -121,3 +121,40 @@ def test_quantized_decode_great_scores(cuda, dtype, exponent, dim):
                    + 2 * n * (2.0 ** -24 * mass + 2.0 ** -40 * 127 * greatest))
             err = (got[0].cpu().double() - want).abs()
             assert bool((err <= tol).all()), (sign, n, float((err / tol).amax()))
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("batch", [2, 9])
+@pytest.mark.parametrize("prefix", [300, 0])
+def test_scale_that_is_no_number(cuda, dtype, batch, prefix):
+    """As the formula and the other attentions have it: NaN wherever a key is visible."""
+    gen = torch.Generator().manual_seed(1)
+    q, k, v = (torch.randn(s, generator=gen).to(dtype).to(cuda)
+               for s in ((batch, 4, 64), (batch, 1, 300, 64), (batch, 1, 300, 64)))
+    got = fpv2.shared_prefix_attention(q, k[:1], v[:1], None, prefix, k, v, None, 40, scale=math.nan)
+    assert bool(got.isnan().all())
+    assert bool(fpv2.decode_attention(q, k, v, None, 40, scale=math.nan).isnan().all())
+    got = fpv2.shared_prefix_attention(q, k[:1], v[:1], None, 0, k, v, None, 0, scale=math.nan)
+    assert not got.any()
+
+
+@pytest.mark.parametrize("batch", [2, 9])
+@pytest.mark.parametrize("scale", [2.0 ** -100, 2.0 ** -120, -2.0 ** -110, 0.0])
+def test_scales_far_below_one(cuda, batch, scale):
+    """Great queries and keys under a tiny scale have ordinary scores; a scale of zero has equal
+    weights."""
+    gen = torch.Generator().manual_seed(2)
+    dim, n, prefix = 64, 500, 300
+    size = 2.0 ** round(-math.log2(abs(scale)) / 2) if scale else 1.0
+    q = (torch.randn((batch, 4, dim), generator=gen) * size).to(BF16)
+    k = (torch.randn((n, dim), generator=gen) * size / 2).to(BF16)
+    v = torch.randn((n, dim), generator=gen).to(BF16)
+    kd, vd = k.to(cuda), v.to(cuda)
+    own = [x[prefix:].expand(batch, 1, n - prefix, dim).contiguous() for x in (kd, vd)]
+    got = fpv2.shared_prefix_attention(q.to(cuda), kd[None, None], vd[None, None], None, prefix, *own, None,
+                                       n - prefix, scale=scale)
+    for b in range(batch):
+        want, mass, most = attention(q[b], k[None], v[None], scale)
+        tol = tolerance(want, mass, most, n, dim, BF16, BF16)
+        err = (got[b].cpu().double() - want).abs()
+        assert bool((err <= tol).all()), (b, float((err / tol).max()))

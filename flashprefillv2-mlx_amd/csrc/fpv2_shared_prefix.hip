@@ -136,7 +136,7 @@ __device__ __forceinline__ Division divide(const PrefixArgs& p, const DecodeArgs
 // 2^-30 of it.  (2^-15 instead of 2^-12: most tiles have a column that exceeds it, 128
 // sequences of an 8191-key prefix 41 us instead of 38.)
 constexpr float kLag = 8.f, kMost = 15.9f, kLeast = 5.f, kHeadroom = 12.f, kBelow = 40.f;
-constexpr float kNone = -3e38f;  // the reference before any score: below all of them
+constexpr float kNone = -3.4028234663852886e38f;  // the reference before any score: no finite one is below
 
 // A tile's exponents of 16 rows from its scores (of 32 keys the ones before `live`, counted
 // from the lane's first); O, l and m of the rows are moved where they have to be.

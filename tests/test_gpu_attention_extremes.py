@@ -158,3 +158,20 @@ def test_scales_far_below_one(cuda, batch, scale):
         tol = tolerance(want, mass, most, n, dim, BF16, BF16)
         err = (got[b].cpu().double() - want).abs()
         assert bool((err <= tol).all()), (b, float((err / tol).max()))
+
+
+@pytest.mark.parametrize("batch", [2, 9])
+@pytest.mark.parametrize("prefix", [100, 0])
+def test_scores_near_the_lowest(cuda, batch, prefix):
+    """Every score next to float32's lowest number: equal weights."""
+    dim = 64
+    q, k = torch.zeros((batch, 4, dim), dtype=BF16), torch.zeros((1, 1, 100, dim), dtype=BF16)
+    q[:, :, 0], k[..., 0] = -1.984375 * 2.0 ** 64, 2.0 ** 63
+    v = torch.randn((1, 1, 100, dim), generator=torch.Generator().manual_seed(3)).to(BF16)
+    own = [x.expand(batch, 1, 100, dim).contiguous().to(cuda) for x in (k, v)]
+    got = fpv2.shared_prefix_attention(q.to(cuda), k.to(cuda), v.to(cuda), None, prefix, *own, None,
+                                       100 if prefix == 0 else 0, scale=LN2)
+    want, mass = v[0, 0].double().mean(0), v[0, 0].double().abs().mean(0)
+    # (equal weights of at most 2^7: exact in bfloat16; sums of 100 terms)
+    err = (got.cpu().double() - want).abs()
+    assert bool((err <= 2.0 ** -8 * want.abs() + 300 * 2.0 ** -24 * mass).all())

@@ -128,7 +128,8 @@ __device__ __forceinline__ Division divide(const PrefixArgs& p, const DecodeArgs
 
 // A column's weights are 2^(x - m), x = scale log2(e) q.k, with a reference m that moves when
 // it has to, so that most tiles rescale nothing.
-//   bfloat16: where a weight exceeds 2^kLag, to the greatest score.
+//   bfloat16: where a weight exceeds 1, to 2^-kLag of the greatest score (not above 1: sums of values
+// next to the type's greatest would leave float32).
 //   float16, which has only 2^-14 to 2^16: where a weight would exceed 2^kMost or the
 // tile's greatest is below 2^kLeast, to 2^-12 of the tile's greatest score (or 2^-40 of the
 // greatest so far, so that no float32 sum overflows).  So weights down to 2^-19 of their
@@ -162,7 +163,7 @@ __device__ __forceinline__ Exponents relate(const f32x4 (&sc)[2], float scale, i
     const uint32_t any = static_cast<uint32_t>(some) | static_cast<uint32_t>(some >> 32);
     move = ((any | any >> 16) & 0xffffu) != 0xffffu || __any(top > kMost);
   } else {
-    move = __any(top > kLag);
+    move = __any(top > 0.f);
   }
   if (move) {
     top = neg_inf();
@@ -180,7 +181,7 @@ __device__ __forceinline__ Exponents relate(const f32x4 (&sc)[2], float scale, i
       if ((top - m > kMost || top - m < kLeast) && greatest > neg_inf())
         to = below(fmaxf(top, greatest - kBelow), kHeadroom);
     } else {
-      to = top > m + kLag ? top : m;
+      to = top > m ? top + kLag : m;
     }
     const float fix = __builtin_amdgcn_exp2f(m - to);
     m = to;

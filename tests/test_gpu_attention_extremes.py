@@ -161,6 +161,29 @@ def test_scales_far_below_one(cuda, batch, scale):
 
 
 @pytest.mark.parametrize("batch", [2, 9])
+@pytest.mark.parametrize("prefix", [400, 200, 0])
+@pytest.mark.parametrize("gap", [0.0, 3.0, 7.5, 8.0, 8.5])
+def test_values_near_the_greatest(cuda, batch, prefix, gap):
+    """One key ``gap`` bits above the ones before it, whose value is next to bfloat16's greatest
+    number, as the result is: no weight leaves more room above a value than ``decode_attention``'s do."""
+    n, dim, at = 400, 64, 390
+    q, k, v = torch.zeros((batch, 4, dim), dtype=BF16), torch.zeros((n, dim), dtype=BF16), torch.zeros((n, dim))
+    q[:, :, 0], k[at, 0] = 1.0, gap
+    v = v.to(BF16)
+    v[at] = 2.0 ** 127 * 1.875
+    kd, vd = k.to(cuda), v.to(cuda)
+    own = [x[prefix:].expand(batch, 1, n - prefix, dim).contiguous() if prefix < n
+           else torch.zeros((batch, 1, 1, dim), dtype=BF16, device=cuda) for x in (kd, vd)]
+    got = fpv2.shared_prefix_attention(q.to(cuda), kd[None, None], vd[None, None], None, prefix, *own, None,
+                                       n - prefix, scale=LN2)
+    want, mass, most = attention(q[0], k[None], v[None], LN2)
+    assert bool(fpv2.decode_attention(q[:1].to(cuda), kd[None, None], vd[None, None], None, n, scale=LN2)
+                .isfinite().all())
+    err = (got.cpu().double() - want).abs()
+    assert bool((err <= tolerance(want, mass, most, n, dim, BF16, BF16)).all())
+
+
+@pytest.mark.parametrize("batch", [2, 9])
 @pytest.mark.parametrize("prefix", [100, 0])
 def test_scores_near_the_lowest(cuda, batch, prefix):
     """Every score next to float32's lowest number: equal weights."""

@@ -32,6 +32,9 @@ from fpv2.decode import (_HALF, MAX_VOCAB, _check_apart, _count, _device, _exten
                          _rows_meet, _rows_overlap, _share_memory)
 from fpv2.kernel import SUPPORTED_HEAD_DIMS
 
+MAX_SEQUENCES = 0xFFFF       # of an attention call
+MAX_QUERY_HEADS = 0xFFFFFF   # of all its sequences together, after a shared prefix
+
 
 def _table(page_table, rows: int | None, name: str):
     """A page table's width and row stride; ``rows`` ``None``: of one sequence, ``[n]``."""

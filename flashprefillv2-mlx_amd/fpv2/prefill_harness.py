@@ -38,7 +38,7 @@ import torch
 import torch.nn.functional as F
 
 from fpv2 import _lib
-from fpv2.batch import shared_prefix_attention, token_logprobs
+from fpv2.batch import MAX_QUERY_HEADS, MAX_SEQUENCES, shared_prefix_attention, token_logprobs
 from fpv2.chunked import ChunkedPrefill
 from fpv2.decode import (GROUP_SIZES, MAX_VOCAB, _device as check_device, _settings,
                          decode_attention, dequantize_weight, quantize_weight, quantized_linear,
@@ -435,10 +435,16 @@ class ChunkedPrefillRunner:
         attention is the runner's, into the caches, which have to be empty.  Tokens as in
         ``prefill`` (of the vocabulary); a text of one token has no score."""
         m, n = self.model, tokens.numel()
+        # (what could be refused is looked at before the text is prefilled)
         if tokens.ndim != 1 or n == 0 or chunk <= 0:
             raise ValueError("score needs a text [tokens] and a positive chunk")
+        if tokens.dtype not in (torch.int32, torch.int64):
+            raise ValueError("tokens must be int32 or int64")
+        if m.embed.shape[0] > MAX_VOCAB:
+            raise ValueError(f"the vocabulary must have 1 to {MAX_VOCAB} tokens")
         if any(cache.length for cache in self.caches):
             raise ValueError("score starts from empty caches: call reset() first")
+        check_device([tokens, m.embed])
         out, rows = [], 512  # rows whose logits are held at a time
         for x, delta, end in self._chunks(tokens, chunk):
             last = _add_rms_norm(x, delta, m.final_norm, m.shape.rms_eps)
@@ -546,6 +552,9 @@ class ChunkedPrefillRunner:
             if isinstance(value, bool) or not isinstance(value, int) or value <= 0:
                 raise ValueError(f"{name} must be a positive integer")
         # (what could be refused is looked at before the prompt is prefilled)
+        if samples > MAX_SEQUENCES or samples * s.query_heads > MAX_QUERY_HEADS:
+            raise ValueError(f"samples must be at most {MAX_SEQUENCES}, and {MAX_QUERY_HEADS} of all "
+                             "their query heads")
         if self.attention == "sdpa":
             raise ValueError("generate_many goes on over the caches of 'fpv2' or 'dense'")
         settings = [rows for rows, _ in _settings(temperature, top_k, top_p, min_p, samples)

@@ -178,3 +178,24 @@ def test_scores_of_samples_and_alternatives(cuda):
     greedy = fpv2.sample_tokens(logits, torch.zeros(33, device=cuda), temperature=0.0)
     assert torch.equal(res.top_tokens[:, 0], greedy)
     assert bool((res.top_logprobs.diff(dim=1)[live] <= 0).all())
+
+
+def test_refused_before_the_prompt_is_prefilled(cuda):
+    """What ``score`` and ``generate_many`` cannot do leaves the caches empty."""
+    runner = ChunkedPrefillRunner(_model(cuda), 64)
+    text = _prompt(cuda, 40)
+    for bad, error in ((text.cpu(), RuntimeError), (text.to(torch.uint8), ValueError),
+                       (text.float(), ValueError), (text[None], ValueError)):
+        with pytest.raises(error):
+            runner.score(bad, 16)
+        assert all(cache.length == 0 for cache in runner.caches)
+    heads = DecoderShape(layers=1, hidden=64, query_heads=512, kv_heads=32, head_dim=64, intermediate=64, vocab=100)
+    for shape, samples in ((SHAPE, 65_536), (heads, 32_768)):
+        many = ChunkedPrefillRunner(RandomDecoder(shape, device=cuda, seed=1), 64)
+        with pytest.raises(ValueError, match="samples must be at most"):
+            many.generate_many(text % 100, 16, 2, samples)
+        assert all(cache.length == 0 for cache in many.caches)
+    runner.model.embed = torch.zeros(((1 << 19) + 1, SHAPE.hidden), dtype=BF16, device=cuda)
+    with pytest.raises(ValueError, match="vocabulary"):
+        runner.score(text, 16)
+    assert all(cache.length == 0 for cache in runner.caches)

@@ -400,12 +400,17 @@ class ChunkedPrefillRunner:
         return _row_logits(last[0], w)
 
     def _angles(self, positions: int) -> tuple:
-        """cos / sin ``[positions or more, head_dim / 2]`` of a decode step's rotation."""
-        if self._tables is None or self._tables[0].shape[0] < positions:
-            pos = torch.arange(max(positions, self.capacity), device=self.model.device)
-            half = self.model.shape.head_dim // 2
-            self._tables = tuple(t[:, :half].contiguous() for t in rope_tables(self.model.shape, pos))
-        return self._tables
+        """cos / sin ``[positions or more, head_dim / 2]`` of a decode step's rotation: the
+        ones kept for the caches' positions (a captured ``decode`` reads them), of more the
+        call's own."""
+        if self._tables is not None and positions <= self.capacity:
+            return self._tables
+        pos = torch.arange(max(positions, self.capacity), device=self.model.device)
+        half = self.model.shape.head_dim // 2
+        tables = tuple(t[:, :half].contiguous() for t in rope_tables(self.model.shape, pos))
+        if positions <= self.capacity:
+            self._tables = tables
+        return tables
 
     def _linear(self, x: torch.Tensor, li: int, name: str) -> torch.Tensor:
         """A decode step's projection, with 4-bit weights where the model has them."""

@@ -199,3 +199,17 @@ def test_refused_before_the_prompt_is_prefilled(cuda):
     with pytest.raises(ValueError, match="vocabulary"):
         runner.score(text, 16)
     assert all(cache.length == 0 for cache in runner.caches)
+
+
+def test_angles_of_the_decode_step_stay(cuda):
+    """Samples past the capacity take angles of their own: a captured ``decode`` reads the runner's."""
+    runner = ChunkedPrefillRunner(_model(cuda), 50)
+    prompt = _prompt(cuda, 40)
+    runner.prefill(prompt, 64)
+    runner.decode(prompt[:1])
+    kept = [x.data_ptr() for x in runner._tables]
+    runner.reset()
+    tokens, _ = runner.generate_many(prompt, 64, 30, 2, temperature=0.0)
+    assert [x.data_ptr() for x in runner._tables] == kept
+    wide = ChunkedPrefillRunner(runner.model, 70)
+    assert torch.equal(wide.generate_many(prompt, 64, 30, 2, temperature=0.0)[0], tokens)

@@ -9,8 +9,9 @@ import pytest
 import torch
 
 import fpv2
-from fpv2 import ChunkedPrefill
-from fpv2.prefill_harness import ChunkedPrefillRunner, DecoderShape, RandomDecoder
+from batch_cases import attention, tolerance
+from fpv2 import ChunkedPrefill, prefill_harness
+from fpv2.prefill_harness import ChunkedPrefillRunner, DecoderShape, RandomDecoder, rope_tables
 
 pytestmark = pytest.mark.gpu
 
@@ -213,3 +214,97 @@ def test_angles_of_the_decode_step_stay(cuda):
     assert [x.data_ptr() for x in runner._tables] == kept
     wide = ChunkedPrefillRunner(runner.model, 70)
     assert torch.equal(wide.generate_many(prompt, 64, 30, 2, temperature=0.0)[0], tokens)
+
+
+def _later(k, by):
+    """Rotated keys ``[Hkv, n, D]`` as they would be ``by`` positions later."""
+    cos, sin = (x.cpu().double() for x in rope_tables(SHAPE, torch.tensor([by])))
+    half = k.shape[-1] // 2
+    return k * cos + torch.cat([-k[..., half:], k[..., :half]], -1) * sin
+
+
+@pytest.mark.parametrize("quantized", [False, True])
+@pytest.mark.parametrize("samples,n", [(1, 20), (3, 3), (5, 300), (40, 130)])
+def test_steps_of_samples(cuda, monkeypatch, quantized, samples, n):
+    """Every attention call of every step sees the prompt and the sample's own tokens, each at its
+    position, and its result is theirs; the logits are those of a sequence that decodes the same tokens.
+
+    Tolerances.  Keys and values against the other run's: rows of a projection differ by a rounding to
+    bfloat16 on either side (2^-8 of an element), a key's norm by as much, its rotation mixes two
+    elements: 6 2^-8 < 2^-5 of the row's greatest.  In the second layer the streams differ by some 12 roundings
+    of 2^-9 / sqrt(3) (0.4 %), which change a projection by as much of its deviation, five times that at
+    most among these rows: still below 2^-5 of the greatest, more than twice the deviation.  Attention: of the
+    call's own operands, as ``batch_cases`` derives it.  Logits: 24 roundings are 0.6 % of a stream
+    of deviation 1, times 16 rows of 0.02: a deviation of 0.002, and 2^-5.6 is ten of them.
+
+    What these see, planted in the reference: a key one position off in every call, the prompt's last
+    key or the last own one left out in some."""
+    layers, new = SHAPE.layers, 6
+    calls, logits = [], []
+
+    def attend(q, *args):
+        out = fpv2.shared_prefix_attention(q, *args)
+        calls.append([x.cpu() if isinstance(x, torch.Tensor) else x for x in (q, *args, out)])
+        return out
+
+    def score(rows, tokens):
+        logits.append(rows)
+        return fpv2.token_logprobs(rows, tokens)
+
+    monkeypatch.setattr(prefill_harness, "shared_prefix_attention", attend)
+    monkeypatch.setattr(prefill_harness, "token_logprobs", score)
+    model = _model(cuda, quantized)
+    runner = ChunkedPrefillRunner(model, n + 8)
+    prompt = _prompt(cuda, n)
+    uniform = torch.rand((samples, new), generator=torch.Generator().manual_seed(1)).to(cuda)
+    tokens, logprobs = runner.generate_many(prompt, 64, new, samples, uniform=uniform, top_k=200)
+    assert len(calls) == layers * (new - 1) and len(logits) == new
+    seen = [0, 0]
+    for b in {0, samples // 2, samples - 1}:
+        other = ChunkedPrefillRunner(model, n + 8)
+        want = _forced(other, prompt, 64, tokens[b])
+        got = torch.stack([rows[b] for rows in logits])
+        assert bool(((got - want).abs() <= 2.0 ** -5.6).all())
+        given = torch.log_softmax(got.double(), 1).gather(1, tokens[b][:, None])[:, 0]
+        assert bool(((logprobs[b] - given).abs() <= 1e-5).all())
+        for c, (q, pk, pv, table, prefix, k, v, own_table, own, out) in enumerate(calls):
+            step, cache = c // layers, other.caches[c % layers]
+            assert table is None and own_table is None and prefix == n and own == step + 1
+            held = [torch.cat([x[0, :, :prefix], y[b, :, :own]], 1).double() for x, y in ((pk, k), (pv, v))]
+            for x, y in zip(held, (cache.k, cache.v)):
+                y = y[:, :n + own].cpu().double()
+                assert torch.equal(x[:, :n], y[:, :n])
+                bound = 2.0 ** -5 * y.abs().amax(-1, keepdim=True)
+                assert bool(((x - y).abs() <= bound).all())
+            for by in (-1, 1):
+                wrong = _later(held[0], by)
+                assert bool(((wrong - held[0]).abs() > bound).any(-1).all())
+            result, mass, size = attention(q[b], *held, 0.125)
+            tol = tolerance(result, mass, size, n + own, 64, BF16, BF16)
+            assert bool(((out[b].double() - result).abs() <= tol).all())
+            for i, gone in enumerate((n - 1, n + own - 1)):
+                keep = torch.arange(n + own) != gone
+                wrong = attention(q[b], *(x[:, keep] for x in held), 0.125)[0]
+                seen[i] += int(((wrong - result).abs() > 2 * tol).any())
+    assert min(seen) > 0, seen
+
+
+@pytest.mark.parametrize("n,chunk", [(2, 8), (65, 64), (700, 128), (1300, 1024)])
+def test_scores_are_of_the_next_tokens(cuda, n, chunk):
+    """Each row's log probability of the token behind it, from the same chunks' last rows.
+
+    Tolerance: a logit is a float32 sum of 256 products, off by 256 2^-24 of their size; the
+    log probability by twice the largest of these and 2^-16 (sums of 1000 weights).  Planted in the reference:
+    rows or tokens one off."""
+    model = _model(cuda)
+    text = _prompt(cuda, n, seed=n)
+    scores = ChunkedPrefillRunner(model, n, attention="dense").score(text, chunk).cpu().double()
+    rows = [prefill_harness._add_rms_norm(x, delta, model.final_norm, SHAPE.rms_eps).cpu().double()
+            for x, delta, _ in ChunkedPrefillRunner(model, n, attention="dense")._chunks(text, chunk)]
+    rows, embed, text = torch.cat(rows), model.embed.cpu().double(), text.cpu()
+    tol = 2 * 256 * 2.0 ** -24 * float((rows.abs() @ embed.abs().T).max()) + 2.0 ** -16
+    logs = torch.log_softmax(rows @ embed.T, 1)
+    want = logs[:-1].gather(1, text[1:, None])[:, 0]
+    assert bool(((scores - want).abs() <= tol).all())
+    for wrong in (logs[1:].gather(1, text[1:, None])[:, 0], logs[:-1].gather(1, text[:-1, None])[:, 0]):
+        assert bool(((want - wrong).abs() > 2 * tol)[:n - 1].any())

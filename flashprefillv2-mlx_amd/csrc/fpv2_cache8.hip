@@ -196,14 +196,6 @@ int check_cache(const char* name, const fpv2_code_pages& c) {
   return FPV2_OK;
 }
 
-// t / page_size = (umulhi(t, mul) + t) >> shift for t below 2^31.
-void page_division(int64_t page_size, uint32_t* mul, uint32_t* shift) {
-  uint32_t s = 0;
-  while ((1ull << s) < static_cast<uint64_t>(page_size)) ++s;
-  *shift = s;
-  *mul = static_cast<uint32_t>((((1ull << s) - page_size) << 32) / page_size + 1);
-}
-
 bool a16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
 template <typename A>

@@ -18,6 +18,14 @@ int fail(int status, const char* fmt, ...);
 int check_launch(const char* kernel);
 int cu_count();  // compute units of the current device
 
+// t / page_size = (umulhi(t, mul) + t) >> shift for t below 2^31.
+inline void page_division(int64_t page_size, uint32_t* mul, uint32_t* shift) {
+  uint32_t s = 0;
+  while ((1ull << s) < static_cast<uint64_t>(page_size)) ++s;
+  *shift = s;
+  *mul = static_cast<uint32_t>((((1ull << s) - page_size) << 32) / page_size + 1);
+}
+
 // ---------------------------------------------------------------------------
 // Vector types.  16-bit element types are carried as raw uint16 bits in
 // memory; the MFMA operands are 8-element vectors of the element type.

@@ -556,14 +556,6 @@ inline int64_t partial_bytes(const fpv2_decode_params& p, const DecodePlan& plan
   return 2LL * plan.grid * plan.item_heads * (p.head_dim + 2) * 4;
 }
 
-// t / page_size = (umulhi(t, mul) + t) >> shift for t below 2^31.
-inline void page_division(int64_t page_size, uint32_t* mul, uint32_t* shift) {
-  uint32_t s = 0;
-  while ((1ull << s) < static_cast<uint64_t>(page_size)) ++s;
-  *shift = s;
-  *mul = static_cast<uint32_t>((((1ull << s) - page_size) << 32) / page_size + 1);
-}
-
 // The launch's arguments but for the pointers.
 inline DecodeArgs decode_args(const fpv2_decode_params& p, const DecodePlan& plan) {
   DecodeArgs a{};

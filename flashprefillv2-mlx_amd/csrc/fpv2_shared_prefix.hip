@@ -18,7 +18,8 @@
 // Measured (32 / 8 heads, D = 128; caches that change from call to call): 40 sequences of 20 to 700 own
 // keys after 32768 in pages of 64, bfloat16, 58 us + the join's 8; 128 of 5 to 300 after 8191, float16,
 // 44 + 10; 64 of up to 32 after 32768 61 + 10.5; 16 / 4 heads of D = 256, 21 of 9 to 1500 after 20011, 40 + 8.
-// Up to 16 rows 4 sequences after 32768 keys 34 + 8, one after 131072 93 + 7.5 (5.7 TB/s).  A launch takes
+// Up to 16 rows 4 sequences after 32768 keys 34 + 8, one after 131072 93 + 7.5 (5.7 TB/s); 16 / 4 heads of
+// D = 256, 4 of 30 after 32768 43 for both.  A launch takes
 // some 5 us of these, and each MB of partials (10 to 33 of them) half a microsecond.
 // Without gain: workgroups of 8 waves in two groups of keys that join in LDS (half the partials,
 // but a barrier of 8 waves in each step), partials past the caches (1.5 us less here, 1.5 more in
@@ -30,7 +31,8 @@ namespace fpv2 {
 namespace {
 
 // What a tile of own keys costs a wave beside what one of the prefix, of more than 16 rows, costs
-// each wave of its workgroup: measured best of 1 to 8, at head dim 256 (kOwnWide) of 1 to 20.
+// each wave of its workgroup: measured best of 1 to 8, at head dim 256 (kOwnWide) of 1 to 20 by one batch, 21
+// sequences of 9 to 1500 after 20011 keys.
 constexpr float kOwnTile = 2.f, kOwnWide = 8.f;
 constexpr int kLong = 24, kCoarse = 8;
 
@@ -193,7 +195,9 @@ __device__ __forceinline__ Exponents relate(const f32x4 (&sc)[2], float scale, i
   }
   return e;
 }
-// Their weights, as the B operand of the product with V, and l's share.
+// Their weights, as the B operand of the product with V, and l's share.  MFMA takes both of one type, so they are
+// rounded to V's: half a step of each, which together is about as much as the result's own rounding (against
+// float64 0.0023 of the result in bfloat16, 0.0017 of it the result's); l is the sum of the unrounded ones.
 template <typename T>
 __device__ __forceinline__ u32x4 weigh(const Exponents& e, float& l) {
   u32x4 pf;

@@ -490,7 +490,7 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, *, top: int = 0) 
     ``logits`` float32, float16 or bfloat16, any strides (rows that are not contiguous
     are copied first).  Sums are in float32.  A token outside the vocabulary (padding, or
     ``sample_tokens``' -1) has -inf.  A NaN logit counts as -inf, magnitudes beyond 2^126 as
-    2^126; a row of nothing but -inf gives -inf, an entropy of 0 and, as for every
+    2^126 in the probabilities (alternatives are in the order of the logits as given); a row of nothing but -inf gives -inf, an entropy of 0 and, as for every
     alternative that is missing because fewer tokens are above -inf, token -1 with -inf.
     """
     if logits.ndim != 2 or logits.dtype not in (torch.float32, *_HALF):

@@ -150,8 +150,8 @@ typedef struct fpv2_logprobs_params {
  *   entropy[r] = -sum p log p, in nats
  *   top_tokens[r][i], top_logprobs[r][i]: the i-th greatest logit's token, of equal ones
  *   the first, and log p of it; -1 and -inf where there is none above -inf
- * A NaN logit counts as -inf, magnitudes beyond 2^126 as 2^126; a row of nothing but -inf has
- * logprob -inf and entropy 0.  float32 arithmetic.  workspace:
+ * A NaN logit counts as -inf, magnitudes beyond 2^126 as 2^126 (in p; the alternatives are in the order of
+ * the logits as given); a row of nothing but -inf has logprob -inf and entropy 0.  float32 arithmetic.  workspace:
  * fpv2_token_logprobs_workspace_bytes bytes for the current device (0: none), 16-byte
  * aligned, not kept between calls; calls that share one on different streams race.
  */
